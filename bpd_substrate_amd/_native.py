@@ -17,6 +17,7 @@ HIP_LIB = os.environ.get("BPDQ_HIP_LIB") or os.path.join(PKG, "libbpdq_hip.so")
 SYNTH_LIB = os.environ.get("BPDQ_SYNTH_LIB") or os.path.join(PKG, "libbpdq_synth.so")
 
 P, I, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+L = ctypes.c_int64
 
 # name -> (restype, argtypes); the full exported surface of include/bpdq.h
 HIP_SIGNATURES = {
@@ -100,6 +101,12 @@ HIP_SIGNATURES = {
     "bpd_residual_rmsnorm_gpu": (None, [P, P, P, P, P, P, I, F]),
     "bpd_expf_gpu": (None, [P, P, I]),
     "bpd_argmax_gpu": (None, [P, I, P]),
+    # include/bpdq_serve.h; the structs are passed by address
+    "bpd_rope_append_paged_gpu": (None, [P, P, P, P, P, L, P, L, P, L, P, L, I, I]),
+    "bpd_attn_paged_gpu": (None, [P, P, P, L, P, L, P, I, I, F, P, L]),
+    "bpd_attn_paged_workspace": (L, [P, P, I]),
+    "bpd_sample_gpu": (None, [P, I, L, I, I, P, P, P, P, P, P, P, P, P, L]),
+    "bpd_sample_workspace": (L, [I, I]),
 }
 
 SYNTH_SIGNATURES = {
