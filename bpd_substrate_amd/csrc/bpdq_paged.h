@@ -99,7 +99,7 @@ struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Vec {
 void launch_rope_append(const Paged& a, int cache_type, const double* turns, int rot, bool neox, const int32_t* pos,
                         const void* q, int64_t qs, const void* k, int64_t ks, const void* v, int64_t vs, void* qo,
                         int64_t qos, int x_type, int H, hipStream_t s);
-int64_t attn_paged_ws(int B, int T, int H, int HKV, int D, int P);
+int64_t attn_paged_ws(const int32_t* q_start, int B, int T, int H, int HKV, int D, int P);
 void launch_attn_paged(const Paged& a, int cache_type, const void* q, int64_t qs, void* out, int64_t os, float* lse,
                        int q_type, int H, float scale, void* ws, hipStream_t s);
 int64_t sample_ws(int n_rows, int vocab);

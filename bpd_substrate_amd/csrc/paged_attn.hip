@@ -31,7 +31,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kKeys = 64;   // keys of a unit
-constexpr int kGroups = 512;  // workgroups that share the units: 2 per CU
+constexpr int kGroupsMax = 512;  // workgroups that share the units: one of 8 waves or two of 4 per CU
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -__builtin_inff();
 
@@ -55,17 +55,27 @@ struct AttnArgs {
     int H, G;
     float scale;
     FastDiv g;  // by G
-    int R, DT;  // rows of a tile, padded head size
+    int R, DT;   // rows of a tile, padded head size
+    int groups;  // workgroups
+    bool planned;  // the items are the plan's; otherwise every token is packed, and sequences are k_attn_wave's
     Plan p;
-    float* part;  // [slot][R][DT]
-    float2* ml;   // [slot][R] reference exponent, sum
+    float* part;   // [slot][R][DT]
+    float2* ml;    // [slot][R] reference exponent, sum
+    int2* where;   // [head][item] first slot of its results and their number, 0 where the output is written
+    int waves;     // k_attn_wave: shares
+    float* part1;  // k_attn_wave's results, [slot][G][DT], and the same of them
+    float2* ml1;
+    int2* where1;  // [head][sequence]
 };
 
 __host__ __device__ constexpr int round64(int v) { return (v + 63) / 64; }
-__device__ __forceinline__ int64_t slot_of(int group, int item, int hkv, int h) {
-    return (int64_t)group + (int64_t)item * hkv + h;
+// Units are numbered head by head, as a head's items may share keys (a prefix), which its neighbours in
+// the order then find in the L2 of their XCD.  [w U / n, (w + 1) U / n) go to share w of n = min(groups, U).
+// A share leaves at most one result per (head, item): share and pair never repeat together
+// in share + pair, as each step along the units raises one or both.
+__device__ __forceinline__ int64_t slot_of(int share, int item, int nitems, int h) {
+    return (int64_t)share + (int64_t)h * nitems + item;
 }
-// Units are dealt as [w U / n, (w + 1) U / n) to workgroup w of n = min(kGroups, U).
 __device__ __forceinline__ int64_t unit_of(int w, int64_t U, int n) { return w * U / n; }
 __device__ __forceinline__ int group_of(int64_t u, int64_t U, int n) { return (int)(((u + 1) * n - 1) / U); }
 
@@ -81,81 +91,98 @@ __device__ __forceinline__ int seen_rows(const Paged& a, int b, int n, int i, in
     return (int)(s < 0 ? 0 : s > own ? own : s);
 }
 
-// One workgroup lays out the items.  Sequences are taken 256 at a time, a thread each.
-__global__ __launch_bounds__(256) void k_attn_plan(AttnArgs g) {
-    __shared__ int s_scan[256];
-    __shared__ int s_run[3];
+// One workgroup lays out the items.  Sequences are taken 1024 at a time, a thread each, then their tiles
+// and tokens, a thread each.
+__global__ __launch_bounds__(1024) void k_attn_plan(AttnArgs g) {
+    constexpr int N = 1024;
+    __shared__ int s_wave[N / 64];
+    __shared__ int s_at[N];   // exclusive sums of a round
     const Paged& a = g.a;
-    const int tid = (int)threadIdx.x;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int ntp = round64(a.P);
-    auto scan = [&](int v) {  // exclusive over the workgroup, the total in s_scan[255] + v of the last
-        s_scan[tid] = v;
-        __syncthreads();
-        for (int d = 1; d < 256; d <<= 1) {
-            const int o = tid >= d ? s_scan[tid - d] : 0;
-            __syncthreads();
-            s_scan[tid] += o;
-            __syncthreads();
+    auto scan = [&](int v) {  // (exclusive sum, total) over the workgroup
+        int x = v;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(x, d);
+            if (lane >= d) x += o;
         }
-        const int r = s_scan[tid] - v, total = s_scan[255];
         __syncthreads();
-        return make_int2(r, total);
+        if (lane == 63) s_wave[wave] = x;
+        __syncthreads();
+        int before = 0, total = 0;
+        for (int i = 0; i < N / 64; i++) {
+            if (i < wave) before += s_wave[i];
+            total += s_wave[i];
+        }
+        return make_int2(before + x - v, total);
     };
-    // the packed rows
+    // the packed tokens
     int packed = 0;
-    if (a.P > 0)
-        for (int b0 = 0; b0 < a.B; b0 += 256) {
+    if (a.P > 0) {
+        for (int b0 = 0; b0 < a.B; b0 += N) {
             const int b = b0 + tid;
             int t0 = 0, n = 0;
             if (b < a.B) seq_tokens(a, b, t0, n);
             const bool in = n > 0 && !is_joint(g, n);
             const int2 at = scan(in ? n : 0);
-            for (int i = 0; i < n; i++) {
-                const int k = packed + at.x + i;
-                if (in && k < a.T) g.p.packed[k] = t0 + i;
-                g.p.place[t0 + i] = in && k < a.T ? k : -1;
-            }
-            packed += at.y;
+            if (in)  // fewer than R / 2G tokens
+                for (int i = 0; i < n; i++) {
+                    const int k = packed + at.x + i;
+                    if (k < a.T) g.p.packed[k] = t0 + i;
+                    g.p.place[t0 + i] = k < a.T ? k : -1;
+                }
+            packed = min(packed + at.y, a.T);
         }
-    packed = min(packed, a.T);
+    }
     const int np = packed > 0 ? (packed * g.G + g.R - 1) / g.R : 0;
-    for (int i = tid; i < np; i += 256) {
+    for (int i = tid; i < np; i += N) {
         g.p.first[i] = i * ntp;
         g.p.seq[i] = -1;
         g.p.rt[i] = i;
     }
-    int items = np, units = np * ntp;
-    // most items there can be: overlapping sequences (offsets that decrease) stop the plan there
+    // the sequences' own tiles
+    int items = np;
+    // more than this many only offsets that decrease can ask for: the plan ends there
     const int most = np + a.B + (int)(((int64_t)a.T * g.G) / g.R);
-    for (int b0 = 0; b0 < a.B; b0 += 256) {
+    for (int b0 = 0; b0 < a.B; b0 += N) {
         const int b = b0 + tid;
         int t0 = 0, n = 0;
         if (b < a.B) seq_tokens(a, b, t0, n);
-        const int own = b < a.B ? own_rows(a, b) : 0;
         const int nrt = n > 0 ? (n * g.G + g.R - 1) / g.R : 0;
-        const int pre = n > 0 && is_joint(g, n) ? ntp : 0;
-        int mine = 0;
-        for (int r = 0; r < nrt; r++)
-            mine += pre + round64(seen_rows(a, b, n, min(n, ((r + 1) * g.R - 1) / g.G + 1) - 1, own));
-        const int2 ai = scan(nrt), au = scan(mine);
-        if (b < a.B) g.p.item0[b] = items + ai.x;
-        int u = units + au.x;
-        for (int r = 0; r < nrt; r++) {
-            const int k = items + ai.x + r;
-            if (k >= most) break;
-            g.p.first[k] = u;
-            g.p.seq[k] = b;
-            g.p.rt[k] = r;
-            u += pre + round64(seen_rows(a, b, n, min(n, ((r + 1) * g.R - 1) / g.G + 1) - 1, own));
-            if (k + 1 == most) s_run[0] = u;
+        const int2 at = scan(nrt);
+        if (b < a.B) g.p.item0[b] = items + at.x;
+        __syncthreads();
+        s_at[tid] = at.x;
+        __syncthreads();
+        for (int k = tid; k < at.y && items + k < most; k += N) {
+            int lo = 0, hi = N;  // the last sequence of the round that starts at or before k
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (s_at[mid] <= k) lo = mid;
+                else hi = mid;
+            }
+            g.p.seq[items + k] = b0 + lo;
+            g.p.rt[items + k] = k - s_at[lo];
         }
-        items += ai.y;
-        units += au.y;
+        items = min(items + at.y, most);
     }
+    __threadfence_block();
     __syncthreads();
-    if (items > most) {
-        items = most;
-        units = s_run[0];
+    // units before each
+    int units = np * ntp;
+    for (int k0 = np; k0 < items; k0 += N) {
+        const int k = k0 + tid;
+        int mine = 0;
+        if (k < items) {
+            const int b = g.p.seq[k], r = g.p.rt[k];
+            int t0, n;
+            seq_tokens(a, b, t0, n);
+            const int last = min(n, ((r + 1) * g.R - 1) / g.G + 1) - 1;
+            mine = (is_joint(g, n) ? ntp : 0) + round64(seen_rows(a, b, n, last, own_rows(a, b)));
+        }
+        const int2 at = scan(mine);
+        if (k < items) g.p.first[k] = units + at.x;
+        units += at.y;
     }
     if (tid == 0) {
         g.p.first[items] = units;
@@ -187,21 +214,80 @@ struct Mfma<BPD_T_BF16> {
 // x as NS values of the cache's type whose sum keeps 11 NS (f16) or 8 NS (bf16) bits of it, 8 elements.
 template <int CT, int NS>
 __device__ __forceinline__ void split8(const float (&x)[8], u32x4 (&out)[NS]) {
-    using T = typename Mfma<CT>::T;
     using V = typename Mfma<CT>::V;
     float r[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) r[i] = x[i];
 #pragma unroll
     for (int s = 0; s < NS; s++) {
-        V v;
+        typedef float F8 __attribute__((ext_vector_type(8)));
+        const V v = __builtin_convertvector((F8){r[0], r[1], r[2], r[3], r[4], r[5], r[6], r[7]}, V);
+        if (s + 1 < NS) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            v[i] = (T)r[i];
-            if (s + 1 < NS) r[i] -= (float)v[i];
+            for (int i = 0; i < 8; i++) r[i] -= (float)v[i];
         }
         out[s] = __builtin_bit_cast(u32x4, v);
     }
+}
+
+// The largest of lanes l, l ^ 16, l ^ 32 and l ^ 48.
+__device__ __forceinline__ float xor_max(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t v = __float_as_uint(fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1])));
+    const auto q = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+
+// Elements 8 (4 k + lg) .. + 7 of a query, in binary32; zeros behind its end and for a row that is none.
+template <int KS, typename Q>
+__device__ __forceinline__ void load_query(const Q* __restrict__ q, bool row, int per, int lg, float sign, float (&x)[KS][8]) {
+#pragma unroll
+    for (int k = 0; k < KS; k++) {
+        const int c = 4 * k + lg;
+        Vec<Q, 8> v;
+#pragma unroll
+        for (int e = 0; e < 8; e++) v.v[e] = (Q)0.f;
+        if (row && c < per) v = *reinterpret_cast<const Vec<Q, 8>*>(q + 8 * c);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[k][e] = sign == 1.f ? (float)v.v[e] : (float)v.v[e] * sign;
+    }
+}
+
+// Scales an fp32 query by a power of two to a largest element in [1, 2), so that two binary16 parts keep
+// 22 bits of that; returns the exponent taken out.
+template <int KS>
+__device__ __forceinline__ int row_exponent(float (&x)[KS][8]) {
+    float top = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[k][e]));
+    top = xor_max(top);
+    int e2 = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+    if (top == 0.f || e2 == 128) e2 = 0;
+    e2 = max(e2, -100);
+#pragma unroll
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[k][e] = ldexpf(x[k][e], -e2);
+    return e2;
+}
+
+// The lane's elements of a row of O, of the first D.
+template <typename Q, int VD, int VB>
+__device__ __forceinline__ void store_row(Q* out, int D, int lg, const f32x4* o, float f) {
+#pragma unroll
+    for (int vb = 0; vb < VB; vb++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int d = vb * 128 + 2 * VD * (4 * lg + r);
+            if (d >= D) continue;
+            Vec<Q, 2 * VD> v;
+#pragma unroll
+            for (int e = 0; e < 2 * VD; e++) v.v[e] = (Q)(o[vb * 8 + e][r] * f);
+            *reinterpret_cast<Vec<Q, 2 * VD>*>(out + d) = v;
+        }
 }
 
 // Which 16-byte chunk slot of a K row in LDS holds chunk c: rows of a 16-lane operand read
@@ -231,18 +317,18 @@ __device__ __forceinline__ uint32_t finite_or_0(uint32_t d) {
     return ((d & e) == e ? 0u : d & 0xFFFFu) | (((d >> 16) & e) == e ? 0u : d & 0xFFFF0000u);
 }
 
-// 4 waves of 16 MT rows each, the units [u0, u1) of this workgroup.  Scores are taken as
+// NW waves of 16 MT rows each, the units [u0, u1) of this workgroup.  Scores are taken as
 // S^T = K Q^T (lane: query l % 16, keys 4 (l / 16) + r), which is the layout in which
 // O^T = V^T P^T takes P: the 32 keys of two score tiles in the order 4g..4g+3, 16+4g..16+4g+3 of
 // lane group g.  V's operand is read in that order of rows, 16 bytes of each, and
 // transposed in registers; row c of it stands for element 8c + e of the head in product e.
-template <int QT, int CT, int NS, int DT, int MT>
-__global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_tile(AttnArgs g) {
+template <int QT, int CT, int NS, int DT, int MT, int NW>
+__global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnArgs g) {
     using M = Mfma<CT>;
     using T = typename M::T;
     using Q = typename Elem<QT>::type;
     constexpr int CPR = DT / 8;           // 16-byte chunks of a row
-    constexpr int NI = kKeys * CPR / 256;  // chunks of K and of V that a thread moves per unit
+    constexpr int NI = kKeys * CPR / (64 * NW);  // chunks of K and of V that a thread moves per unit
     constexpr int KS = DT / 32;           // products of a score tile
     constexpr int NE = DT / 16;           // products of O
     constexpr int VD = DT < 128 ? 2 : 4;  // dwords of a V row in one operand read
@@ -252,10 +338,13 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_tile(AttnArgs g
     const Paged& a = g.a;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, lg = lane >> 4;
-    const int nitems = g.p.info[0];
-    const int64_t U = (int64_t)g.p.info[1] * a.hkv;
-    const int n_groups = (int)(U < kGroups ? U : kGroups);
-    const int w = (int)blockIdx.x;
+    const int ntiles = round64(a.P);
+    const int nitems = g.planned ? g.p.info[0] : (a.T * g.G + g.R - 1) / g.R;
+    const int UH = g.planned ? g.p.info[1] : nitems * ntiles;
+    const int64_t U = (int64_t)UH * a.hkv;
+    const int n_groups = (int)(U < g.groups ? U : g.groups);
+    // workgroups go to the 8 XCDs in turn: each XCD takes an eighth of the shares in a row
+    const int w = n_groups == g.groups ? (int)((blockIdx.x & 7) * (g.groups >> 3) + (blockIdx.x >> 3)) : (int)blockIdx.x;
     if (w >= n_groups) return;
     int64_t u = unit_of(w, U, n_groups);
     const int64_t u1 = unit_of(w + 1, U, n_groups);
@@ -265,22 +354,34 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_tile(AttnArgs g
 
     while (u < u1) {
         // ---- the item of unit u
-        const int per_head = (int)(u / a.hkv);
-        const int item = __builtin_amdgcn_readfirstlane(count_le(g.p.first, nitems, per_head) - 1);
-        const int f0 = g.p.first[item], nk = g.p.first[item + 1] - f0;
-        const int64_t in = u - (int64_t)f0 * a.hkv;
-        const int head = (int)(in / nk);
-        int kt = (int)(in - (int64_t)head * nk);
-        const int k1 = (int)(u1 - u < nk - kt ? kt + (u1 - u) : nk);
-        const bool whole = kt == 0 && k1 == nk;
-        const int b = g.p.seq[item], rt = g.p.rt[item];
-        int t0 = 0, n = 0, own = 0, ntp = round64(a.P);
-        if (b >= 0) {
-            seq_tokens(a, b, t0, n);
-            own = own_rows(a, b);
-            if (!is_joint(g, n)) ntp = 0;
+        const int head = (int)(u / UH), in = (int)(u - (int64_t)head * UH);
+        int item, f0, nk, b = -1, rt, t0 = 0, n = a.T, own = 0, ntp = ntiles;
+        if (g.planned) {
+            item = __builtin_amdgcn_readfirstlane(count_le(g.p.first, nitems, in) - 1);
+            f0 = g.p.first[item];
+            nk = g.p.first[item + 1] - f0;
+            b = g.p.seq[item];
+            rt = g.p.rt[item];
+            if (b >= 0) {
+                seq_tokens(a, b, t0, n);
+                own = own_rows(a, b);
+                if (!is_joint(g, n)) ntp = 0;
+            } else {
+                n = g.p.info[2];
+            }
         } else {
-            n = g.p.info[2];
+            rt = item = in / ntiles;
+            f0 = item * ntiles;
+            nk = ntiles;
+        }
+        int kt = in - f0;
+        const int k0 = kt;
+        const int k1 = (int)(u1 - u < nk - kt ? kt + (u1 - u) : nk);
+        const bool last_word = kt == 0 && k1 == nk && b >= 0 && (ntp > 0 || a.P == 0);
+        if (kt == 0 && tid == 0) {
+            const int64_t ue = (int64_t)head * UH + f0 + nk - 1;
+            g.where[(int64_t)head * nitems + item] =
+                make_int2((int)slot_of(w, item, nitems, head), last_word ? 0 : group_of(ue, U, n_groups) - w + 1);
         }
         const int64_t hoff = (int64_t)head * a.head_stride;
         const int32_t* table = b >= 0 ? a.table + (int64_t)b * a.table_stride : nullptr;
@@ -297,49 +398,15 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_tile(AttnArgs g
             hq[m] = head * g.G + (row - i * g.G);
             lim[m] = -1;
             tok[m] = -1;
-            float top = 0.f;
-            float x[KS][8];
             if (i < n) {
-                tok[m] = b >= 0 ? t0 + i : g.p.packed[i];
+                tok[m] = b >= 0 ? t0 + i : g.planned ? g.p.packed[i] : i;
                 lim[m] = b >= 0 ? seen_rows(a, b, n, i, own) : 0;
-                const Q* q = reinterpret_cast<const Q*>(g.q) + tok[m] * g.qs + (int64_t)hq[m] * a.D;
-#pragma unroll
-                for (int k = 0; k < KS; k++) {
-                    const int c = 4 * k + lg;
-                    if (c < per) {
-                        const Vec<Q, 8> v = *reinterpret_cast<const Vec<Q, 8>*>(q + 8 * c);
-#pragma unroll
-                        for (int e = 0; e < 8; e++) x[k][e] = sign == 1.f ? (float)v.v[e] : (float)v.v[e] * sign;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; e++) x[k][e] = 0.f;
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < KS; k++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[k][e] = 0.f;
             }
+            float x[KS][8];
+            load_query<KS>(reinterpret_cast<const Q*>(g.q) + max(tok[m], 0) * g.qs + (int64_t)hq[m] * a.D, i < n, per, lg,
+                           sign, x);
             qscale[m] = scale2;
-            if constexpr (NS > 1 && CT == BPD_T_F16) {
-                // an fp32 row scaled by a power of two to a largest element in [1, 2), so that two
-                // binary16 parts keep 22 bits of that
-#pragma unroll
-                for (int k = 0; k < KS; k++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[k][e]));
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                int e2 = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-                if (top == 0.f || e2 == 128) e2 = 0;
-                e2 = max(e2, -100);
-#pragma unroll
-                for (int k = 0; k < KS; k++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[k][e] = ldexpf(x[k][e], -e2);
-                qscale[m] = ldexpf(scale2, e2);
-            }
+            if constexpr (NS > 1 && CT == BPD_T_F16) qscale[m] = ldexpf(scale2, row_exponent<KS>(x));
 #pragma unroll
             for (int k = 0; k < KS; k++) split8<CT, NS>(x[k], qf[m][k]);
         }
@@ -355,14 +422,14 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_tile(AttnArgs g
             for (int e = 0; e < NE; e++) o[m][e] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
 
-        // ---- staging of one unit's rows: a thread moves chunk slot tid % CPR of rows tid / CPR + 256 / CPR j
+        // ---- staging of one unit's rows: a thread moves chunk slot tid % CPR of rows tid / CPR + 64 NW / CPR j
         const int srow = tid / CPR, sc = tid % CPR;
         int pg[NI];
         uint4 rk[NI], rv[NI];
         bool rin[NI];
         auto key_of = [&](int t, int j, int& i, int& top) {
             const bool pre = t < ntp;
-            i = (pre ? t : t - ntp) * kKeys + srow + (256 / CPR) * j;
+            i = (pre ? t : t - ntp) * kKeys + srow + (64 * NW / CPR) * j;
             top = pre ? a.P : own;
             return pre ? a.prefix : table;
         };
@@ -392,7 +459,7 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_tile(AttnArgs g
         auto store = [&](int buf) {
 #pragma unroll
             for (int j = 0; j < NI; j++) {
-                const int row = srow + (256 / CPR) * j;
+                const int row = srow + (64 * NW / CPR) * j;
                 s.k[buf][row][k_slot<DT>(row, sc)] = rk[j];
                 s.v[buf][row][sc] = rv[j];
                 if (sc == 0) s.bias[buf][row] = rin[j] ? 0.f : kNegInf;
@@ -435,41 +502,43 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_tile(AttnArgs g
                         for (int m = 0; m < MT; m++) d |= lim[m] >= 0 && lim[m] < min(own, key0 + half * 32 + 32);
                         diag = __ballot(d) != 0;
                     }
-                    u32x4 pf[MT][NS];
+                    float top[MT];
+                    bool grow = false;
 #pragma unroll
                     for (int m = 0; m < MT; m++) {
-                        float x[8];
-#pragma unroll
-                        for (int e = 0; e < 8; e++) x[e] = sc4[e >> 2][m][e & 3] * qscale[m];
                         if (diag) {
 #pragma unroll
                             for (int e = 0; e < 8; e++)
-                                if (key0 + half * 32 + (e >> 2) * 16 + 4 * lg + (e & 3) >= lim[m]) x[e] = kNegInf;
+                                if (key0 + half * 32 + (e >> 2) * 16 + 4 * lg + (e & 3) >= lim[m])
+                                    sc4[e >> 2][m][e & 3] = kNegInf;
                         }
-                        float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
-                                          fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-                        top = fmaxf(top, __shfl_xor(top, 16));
-                        top = fmaxf(top, __shfl_xor(top, 32));
-                        // weights are 2^(x - ref) with the largest met so far between 2^12 and 2^15:
-                        // binary16 weights stay normal 26 binary places below it
-                        const bool grow = top - 15.f > ref[m];
-                        if (__ballot(grow) != 0) {
-                            const float nr = grow ? top - 12.f : ref[m];
-                            const float f = ref[m] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ref[m] - nr);
-                            if (grow) {
-                                l[m] *= f;
+                        const f32x4 x = sc4[0][m], y = sc4[1][m];
+                        top[m] = xor_max(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                                               fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])))) * qscale[m];
+                        grow |= top[m] - 15.f > ref[m];
+                    }
+                    // weights are 2^(x - ref) with the largest met so far between 2^12 and 2^15: binary16
+                    // weights stay normal 26 binary places below it
+                    if (__ballot(grow) != 0) {
 #pragma unroll
-                                for (int e = 0; e < NE; e++) o[m][e] *= f;
-                                ref[m] = nr;
-                            }
+                        for (int m = 0; m < MT; m++) {
+                            const float nr = top[m] - 15.f > ref[m] ? top[m] - 12.f : ref[m];
+                            const float f = nr == ref[m] ? 1.f : __builtin_amdgcn_exp2f(ref[m] - nr);
+                            l[m] *= f;
+#pragma unroll
+                            for (int e = 0; e < NE; e++) o[m][e] *= f;
+                            ref[m] = nr;
                         }
+                    }
+                    u32x4 pf[MT][NS];
+#pragma unroll
+                    for (int m = 0; m < MT; m++) {
                         const float base = ref[m] == kNegInf ? 0.f : ref[m];
                         float p[8];
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            p[e] = __builtin_amdgcn_exp2f(x[e] - base);
-                            l[m] += p[e];
-                        }
+                        for (int e = 0; e < 8; e++)
+                            p[e] = __builtin_amdgcn_exp2f(fmaf(sc4[e >> 2][m][e & 3], qscale[m], -base));
+                        l[m] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
                         split8<CT, NS>(p, pf[m]);
                     }
                     // ---- O^T += V^T P^T
@@ -550,155 +619,475 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_tile(AttnArgs g
 
         // ---- the item's rows, or this workgroup's part of them
         if (busy) {
-            const bool last_word = whole && b >= 0 && (ntp > 0 || a.P == 0);
-            const int64_t slot = slot_of(w, item, a.hkv, head);
+            const int64_t slot = slot_of(w, item, nitems, head);
 #pragma unroll
             for (int m = 0; m < MT; m++) {
                 l[m] += __shfl_xor(l[m], 16);
                 l[m] += __shfl_xor(l[m], 32);
                 if (tok[m] < 0) continue;
                 if (last_word) {
-                    const bool any = ref[m] != kNegInf || l[m] != 0.f;
-                    const float inv = any ? 1.f / l[m] : 0.f;
-                    Q* out = reinterpret_cast<Q*>(g.out) + tok[m] * g.os + (int64_t)hq[m] * a.D;
-#pragma unroll
-                    for (int vb = 0; vb < VB; vb++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            const int d = vb * 128 + 2 * VD * (4 * lg + r);
-                            if (d >= a.D) continue;
-                            Vec<Q, 2 * VD> v;
-#pragma unroll
-                            for (int e = 0; e < 2 * VD; e++) v.v[e] = (Q)(o[m][vb * 8 + e][r] * inv);
-                            *reinterpret_cast<Vec<Q, 2 * VD>*>(out + d) = v;
-                        }
+                    store_row<Q, VD, VB>(reinterpret_cast<Q*>(g.out) + tok[m] * g.os + (int64_t)hq[m] * a.D, a.D, lg, o[m],
+                                         l[m] != 0.f ? 1.f / l[m] : 0.f);
                     if (g.lse != nullptr && lg == 0)
-                        g.lse[(int64_t)tok[m] * g.H + hq[m]] = any ? (ref[m] + __builtin_log2f(l[m])) * kLn2 : kNegInf;
+                        g.lse[(int64_t)tok[m] * g.H + hq[m]] = l[m] != 0.f ? (ref[m] + __builtin_log2f(l[m])) * kLn2 : kNegInf;
                 } else {
-                    const int row = (wave * MT + m) * 16 + col;
-                    float* part = g.part + (slot * g.R + row) * DT;
-#pragma unroll
-                    for (int vb = 0; vb < VB; vb++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            Vec<float, 2 * VD> v;
-#pragma unroll
-                            for (int e = 0; e < 2 * VD; e++) v.v[e] = o[m][vb * 8 + e][r];
-                            *reinterpret_cast<Vec<float, 2 * VD>*>(part + vb * 128 + 2 * VD * (4 * lg + r)) = v;
-                        }
-                    if (lg == 0) g.ml[slot * g.R + row] = make_float2(ref[m], l[m]);
+                    const int64_t row = slot * g.R + (wave * MT + m) * 16 + col;
+                    store_row<float, VD, VB>(g.part + row * DT, DT, lg, o[m], 1.f);
+                    if (lg == 0) g.ml[row] = make_float2(ref[m], l[m]);
                 }
             }
         }
-        u += k1 - (int)(in - (int64_t)head * nk);
+        u += k1 - k0;
     }
 }
 
-// Joins what the workgroups left of each (token, query head): one wave per row, 4 elements of the
-// head per lane.
-template <int QT>
+// One new token per sequence: its G <= 16 query heads of a kv head are the columns of one 16-row tile, and
+// a wave reads the keys by itself, 32 at a time, straight into the operands' registers: no LDS, no
+// barrier.  The shares of all waves are dealt as k_attn_tile's, in units of 32 keys.
+// UNI: pages hold multiples of 16 rows, so the 16 rows of a score tile share a page and its lookup.
+template <int QT, int CT, int NS, int DT, bool UNI>
+__global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_wave(AttnArgs g) {
+    using M = Mfma<CT>;
+    using T = typename M::T;
+    using Q = typename Elem<QT>::type;
+    constexpr int KS = DT / 32, NE = DT / 16, VD = DT < 128 ? 2 : 4, VB = DT < 128 ? 1 : DT / 128;
+    const Paged& a = g.a;
+    const int lane = (int)threadIdx.x & 63, col = lane & 15, lg = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    const int per = a.D / 8;
+    int UH = 0;
+    for (int b = lane; b < a.B; b += 64) UH += (own_rows(a, b) + 31) >> 5;
+    for (int d = 1; d < 64; d <<= 1) UH += __shfl_xor(UH, d);
+    UH = __builtin_amdgcn_readfirstlane(UH);
+    const int64_t U = (int64_t)UH * a.hkv;
+    const int n_waves = (int)(U < g.waves ? U : g.waves);
+    if (w >= n_waves) return;
+    int64_t u = unit_of(w, U, n_waves);
+    const int64_t u1 = unit_of(w + 1, U, n_waves);
+    int head = (int)(u / UH), b = 0, before = 0;  // units of the head before sequence b
+    {
+        const int in = (int)(u - (int64_t)head * UH);
+        for (int b0 = 0;; b0 += 64) {
+            int x = b0 + lane < a.B ? (own_rows(a, b0 + lane) + 31) >> 5 : 0;
+            const int mine = x;
+            for (int d = 1; d < 64; d <<= 1) {
+                const int o = __shfl_up(x, d);
+                if (lane >= d) x += o;
+            }
+            const uint64_t over = __ballot(before + x > in);
+            if (over != 0 || b0 + 64 >= a.B) {
+                const int at = over != 0 ? __builtin_ctzll(over) : 63;
+                b = b0 + at;
+                before += __shfl(x - mine, at);
+                break;
+            }
+            before += __shfl(x, 63);
+        }
+        b = __builtin_amdgcn_readfirstlane(b);
+        before = __builtin_amdgcn_readfirstlane(before);
+    }
+    const float sign = g.scale > 0.f ? 1.f : g.scale < 0.f ? -1.f : 0.f;
+    const float scale2 = (g.scale == 0.f ? 1.f : __builtin_fabsf(g.scale)) * kLog2e;
+
+    while (u < u1) {
+        const int own = own_rows(a, b), nk = (own + 31) >> 5;
+        const int in = (int)(u - (int64_t)head * UH);
+        if (in >= before + nk) {  // the next sequence, or the next head's first
+            before += nk;
+            b++;
+            if (b == a.B) {
+                b = 0;
+                before = 0;
+                head++;
+            }
+            continue;
+        }
+        int kt = in - before;
+        const int k0 = kt, k1 = (int)(u1 - u < nk - kt ? kt + (u1 - u) : nk);
+        const bool last_word = kt == 0 && k1 == nk && a.P == 0;
+        const int64_t slot = slot_of(w, b, a.B, head);
+        if (kt == 0 && lane == 0) {
+            const int64_t ue = (int64_t)head * UH + before + nk - 1;
+            g.where1[(int64_t)head * a.B + b] = make_int2((int)slot, last_word ? 0 : group_of(ue, U, n_waves) - w + 1);
+        }
+        const int32_t* table = a.table + (int64_t)b * a.table_stride;
+        const int64_t hoff = (int64_t)head * a.head_stride;
+        const T* kbase = reinterpret_cast<const T*>(a.k) + hoff;
+        const T* vbase = reinterpret_cast<const T*>(a.v) + hoff;
+
+        u32x4 kr[2][KS], vr[8][VB];  // operands of the unit in flight
+        bool in0 = false, in1 = false;    // UNI: the unit's two pages are there
+        uint32_t here = 0;                // else: bits 0..1 the lane's key rows, 8.. its value rows
+        int pg[2] = {-1, -1};
+        auto look = [&](int t) {
+            if constexpr (UNI) {
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const int i = t * 32 + 16 * x;
+                    pg[x] = i < own ? table[fdiv(a.page, i)] : -1;
+                }
+            }
+        };
+        auto row_of = [&](int i, bool& ok) -> int64_t {
+            const int p = fdiv(a.page, i), page = i < own ? table[p] : -1;
+            ok = page >= 0 && page < a.n_pages;
+            return ok ? page * a.page_stride + (i - p * (int)a.page.d) * a.row_stride : 0;
+        };
+        auto load_k = [&](int t) {
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                int64_t at;
+                bool ok;
+                if constexpr (UNI) {
+                    const int i = t * 32 + 16 * x, p = fdiv(a.page, i);
+                    ok = pg[x] >= 0 && pg[x] < a.n_pages;
+                    (x == 0 ? in0 : in1) = ok;
+                    at = pg[x] * a.page_stride + (i - p * (int)a.page.d + col) * a.row_stride;
+                } else {
+                    at = row_of(t * 32 + 16 * x + col, ok);
+                    if (x == 0) here = 0;
+                    here |= ok ? 1u << x : 0u;
+                }
+#pragma unroll
+                for (int k = 0; k < KS; k++)
+                    kr[x][k] = ok && 4 * k + lg < per ? *reinterpret_cast<const u32x4*>(kbase + at + 8 * (4 * k + lg))
+                                                      : u32x4{0u, 0u, 0u, 0u};
+            }
+        };
+        auto load_v = [&](int t, bool i0, bool i1, const int (&pgv)[2]) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int x = j >> 2, i = t * 32 + 16 * x + 4 * lg + (j & 3);
+                int64_t at;
+                bool ok;
+                if constexpr (UNI) {
+                    const int p = fdiv(a.page, t * 32 + 16 * x);
+                    ok = (x == 0 ? i0 : i1) && i < own;
+                    at = pgv[x] * a.page_stride + (i - p * (int)a.page.d) * a.row_stride;
+                } else {
+                    at = row_of(i, ok);
+                }
+#pragma unroll
+                for (int vb = 0; vb < VB; vb++) {
+                    const int d = vb * 128 + 2 * VD * col;
+                    vr[j][vb] = u32x4{0u, 0u, 0u, 0u};
+                    if (ok && d < a.D) {
+                        if constexpr (VD == 4) {
+                            vr[j][vb] = *reinterpret_cast<const u32x4*>(vbase + at + d);
+                        } else {
+                            const u32x2 y = *reinterpret_cast<const u32x2*>(vbase + at + d);
+                            vr[j][vb][0] = y[0];
+                            vr[j][vb][1] = y[1];
+                        }
+                    }
+                }
+            }
+        };
+        look(kt);
+        load_k(kt);
+        load_v(kt, in0, in1, pg);
+
+        // the queries
+        u32x4 qf[KS][NS];
+        float qscale = scale2;
+        {
+            const bool row = col < g.G;
+            const Q* q = reinterpret_cast<const Q*>(g.q) + b * g.qs + (int64_t)(head * g.G + (row ? col : 0)) * a.D;
+            float x[KS][8];
+            load_query<KS>(q, row, per, lg, sign, x);
+            if constexpr (NS > 1 && CT == BPD_T_F16) qscale = ldexpf(scale2, row_exponent<KS>(x));
+#pragma unroll
+            for (int k = 0; k < KS; k++) split8<CT, NS>(x[k], qf[k]);
+        }
+        f32x4 o[NE];
+#pragma unroll
+        for (int e = 0; e < NE; e++) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float ref = kNegInf, l = 0.f;
+        for (; kt < k1; kt++) {
+            const bool more = kt + 1 < k1;
+            f32x4 sc[2];
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                sc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KS; k++)
+#pragma unroll
+                    for (int p = 0; p < NS; p++) sc[x] = M::go(kr[x][k], qf[k][p], sc[x]);
+            }
+            // keys that are not there
+            if constexpr (UNI) {
+                if (!in0 || !in1 || kt * 32 + 32 > own) {
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            if (!(x == 0 ? in0 : in1) || kt * 32 + 16 * x + 4 * lg + r >= own) sc[x][r] = kNegInf;
+                }
+            } else {
+                const uint32_t all = here;  // of the lane's own key rows: asked of the lanes that hold them
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (!((__shfl(all, 4 * lg + r) >> x) & 1u)) sc[x][r] = kNegInf;
+            }
+            int pgv[2];
+            bool n0 = false, n1 = false;
+            if (more) {
+                look(kt + 1);
+                load_k(kt + 1);
+                n0 = in0;
+                n1 = in1;
+            }
+            pgv[0] = pg[0];
+            pgv[1] = pg[1];
+            const float top = xor_max(fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                                            fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])))) * qscale;
+            if (__ballot(top - 15.f > ref) != 0) {
+                const float nr = top - 15.f > ref ? top - 12.f : ref;
+                const float f = nr == ref ? 1.f : __builtin_amdgcn_exp2f(ref - nr);
+                l *= f;
+#pragma unroll
+                for (int e = 0; e < NE; e++) o[e] *= f;
+                ref = nr;
+            }
+            const float base = ref == kNegInf ? 0.f : ref;
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e >> 2][e & 3], qscale, -base));
+            l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            u32x4 pf[NS];
+            split8<CT, NS>(p, pf);
+#pragma unroll
+            for (int vb = 0; vb < VB; vb++)
+#pragma unroll
+                for (int e = 0; e < 2 * VD; e++) {
+                    const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+                    u32x4 vf;
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        vf[j] = __builtin_amdgcn_perm(vr[2 * j + 1][vb][e >> 1], vr[2 * j][vb][e >> 1], sel);
+#pragma unroll
+                    for (int x = 0; x < NS; x++) o[vb * 8 + e] = M::go(vf, pf[x], o[vb * 8 + e]);
+                }
+            if (more) load_v(kt + 1, n0, n1, pgv);
+        }
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        if (col < g.G) {
+            const int h = head * g.G + col;
+            if (last_word) {
+                const float inv = l != 0.f ? 1.f / l : 0.f;
+                Q* out = reinterpret_cast<Q*>(g.out) + b * g.os + (int64_t)h * a.D;
+                store_row<Q, VD, VB>(out, a.D, lg, o, inv);
+                if (g.lse != nullptr && lg == 0) g.lse[(int64_t)b * g.H + h] = l != 0.f ? (ref + __builtin_log2f(l)) * kLn2 : kNegInf;
+            } else {
+                store_row<float, VD, VB>(g.part1 + (slot * g.G + col) * DT, DT, lg, o, 1.f);
+                if (lg == 0) g.ml1[slot * g.G + col] = make_float2(ref, l);
+            }
+        }
+        u += k1 - k0;
+    }
+}
+
+// Joins what was left of each (token, query head): its packed results, then its sequence's.  A
+// workgroup takes a token and HW heads for each of its 4 waves; a lane looks up one of the wave's heads.
+template <int QT, int HW>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs g) {
     using Q = typename Elem<QT>::type;
     const Paged& a = g.a;
-    const int lane = (int)threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= (int64_t)a.T * g.H) return;
-    const int t = (int)(row / g.H), h = (int)(row - (int64_t)t * g.H), head = fdiv(g.g, h), gq = h - head * g.G;
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int t = (int)blockIdx.x, h0 = ((int)blockIdx.y * 4 + wave) * HW;
+    if (h0 >= g.H) return;
     int b = t, i = 0;
     if (a.q_start != nullptr) {
-        b = count_le(a.q_start, a.B + 1, t) - 1;
+        b = __builtin_amdgcn_readfirstlane(count_le(a.q_start, a.B + 1, t) - 1);
         if (b < 0 || b >= a.B) return;
         i = t - a.q_start[b];
     }
-    int t0, n;
-    seq_tokens(a, b, t0, n);
-    const int nitems = g.p.info[0];
-    const int64_t U = (int64_t)g.p.info[1] * a.hkv;
-    const int n_groups = (int)(U < kGroups ? U : kGroups);
-    const bool joint = is_joint(g, n);
-    float m = kNegInf, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int which = 0; which < 2; which++) {
-        int item, r;
-        if (which == 0) {
-            if (a.P == 0 || joint) continue;
-            const int at = g.p.place[t];
-            if (at < 0) continue;
-            item = (at * g.G + gq) / g.R;
-            r = at * g.G + gq - item * g.R;
+    int2 wp = make_int2(0, 0), wo = make_int2(0, 0);  // this lane's head: packed results, the sequence's
+    int rp = 0, ro = 0;
+    bool done = lane >= HW || h0 + lane >= g.H;
+    if (!done) {
+        const int h = h0 + lane, head = fdiv(g.g, h), gq = h - head * g.G;
+        if (g.planned) {
+            int t0, n;
+            seq_tokens(a, b, t0, n);
+            const int nitems = g.p.info[0];
+            const bool packed = a.P > 0 && !is_joint(g, n);
+            const int at = packed ? g.p.place[t] : -1;
+            if (at >= 0) {
+                const int r = at * g.G + gq, item = r / g.R;
+                if (item < nitems) wp = g.where[(int64_t)head * nitems + item];
+                rp = r - item * g.R;
+            }
+            const int r = i * g.G + gq, rt = r / g.R, item = g.p.item0[b] + rt;
+            if (item < nitems && g.p.first[item + 1] > g.p.first[item]) {
+                wo = g.where[(int64_t)head * nitems + item];
+                done = wo.y == 0;
+            }
+            ro = r - rt * g.R;
         } else {
-            const int rt = (i * g.G + gq) / g.R;
-            item = g.p.item0[b] + rt;
-            r = i * g.G + gq - rt * g.R;
+            if (a.P > 0) {
+                const int r = t * g.G + gq, item = r / g.R, nitems = (a.T * g.G + g.R - 1) / g.R;
+                wp = g.where[(int64_t)head * nitems + item];
+                rp = r - item * g.R;
+            }
+            if (own_rows(a, b) > 0) {
+                wo = g.where1[(int64_t)head * a.B + b];
+                done = wo.y == 0;
+            }
+            ro = gq;
         }
-        if (item >= nitems) continue;
-        const int f0 = g.p.first[item], nk = g.p.first[item + 1] - f0;
-        if (nk == 0) continue;
-        const int64_t ua = (int64_t)f0 * a.hkv + (int64_t)head * nk;
-        const int w0 = group_of(ua, U, n_groups), w1 = group_of(ua + nk - 1, U, n_groups);
-        if (which == 1 && w0 == w1 && (joint || a.P == 0)) return;  // written by k_attn_tile
-        for (int w = w0; w <= w1; w++) {
-            const int64_t slot = slot_of(w, item, a.hkv, head) * g.R + r;
-            const float2 x = g.ml[slot];
-            if (x.x == kNegInf && x.y == 0.f) continue;
-            const float nm = fmaxf(m, x.x);
-            const float f = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m - nm), f2 = __builtin_amdgcn_exp2f(x.x - nm);
-            m = nm;
-            l = l * f + x.y * f2;
-            if (4 * lane < a.D) {
-                const f32x4 v = *reinterpret_cast<const f32x4*>(g.part + slot * g.DT + 4 * lane);
+    }
+    const float* part1 = g.planned ? g.part : g.part1;
+    const float2* ml1 = g.planned ? g.ml : g.ml1;
+    const int R1 = g.planned ? g.R : g.G;
+    uint64_t todo = __ballot(!done);
+    // a row of the head in 16-byte pieces by DT / 4 lanes: 64 / (DT / 4) results at a time
+    const int lanes = g.DT >> 2, sub = lane / lanes, piece = lane - sub * lanes, step = 64 / lanes;
+    while (todo != 0) {
+        const int j = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        const int np = __shfl(wp.y, j), no = __shfl(wo.y, j);
+        const int64_t sp = (int64_t)__shfl(wp.x, j) * g.R + __shfl(rp, j), so = (int64_t)__shfl(wo.x, j) * R1 + __shfl(ro, j);
+        auto ml_at = [&](int k) {
+            return k < np ? g.ml[sp + (int64_t)k * g.R] : ml1[so + (int64_t)(k - np) * R1];
+        };
+        float m = kNegInf;
+        for (int k = lane; k < np + no; k += 64) m = fmaxf(m, ml_at(k).x);
+        for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+        float l = 0.f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int k0 = 0; k0 < np + no; k0 += 64) {
+            float f = 0.f;  // the weight of result k0 + lane
+            if (k0 + lane < np + no) {
+                const float2 x = ml_at(k0 + lane);
+                // an untouched result (-inf, 0) weighs nothing; one of NaN scores alone keeps its NaN
+                f = x.x == kNegInf ? (x.y != 0.f ? x.y : 0.f) : __builtin_amdgcn_exp2f(x.x - m);
+                l += x.y * f;
+            }
+            const int top = min(64, np + no - k0);
+            for (int k = 0; k < top; k += 4 * step) {
+                f32x4 v[4];
+                float fk[4];
 #pragma unroll
-                for (int c = 0; c < 4; c++) acc[c] = acc[c] * f + v[c] * f2;
+                for (int x = 0; x < 4; x++) {
+                    const int kx = k + x * step + sub, kk = k0 + kx;
+                    fk[x] = __shfl(f, kx & 63);
+                    v[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    if (kx >= top) fk[x] = 0.f;
+                    if (fk[x] != 0.f)  // nothing, or what is not there
+                        v[x] = *reinterpret_cast<const f32x4*>(
+                            (kk < np ? g.part + (sp + (int64_t)kk * g.R) * g.DT
+                                     : part1 + (so + (int64_t)(kk - np) * R1) * g.DT) + 4 * piece);
+                }
+#pragma unroll
+                for (int x = 0; x < 4; x++) acc += v[x] * fk[x];
             }
         }
-    }
-    const bool any = m != kNegInf || l != 0.f;
-    const float inv = any ? 1.f / l : 0.f;
-    if (4 * lane < a.D) {
-        Vec<Q, 4> v;
+        for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
+        for (int d = lanes; d < 64; d <<= 1)
 #pragma unroll
-        for (int c = 0; c < 4; c++) v.v[c] = (Q)(acc[c] * inv);
-        *reinterpret_cast<Vec<Q, 4>*>(reinterpret_cast<Q*>(g.out) + t * g.os + (int64_t)h * a.D + 4 * lane) = v;
+            for (int c = 0; c < 4; c++) acc[c] += __shfl_xor(acc[c], d);
+        const bool any = l != 0.f;
+        const float inv = any ? 1.f / l : 0.f;
+        const int h = h0 + j;
+        if (sub == 0 && 4 * piece < a.D) {
+            Vec<Q, 4> v;
+#pragma unroll
+            for (int c = 0; c < 4; c++) v.v[c] = (Q)(acc[c] * inv);
+            *reinterpret_cast<Vec<Q, 4>*>(reinterpret_cast<Q*>(g.out) + t * g.os + (int64_t)h * a.D + 4 * piece) = v;
+        }
+        if (g.lse != nullptr && lane == 0) g.lse[(int64_t)t * g.H + h] = any ? (m + __builtin_log2f(l)) * kLn2 : kNegInf;
     }
-    if (g.lse != nullptr && lane == 0) g.lse[row] = any ? (m + __builtin_log2f(l)) * kLn2 : kNegInf;
 }
 
 // ---------------------------------------------------------------- host
 
 int padded(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
-// Rows of a tile: 4 waves of 16 or 32.  32 where the accumulators and the parts of the queries fit the
-// 256 registers of two waves per SIMD.
-int rows_of(int D, int parts) { return D <= 64 || (D <= 128 && parts == 1) ? 128 : 64; }
+// Waves of a workgroup and 16-row tiles of a wave: 8 waves of 32 rows where the accumulators and the
+// parts of the queries fit the 256 registers of two waves per SIMD.
+struct Tile {
+    int mt, nw;
+};
+Tile tile_of(int D, int parts) {
+    if (D <= 64) return {2, 8};
+    if (D <= 128) return {parts == 1 ? 2 : 1, 8};
+    return {1, 4};
+}
+
+int rows_of(int D, int parts) {
+    const Tile t = tile_of(D, parts);
+    return 16 * t.mt * t.nw;
+}
 
 int64_t up16(int64_t v) { return (v + 15) / 16 * 16; }
 
+constexpr int kWaves = 2048;  // k_attn_wave's: two per SIMD
+
+// The workspace of either way: planned, or one token per sequence by k_attn_wave with the prefix packed.
 struct Sizes {
-    int64_t items, slots, ints, part, ml, total;
+    int64_t items, ints, part, ml, where, part1, ml1, where1, total;
 };
-Sizes sizes(int B, int T, int G, int HKV, int R, int DT) {
-    Sizes s;
-    const int64_t per_rows = (int64_t)T * G / R;
-    s.items = per_rows + 1 + B + per_rows;  // packed, own
-    s.slots = kGroups + s.items * HKV;
-    s.ints = up16(4 * (4 + (s.items + 1) + 2 * s.items + B + 2 * (int64_t)T));
-    s.part = s.slots * R * DT * 4;
-    s.ml = s.slots * R * 8;
-    s.total = s.ints + s.part + s.ml;
+Sizes sizes(bool planned, int B, int T, int G, int HKV, int R, int DT, int P) {
+    Sizes s = {};
+    const int64_t per_rows = (int64_t)T * G / R + 1;
+    s.items = planned ? 2 * per_rows + B : P > 0 ? per_rows : 0;
+    const int64_t slots = s.items > 0 ? kGroupsMax + s.items * HKV : 0;
+    s.ints = planned ? up16(4 * (4 + (s.items + 1) + 2 * s.items + B + 2 * (int64_t)T)) : 0;
+    s.part = slots * R * DT * 4;
+    s.ml = up16(slots * R * 8);
+    s.where = up16(s.items * HKV * 8);
+    if (!planned) {
+        const int64_t n = (kWaves + (int64_t)B * HKV) * G;
+        s.part1 = n * DT * 4;
+        s.ml1 = up16(n * 8);
+        s.where1 = up16((int64_t)B * HKV * 8);
+    }
+    s.total = s.ints + s.part + s.ml + s.where + s.part1 + s.ml1 + s.where1;
     return s;
 }
+bool planned_way(const int32_t* q_start, int G) { return q_start != nullptr || G > 16; }
 
 template <int QT, int CT, int NS>
 void launch_tile(const AttnArgs& g, hipStream_t s) {
-    const dim3 grid(kGroups), block(256);
-    if (g.DT == 64) hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, 64, 2>), grid, block, 0, s, g);
-    else if (g.DT == 128) hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, 128, NS == 1 ? 2 : 1>), grid, block, 0, s, g);
-    else hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, 256, 1>), grid, block, 0, s, g);
+    const dim3 grid((unsigned)g.groups);
+    if (g.DT == 64) hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, 64, 2, 8>), grid, dim3(512), 0, s, g);
+    else if (g.DT == 128) hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, 128, NS == 1 ? 2 : 1, 8>), grid, dim3(512), 0, s, g);
+    else hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, 256, 1, 4>), grid, dim3(256), 0, s, g);
+}
+
+template <int QT, int CT, int NS, int DT>
+void launch_wave(const AttnArgs& g, hipStream_t s) {
+    const dim3 grid((unsigned)(g.waves / 4)), block(256);
+    if (g.a.page.d % 16 == 0) hipLaunchKernelGGL((k_attn_wave<QT, CT, NS, DT, true>), grid, block, 0, s, g);
+    else hipLaunchKernelGGL((k_attn_wave<QT, CT, NS, DT, false>), grid, block, 0, s, g);
+}
+
+template <int QT, int CT, int NS>
+void launch_types(const AttnArgs& g, hipStream_t s) {
+    if (g.planned) hipLaunchKernelGGL(k_attn_plan, dim3(1), dim3(1024), 0, s, g);
+    if (g.planned || g.a.P > 0) launch_tile<QT, CT, NS>(g, s);
+    if (!g.planned && g.a.W > 0) {
+        if (g.DT == 64) launch_wave<QT, CT, NS, 64>(g, s);
+        else if (g.DT == 128) launch_wave<QT, CT, NS, 128>(g, s);
+        else launch_wave<QT, CT, NS, 256>(g, s);
+    }
+    // one head per wave while that fills the chip twice at most, more where most rows are done
+    if ((int64_t)g.a.T * g.H <= 32768)
+        hipLaunchKernelGGL((k_attn_join<QT, 1>), dim3((unsigned)g.a.T, (unsigned)((g.H + 3) / 4)), dim3(256), 0, s, g);
+    else
+        hipLaunchKernelGGL((k_attn_join<QT, 8>), dim3((unsigned)g.a.T, (unsigned)((g.H + 31) / 32)), dim3(256), 0, s, g);
 }
 
 }  // namespace
 
-int64_t attn_paged_ws(int B, int T, int H, int HKV, int D, int) {
+int64_t attn_paged_ws(const int32_t* q_start, int B, int T, int H, int HKV, int D, int P) {
     const int G = H / HKV, DT = padded(D);  // for either type of q
-    const int64_t x = sizes(B, T, G, HKV, rows_of(D, 1), DT).total, y = sizes(B, T, G, HKV, rows_of(D, 2), DT).total;
+    const bool pl = planned_way(q_start, G);
+    const int64_t x = sizes(pl, B, T, G, HKV, rows_of(D, 1), DT, P).total;
+    const int64_t y = sizes(pl, B, T, G, HKV, rows_of(D, 2), DT, P).total;
     return x > y ? x : y;
 }
 
@@ -719,8 +1108,17 @@ void launch_attn_paged(const Paged& a0, int cache_type, const void* q, int64_t q
     g.scale = scale;
     g.R = rows_of(a.D, q_type == BPD_T_F32 ? 2 : 1);
     g.DT = padded(a.D);
-    const Sizes z = sizes(a.B, a.T, g.G, a.hkv, g.R, g.DT);
-    int32_t* p = static_cast<int32_t*>(ws);
+    g.groups = 256;
+    g.waves = kWaves;
+    g.planned = planned_way(a.q_start, g.G);
+    const Sizes z = sizes(g.planned, a.B, a.T, g.G, a.hkv, g.R, g.DT, a.P);
+    uint8_t* at = static_cast<uint8_t*>(ws);
+    auto take = [&](int64_t n) {
+        uint8_t* p = at;
+        at += n;
+        return p;
+    };
+    int32_t* p = reinterpret_cast<int32_t*>(take(z.ints));
     g.p.info = p;
     g.p.first = p + 4;
     g.p.seq = g.p.first + z.items + 1;
@@ -728,18 +1126,17 @@ void launch_attn_paged(const Paged& a0, int cache_type, const void* q, int64_t q
     g.p.item0 = g.p.rt + z.items;
     g.p.packed = g.p.item0 + a.B;
     g.p.place = g.p.packed + a.T;
-    g.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + z.ints);
-    g.ml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(g.part) + z.part);
-    hipLaunchKernelGGL(k_attn_plan, dim3(1), dim3(256), 0, s, g);
+    g.part = reinterpret_cast<float*>(take(z.part));
+    g.ml = reinterpret_cast<float2*>(take(z.ml));
+    g.where = reinterpret_cast<int2*>(take(z.where));
+    g.part1 = reinterpret_cast<float*>(take(z.part1));
+    g.ml1 = reinterpret_cast<float2*>(take(z.ml1));
+    g.where1 = reinterpret_cast<int2*>(take(z.where1));
     const bool bf = cache_type == BPD_T_BF16;
-    if (q_type == BPD_T_F32 && bf) launch_tile<BPD_T_F32, BPD_T_BF16, 3>(g, s);
-    else if (q_type == BPD_T_F32) launch_tile<BPD_T_F32, BPD_T_F16, 2>(g, s);
-    else if (bf) launch_tile<BPD_T_BF16, BPD_T_BF16, 1>(g, s);
-    else launch_tile<BPD_T_F16, BPD_T_F16, 1>(g, s);
-    const dim3 grid((unsigned)(((int64_t)a.T * H + 3) / 4)), block(256);
-    if (q_type == BPD_T_F32) hipLaunchKernelGGL(k_attn_join<BPD_T_F32>, grid, block, 0, s, g);
-    else if (bf) hipLaunchKernelGGL(k_attn_join<BPD_T_BF16>, grid, block, 0, s, g);
-    else hipLaunchKernelGGL(k_attn_join<BPD_T_F16>, grid, block, 0, s, g);
+    if (q_type == BPD_T_F32 && bf) launch_types<BPD_T_F32, BPD_T_BF16, 3>(g, s);
+    else if (q_type == BPD_T_F32) launch_types<BPD_T_F32, BPD_T_F16, 2>(g, s);
+    else if (bf) launch_types<BPD_T_BF16, BPD_T_BF16, 1>(g, s);
+    else launch_types<BPD_T_F16, BPD_T_F16, 1>(g, s);
 }
 
 }  // namespace bpdq

@@ -153,7 +153,7 @@ int64_t bpd_attn_paged_workspace(const bpd_paged_cache* kv, const bpd_paged_batc
     c.shape(n_heads >= 1 && n_heads % kv->n_kv_heads == 0, "n_heads is no multiple of n_kv_heads above 0");
     c.shape((int64_t)b->n_tokens * n_heads < INT_MAX, "n_tokens * n_heads is 2^31 or more");
     if (!c.ok) return -1;
-    return bpdq::attn_paged_ws(b->n_seqs, b->n_tokens, n_heads, kv->n_kv_heads, kv->head_dim, b->prefix_len);
+    return bpdq::attn_paged_ws(b->q_start, b->n_seqs, b->n_tokens, n_heads, kv->n_kv_heads, kv->head_dim, b->prefix_len);
 }
 
 void bpd_attn_paged_gpu(const bpd_paged_cache* kv, const bpd_paged_batch* b, const void* q, int64_t q_stride,
@@ -173,7 +173,7 @@ void bpd_attn_paged_gpu(const bpd_paged_cache* kv, const bpd_paged_batch* b, con
     if (lse != nullptr) c.ptr(lse, 4, "lse");
     if (!c.ok) return;
     bpdq::WsLease lease;
-    void* w = work_space(lease, ws, ws_bytes, bpdq::attn_paged_ws(b->n_seqs, b->n_tokens, n_heads, kv->n_kv_heads,
+    void* w = work_space(lease, ws, ws_bytes, bpdq::attn_paged_ws(b->q_start, b->n_seqs, b->n_tokens, n_heads, kv->n_kv_heads,
                                                                   kv->head_dim, b->prefix_len), fn);
     if (w == nullptr) return;
     bpdq::launch_attn_paged(paged(*kv, *b), kv->type, q, q_stride, out, out_stride, lse, q_type, n_heads, scale, w,

@@ -321,7 +321,7 @@ def test_decode_steps_together_in_a_graph(dev):
         assert (np.abs(O.f64(captured[0]) - ref) <= eo).all()
         for j in range(B):
             O.check_sample(O.f64(captured[1])[j], int(captured[2][j]), float(captured[3][j]), int(captured[4][j]),
-                           float(u[j]), 0.8, top_p=float(tp[j]))
+                           float(u[j]), float(t[j]), top_p=float(tp[j]))
 
 
 def test_two_graphs_of_one_stream_replayed_side_by_side(dev):
