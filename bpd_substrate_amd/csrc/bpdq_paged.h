@@ -29,7 +29,7 @@ struct Paged {
     uint8_t *k, *v;
     int n_pages, hkv, D;
     FastDiv page;  // by the page size
-    int64_t page_stride, row_stride, head_stride;
+    int page_stride, row_stride, head_stride;  // below 2^30: elements of a product with a page or row fit 61 bits
     const int32_t* table;
     int64_t table_stride;
     int W;

@@ -105,29 +105,29 @@ __global__ __launch_bounds__(256) void k_rope_append(AppendArgs g) {
         const int pg = fdiv(a.page, idx);
         const int page = pg < a.W ? a.table[(int64_t)b * a.table_stride + pg] : -1;
         if (page >= 0 && page < a.n_pages) {
-            const int64_t at = page * a.page_stride + (idx - pg * (int)a.page.d) * a.row_stride;
+            const int64_t at = (int64_t)page * a.page_stride + (int64_t)(idx - pg * (int)a.page.d) * a.row_stride;
             kc = reinterpret_cast<C*>(a.k) + at;
             vc = reinterpret_cast<C*>(a.v) + at;
         }
     }
-    const X* q = reinterpret_cast<const X*>(g.q) + t * g.qs;
-    X* qo = reinterpret_cast<X*>(g.qo) + t * g.qos;
+    const X* q = reinterpret_cast<const X*>(g.q) + (int64_t)t * g.qs;
+    X* qo = reinterpret_cast<X*>(g.qo) + (int64_t)t * g.qos;
     const int nq = g.H * (int)g.per.d;
     for (int i = (int)threadIdx.x; i < nq; i += 256) {
         const int h = fdiv(g.per, i);
         turn<X, X, N, NEOX>(q + h * a.D, qo + h * a.D, i - h * (int)g.per.d, g.rot, cs);
     }
     if (kc == nullptr) return;
-    const X* k = reinterpret_cast<const X*>(g.k) + t * g.ks;
-    const X* v = reinterpret_cast<const X*>(g.v) + t * g.vs;
+    const X* k = reinterpret_cast<const X*>(g.k) + (int64_t)t * g.ks;
+    const X* v = reinterpret_cast<const X*>(g.v) + (int64_t)t * g.vs;
     const int nk = a.hkv * (int)g.per.d, nv = a.hkv * (int)g.perv.d;
     for (int i = (int)threadIdx.x; i < nk; i += 256) {
         const int h = fdiv(g.per, i);
-        turn<X, C, N, NEOX>(k + h * a.D, kc + h * a.head_stride, i - h * (int)g.per.d, g.rot, cs);
+        turn<X, C, N, NEOX>(k + h * a.D, kc + (int64_t)h * a.head_stride, i - h * (int)g.per.d, g.rot, cs);
     }
     for (int i = (int)threadIdx.x; i < nv; i += 256) {
         const int h = fdiv(g.perv, i);
-        turn<X, C, 8, false>(v + h * a.D, vc + h * a.head_stride, i - h * (int)g.perv.d, 0, cs);
+        turn<X, C, 8, false>(v + h * a.D, vc + (int64_t)h * a.head_stride, i - h * (int)g.perv.d, 0, cs);
     }
 }
 

@@ -192,6 +192,11 @@ __global__ __launch_bounds__(1024) void k_attn_plan(AttnArgs g) {
     }
 }
 
+// Element offset of row i % page_size of a page.
+__device__ __forceinline__ int64_t row_at(const Paged& a, int page, int in_page) {
+    return (int64_t)page * a.page_stride + (int64_t)in_page * a.row_stride;
+}
+
 template <int CT>
 struct Mfma;
 template <>
@@ -304,17 +309,15 @@ struct Lds {
     float bias[2][kKeys];  // 0, or -inf for a row that is not there
 };
 
-// Whether any of 8 packed 16-bit values is an infinity or NaN.
+// Bit 15 of each half: that 16-bit value is an infinity or NaN (the exponent's carry).
 template <int CT>
-__device__ __forceinline__ bool not_finite(uint32_t d) {
-    constexpr uint32_t e = CT == BPD_T_F16 ? 0x7C00u : 0x7F80u;
-    return (d & e) == e || ((d >> 16) & e) == e;
+__device__ __forceinline__ uint32_t not_finite(uint32_t d) {
+    constexpr uint32_t e = CT == BPD_T_F16 ? 0x7C007C00u : 0x7F807F80u, one = CT == BPD_T_F16 ? 0x04000400u : 0x00800080u;
+    return ((d & e) + one) & 0x80008000u;
 }
-
 template <int CT>
 __device__ __forceinline__ uint32_t finite_or_0(uint32_t d) {
-    constexpr uint32_t e = CT == BPD_T_F16 ? 0x7C00u : 0x7F80u;
-    return ((d & e) == e ? 0u : d & 0xFFFFu) | (((d >> 16) & e) == e ? 0u : d & 0xFFFF0000u);
+    return d & ~((not_finite<CT>(d) >> 15) * 0xFFFFu);
 }
 
 // NW waves of 16 MT rows each, the units [u0, u1) of this workgroup.  Scores are taken as
@@ -424,6 +427,7 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
 
         // ---- staging of one unit's rows: a thread moves chunk slot tid % CPR of rows tid / CPR + 64 NW / CPR j
         const int srow = tid / CPR, sc = tid % CPR;
+        const uint8_t *kthread = a.k + 2 * (hoff + 8 * sc), *vthread = a.v + 2 * (hoff + 8 * sc);
         int pg[NI];
         uint4 rk[NI], rv[NI];
         bool rin[NI];
@@ -449,10 +453,9 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
                 rin[j] = pg[j] >= 0 && pg[j] < a.n_pages;
                 rk[j] = rv[j] = make_uint4(0, 0, 0, 0);
                 if (rin[j] && sc < per) {
-                    const int64_t at = pg[j] * a.page_stride + (i - fdiv(a.page, i) * (int)a.page.d) * a.row_stride +
-                                       hoff + 8 * sc;
-                    rk[j] = *reinterpret_cast<const uint4*>(a.k + 2 * at);
-                    rv[j] = *reinterpret_cast<const uint4*>(a.v + 2 * at);
+                    const int64_t at = 2 * row_at(a, pg[j], i - fdiv(a.page, i) * (int)a.page.d);
+                    rk[j] = *reinterpret_cast<const uint4*>(kthread + at);
+                    rv[j] = *reinterpret_cast<const uint4*>(vthread + at);
                 }
             }
         };
@@ -479,22 +482,41 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
                 const int key0 = (kt - ntp) * kKeys;  // own index of the unit's first key; below 0 in the prefix
 #pragma unroll 1
                 for (int half = 0; half < 2; half++) {
-                    f32x4 sc4[2][MT];
+                    f32x4 sc4[2][MT], bias[2];
+                    u32x4 kf[2][KS];
 #pragma unroll
                     for (int kk = 0; kk < 2; kk++) {
                         const int r0 = half * 32 + kk * 16;
-                        const f32x4 bias = *reinterpret_cast<const f32x4*>(&s.bias[buf][r0 + 4 * lg]);
+                        bias[kk] = *reinterpret_cast<const f32x4*>(&s.bias[buf][r0 + 4 * lg]);
 #pragma unroll
-                        for (int m = 0; m < MT; m++) sc4[kk][m] = bias;
+                        for (int k = 0; k < KS; k++)
+                            kf[kk][k] = __builtin_bit_cast(u32x4, s.k[buf][r0 + col][k_slot<DT>(col, 4 * k + lg)]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);  // every operand read is under way before the first product
 #pragma unroll
-                        for (int k = 0; k < KS; k++) {
-                            const u32x4 kf = __builtin_bit_cast(u32x4, s.k[buf][r0 + col][k_slot<DT>(col, 4 * k + lg)]);
+                    for (int k = 0; k < KS; k++)
+#pragma unroll
+                        for (int kk = 0; kk < 2; kk++)
 #pragma unroll
                             for (int m = 0; m < MT; m++)
 #pragma unroll
-                                for (int x = 0; x < NS; x++) sc4[kk][m] = M::go(kf, qf[m][k][x], sc4[kk][m]);
+                                for (int x = 0; x < NS; x++)
+                                    sc4[kk][m] = M::go(kf[kk][k], qf[m][k][x], k == 0 && x == 0 ? bias[kk] : sc4[kk][m]);
+                    uint32_t vr[VB][8][VD];
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++)
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const int row = half * 32 + (j >> 2) * 16 + 4 * lg + (j & 3);
+                            if constexpr (VD == 4) {
+                                const uint4 t = s.v[buf][row][vb * 16 + col];
+                                vr[vb][j][0] = t.x, vr[vb][j][1] = t.y, vr[vb][j][2] = t.z, vr[vb][j][3] = t.w;
+                            } else {
+                                const u32x2 t = reinterpret_cast<const u32x2*>(&s.v[buf][row][0])[col];
+                                vr[vb][j][0] = t[0], vr[vb][j][1] = t[1];
+                            }
                         }
-                    }
+                    __builtin_amdgcn_sched_barrier(0);  // V's reads run behind the softmax
                     bool diag = false;
                     if (kt >= ntp && b >= 0) {
                         bool d = false;
@@ -544,31 +566,19 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
                     // ---- O^T += V^T P^T
 #pragma unroll
                     for (int vb = 0; vb < VB; vb++) {
-                        uint32_t vr[8][VD];
-#pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            const int row = half * 32 + (j >> 2) * 16 + 4 * lg + (j & 3);
-                            if constexpr (VD == 4) {
-                                const uint4 t = s.v[buf][row][vb * 16 + col];
-                                vr[j][0] = t.x, vr[j][1] = t.y, vr[j][2] = t.z, vr[j][3] = t.w;
-                            } else {
-                                const u32x2 t = reinterpret_cast<const u32x2*>(&s.v[buf][row][0])[col];
-                                vr[j][0] = t[0], vr[j][1] = t[1];
-                            }
-                        }
                         if (diag) {
                             // an infinity or NaN in a row that some queries do not see: 0 times it is no 0.  It
                             // counts as 0 here, and is added to the rows that see it after the last unit
-                            bool x = false;
+                            uint32_t x = 0;
 #pragma unroll
                             for (int j = 0; j < 8; j++)
 #pragma unroll
-                                for (int d = 0; d < VD; d++) x |= not_finite<CT>(vr[j][d]);
-                            if (__ballot(x) != 0) {
+                                for (int d = 0; d < VD; d++) x |= not_finite<CT>(vr[vb][j][d]);
+                            if (__ballot(x != 0) != 0) {
 #pragma unroll
                                 for (int j = 0; j < 8; j++)
 #pragma unroll
-                                    for (int d = 0; d < VD; d++) vr[j][d] = finite_or_0<CT>(vr[j][d]);
+                                    for (int d = 0; d < VD; d++) vr[vb][j][d] = finite_or_0<CT>(vr[vb][j][d]);
                                 mend0 = min(mend0, key0 + half * 32);
                                 mend1 = key0 + half * 32 + 32;
                             }
@@ -579,7 +589,7 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
                             u32x4 vf;
 #pragma unroll
                             for (int j = 0; j < 4; j++)
-                                vf[j] = __builtin_amdgcn_perm(vr[2 * j + 1][e >> 1], vr[2 * j][e >> 1], sel);
+                                vf[j] = __builtin_amdgcn_perm(vr[vb][2 * j + 1][e >> 1], vr[vb][2 * j][e >> 1], sel);
 #pragma unroll
                             for (int m = 0; m < MT; m++)
 #pragma unroll
@@ -596,8 +606,7 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
         for (int key = mend0; key < min(mend1, own); key++) {
             const int pgi = fdiv(a.page, key), page = table[pgi];
             if (page < 0 || page >= a.n_pages) continue;
-            const T* v = reinterpret_cast<const T*>(a.v) + page * a.page_stride +
-                         (key - pgi * (int)a.page.d) * a.row_stride + hoff;
+            const T* v = reinterpret_cast<const T*>(a.v) + row_at(a, page, key - pgi * (int)a.page.d) + hoff;
 #pragma unroll
             for (int vb = 0; vb < VB; vb++)
 #pragma unroll
@@ -731,7 +740,7 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_wave(AttnArgs g
         auto row_of = [&](int i, bool& ok) -> int64_t {
             const int p = fdiv(a.page, i), page = i < own ? table[p] : -1;
             ok = page >= 0 && page < a.n_pages;
-            return ok ? page * a.page_stride + (i - p * (int)a.page.d) * a.row_stride : 0;
+            return ok ? row_at(a, page, i - p * (int)a.page.d) : 0;
         };
         auto load_k = [&](int t) {
 #pragma unroll
@@ -742,7 +751,7 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_wave(AttnArgs g
                     const int i = t * 32 + 16 * x, p = fdiv(a.page, i);
                     ok = pg[x] >= 0 && pg[x] < a.n_pages;
                     (x == 0 ? in0 : in1) = ok;
-                    at = pg[x] * a.page_stride + (i - p * (int)a.page.d + col) * a.row_stride;
+                    at = row_at(a, pg[x], i - p * (int)a.page.d + col);
                 } else {
                     at = row_of(t * 32 + 16 * x + col, ok);
                     if (x == 0) here = 0;
@@ -763,7 +772,7 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_wave(AttnArgs g
                 if constexpr (UNI) {
                     const int p = fdiv(a.page, t * 32 + 16 * x);
                     ok = (x == 0 ? i0 : i1) && i < own;
-                    at = pgv[x] * a.page_stride + (i - p * (int)a.page.d) * a.row_stride;
+                    at = row_at(a, pgv[x], i - p * (int)a.page.d);
                 } else {
                     at = row_of(i, ok);
                 }

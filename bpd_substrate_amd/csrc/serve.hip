@@ -82,9 +82,9 @@ bpdq::Paged paged(const bpd_paged_cache& kv, const bpd_paged_batch& b) {
     a.hkv = kv.n_kv_heads;
     a.D = kv.head_dim;
     a.page = bpdq::fast_div(kv.page_size);
-    a.page_stride = kv.page_stride;
-    a.row_stride = kv.row_stride;
-    a.head_stride = kv.head_stride;
+    a.page_stride = (int)kv.page_stride;
+    a.row_stride = (int)kv.row_stride;
+    a.head_stride = (int)kv.head_stride;
     a.table = b.table;
     a.table_stride = b.table_stride;
     a.W = b.table_width;
