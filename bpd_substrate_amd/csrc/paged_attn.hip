@@ -279,7 +279,8 @@ __device__ __forceinline__ int row_exponent(float (&x)[KS][8]) {
     return e2;
 }
 
-// The lane's elements of a row of O, of the first D.
+// The lane's elements of a row of O, of the first D, where row c of product 8 vb + e holds element
+// 128 vb + 2 VD c + e.
 template <typename Q, int VD, int VB>
 __device__ __forceinline__ void store_row(Q* out, int D, int lg, const f32x4* o, float f) {
 #pragma unroll
@@ -295,11 +296,30 @@ __device__ __forceinline__ void store_row(Q* out, int D, int lg, const f32x4* o,
         }
 }
 
-// Which 16-byte chunk slot of a K row in LDS holds chunk c: rows of a 16-lane operand read
-// differ in it, so that the read meets every bank once.
+// The same where product e holds elements 16 e .. 16 e + 15.
+template <typename Q, int NE>
+__device__ __forceinline__ void store_row4(Q* out, int D, int lg, const f32x4* o, float f) {
+#pragma unroll
+    for (int e = 0; e < NE; e++) {
+        const int d = 16 * e + 4 * lg;
+        if (d >= D) continue;
+        Vec<Q, 4> v;
+#pragma unroll
+        for (int r = 0; r < 4; r++) v.v[r] = (Q)(o[e][r] * f);
+        *reinterpret_cast<Vec<Q, 4>*>(out + d) = v;
+    }
+}
+
+// Which 16-byte chunk slot of a row in LDS holds chunk c.  K: the 16 rows of an operand read differ in it, so
+// that the read meets every bank once.  V: a transposing read takes 32 bytes of each of 16 rows, so pairs
+// of chunks differ.
 template <int DT>
 __device__ __forceinline__ int k_slot(int row, int c) {
     return DT == 64 ? c ^ ((row >> 1) & 7) : c ^ (row & 15);
+}
+template <int DT>
+__device__ __forceinline__ int v_slot(int row, int c) {
+    return DT == 64 ? c ^ (((row >> 1) & 3) << 1) : c ^ ((row & 7) << 1);
 }
 
 template <int DT>
@@ -320,12 +340,21 @@ __device__ __forceinline__ uint32_t finite_or_0(uint32_t d) {
     return d & ~((not_finite<CT>(d) >> 15) * 0xFFFFu);
 }
 
+// The 4 x 16 transposing LDS read: of each 16 lanes, lane 4 i + c gives the place of elements 4 c .. 4 c + 3 of
+// row i, and lane l gets element l of rows 0..3.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x2 read_tr(const uint8_t* p) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                         (__attribute__((address_space(3))) s16x4*)(const_cast<uint8_t*>(p))));
+}
+
 // NW waves of 16 MT rows each, the units [u0, u1) of this workgroup.  Scores are taken as
 // S^T = K Q^T (lane: query l % 16, keys 4 (l / 16) + r), which is the layout in which
 // O^T = V^T P^T takes P: the 32 keys of two score tiles in the order 4g..4g+3, 16+4g..16+4g+3 of
-// lane group g.  V's operand is read in that order of rows, 16 bytes of each, and
-// transposed in registers; row c of it stands for element 8c + e of the head in product e.
-template <int QT, int CT, int NS, int DT, int MT, int NW>
+// lane group g.  V's operand comes in that order from two transposing reads; row c of it is
+// element 16 e + c of the head in product e.
+// UNI: pages hold multiples of 16 rows, so the rows that a wave's lanes move at a time share a page.
+template <int QT, int CT, int NS, int DT, int MT, int NW, bool UNI>
 __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnArgs g) {
     using M = Mfma<CT>;
     using T = typename M::T;
@@ -334,9 +363,8 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
     constexpr int NI = kKeys * CPR / (64 * NW);  // chunks of K and of V that a thread moves per unit
     constexpr int KS = DT / 32;           // products of a score tile
     constexpr int NE = DT / 16;           // products of O
-    constexpr int VD = DT < 128 ? 2 : 4;  // dwords of a V row in one operand read
-    constexpr int VB = DT < 128 ? 1 : DT / 128;
-    static_assert(NI >= 1, "a chunk per thread");
+    constexpr int LR = 64 / CPR;          // rows that a wave moves at a time
+    static_assert(NI >= 1 && 16 % LR == 0, "a chunk per thread, rows of one page");
     __shared__ Lds<DT> s;
     const Paged& a = g.a;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -391,28 +419,30 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
 
         // ---- this wave's queries
         u32x4 qf[MT][KS][NS];
-        float qscale[MT];
+        int e2[MT];   // the exponents taken out of them
         int lim[MT];  // own keys that the lane's query sees, -1: no query
-        int tok[MT], hq[MT];
+        auto query_of = [&](int m, int& tok, int& hq) {
+            const int row = rt * g.R + (wave * MT + m) * 16 + col, i = fdiv(g.g, row);
+            hq = head * g.G + (row - i * g.G);
+            tok = i >= n ? -1 : b >= 0 ? t0 + i : g.planned ? g.p.packed[i] : i;
+            return i;
+        };
 #pragma unroll
         for (int m = 0; m < MT; m++) {
-            const int row = rt * g.R + (wave * MT + m) * 16 + col;
-            const int i = fdiv(g.g, row);
-            hq[m] = head * g.G + (row - i * g.G);
-            lim[m] = -1;
-            tok[m] = -1;
-            if (i < n) {
-                tok[m] = b >= 0 ? t0 + i : g.planned ? g.p.packed[i] : i;
-                lim[m] = b >= 0 ? seen_rows(a, b, n, i, own) : 0;
-            }
+            int tok, hq;
+            const int i = query_of(m, tok, hq);
+            lim[m] = tok < 0 ? -1 : b >= 0 ? seen_rows(a, b, n, i, own) : 0;
             float x[KS][8];
-            load_query<KS>(reinterpret_cast<const Q*>(g.q) + max(tok[m], 0) * g.qs + (int64_t)hq[m] * a.D, i < n, per, lg,
-                           sign, x);
-            qscale[m] = scale2;
-            if constexpr (NS > 1 && CT == BPD_T_F16) qscale[m] = ldexpf(scale2, row_exponent<KS>(x));
+            load_query<KS>(reinterpret_cast<const Q*>(g.q) + max(tok, 0) * g.qs + (int64_t)hq * a.D, tok >= 0, per, lg, sign,
+                           x);
+            e2[m] = 0;
+            if constexpr (NS > 1 && CT == BPD_T_F16) e2[m] = row_exponent<KS>(x);
 #pragma unroll
             for (int k = 0; k < KS; k++) split8<CT, NS>(x[k], qf[m][k]);
         }
+        float qscale[MT];
+#pragma unroll
+        for (int m = 0; m < MT; m++) qscale[m] = NS > 1 && CT == BPD_T_F16 ? ldexpf(scale2, e2[m]) : scale2;
         const bool busy = __ballot(lim[0] >= 0) != 0;  // rows of a wave fill from its first
         f32x4 o[MT][NE];
         float ref[MT], l[MT];
@@ -425,15 +455,21 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
             for (int e = 0; e < NE; e++) o[m][e] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
 
-        // ---- staging of one unit's rows: a thread moves chunk slot tid % CPR of rows tid / CPR + 64 NW / CPR j
+        // ---- staging of one unit's rows: a thread moves chunk tid % CPR of rows tid / CPR + 64 NW / CPR j
         const int srow = tid / CPR, sc = tid % CPR;
         const uint8_t *kthread = a.k + 2 * (hoff + 8 * sc), *vthread = a.v + 2 * (hoff + 8 * sc);
+        if constexpr (UNI) {
+            const int64_t at = 2 * (int64_t)(lane / CPR) * a.row_stride;
+            kthread += at;
+            vthread += at;
+        }
         int pg[NI];
         uint4 rk[NI], rv[NI];
         bool rin[NI];
+        // own or prefix index of this thread's (UNI: its wave's first) row j of unit t, rows there are
         auto key_of = [&](int t, int j, int& i, int& top) {
             const bool pre = t < ntp;
-            i = (pre ? t : t - ntp) * kKeys + srow + (64 * NW / CPR) * j;
+            i = (pre ? t : t - ntp) * kKeys + (UNI ? wave * LR : srow) + NW * LR * j;
             top = pre ? a.P : own;
             return pre ? a.prefix : table;
         };
@@ -450,24 +486,33 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
             for (int j = 0; j < NI; j++) {
                 int i, top;
                 key_of(t, j, i, top);
-                rin[j] = pg[j] >= 0 && pg[j] < a.n_pages;
+                const bool there = pg[j] >= 0 && pg[j] < a.n_pages;
+                const int64_t at = 2 * row_at(a, pg[j], i - fdiv(a.page, i) * (int)a.page.d);
+                const auto *kp = reinterpret_cast<const uint4*>(kthread + at), *vp = reinterpret_cast<const uint4*>(vthread + at);
+                if (UNI && there && i + LR <= top && per == CPR) {  // all lanes
+                    rin[j] = true;
+                    rk[j] = *kp;
+                    rv[j] = *vp;
+                    continue;
+                }
+                rin[j] = there && i + (UNI ? lane / CPR : 0) < top;
                 rk[j] = rv[j] = make_uint4(0, 0, 0, 0);
                 if (rin[j] && sc < per) {
-                    const int64_t at = 2 * row_at(a, pg[j], i - fdiv(a.page, i) * (int)a.page.d);
-                    rk[j] = *reinterpret_cast<const uint4*>(kthread + at);
-                    rv[j] = *reinterpret_cast<const uint4*>(vthread + at);
+                    rk[j] = *kp;
+                    rv[j] = *vp;
                 }
             }
         };
         auto store = [&](int buf) {
 #pragma unroll
             for (int j = 0; j < NI; j++) {
-                const int row = srow + (64 * NW / CPR) * j;
+                const int row = srow + NW * LR * j;
                 s.k[buf][row][k_slot<DT>(row, sc)] = rk[j];
-                s.v[buf][row][sc] = rv[j];
+                s.v[buf][row][v_slot<DT>(row, sc)] = rv[j];
                 if (sc == 0) s.bias[buf][row] = rin[j] ? 0.f : kNegInf;
             }
         };
+        bool fresh = true;  // a query of the wave has not met a key yet
         look(kt);
         load(kt);
         if (kt + 1 < k1) look(kt + 1);
@@ -502,19 +547,17 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
 #pragma unroll
                                 for (int x = 0; x < NS; x++)
                                     sc4[kk][m] = M::go(kf[kk][k], qf[m][k][x], k == 0 && x == 0 ? bias[kk] : sc4[kk][m]);
-                    uint32_t vr[VB][8][VD];
+                    u32x4 vf[NE];
 #pragma unroll
-                    for (int vb = 0; vb < VB; vb++)
+                    for (int e = 0; e < NE; e++)
 #pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            const int row = half * 32 + (j >> 2) * 16 + 4 * lg + (j & 3);
-                            if constexpr (VD == 4) {
-                                const uint4 t = s.v[buf][row][vb * 16 + col];
-                                vr[vb][j][0] = t.x, vr[vb][j][1] = t.y, vr[vb][j][2] = t.z, vr[vb][j][3] = t.w;
-                            } else {
-                                const u32x2 t = reinterpret_cast<const u32x2*>(&s.v[buf][row][0])[col];
-                                vr[vb][j][0] = t[0], vr[vb][j][1] = t[1];
-                            }
+                        for (int kk = 0; kk < 2; kk++) {
+                            const int row = half * 32 + kk * 16 + 4 * lg + (col >> 2);
+                            const u32x2 t = read_tr(reinterpret_cast<const uint8_t*>(
+                                                        &s.v[buf][row][v_slot<DT>(row, 2 * e + ((col >> 1) & 1))]) +
+                                                    8 * (col & 1));
+                            vf[e][2 * kk] = t[0];
+                            vf[e][2 * kk + 1] = t[1];
                         }
                     __builtin_amdgcn_sched_barrier(0);  // V's reads run behind the softmax
                     bool diag = false;
@@ -524,79 +567,79 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
                         for (int m = 0; m < MT; m++) d |= lim[m] >= 0 && lim[m] < min(own, key0 + half * 32 + 32);
                         diag = __ballot(d) != 0;
                     }
-                    float top[MT];
-                    bool grow = false;
+                    if (diag) {
 #pragma unroll
-                    for (int m = 0; m < MT; m++) {
-                        if (diag) {
+                        for (int m = 0; m < MT; m++)
 #pragma unroll
                             for (int e = 0; e < 8; e++)
                                 if (key0 + half * 32 + (e >> 2) * 16 + 4 * lg + (e & 3) >= lim[m])
                                     sc4[e >> 2][m][e & 3] = kNegInf;
-                        }
-                        const f32x4 x = sc4[0][m], y = sc4[1][m];
-                        top[m] = xor_max(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
-                                               fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])))) * qscale[m];
-                        grow |= top[m] - 15.f > ref[m];
                     }
-                    // weights are 2^(x - ref) with the largest met so far between 2^12 and 2^15: binary16
-                    // weights stay normal 26 binary places below it
-                    if (__ballot(grow) != 0) {
+                    // weights 2^(x - ref), x = score log2(e).  Only where the 8 of a lane add up to more than
+                    // 2^15.5 is the largest score looked for, and ref set to 10 below it: binary16 weights
+                    // stay below their largest value, and normal 24 places below the largest weight
+                    float p[MT][8], s8[MT];
+                    auto weigh = [&](int m) {
+                        const float base = ref[m] == kNegInf ? 0.f : ref[m];
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            p[m][e] = __builtin_amdgcn_exp2f(fmaf(sc4[e >> 2][m][e & 3], qscale[m], -base));
+                        s8[m] = ((p[m][0] + p[m][1]) + (p[m][2] + p[m][3])) + ((p[m][4] + p[m][5]) + (p[m][6] + p[m][7]));
+                    };
+                    bool over = fresh;
+#pragma unroll
+                    for (int m = 0; m < MT; m++) {
+                        weigh(m);
+                        over |= !(s8[m] <= 46340.f);
+                    }
+                    if (__ballot(over) != 0) {
+                        bool none = false;
 #pragma unroll
                         for (int m = 0; m < MT; m++) {
-                            const float nr = top[m] - 15.f > ref[m] ? top[m] - 12.f : ref[m];
+                            const f32x4 x = sc4[0][m], y = sc4[1][m];
+                            const float top = xor_max(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                                                            fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])))) * qscale[m];
+                            const float nr = top - 12.f > ref[m] ? top - 10.f : ref[m];
                             const float f = nr == ref[m] ? 1.f : __builtin_amdgcn_exp2f(ref[m] - nr);
                             l[m] *= f;
 #pragma unroll
                             for (int e = 0; e < NE; e++) o[m][e] *= f;
                             ref[m] = nr;
+                            none |= lim[m] >= 0 && nr == kNegInf;
+                            weigh(m);
                         }
+                        fresh = __ballot(none) != 0;
                     }
                     u32x4 pf[MT][NS];
 #pragma unroll
                     for (int m = 0; m < MT; m++) {
-                        const float base = ref[m] == kNegInf ? 0.f : ref[m];
-                        float p[8];
+                        l[m] += s8[m];
+                        split8<CT, NS>(p[m], pf[m]);
+                    }
+                    if (diag) {
+                        // an infinity or NaN in a row that some queries do not see: 0 times it is no 0.  It
+                        // counts as 0 here, and is added to the rows that see it after the last unit
+                        uint32_t x = 0;
 #pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            p[e] = __builtin_amdgcn_exp2f(fmaf(sc4[e >> 2][m][e & 3], qscale[m], -base));
-                        l[m] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-                        split8<CT, NS>(p, pf[m]);
+                        for (int e = 0; e < NE; e++)
+#pragma unroll
+                            for (int d = 0; d < 4; d++) x |= not_finite<CT>(vf[e][d]);
+                        if (__ballot(x != 0) != 0) {
+#pragma unroll
+                            for (int e = 0; e < NE; e++)
+#pragma unroll
+                                for (int d = 0; d < 4; d++) vf[e][d] = finite_or_0<CT>(vf[e][d]);
+                            mend0 = min(mend0, key0 + half * 32);
+                            mend1 = key0 + half * 32 + 32;
+                        }
                     }
                     // ---- O^T += V^T P^T
 #pragma unroll
-                    for (int vb = 0; vb < VB; vb++) {
-                        if (diag) {
-                            // an infinity or NaN in a row that some queries do not see: 0 times it is no 0.  It
-                            // counts as 0 here, and is added to the rows that see it after the last unit
-                            uint32_t x = 0;
+                    for (int e = 0; e < NE; e++)
 #pragma unroll
-                            for (int j = 0; j < 8; j++)
+                        for (int m = 0; m < MT; m++)
 #pragma unroll
-                                for (int d = 0; d < VD; d++) x |= not_finite<CT>(vr[vb][j][d]);
-                            if (__ballot(x != 0) != 0) {
-#pragma unroll
-                                for (int j = 0; j < 8; j++)
-#pragma unroll
-                                    for (int d = 0; d < VD; d++) vr[vb][j][d] = finite_or_0<CT>(vr[vb][j][d]);
-                                mend0 = min(mend0, key0 + half * 32);
-                                mend1 = key0 + half * 32 + 32;
-                            }
-                        }
-#pragma unroll
-                        for (int e = 0; e < 2 * VD; e++) {
-                            const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
-                            u32x4 vf;
-#pragma unroll
-                            for (int j = 0; j < 4; j++)
-                                vf[j] = __builtin_amdgcn_perm(vr[vb][2 * j + 1][e >> 1], vr[vb][2 * j][e >> 1], sel);
-#pragma unroll
-                            for (int m = 0; m < MT; m++)
-#pragma unroll
-                                for (int x = 0; x < NS; x++)
-                                    o[m][vb * 8 + e] = M::go(vf, pf[m][x], o[m][vb * 8 + e]);
-                        }
-                    }
+                            for (int x = 0; x < NS; x++) o[m][e] = M::go(vf[e], pf[m][x], o[m][e]);
                 }
             }
             if (kt + 1 < k1) store((kt + 1) & 1);
@@ -608,22 +651,20 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
             if (page < 0 || page >= a.n_pages) continue;
             const T* v = reinterpret_cast<const T*>(a.v) + row_at(a, page, key - pgi * (int)a.page.d) + hoff;
 #pragma unroll
-            for (int vb = 0; vb < VB; vb++)
+            for (int e = 0; e < NE; e++) {
+                const int d = 16 * e + 4 * lg;
+                if (d >= a.D) continue;
+                const Vec<T, 4> x = *reinterpret_cast<const Vec<T, 4>*>(v + d);
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int d = vb * 128 + 2 * VD * (4 * lg + r);
-                    if (d >= a.D) continue;
-                    const Vec<T, 2 * VD> x = *reinterpret_cast<const Vec<T, 2 * VD>*>(v + d);
+                for (int m = 0; m < MT; m++) {
+                    if (key >= lim[m]) continue;
 #pragma unroll
-                    for (int m = 0; m < MT; m++) {
-                        if (key >= lim[m]) continue;
-#pragma unroll
-                        for (int e = 0; e < 2 * VD; e++) {
-                            const float y = (float)x.v[e];
-                            if (!(__builtin_fabsf(y) < -kNegInf)) o[m][vb * 8 + e][r] += y;
-                        }
+                    for (int r = 0; r < 4; r++) {
+                        const float y = (float)x.v[r];
+                        if (!(__builtin_fabsf(y) < -kNegInf)) o[m][e][r] += y;
                     }
                 }
+            }
         }
 
         // ---- the item's rows, or this workgroup's part of them
@@ -633,15 +674,17 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
             for (int m = 0; m < MT; m++) {
                 l[m] += __shfl_xor(l[m], 16);
                 l[m] += __shfl_xor(l[m], 32);
-                if (tok[m] < 0) continue;
+                int tok, hq;
+                query_of(m, tok, hq);
+                if (tok < 0) continue;
                 if (last_word) {
-                    store_row<Q, VD, VB>(reinterpret_cast<Q*>(g.out) + tok[m] * g.os + (int64_t)hq[m] * a.D, a.D, lg, o[m],
+                    store_row4<Q, NE>(reinterpret_cast<Q*>(g.out) + tok * g.os + (int64_t)hq * a.D, a.D, lg, o[m],
                                          l[m] != 0.f ? 1.f / l[m] : 0.f);
                     if (g.lse != nullptr && lg == 0)
-                        g.lse[(int64_t)tok[m] * g.H + hq[m]] = l[m] != 0.f ? (ref[m] + __builtin_log2f(l[m])) * kLn2 : kNegInf;
+                        g.lse[(int64_t)tok * g.H + hq] = l[m] != 0.f ? (ref[m] + __builtin_log2f(l[m])) * kLn2 : kNegInf;
                 } else {
                     const int64_t row = slot * g.R + (wave * MT + m) * 16 + col;
-                    store_row<float, VD, VB>(g.part + row * DT, DT, lg, o[m], 1.f);
+                    store_row4<float, NE>(g.part + row * DT, DT, lg, o[m], 1.f);
                     if (lg == 0) g.ml[row] = make_float2(ref[m], l[m]);
                 }
             }
@@ -1059,12 +1102,13 @@ Sizes sizes(bool planned, int B, int T, int G, int HKV, int R, int DT, int P) {
 }
 bool planned_way(const int32_t* q_start, int G) { return q_start != nullptr || G > 16; }
 
-template <int QT, int CT, int NS>
+template <int QT, int CT, int NS, bool UNI>
 void launch_tile(const AttnArgs& g, hipStream_t s) {
     const dim3 grid((unsigned)g.groups);
-    if (g.DT == 64) hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, 64, 2, 8>), grid, dim3(512), 0, s, g);
-    else if (g.DT == 128) hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, 128, NS == 1 ? 2 : 1, 8>), grid, dim3(512), 0, s, g);
-    else hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, 256, 1, 4>), grid, dim3(256), 0, s, g);
+    if (g.DT == 64) hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, 64, 2, 8, UNI>), grid, dim3(512), 0, s, g);
+    else if (g.DT == 128)
+        hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, 128, NS == 1 ? 2 : 1, 8, UNI>), grid, dim3(512), 0, s, g);
+    else hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, 256, 1, 4, UNI>), grid, dim3(256), 0, s, g);
 }
 
 template <int QT, int CT, int NS, int DT>
@@ -1077,7 +1121,7 @@ void launch_wave(const AttnArgs& g, hipStream_t s) {
 template <int QT, int CT, int NS>
 void launch_types(const AttnArgs& g, hipStream_t s) {
     if (g.planned) hipLaunchKernelGGL(k_attn_plan, dim3(1), dim3(1024), 0, s, g);
-    if (g.planned || g.a.P > 0) launch_tile<QT, CT, NS>(g, s);
+    if (g.planned || g.a.P > 0) g.a.page.d % 16 == 0 ? launch_tile<QT, CT, NS, true>(g, s) : launch_tile<QT, CT, NS, false>(g, s);
     if (!g.planned && g.a.W > 0) {
         if (g.DT == 64) launch_wave<QT, CT, NS, 64>(g, s);
         else if (g.DT == 128) launch_wave<QT, CT, NS, 128>(g, s);
