@@ -31,7 +31,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kKeys = 64;   // keys of a unit
-constexpr int kGroupsMax = 512;  // workgroups that share the units: one of 8 waves or two of 4 per CU
+constexpr int kGroupsMax = 256;  // workgroups that share the units: one per CU
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -__builtin_inff();
 
@@ -63,6 +63,7 @@ struct AttnArgs {
     float2* ml;    // [slot][R] reference exponent, sum
     int2* where;   // [head][item] first slot of its results and their number, 0 where the output is written
     int waves;     // k_attn_wave: shares
+    float tile_cost, wave_cost;
     float* part1;  // k_attn_wave's results, [slot][G][DT], and the same of them
     float2* ml1;
     int2* where1;  // [head][sequence]
@@ -195,6 +196,11 @@ __global__ __launch_bounds__(1024) void k_attn_plan(AttnArgs g) {
 // Element offset of row i % page_size of a page.
 __device__ __forceinline__ int64_t row_at(const Paged& a, int page, int in_page) {
     return (int64_t)page * a.page_stride + (int64_t)in_page * a.row_stride;
+}
+
+// A value at an address that is the same in every lane, through the scalar cache.
+__device__ __forceinline__ int load_uniform(const int32_t* p) {
+    return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
 }
 
 template <int CT>
@@ -355,7 +361,7 @@ __device__ __forceinline__ u32x2 read_tr(const uint8_t* p) {
 // element 16 e + c of the head in product e.
 // UNI: pages hold multiples of 16 rows, so the rows that a wave's lanes move at a time share a page.
 template <int QT, int CT, int NS, int DT, int MT, int NW, bool UNI>
-__global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnArgs g) {
+__device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w, int groups) {
     using M = Mfma<CT>;
     using T = typename M::T;
     using Q = typename Elem<QT>::type;
@@ -365,7 +371,6 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
     constexpr int NE = DT / 16;           // products of O
     constexpr int LR = 64 / CPR;          // rows that a wave moves at a time
     static_assert(NI >= 1 && 16 % LR == 0, "a chunk per thread, rows of one page");
-    __shared__ Lds<DT> s;
     const Paged& a = g.a;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, lg = lane >> 4;
@@ -373,9 +378,7 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
     const int nitems = g.planned ? g.p.info[0] : (a.T * g.G + g.R - 1) / g.R;
     const int UH = g.planned ? g.p.info[1] : nitems * ntiles;
     const int64_t U = (int64_t)UH * a.hkv;
-    const int n_groups = (int)(U < g.groups ? U : g.groups);
-    // workgroups go to the 8 XCDs in turn: each XCD takes an eighth of the shares in a row
-    const int w = n_groups == g.groups ? (int)((blockIdx.x & 7) * (g.groups >> 3) + (blockIdx.x >> 3)) : (int)blockIdx.x;
+    const int n_groups = (int)(U < groups ? U : groups);
     if (w >= n_groups) return;
     int64_t u = unit_of(w, U, n_groups);
     const int64_t u1 = unit_of(w + 1, U, n_groups);
@@ -478,7 +481,7 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
             for (int j = 0; j < NI; j++) {
                 int i, top;
                 const int32_t* tab = key_of(t, j, i, top);
-                pg[j] = i < top ? tab[fdiv(a.page, i)] : -1;
+                pg[j] = i < top ? UNI ? load_uniform(tab + fdiv(a.page, i)) : tab[fdiv(a.page, i)] : -1;
             }
         };
         auto load = [&](int t) {
@@ -694,25 +697,21 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnAr
 }
 
 // One new token per sequence: its G <= 16 query heads of a kv head are the columns of one 16-row tile, and
-// a wave reads the keys by itself, 32 at a time, straight into the operands' registers: no LDS, no
-// barrier.  The shares of all waves are dealt as k_attn_tile's, in units of 32 keys.
+// a wave reads the keys by itself, 32 at a time, V straight into the operand's registers, K through LDS of
+// its own: no barrier.  The shares of all waves are dealt as k_attn_tile's, in units of 32 keys.
 // UNI: pages hold multiples of 16 rows, so the 16 rows of a score tile share a page and its lookup.
 template <int QT, int CT, int NS, int DT, bool UNI>
-__global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_wave(AttnArgs g) {
+__device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT / 8], int w, int waves, int UH) {
     using M = Mfma<CT>;
     using T = typename M::T;
     using Q = typename Elem<QT>::type;
     constexpr int KS = DT / 32, NE = DT / 16, VD = DT < 128 ? 2 : 4, VB = DT < 128 ? 1 : DT / 128;
+    constexpr int BUF = UNI && (DT == 64 || (DT == 128 && NS == 1)) ? 2 : 1;  // units in flight: what 256 registers hold
     const Paged& a = g.a;
     const int lane = (int)threadIdx.x & 63, col = lane & 15, lg = lane >> 4;
-    const int w = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
     const int per = a.D / 8;
-    int UH = 0;
-    for (int b = lane; b < a.B; b += 64) UH += (own_rows(a, b) + 31) >> 5;
-    for (int d = 1; d < 64; d <<= 1) UH += __shfl_xor(UH, d);
-    UH = __builtin_amdgcn_readfirstlane(UH);
     const int64_t U = (int64_t)UH * a.hkv;
-    const int n_waves = (int)(U < g.waves ? U : g.waves);
+    const int n_waves = (int)(U < waves ? U : waves);
     if (w >= n_waves) return;
     int64_t u = unit_of(w, U, n_waves);
     const int64_t u1 = unit_of(w + 1, U, n_waves);
@@ -767,77 +766,63 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_wave(AttnArgs g
         const T* kbase = reinterpret_cast<const T*>(a.k) + hoff;
         const T* vbase = reinterpret_cast<const T*>(a.v) + hoff;
 
-        u32x4 kr[2][KS], vr[8][VB];  // operands of the unit in flight
-        bool in0 = false, in1 = false;    // UNI: the unit's two pages are there
-        uint32_t here = 0;                // else: bits 0..1 the lane's key rows, 8.. its value rows
-        int pg[2] = {-1, -1};
-        auto look = [&](int t) {
+        // the rows of units in flight: row 16 (j / 4) + 4 lg + j % 4, 16 lanes across it
+        struct Unit {
+            u32x4 k[8][VB], v[8][VB];
+            uint32_t ok;  // bit j: row j is there
+        };
+        Unit un[BUF];
+        int pg[BUF][2];
+        auto look = [&](int (&p)[2], int t) {
             if constexpr (UNI) {
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
                     const int i = t * 32 + 16 * x;
-                    pg[x] = i < own ? table[fdiv(a.page, i)] : -1;
+                    p[x] = t < k1 && i < own ? load_uniform(table + fdiv(a.page, i)) : -1;
                 }
             }
         };
-        auto row_of = [&](int i, bool& ok) -> int64_t {
-            const int p = fdiv(a.page, i), page = i < own ? table[p] : -1;
-            ok = page >= 0 && page < a.n_pages;
-            return ok ? row_at(a, page, i - p * (int)a.page.d) : 0;
-        };
-        auto load_k = [&](int t) {
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                int64_t at;
-                bool ok;
-                if constexpr (UNI) {
-                    const int i = t * 32 + 16 * x, p = fdiv(a.page, i);
-                    ok = pg[x] >= 0 && pg[x] < a.n_pages;
-                    (x == 0 ? in0 : in1) = ok;
-                    at = row_at(a, pg[x], i - p * (int)a.page.d + col);
-                } else {
-                    at = row_of(t * 32 + 16 * x + col, ok);
-                    if (x == 0) here = 0;
-                    here |= ok ? 1u << x : 0u;
-                }
-#pragma unroll
-                for (int k = 0; k < KS; k++)
-                    kr[x][k] = ok && 4 * k + lg < per ? *reinterpret_cast<const u32x4*>(kbase + at + 8 * (4 * k + lg))
-                                                      : u32x4{0u, 0u, 0u, 0u};
-            }
-        };
-        auto load_v = [&](int t, bool i0, bool i1, const int (&pgv)[2]) {
+        auto load = [&](u32x4 (&to)[8][VB], uint32_t& oks, const T* base, const int (&p)[2], int t) {
+            oks = 0;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const int x = j >> 2, i = t * 32 + 16 * x + 4 * lg + (j & 3);
-                int64_t at;
-                bool ok;
+                const int x = j >> 2, i0 = t * 32 + 16 * x, i = i0 + 4 * lg + (j & 3);
+                int page, in_page;
                 if constexpr (UNI) {
-                    const int p = fdiv(a.page, t * 32 + 16 * x);
-                    ok = (x == 0 ? i0 : i1) && i < own;
-                    at = row_at(a, pgv[x], i - p * (int)a.page.d);
+                    page = p[x];
+                    in_page = i - fdiv(a.page, i0) * (int)a.page.d;
                 } else {
-                    at = row_of(i, ok);
+                    const int at = fdiv(a.page, i);
+                    page = i < own ? table[at] : -1;
+                    in_page = i - at * (int)a.page.d;
                 }
+                const bool ok = page >= 0 && page < a.n_pages && i < own;
+                oks |= ok ? 1u << j : 0u;
+                const int64_t at = row_at(a, page, in_page);
 #pragma unroll
                 for (int vb = 0; vb < VB; vb++) {
                     const int d = vb * 128 + 2 * VD * col;
-                    vr[j][vb] = u32x4{0u, 0u, 0u, 0u};
+                    to[j][vb] = u32x4{0u, 0u, 0u, 0u};
                     if (ok && d < a.D) {
                         if constexpr (VD == 4) {
-                            vr[j][vb] = *reinterpret_cast<const u32x4*>(vbase + at + d);
+                            to[j][vb] = *reinterpret_cast<const u32x4*>(base + at + d);
                         } else {
-                            const u32x2 y = *reinterpret_cast<const u32x2*>(vbase + at + d);
-                            vr[j][vb][0] = y[0];
-                            vr[j][vb][1] = y[1];
+                            const u32x2 y = *reinterpret_cast<const u32x2*>(base + at + d);
+                            to[j][vb][0] = y[0];
+                            to[j][vb][1] = y[1];
                         }
                     }
                 }
             }
         };
-        look(kt);
-        load_k(kt);
-        load_v(kt, in0, in1, pg);
+#pragma unroll
+        for (int i = 0; i < BUF; i++) look(pg[i], kt + i);
+#pragma unroll
+        for (int i = 0; i < BUF; i++) {
+            if (kt + i >= k1) break;
+            load(un[i].k, un[i].ok, kbase, pg[i], kt + i);
+            load(un[i].v, un[i].ok, vbase, pg[i], kt + i);
+        }
 
         // the queries
         u32x4 qf[KS][NS];
@@ -855,44 +840,46 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_wave(AttnArgs g
 #pragma unroll
         for (int e = 0; e < NE; e++) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
         float ref = kNegInf, l = 0.f;
-        for (; kt < k1; kt++) {
-            const bool more = kt + 1 < k1;
-            f32x4 sc[2];
+        // unit t, held in n; then the unit BUF further on is asked for
+        auto step = [&](Unit& n, int (&p)[2], int t) {
+            // K's rows through the wave's own LDS into the order of the product's operand: read from memory as
+            // the operand takes them, 16 lanes would meet 16 rows at a time
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-                sc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int vb = 0; vb < VB; vb++) {
+                    const int row = 16 * (j >> 2) + 4 * lg + (j & 3);
+                    if constexpr (VD == 4)
+                        *reinterpret_cast<u32x4*>(&ks[row][k_slot<DT>(row, vb * 16 + col)]) = n.k[j][vb];
+                    else
+                        reinterpret_cast<u32x2*>(&ks[row][k_slot<DT>(row, col >> 1)])[col & 1] = u32x2{n.k[j][vb][0], n.k[j][vb][1]};
+                }
+            const uint32_t ok = n.ok;
+            const bool more = t + BUF < k1;
+            int pn[2] = {p[0], p[1]};
+            if (more) {
+                load(n.k, n.ok, kbase, pn, t + BUF);
+                look(p, t + 2 * BUF);
+            }
+            u32x4 kf[2][KS];
+#pragma unroll
+            for (int x = 0; x < 2; x++)
 #pragma unroll
                 for (int k = 0; k < KS; k++)
+                    kf[x][k] = __builtin_bit_cast(u32x4, ks[16 * x + col][k_slot<DT>(col, 4 * k + lg)]);
+            f32x4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-                    for (int p = 0; p < NS; p++) sc[x] = M::go(kr[x][k], qf[k][p], sc[x]);
-            }
-            // keys that are not there
-            if constexpr (UNI) {
-                if (!in0 || !in1 || kt * 32 + 32 > own) {
-#pragma unroll
-                    for (int x = 0; x < 2; x++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++)
-                            if (!(x == 0 ? in0 : in1) || kt * 32 + 16 * x + 4 * lg + r >= own) sc[x][r] = kNegInf;
-                }
-            } else {
-                const uint32_t all = here;  // of the lane's own key rows: asked of the lanes that hold them
+            for (int k = 0; k < KS; k++)
 #pragma unroll
                 for (int x = 0; x < 2; x++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if (!((__shfl(all, 4 * lg + r) >> x) & 1u)) sc[x][r] = kNegInf;
+                    for (int y = 0; y < NS; y++) sc[x] = M::go(kf[x][k], qf[k][y], sc[x]);
+            // keys that are not there: the lane's scores are those of the rows that it read
+            if (__ballot(ok != 255u) != 0) {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (!((ok >> e) & 1u)) sc[e >> 2][e & 3] = kNegInf;
             }
-            int pgv[2];
-            bool n0 = false, n1 = false;
-            if (more) {
-                look(kt + 1);
-                load_k(kt + 1);
-                n0 = in0;
-                n1 = in1;
-            }
-            pgv[0] = pg[0];
-            pgv[1] = pg[1];
             const float top = xor_max(fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                                             fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])))) * qscale;
             if (__ballot(top - 15.f > ref) != 0) {
@@ -904,12 +891,12 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_wave(AttnArgs g
                 ref = nr;
             }
             const float base = ref == kNegInf ? 0.f : ref;
-            float p[8];
+            float w8[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e >> 2][e & 3], qscale, -base));
-            l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            for (int e = 0; e < 8; e++) w8[e] = __builtin_amdgcn_exp2f(fmaf(sc[e >> 2][e & 3], qscale, -base));
+            l += ((w8[0] + w8[1]) + (w8[2] + w8[3])) + ((w8[4] + w8[5]) + (w8[6] + w8[7]));
             u32x4 pf[NS];
-            split8<CT, NS>(p, pf);
+            split8<CT, NS>(w8, pf);
 #pragma unroll
             for (int vb = 0; vb < VB; vb++)
 #pragma unroll
@@ -918,11 +905,23 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_wave(AttnArgs g
                     u32x4 vf;
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-                        vf[j] = __builtin_amdgcn_perm(vr[2 * j + 1][vb][e >> 1], vr[2 * j][vb][e >> 1], sel);
+                        vf[j] = __builtin_amdgcn_perm(n.v[2 * j + 1][vb][e >> 1], n.v[2 * j][vb][e >> 1], sel);
 #pragma unroll
                     for (int x = 0; x < NS; x++) o[vb * 8 + e] = M::go(vf, pf[x], o[vb * 8 + e]);
                 }
-            if (more) load_v(kt + 1, n0, n1, pgv);
+            if (more) load(n.v, n.ok, vbase, pn, t + BUF);
+        };
+        // the pages of the units behind those in flight
+#pragma unroll
+        for (int i = 0; i < BUF; i++) look(pg[i], kt + BUF + i);
+        while (true) {
+#pragma unroll
+            for (int i = 0; i < BUF; i++) {
+                if (kt + i >= k1) break;
+                step(un[i], pg[i], kt + i);
+            }
+            kt += BUF;
+            if (kt >= k1) break;
         }
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
@@ -939,6 +938,55 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_wave(AttnArgs g
             }
         }
         u += k1 - k0;
+    }
+}
+
+// Units of 32 keys of one kv head's sequences.
+__device__ __forceinline__ int wave_units(const Paged& a) {
+    int n = 0;
+    for (int b = (int)threadIdx.x & 63; b < a.B; b += 64) n += (own_rows(a, b) + 31) >> 5;
+    for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
+    return __builtin_amdgcn_readfirstlane(n);
+}
+
+// Workgroups go to the 8 XCDs in turn: each XCD takes an eighth of the tiles' shares in a row.
+__device__ __forceinline__ int xcd_share(int block, int groups) {
+    return groups % 8 == 0 ? (block & 7) * (groups >> 3) + (block >> 3) : block;
+}
+
+template <int QT, int CT, int NS, int DT, int MT, int NW, bool UNI>
+__global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_tile(AttnArgs g) {
+    __shared__ Lds<DT> s;
+    tile_share<QT, CT, NS, DT, MT, NW, UNI>(g, s, xcd_share((int)blockIdx.x, g.groups), g.groups);
+}
+
+template <int QT, int CT, int NS, int DT, bool UNI>
+__global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_wave(AttnArgs g) {
+    __shared__ uint4 ks[4][32][DT / 8];
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    wave_share<QT, CT, NS, DT, UNI>(g, ks[wave], (int)blockIdx.x * 4 + wave, g.waves, wave_units(g.a));
+}
+
+// One token per sequence behind a prefix: x of the workgroups take the prefix's tiles, which the matrix
+// units bound, the others the sequences' own keys, which memory bounds, at the same time.  x by
+// the time that a unit of each takes a CU: kTileCost (64 keys x R rows) against kWaveCost (32 keys x 16).
+template <int QT, int CT, int NS, int DT, int MT, int NW, bool UNI>
+__global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_both(AttnArgs g) {
+    __shared__ union {
+        Lds<DT> tile;
+        uint4 k[NW][32][DT / 8];
+    } s;
+    const Paged& a = g.a;
+    const int uw = wave_units(a), eighths = g.groups >> 3;
+    const float ct = (float)(((a.T * g.G + g.R - 1) / g.R) * round64(a.P)) * g.tile_cost, cw = (float)uw * g.wave_cost;
+    const int x8 = cw == 0.f ? eighths : max(1, min(eighths - 1, (int)((float)eighths * ct / (ct + cw) + 0.5f)));
+    const int row = (int)blockIdx.x >> 3;
+    if (row < x8) {
+        tile_share<QT, CT, NS, DT, MT, NW, UNI>(g, s.tile, ((int)blockIdx.x & 7) * x8 + row, 8 * x8);
+    } else {
+        const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+        const int w = (((int)blockIdx.x & 7) * (eighths - x8) + row - x8) * NW + wave;
+        wave_share<QT, CT, NS, DT, UNI>(g, s.k[wave], w, 8 * (eighths - x8) * NW, uw);
     }
 }
 
@@ -1102,31 +1150,31 @@ Sizes sizes(bool planned, int B, int T, int G, int HKV, int R, int DT, int P) {
 }
 bool planned_way(const int32_t* q_start, int G) { return q_start != nullptr || G > 16; }
 
-template <int QT, int CT, int NS, bool UNI>
-void launch_tile(const AttnArgs& g, hipStream_t s) {
-    const dim3 grid((unsigned)g.groups);
-    if (g.DT == 64) hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, 64, 2, 8, UNI>), grid, dim3(512), 0, s, g);
-    else if (g.DT == 128)
-        hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, 128, NS == 1 ? 2 : 1, 8, UNI>), grid, dim3(512), 0, s, g);
-    else hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, 256, 1, 4, UNI>), grid, dim3(256), 0, s, g);
+template <int QT, int CT, int NS, int DT, int MT, int NW, bool UNI>
+void launch_dim(const AttnArgs& g, hipStream_t s) {
+    const dim3 grid((unsigned)g.groups), block(64 * NW);
+    if (g.planned)
+        hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, DT, MT, NW, UNI>), grid, block, 0, s, g);
+    else if (g.a.P > 0 && g.a.W > 0)
+        hipLaunchKernelGGL((k_attn_both<QT, CT, NS, DT, MT, NW, UNI>), grid, block, 0, s, g);
+    else if (g.a.P > 0)
+        hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, DT, MT, NW, UNI>), grid, block, 0, s, g);
+    else if (g.a.W > 0)
+        hipLaunchKernelGGL((k_attn_wave<QT, CT, NS, DT, UNI>), dim3((unsigned)(g.waves / 4)), dim3(256), 0, s, g);
 }
 
-template <int QT, int CT, int NS, int DT>
-void launch_wave(const AttnArgs& g, hipStream_t s) {
-    const dim3 grid((unsigned)(g.waves / 4)), block(256);
-    if (g.a.page.d % 16 == 0) hipLaunchKernelGGL((k_attn_wave<QT, CT, NS, DT, true>), grid, block, 0, s, g);
-    else hipLaunchKernelGGL((k_attn_wave<QT, CT, NS, DT, false>), grid, block, 0, s, g);
+template <int QT, int CT, int NS, bool UNI>
+void launch_uni(const AttnArgs& g, hipStream_t s) {
+    if (g.DT == 64) launch_dim<QT, CT, NS, 64, 2, 8, UNI>(g, s);
+    else if (g.DT == 128) launch_dim<QT, CT, NS, 128, NS == 1 ? 2 : 1, 8, UNI>(g, s);
+    else launch_dim<QT, CT, NS, 256, 1, 4, UNI>(g, s);
 }
 
 template <int QT, int CT, int NS>
 void launch_types(const AttnArgs& g, hipStream_t s) {
     if (g.planned) hipLaunchKernelGGL(k_attn_plan, dim3(1), dim3(1024), 0, s, g);
-    if (g.planned || g.a.P > 0) g.a.page.d % 16 == 0 ? launch_tile<QT, CT, NS, true>(g, s) : launch_tile<QT, CT, NS, false>(g, s);
-    if (!g.planned && g.a.W > 0) {
-        if (g.DT == 64) launch_wave<QT, CT, NS, 64>(g, s);
-        else if (g.DT == 128) launch_wave<QT, CT, NS, 128>(g, s);
-        else launch_wave<QT, CT, NS, 256>(g, s);
-    }
+    if (g.a.page.d % 16 == 0) launch_uni<QT, CT, NS, true>(g, s);
+    else launch_uni<QT, CT, NS, false>(g, s);
     // one head per wave while that fills the chip twice at most, more where most rows are done
     if ((int64_t)g.a.T * g.H <= 32768)
         hipLaunchKernelGGL((k_attn_join<QT, 1>), dim3((unsigned)g.a.T, (unsigned)((g.H + 3) / 4)), dim3(256), 0, s, g);
@@ -1163,6 +1211,8 @@ void launch_attn_paged(const Paged& a0, int cache_type, const void* q, int64_t q
     g.DT = padded(a.D);
     g.groups = 256;
     g.waves = kWaves;
+    g.tile_cost = 3.4f;
+    g.wave_cost = 0.25f;
     g.planned = planned_way(a.q_start, g.G);
     const Sizes z = sizes(g.planned, a.B, a.T, g.G, a.hkv, g.R, g.DT, a.P);
     uint8_t* at = static_cast<uint8_t*>(ws);
