@@ -699,7 +699,8 @@ __device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w,
 // One new token per sequence: its G <= 16 query heads of a kv head are the columns of one 16-row tile, and
 // a wave reads the keys by itself, 32 at a time, V straight into the operand's registers, K through LDS of
 // its own: no barrier.  The shares of all waves are dealt as k_attn_tile's, in units of 32 keys.
-// UNI: pages hold multiples of 16 rows, so the 16 rows of a score tile share a page and its lookup.
+// UNI: pages hold multiples of 16 rows, which span less than 2^32 bytes, so the 16 rows of a score tile share
+// a page, its lookup and the high half of their addresses.
 template <int QT, int CT, int NS, int DT, bool UNI>
 __device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT / 8], int w, int waves, int UH) {
     using M = Mfma<CT>;
@@ -773,6 +774,8 @@ __device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT
         };
         Unit un[BUF];
         int pg[BUF][2];
+        const uint32_t row_bytes = 2u * (uint32_t)a.row_stride, lane_at = 4u * lg * row_bytes + 4u * VD * col;
+        const bool all_lanes = a.D == DT;
         auto look = [&](int (&p)[2], int t) {
             if constexpr (UNI) {
 #pragma unroll
@@ -783,6 +786,28 @@ __device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT
             }
         };
         auto load = [&](u32x4 (&to)[8][VB], uint32_t& oks, const T* base, const int (&p)[2], int t) {
+            if (UNI && all_lanes && t * 32 + 32 <= own && (uint32_t)p[0] < (uint32_t)a.n_pages &&
+                (uint32_t)p[1] < (uint32_t)a.n_pages) {  // a whole unit: two scalar bases, the lane's part the same for each
+                oks = 255u;
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const int i0 = t * 32 + 16 * x;
+                    const auto* at = reinterpret_cast<const uint8_t*>(base + row_at(a, p[x], i0 - fdiv(a.page, i0) * (int)a.page.d));
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int vb = 0; vb < VB; vb++) {
+                            const auto* q = at + (uint32_t)(lane_at + (uint32_t)j * row_bytes + 256 * vb);
+                            if constexpr (VD == 4) {
+                                to[4 * x + j][vb] = *reinterpret_cast<const u32x4*>(q);
+                            } else {
+                                const u32x2 y = *reinterpret_cast<const u32x2*>(q);
+                                to[4 * x + j][vb] = u32x4{y[0], y[1], 0u, 0u};
+                            }
+                        }
+                }
+                return;
+            }
             oks = 0;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -1173,7 +1198,7 @@ void launch_uni(const AttnArgs& g, hipStream_t s) {
 template <int QT, int CT, int NS>
 void launch_types(const AttnArgs& g, hipStream_t s) {
     if (g.planned) hipLaunchKernelGGL(k_attn_plan, dim3(1), dim3(1024), 0, s, g);
-    if (g.a.page.d % 16 == 0) launch_uni<QT, CT, NS, true>(g, s);
+    if (g.a.page.d % 16 == 0 && g.a.row_stride < 1 << 26) launch_uni<QT, CT, NS, true>(g, s);
     else launch_uni<QT, CT, NS, false>(g, s);
     // one head per wave while that fills the chip twice at most, more where most rows are done
     if ((int64_t)g.a.T * g.H <= 32768)
@@ -1211,8 +1236,10 @@ void launch_attn_paged(const Paged& a0, int cache_type, const void* q, int64_t q
     g.DT = padded(a.D);
     g.groups = 256;
     g.waves = kWaves;
-    g.tile_cost = 3.4f;
-    g.wave_cost = 0.25f;
+    // us of a CU: 64 keys x 256 rows of 128 by 8 waves (630 TFLOP/s), 32 keys of 128 (one CU alone draws 48 GB/s)
+    const int parts = q_type != BPD_T_F32 ? 1 : cache_type == BPD_T_BF16 ? 3 : 2;
+    g.tile_cost = 3.4f * (float)(g.R * g.DT * parts) / (256.f * 128.f) * (g.DT == 256 ? 2.f : 1.f);
+    g.wave_cost = 0.35f * (float)g.DT / 128.f;
     g.planned = planned_way(a.q_start, g.G);
     const Sizes z = sizes(g.planned, a.B, a.T, g.G, a.hkv, g.R, g.DT, a.P);
     uint8_t* at = static_cast<uint8_t*>(ws);
