@@ -21,10 +21,12 @@ namespace bpdq {
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of a row's workgroup
+constexpr int kRow = 32768;  // elements of a row that its workgroup holds in registers
 constexpr int kSliceThreads = 512;
 constexpr int kBuckets = 1024;
 constexpr int kList = 4096;  // entries of a list that is sorted
 constexpr int kTable = 64;
+constexpr int kSlices = 256;  // at most: vocab up to 2^22
 typedef unsigned long long u64;
 
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -62,23 +64,23 @@ struct Row {
         p *= table[k & (kTable - 1)];
         return __longlong_as_double(__double_as_longlong(p) + ((long long)((k >> 6) + up) << 52));
     }
+    // at most 2^44: adding 2^52 rounds to an integer and leaves it in the low bits.  The largest logit's is exactly
+    // 2^shift: its exponent is off by what off rounds to, 2^-53 of it
     __device__ __forceinline__ u64 weight(float x) const {
-        // at most 2^44: adding 2^52 rounds to an integer and leaves it in the low bits
-        const u64 w = (u64)__double_as_longlong(power(x, shift) + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
-        return x == top ? 1ull << shift : w;
+        return (u64)__double_as_longlong(power(x, shift) + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
     }
-    __device__ __forceinline__ u64 weight_of(uint32_t key) const { return weight(logit_of(key)); }
+    // where the largest may be infinite
+    __device__ __forceinline__ u64 weight_of(uint32_t key) const {
+        return logit_of(key) == top ? 1ull << shift : weight(logit_of(key));
+    }
     __device__ __forceinline__ bool passes(uint32_t key, float min_p) const {
         const float x = logit_of(key);
         return !(min_p > 0.f) || x == top || (min_p < 1.f && power(x, 0) >= (double)min_p && min_p > 0x1p-59f) ||
                (min_p <= 0x1p-59f && exp2(__builtin_fma((double)x, per, off)) >= (double)min_p);
     }
-    // Distance from the largest logit in buckets: does not fall as logits do; NaN only for NaN
-    __device__ __forceinline__ float distance(float x) const { return x == top ? 0.f : (top - x) * buckets; }
-    __device__ __forceinline__ int bucket(float x) const {
-        const float d = distance(x);
-        return d < (float)(kBuckets - 1) ? (int)d : kBuckets - 1;
-    }
+    // Distance from the largest logit, which is finite, in buckets: does not fall as logits do; NaN only for NaN
+    __device__ __forceinline__ float distance(float x) const { return (top - x) * buckets; }
+    __device__ __forceinline__ int bucket(float x) const { return (int)fminf(distance(x), (float)(kBuckets - 1)); }
 };
 
 template <typename T>
@@ -99,13 +101,15 @@ __device__ __forceinline__ T scan_block(T v, T& all, T* s_part) {
     __syncthreads();
     if (lane == 63) s_part[wave] = run;
     __syncthreads();
-    T before = run - v;
-    all = 0;
-    for (int i = 0; i < THREADS / 64; i++) {
-        if (i < wave) before += s_part[i];
-        all += s_part[i];
+    constexpr int W = THREADS / 64;
+    T sums = s_part[lane & (W - 1)];
+    for (int d = 1; d < W; d <<= 1) {
+        const T o = __shfl_up(sums, d);
+        if (lane >= d) sums += o;
     }
-    return before;
+    all = __shfl(sums, W - 1);
+    const T before = __shfl(sums, (wave + 63) & 63);  // of the waves before this one
+    return (wave > 0 ? before : 0) + run - v;
 }
 
 // The settings of a row.
@@ -187,11 +191,12 @@ __device__ __forceinline__ void join_wave(Max& a) {
     for (int d = 1; d < 64; d <<= 1) join(a, __shfl_xor(a.top, d), __shfl_xor(a.low, d), __shfl_xor(a.n, d));
 }
 
-// ---- max: of [lo, hi), in every thread
-template <typename X, int THREADS>
-__device__ __forceinline__ Max part_max(const X* x, int lo, int hi, Max* s_part) {
+// ---- max: in every thread
+// (visit(f) calls f(index, logit) for a thread's part of the elements)
+template <int THREADS, typename VISIT>
+__device__ __forceinline__ Max part_max(VISIT&& visit, Max* s_part) {
     Max m = {-__builtin_inff(), __builtin_inff(), 0u};
-    each<X, THREADS>(x, lo, hi, [&](int, float v) {
+    visit([&](int, float v) {
         const bool is = v > -__builtin_inff();
         m.top = fmaxf(m.top, v);
         m.low = is ? fminf(m.low, v) : m.low;
@@ -215,37 +220,33 @@ __device__ __forceinline__ Row row_of(const Set& set, const Max& m, int shift, c
     r.table = table;
     // 32 to a unit of (l - max) / t, which weighs nothing beyond kBuckets of them; a smaller range of logits
     // is cut finer
-    r.buckets = fmaxf(32.f / set.t, 0.999f * (float)kBuckets / (m.top - m.low));
+    r.buckets = fminf(fmaxf(32.f / set.t, 0.999f * (float)kBuckets / (m.top - m.low)), 1e30f);
     return r;
 }
 
 __device__ __forceinline__ Mode mode_of(const Set& s, const Max& m) {
     if (m.n == 0) return kNone;
     if (s.greedy) return kGreedy;
+    if (m.top == __builtin_inff()) return kSearch;
     if (s.k > 0 && (uint32_t)s.k < m.n) return s.k > kList ? kSearch : kTopK;
     return kWeights;
 }
 
-// ---- hist: of [lo, hi), into hw (kTopK: counts in its first half), cleared before; ends with a barrier
-template <typename X, int THREADS>
-__device__ __forceinline__ void part_hist(const X* x, int lo, int hi, const Row& r, Mode mode, u64* hw) {
+// ---- hist: into hw (kTopK: counts in its first half), cleared before; ends with a barrier
+template <typename VISIT>
+__device__ __forceinline__ void part_hist(VISIT&& visit, const Row& r, Mode mode, u64* hw) {
     if (mode == kTopK) {
         uint32_t* hc = reinterpret_cast<uint32_t*>(hw);
-        each<X, THREADS>(x, lo, hi, [&](int, float v) {
+        visit([&](int, float v) {
             // the last bucket's are what the others leave, and not asked for
             const float d = r.distance(v);
             if (d < (float)(kBuckets - 1)) atomicAdd(&hc[(int)d], 1u);
         });
     } else {
-        u64 rest = 0;  // the last bucket's, by thread
-        each<X, THREADS>(x, lo, hi, [&](int, float v) {
+        visit([&](int, float v) {  // in the last bucket few weigh anything
             const u64 w = r.weight(v);
-            const int b = r.bucket(v);
-            if (b == kBuckets - 1) rest += w;
-            else if (w != 0) atomicAdd(&hw[b], w);
+            if (w != 0) atomicAdd(&hw[r.bucket(v)], w);
         });
-        rest = wave_sum(rest);
-        if ((threadIdx.x & 63) == 0 && rest != 0) atomicAdd(&hw[kBuckets - 1], rest);
     }
     __syncthreads();
 }
@@ -306,16 +307,19 @@ __device__ __forceinline__ Pick find_buckets(const T* hist, int stride, int S, c
     return p;
 }
 
-// ---- pick, second half: put(index) for what is listed of [lo, hi); how many stay, by thread
-template <typename X, int THREADS, typename F>
-__device__ __forceinline__ uint32_t part_pick(const X* x, int lo, int hi, const Row& r, const Pick& p, F&& put) {
+// ---- pick, second half: bit k of `listed` for the k-th element that visit shows the thread, 32 at most; returns
+// how many stay, by thread
+template <typename VISIT>
+__device__ __forceinline__ uint32_t part_pick(VISIT&& visit, const Row& r, const Pick& p, uint32_t& listed) {
     const float first = (float)p.first, last = p.last < kBuckets - 1 ? (float)(p.last + 1) : __builtin_inff();
-    uint32_t n = 0;
-    each<X, THREADS>(x, lo, hi, [&](int i, float v) {
+    uint32_t n = 0, bit = 1;
+    listed = 0;
+    visit([&](int, float v) {
         const float d = r.distance(v);
         const bool stays = d < first;
         n += stays;
-        if (!stays && (d < last || (last > (float)kBuckets && v > -__builtin_inff()))) put(i);
+        if (!stays && (d < last || (last > (float)kBuckets && v > -__builtin_inff()))) listed |= bit;
+        bit <<= 1;
     });
     return n;
 }
@@ -543,22 +547,32 @@ __device__ __forceinline__ void search_row(const SampleArgs& g, int row, const X
     }
 }
 
-// Sorts n values of LDS, falling; they differ.  Up to 1024 each finds its place by counting those above it.
+// Sorts n values of LDS, falling, by a bitonic network.  Up to 1024 each thread holds one, and partners less than 64
+// apart are asked by shuffles.
 __device__ __forceinline__ void sort_falling(u64* a, int n) {
     const int tid = (int)threadIdx.x;
     if (n <= kThreads) {
-        const u64 mine = tid < n ? a[tid] : 0;
-        int rank = 0;
-        if ((tid & ~63) < n) {
-#pragma unroll 8
-            for (int j = 0; j < n; j++) rank += a[j] > mine;
-        }
+        u64 v = tid < n ? a[tid] : 0;
+        for (int k = 2; k < 2 * n; k <<= 1)
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                u64 o;
+                if (j >= 64) {
+                    __syncthreads();
+                    a[tid] = v;
+                    __syncthreads();
+                    o = a[tid ^ j];
+                } else {
+                    o = __shfl_xor(v, j);
+                }
+                const bool larger = ((tid & k) == 0) == ((tid & j) == 0);
+                v = (v > o) == larger ? v : o;
+            }
         __syncthreads();
-        if (tid < n) a[rank] = mine;
+        a[tid] = v;
         __syncthreads();
         return;
     }
-    int n2 = kThreads;
+    int n2 = 2 * kThreads;
     while (n2 < n) n2 <<= 1;
     for (int i = n + tid; i < n2; i += kThreads) a[i] = 0;
     __syncthreads();
@@ -576,7 +590,7 @@ __device__ __forceinline__ void sort_falling(u64* a, int n) {
 struct DrawLds {
     u64 list[kList];  // (key, ~index), later (~index, key)
     u64 part[kWaves];
-    u64 slice[256];
+    u64 slice[kSlices];
     u64 before;
     uint32_t n, kept;
     int chosen;
@@ -588,30 +602,31 @@ template <typename X>
 __device__ __forceinline__ void draw_row(const SampleArgs& g, int row, const X* x, const Row& r, const Set& set, Mode mode,
                                          const Pick& pick, const Sum* sums, int S, int len, uint32_t n_list, uint32_t n_stay,
                                          DrawLds& s) {
-    constexpr int PER = kList / kThreads;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     sort_falling(s.list, (int)n_list);  // by logit, equal ones by index
-    // how many of the list stay
-    u64 v[PER], mine = 0, total;
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-        const int i = tid * PER + j;
-        v[j] = i < (int)n_list && (mode != kTopK || i < set.k) ? r.weight_of((uint32_t)(s.list[i] >> 32)) : 0;
-        mine += v[j];
+    // how many of the list stay.  Every loop here is kept rolled: a row's workgroup runs through this code
+    // once, and waits for its instructions more than for its data
+    const int n_ranked = mode == kTopK ? min((int)n_list, set.k) : (int)n_list;
+    u64 total = 0, want = pick.want;
+    if (mode == kTopK && set.p < 1.f) {  // the total of the top-k first
+        u64 mine = 0;
+#pragma unroll 1
+        for (int i = tid; i < n_ranked; i += kThreads) mine += r.weight_of((uint32_t)(s.list[i] >> 32));
+        scan_block<kThreads>(mine, total, s.part);
+        want = reach(set.p, total);
     }
-    u64 run = scan_block<kThreads>(mine, total, s.part);
-    const u64 want = mode != kTopK ? pick.want : set.p < 1.f ? reach(set.p, total) : ~0ull;
-    uint32_t stay = 0;
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-        const int i = tid * PER + j;
+    u64 run0 = 0;
+#pragma unroll 1
+    for (int i0 = 0; i0 < n_ranked; i0 += kThreads) {
+        const int i = i0 + tid;
+        const uint32_t k = i < n_ranked ? (uint32_t)(s.list[i] >> 32) : 0;
+        u64 all = 0, run = run0;
+        if (want != ~0ull) run += scan_block<kThreads>(i < n_ranked ? r.weight_of(k) : 0, all, s.part);
         // what stands before it falls short of what is wanted
-        if (i < (int)n_list && (mode != kTopK || i < set.k) && run < want && r.passes((uint32_t)(s.list[i] >> 32), set.m))
-            stay++;
-        run += v[j];
+        const uint64_t stay = __ballot(i < n_ranked && run < want && r.passes(k, set.m));
+        if (lane == 0 && stay != 0) atomicAdd(&s.kept, (uint32_t)__popcll(stay));
+        run0 += all;
     }
-    stay = wave_sum(stay);
-    if (lane == 0 && stay) atomicAdd(&s.kept, stay);
     __syncthreads();
     const uint32_t kept_list = s.kept, kept = kept_list + n_stay;
 
@@ -623,83 +638,84 @@ __device__ __forceinline__ void draw_row(const SampleArgs& g, int row, const X* 
         }
         __syncthreads();
         sort_falling(s.list, (int)kept_list);  // ~index falls
-        mine = 0;
-#pragma unroll
-        for (int j = 0; j < PER; j++) {
-            const int i = tid * PER + j;
-            v[j] = i < (int)kept_list ? r.weight_of((uint32_t)s.list[i]) : 0;
-            mine += v[j];
-        }
-        run = scan_block<kThreads>(mine, total, s.part);
-        const u64 target = draw_target(set.u, total);
-#pragma unroll
-        for (int j = 0; j < PER; j++) {
-            if (run <= target && run + v[j] > target)
-                answer(g, row, (int)~(uint32_t)(s.list[tid * PER + j] >> 32), (float)log((double)v[j] / (double)total), kept);
-            run += v[j];
+        for (int pass = 0; pass < 2; pass++) {  // the total, then the place
+            const u64 target = pass == 0 ? 0 : draw_target(set.u, total);
+            run0 = 0;
+#pragma unroll 1
+            for (int i0 = 0; i0 < (int)kept_list; i0 += kThreads) {
+                const int i = i0 + tid;
+                const u64 e = i < (int)kept_list ? s.list[i] : 0, v = i < (int)kept_list ? r.weight_of((uint32_t)e) : 0;
+                u64 all;
+                const u64 run = run0 + scan_block<kThreads>(v, all, s.part);
+                run0 += all;
+                if (pass == 0 && kept_list > (uint32_t)kThreads) continue;
+                const u64 t = kept_list > (uint32_t)kThreads ? target : draw_target(set.u, all), sum = pass == 0 ? all : total;
+                if (run <= t && run + v > t)
+                    answer(g, row, (int)~(uint32_t)(e >> 32), (float)log((double)v / (double)sum), kept);
+            }
+            total = run0;
+            if (kept_list <= (uint32_t)kThreads) break;  // one round said it all
         }
         return;
     }
     // a head of the list stays, up to this one; where none does, the buckets before it alone
     const u64 cut = kept_list > 0 ? s.list[kept_list - 1] : 0;
     // the slice: what stays of each is its sum and its part of the list
-    total = 0;
-    for (int pass = 0; pass < 2; pass++) {  // the total, then the slice
-        u64 before = 0;
-        const u64 target = pass == 0 ? 0 : draw_target(set.u, total);
-        for (int s0 = 0; s0 < S; s0 += 256) {
-            __syncthreads();
-            if (tid < 256) s.slice[tid] = s0 + tid < S ? sums[s0 + tid].w : 0;
-            __syncthreads();
-            for (int i = tid; i < (int)kept_list; i += kThreads) {
-                const int at = S == 1 ? 0 : (int)(~(uint32_t)s.list[i]) / len - s0;
-                if (at >= 0 && at < 256) atomicAdd(&s.slice[at], r.weight_of((uint32_t)(s.list[i] >> 32)));
-            }
-            __syncthreads();
-            const u64 ws = tid < 256 ? s.slice[tid] : 0;
-            u64 all;
-            const u64 at = before + scan_block<kThreads>(ws, all, s.part);
-            if (pass == 1 && at <= target && at + ws > target) {
-                s.chosen = s0 + tid;
-                s.before = at;
-            }
-            before += all;
+    if (tid < kSlices) s.slice[tid] = tid < S ? sums[tid].w : 0;
+    __syncthreads();
+    for (int i = tid; i < (int)kept_list; i += kThreads)
+        atomicAdd(&s.slice[S == 1 ? 0 : (int)(~(uint32_t)s.list[i]) / len], r.weight_of((uint32_t)(s.list[i] >> 32)));
+    __syncthreads();
+    {
+        const u64 w = tid < kSlices ? s.slice[tid] : 0, at = scan_block<kThreads>(w, total, s.part);
+        const u64 target = draw_target(set.u, total);
+        if (at <= target && at + w > target) {
+            s.chosen = tid;
+            s.before = at;
         }
-        total = before;
-        if (S == 1) break;
     }
     __syncthreads();
     // the place in the slice: by the waves' parts of it, then 64 at a time
     const u64 target = draw_target(set.u, total);
-    const int lo = S == 1 ? 0 : s.chosen * len, hi = min(g.V, lo + len), seg = (min(len, g.V) + kWaves * 64 - 1) / (kWaves * 64) * 64;
-    const int wlo = min(hi, lo + wave * seg), whi = min(hi, wlo + seg);
+    const int lo = s.chosen * len, hi = min(g.V, lo + len), seg = (min(len, g.V) + kWaves * 64 - 1) / (kWaves * 64) * 64;
+    const int wlo = lo + wave * seg, whi = min(hi, wlo + seg);
     const float first = (float)pick.first;
-    auto weight_at = [&](int i) -> u64 {
-        if (i >= whi) return 0;
-        const float f = (float)x[i];
+    auto weight_at = [&](float f, int i) -> u64 {
         const bool in = r.distance(f) < first || (cut != 0 && ((u64)key_of(f) << 32 | (uint32_t)~(uint32_t)i) >= cut);
         return in ? r.weight(f) : 0;
     };
-    mine = 0;
-    for (int i = wlo + lane; i < whi; i += 64) mine += weight_at(i);
+    u64 mine = 0;
+#pragma unroll 1
+    for (int i0 = wlo + lane; i0 < whi; i0 += 8 * 64) {
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) f[j] = i0 + 64 * j < whi ? (float)x[i0 + 64 * j] : -__builtin_inff();
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const u64 v = weight_at(f[j], i0 + 64 * j);
+            mine += v;
+        }
+    }
     mine = wave_sum(mine);
     __syncthreads();
     if (lane == 0) s.part[wave] = mine;
     __syncthreads();
-    u64 before = S == 1 ? 0 : s.before;
+    u64 before = s.before;
     int chosen = 0;
     for (; chosen < kWaves - 1 && before + s.part[chosen] <= target; chosen++) before += s.part[chosen];
     if (wave != chosen) return;
+#pragma unroll 1
     for (int i0 = wlo; i0 < whi; i0 += 64) {
-        const u64 v1 = weight_at(i0 + lane);
-        u64 sum = v1;
+        const int i = i0 + lane;
+        const u64 v = i < whi ? weight_at((float)x[i], i) : 0;
+        u64 sum = v;
         for (int d = 1; d < 64; d <<= 1) {
             const u64 o = __shfl_up(sum, d);
             if (lane >= d) sum += o;
         }
         const uint64_t over = __ballot(before + sum > target);
         if (over != 0) {
-            if (lane == __builtin_ctzll(over)) answer(g, row, i0 + lane, (float)log((double)v1 / (double)total), kept);
+            if (lane == __builtin_ctzll(over)) answer(g, row, i, (float)log((double)v / (double)total), kept);
             return;
         }
         before += __shfl(sum, 63);
@@ -742,7 +758,29 @@ __global__ __launch_bounds__(kThreads) void k_sample_row(SampleArgs g, int shift
     fill_table(table);
     hw[tid] = 0;
     if (tid == 0) s.draw.n = s.draw.kept = 0;
-    const Max m = part_max<X, kThreads>(x, 0, g.V, s_max);
+    // the row's kRow elements at most stay in registers
+    constexpr int N = 16 / (int)sizeof(X), NV = kRow / (kThreads * N);
+    Vec<X, N> held[NV];
+    const bool aligned = ((uintptr_t)x & 15) == 0;
+#pragma unroll
+    for (int c = 0; c < NV; c++) {
+        const int i = (c * kThreads + tid) * N;
+        if (aligned && i + N <= g.V) {
+            held[c] = *reinterpret_cast<const Vec<X, N>*>(x + i);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j++) held[c].v[j] = i + j < g.V ? x[i + j] : (X)-__builtin_inff();
+        }
+    }
+    auto visit = [&](auto&& f) {
+#pragma unroll
+        for (int c = 0; c < NV; c++) {
+            if (c * kThreads * N >= g.V) break;
+#pragma unroll
+            for (int j = 0; j < N; j++) f((c * kThreads + tid) * N + j, (float)held[c].v[j]);
+        }
+    };
+    const Max m = part_max<kThreads>(visit, s_max);
     const Mode mode = mode_of(set, m);
     if (mode == kNone) {
         if (tid == 0) answer(g, row, -1, __builtin_nanf(""), 0);
@@ -754,21 +792,26 @@ __global__ __launch_bounds__(kThreads) void k_sample_row(SampleArgs g, int shift
     }
     const Row r = row_of(set, m, shift, table);
     if (mode != kSearch) {
-        part_hist<X, kThreads>(x, 0, g.V, r, mode, hw);
+        part_hist(visit, r, mode, hw);
         const Pick pick = mode == kTopK ? find_buckets<kThreads>(reinterpret_cast<const uint32_t*>(hw), 0, 1, r, set, mode,
                                                                  reinterpret_cast<uint32_t*>(s_part),
                                                                  reinterpret_cast<uint32_t*>(&s_before), &s_bucket)
                                         : find_buckets<kThreads>(hw, 0, 1, r, set, mode, s_part, &s_before, &s_bucket);
-        uint32_t n_stay = m.n;
+        uint32_t n_stay = m.n, n_list = 0;
         if (pick.first < kBuckets) {
-            const uint32_t n = part_pick<X, kThreads>(x, 0, g.V, r, pick, [&](int i) {
-                const uint32_t at = atomicAdd(&s.draw.n, 1u);
-                if (at < (uint32_t)kList) s.draw.list[at] = (u64)key_of((float)x[i]) << 32 | (uint32_t)~(uint32_t)i;
-            });
-            scan_block<kThreads>(n, n_stay, reinterpret_cast<uint32_t*>(s_part));
+            uint32_t listed;
+            const uint32_t n = part_pick(visit, r, pick, listed);
+            u64 both;  // staying above, listed below
+            const u64 at = scan_block<kThreads>((u64)n << 32 | (uint32_t)__popc(listed), both, s_part);
+            n_stay = (uint32_t)(both >> 32);
+            n_list = (uint32_t)both;
+            uint32_t to = (uint32_t)at;
+            for (; listed != 0 && n_list <= (uint32_t)kList; listed &= listed - 1) {
+                const int k = __builtin_ctz(listed), i = (k / N * kThreads + tid) * N + k % N;
+                s.draw.list[to++] = (u64)key_of((float)x[i]) << 32 | (uint32_t)~(uint32_t)i;
+            }
         }
         __syncthreads();
-        const uint32_t n_list = s.draw.n;
         if (n_list <= (uint32_t)kList) {
             u64 w_stay = 0;
             if (mode == kWeights) scan_block<kThreads>(staying<kThreads>(hw, pick), w_stay, s_part);
@@ -800,7 +843,8 @@ __global__ __launch_bounds__(kSliceThreads) void k_max(SampleArgs g, Work w) {
     __shared__ Max part[kSliceThreads / 64];
     const int row = (int)(blockIdx.x / (unsigned)w.S), slice = (int)(blockIdx.x % (unsigned)w.S);
     const int lo = slice * w.len, hi = min(g.V, lo + w.len);
-    const Max m = part_max<X, kSliceThreads>(reinterpret_cast<const X*>(g.logits) + (int64_t)row * g.stride, lo, hi, part);
+    const X* x = reinterpret_cast<const X*>(g.logits) + (int64_t)row * g.stride;
+    const Max m = part_max<kSliceThreads>([&](auto&& f) { each<X, kSliceThreads>(x, lo, hi, f); }, part);
     if (threadIdx.x == 0) w.max[blockIdx.x] = m;
 }
 
@@ -818,8 +862,8 @@ __global__ __launch_bounds__(kSliceThreads) void k_hist(SampleArgs g, Work w) {
     for (int i = tid; i < kBuckets; i += kSliceThreads) hw[i] = 0;
     __syncthreads();
     const int lo = slice * w.len, hi = min(g.V, lo + w.len);
-    part_hist<X, kSliceThreads>(reinterpret_cast<const X*>(g.logits) + (int64_t)row * g.stride, lo, hi,
-                                row_of(set, m, w.shift, table), mode, hw);
+    const X* x = reinterpret_cast<const X*>(g.logits) + (int64_t)row * g.stride;
+    part_hist([&](auto&& f) { each<X, kSliceThreads>(x, lo, hi, f); }, row_of(set, m, w.shift, table), mode, hw);
     const int64_t at = (int64_t)blockIdx.x * kBuckets;
     const int n = mode == kTopK ? kBuckets / 2 : kBuckets;
     for (int i = tid; i < n; i += kSliceThreads) w.weight[at + i] = hw[i];
@@ -848,28 +892,34 @@ __global__ __launch_bounds__(kSliceThreads) void k_pick(SampleArgs g, Work w) {
     using X = typename Elem<TYPE>::type;
     constexpr int T = kSliceThreads;
     __shared__ u64 s_part[T / 64];
-    __shared__ uint32_t s_list;
     const int row = (int)(blockIdx.x / (unsigned)w.S), slice = (int)(blockIdx.x % (unsigned)w.S), tid = (int)threadIdx.x;
     const Set set = settings(g, row);
     const Max m = row_max(w, row);
     const Mode mode = mode_of(set, m);
     if (mode != kWeights && mode != kTopK) return;
-    if (tid == 0) s_list = 0;
-    __syncthreads();
     const Row r = row_of(set, m, w.shift, nullptr);  // no weights here
     const Pick pick = w.pick[row];
     const int lo = slice * w.len, hi = min(g.V, lo + w.len);
     uint16_t* list = w.list + (int64_t)blockIdx.x * w.len;
-    uint32_t n_all = w.max[blockIdx.x].n;
+    uint32_t n_all = w.max[blockIdx.x].n, n_list = 0;
     if (pick.first < kBuckets) {
-        const uint32_t n = part_pick<X, T>(reinterpret_cast<const X*>(g.logits) + (int64_t)row * g.stride, lo, hi, r, pick,
-                                           [&](int i) { list[atomicAdd(&s_list, 1u)] = (uint16_t)(i - lo); });
-        scan_block<T>(n, n_all, reinterpret_cast<uint32_t*>(s_part));
+        const X* x = reinterpret_cast<const X*>(g.logits) + (int64_t)row * g.stride;
+        uint32_t listed;
+        const uint32_t n = part_pick([&](auto&& f) { each<X, T>(x, lo, hi, f); }, r, pick, listed);
+        u64 both;  // staying above, listed below
+        const u64 at = scan_block<T>((u64)n << 32 | (uint32_t)__popc(listed), both, s_part);
+        n_all = (uint32_t)(both >> 32);
+        n_list = (uint32_t)both;
+        constexpr int N = 16 / (int)sizeof(X);
+        for (uint32_t to = (uint32_t)at; listed != 0; listed &= listed - 1) {
+            const int k = __builtin_ctz(listed);
+            list[to++] = (uint16_t)((k / N * T + tid) * N + k % N);
+        }
     }
     u64 w_all = 0;
     if (mode == kWeights) scan_block<T>(staying<T>(w.weight + (int64_t)blockIdx.x * kBuckets, pick), w_all, s_part);
     __syncthreads();
-    if (tid == 0) w.sum[blockIdx.x] = {w_all, n_all, s_list};
+    if (tid == 0) w.sum[blockIdx.x] = {w_all, n_all, n_list};
 }
 
 template <int TYPE>
@@ -930,7 +980,7 @@ int shift_of(int V) {
     return bits <= 18 ? 44 : 62 - bits;
 }
 
-// Elements of a slice: enough workgroups for the chip, up to 16384 (16-bit places in a slice's list).
+// Elements of a slice: enough workgroups for the chip, up to 16384 (32 for a thread, marked in one word).
 int slice_len(int B, int V) {
     int len = 16384;
     while (len > 2048 && (int64_t)B * ((V + len - 1) / len) < 1024) len >>= 1;
@@ -938,7 +988,7 @@ int slice_len(int B, int V) {
 }
 
 // Whether rows take one workgroup each or one per slice.
-bool by_row(int, int V) { return V <= 32768; }
+bool by_row(int V) { return V <= kRow; }
 
 int64_t up16(int64_t v) { return (v + 15) / 16 * 16; }
 
@@ -948,7 +998,7 @@ struct Layout {
 };
 Layout layout(int B, int V) {
     Layout l = {};
-    if (by_row(B, V)) {
+    if (by_row(V)) {
         l.total = 16;
         return l;
     }
@@ -965,7 +1015,7 @@ Layout layout(int B, int V) {
 
 template <int TYPE>
 void launch_type(const SampleArgs& a, const Work& w, hipStream_t s) {
-    if (by_row(a.B, a.V)) {
+    if (by_row(a.V)) {
         hipLaunchKernelGGL(k_sample_row<TYPE>, dim3((unsigned)a.B), dim3(kThreads), 0, s, a, w.shift);
         return;
     }

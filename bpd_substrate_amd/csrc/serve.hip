@@ -183,7 +183,8 @@ void bpd_attn_paged_gpu(const bpd_paged_cache* kv, const bpd_paged_batch* b, con
 
 int64_t bpd_sample_workspace(int n_rows, int vocab) {
     Args c("bpd_sample_workspace");
-    c.shape(n_rows >= 0, "n_rows is negative").shape(vocab >= 0, "vocab is negative");
+    c.shape(n_rows >= 0, "n_rows is negative").shape(vocab >= 0, "vocab is negative").need(
+        vocab <= 1 << 22, BPDQ_ERR_LIMIT, "vocab is above 2^22");
     return c.ok ? bpdq::sample_ws(n_rows, vocab) : -1;
 }
 
@@ -194,6 +195,7 @@ void bpd_sample_gpu(const void* logits, int type, int64_t row_stride, int n_rows
     Args c(fn);
     c.shape(type == BPD_T_F32 || type == BPD_T_F16 || type == BPD_T_BF16, "type is unknown");
     c.shape(n_rows >= 0, "n_rows is negative").shape(vocab >= 0, "vocab is negative");
+    c.need(vocab <= 1 << 22, BPDQ_ERR_LIMIT, "vocab is above 2^22");
     c.shape(row_stride >= vocab && row_stride <= kMaxStride, "row_stride is shorter than a row, or 2^30 or more");
     if (!c.ok || n_rows == 0) return;
     if (vocab > 0) c.ptr(logits, (uintptr_t)esize(type), "logits");

@@ -105,7 +105,7 @@ void bpd_attn_paged_gpu(const bpd_paged_cache* cache, const bpd_paged_batch* bat
 int64_t bpd_attn_paged_workspace(const bpd_paged_cache* cache, const bpd_paged_batch* batch, int n_heads);
 
 /* One token per row of logits [n_rows][vocab] (type, rows row_stride elements
- * apart, aligned to an element).  In order, each over what the one before left, equal
+ * apart, aligned to an element; vocab up to 2^22, more is BPDQ_ERR_LIMIT).  In order, each over what the one before left, equal
  * logits ranked by index:
  *   temperature  weights w_i = exp((l_i - max l) / temperature); not above 0: the
  *                largest logit alone
