@@ -1071,6 +1071,51 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs g) {
     uint64_t todo = __ballot(!done);
     // a row of the head in 16-byte pieces by DT / 4 lanes: 64 / (DT / 4) results at a time
     const int lanes = g.DT >> 2, sub = lane / lanes, piece = lane - sub * lanes, step = 64 / lanes;
+    constexpr int FEW = 4;
+    if (HW > 1 && __ballot(!done && wp.y + wo.y > FEW) == 0) {
+        // few results each: a lane weighs its head's, then each group of lanes adds up a head
+        const int64_t sp = (int64_t)wp.x * g.R + rp, so = (int64_t)wo.x * R1 + ro;
+        float2 x[FEW];
+        float m = kNegInf, l = 0.f, f[FEW];
+#pragma unroll
+        for (int k = 0; k < FEW; k++) {
+            x[k] = make_float2(kNegInf, 0.f);
+            if (!done && k < wp.y + wo.y) x[k] = k < wp.y ? g.ml[sp + (int64_t)k * g.R] : ml1[so + (int64_t)(k - wp.y) * R1];
+            m = fmaxf(m, x[k].x);
+        }
+#pragma unroll
+        for (int k = 0; k < FEW; k++) {
+            f[k] = x[k].x == kNegInf ? (x[k].y != 0.f ? x[k].y : 0.f) : __builtin_amdgcn_exp2f(x[k].x - m);
+            l += x[k].y * f[k];
+        }
+        const bool any = l != 0.f;
+        if (!done && g.lse != nullptr)
+            g.lse[(int64_t)t * g.H + h0 + lane] = any ? (m + __builtin_log2f(l)) * kLn2 : kNegInf;
+#pragma unroll
+        for (int k = 0; k < FEW; k++) f[k] = any ? f[k] / l : 0.f;
+#pragma unroll 4
+        for (int j0 = 0; j0 < HW; j0 += step) {
+            const int j = j0 + sub;  // below 64: HW is 8 at most, sub 4
+            const int np = __shfl(wp.y, j), n = np + __shfl(wo.y, j);
+            const int64_t p0 = __shfl(sp, j), p1 = __shfl(so, j);
+            const bool skip = __shfl((int)done, j) != 0 || j >= HW;
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < FEW; k++) {
+                const float fk = __shfl(f[k], j);
+                if (skip || k >= n || fk == 0.f) continue;  // nothing, or what is not there
+                const float* p = k < np ? g.part + (p0 + (int64_t)k * g.R) * g.DT : part1 + (p1 + (int64_t)(k - np) * R1) * g.DT;
+                acc += *reinterpret_cast<const f32x4*>(p + 4 * piece) * fk;
+            }
+            if (!skip && 4 * piece < a.D) {
+                Vec<Q, 4> v;
+#pragma unroll
+                for (int c = 0; c < 4; c++) v.v[c] = (Q)acc[c];
+                *reinterpret_cast<Vec<Q, 4>*>(reinterpret_cast<Q*>(g.out) + t * g.os + (int64_t)(h0 + j) * a.D + 4 * piece) = v;
+            }
+        }
+        return;
+    }
     while (todo != 0) {
         const int j = __builtin_ctzll(todo);
         todo &= todo - 1;

@@ -17,6 +17,7 @@ workspace comes from torch's allocator, so calls on several streams, from severa
 in several captured graphs do not share one.
 """
 import ctypes
+import functools
 import math
 import threading
 
@@ -78,25 +79,18 @@ def _rows(t, what, shape, dtype, device):
 _lock = threading.Lock()
 
 
-def _launch(device, name, *args):
+def _launch(device, fn, *args):
+    """fn(*args), an entry point of the library, on torch's current stream of `device`."""
     if device.type != "cuda":
-        _bad(f"{name}: the tensors are on {device}, not on a GPU")
-    if device.index != torch.cuda.current_device():
+        _bad(f"{fn.__name__}: the tensors are on {device}, not on a GPU")
+    index = device.index
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
-            return _launch(device, name, *args)
-    fn, err = gpu._fn(name), gpu._fn("bpd_gpu_last_error")
+            return _launch(device, fn, *args)
     with _lock:
-        gpu._fn("bpd_gpu_set_stream")(torch._C._cuda_getCurrentRawStream(device.index))
-        err()   # what an unchecked call left is not this one's
+        gpu._fn("bpd_gpu_set_stream")(torch._C._cuda_getCurrentRawStream(index))
         fn(*args)
     gpu.check()
-
-
-def _workspace(name, device, *args):
-    n = gpu._fn(name)(*args)
-    if n < 0:
-        gpu.check()
-    return torch.empty(n, dtype=torch.uint8, device=device), n
 
 
 class PagedCache:
@@ -162,12 +156,23 @@ class PagedBatch:
         self.c = _Batch(p(table), table.stride(0) if n > 1 else w, w, p(lens), p(q_start), n, self.n_tokens, p(prefix),
                         prefix_len)
         self._p = ctypes.addressof(self.c)
+        self._bytes = {}
 
     def _check(self, cache):
         if self.device != cache.device:
             _bad(f"the batch is on {self.device}, the cache on {cache.device}")
         if self.prefix_len > (0 if self.prefix is None else self.prefix.shape[0]) * cache.page_size:
             _bad(f"prefix_len {self.prefix_len} is more than its pages hold")
+
+
+    def _workspace(self, cache, heads):
+        """Bytes that an attention call needs, which go by shapes alone."""
+        key = (heads, cache.n_kv_heads, cache.head_dim)
+        n = self._bytes.get(key)
+        if n is None:
+            n = gpu.call("bpd_attn_paged_workspace", cache._p, self._p, heads)
+            self._bytes[key] = n
+        return n
 
 
 class Rope:
@@ -223,7 +228,7 @@ def rope_append(cache, batch, q, k, v, rope=None, pos=None, q_out=None):
         _tensor(pos, "pos", (torch.int32,), 1, dev, contiguous=True)
         if pos.shape[0] != T:
             _bad(f"pos has {pos.shape[0]} values for {T} tokens")
-    _launch(dev, "bpd_rope_append_paged_gpu", cache._p, batch._p, None if rope is None else rope._p,
+    _launch(dev, gpu._fn("bpd_rope_append_paged_gpu"), cache._p, batch._p, None if rope is None else rope._p,
             None if pos is None else pos.data_ptr(), qp, qs, kp, ks, vp, vs, op, os_, TYPES[x.dtype], H)
     return q_out
 
@@ -245,11 +250,17 @@ def attention(cache, batch, q, scale=None, out=None, return_lse=False):
         out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
     os_ = _rows(out, "out", (T, H, D), q.dtype, dev)
     lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
-    ws, n = _workspace("bpd_attn_paged_workspace", dev, cache._p, batch._p, H)
-    _launch(dev, "bpd_attn_paged_gpu", cache._p, batch._p, q.data_ptr(), qs, out.data_ptr(), os_,
+    n = batch._workspace(cache, H)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    _launch(dev, gpu._fn("bpd_attn_paged_gpu"), cache._p, batch._p, q.data_ptr(), qs, out.data_ptr(), os_,
             None if lse is None else lse.data_ptr(), TYPES[q.dtype], H, D ** -0.5 if scale is None else float(scale),
             ws.data_ptr(), n)
     return (out, lse) if return_lse else out
+
+
+@functools.lru_cache(maxsize=256)
+def _sample_workspace(rows, vocab):
+    return gpu.call("bpd_sample_workspace", rows, vocab)
 
 
 def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
@@ -275,7 +286,8 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
         ptrs.append(t.data_ptr())
     res = torch.empty((3, B), dtype=torch.int32, device=dev)
     token, logprob, kept = res[0], res[1].view(torch.float32), res[2]
-    ws, n = _workspace("bpd_sample_workspace", dev, B, V)
-    _launch(dev, "bpd_sample_gpu", logits.data_ptr(), TYPES[logits.dtype], logits.stride(0) if B > 1 else V, B, V,
+    n = _sample_workspace(B, V)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    _launch(dev, gpu._fn("bpd_sample_gpu"), logits.data_ptr(), TYPES[logits.dtype], logits.stride(0) if B > 1 else V, B, V,
             *ptrs, token.data_ptr(), logprob.data_ptr(), kept.data_ptr(), ws.data_ptr(), n)
     return token, logprob, kept
