@@ -18,6 +18,8 @@
 // not depend on the batch: a workgroup runs through its units, and where an item ends in the
 // middle leaves its O, r and l for k_attn_join, in a place of its own.  The plan (k_attn_plan) is
 // made on the device, as the lengths are there.
+#include <type_traits>
+
 #include "bpdq_paged.h"
 
 namespace bpdq {
@@ -740,6 +742,9 @@ __device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT
     }
     const float sign = g.scale > 0.f ? 1.f : g.scale < 0.f ? -1.f : 0.f;
     const float scale2 = (g.scale == 0.f ? 1.f : __builtin_fabsf(g.scale)) * kLog2e;
+    // keys and values beyond the 256 MB of the MALL are read past it (128 -> 114 us for 670 MB); fewer may be there
+    // from the call before (27.4 us for 74 MB, 30 read past it)
+    const bool stream = U * 32 * a.D * 4 > (int64_t)256 << 20;
 
     while (u < u1) {
         const int own = own_rows(a, b), nk = (own + 31) >> 5;
@@ -789,22 +794,32 @@ __device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT
             if (UNI && all_lanes && t * 32 + 32 <= own && (uint32_t)p[0] < (uint32_t)a.n_pages &&
                 (uint32_t)p[1] < (uint32_t)a.n_pages) {  // a whole unit: two scalar bases, the lane's part the same for each
                 oks = 255u;
+                auto get = [&](auto nt) {
 #pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const int i0 = t * 32 + 16 * x;
-                    const auto* at = reinterpret_cast<const uint8_t*>(base + row_at(a, p[x], i0 - fdiv(a.page, i0) * (int)a.page.d));
+                    for (int x = 0; x < 2; x++) {
+                        const int i0 = t * 32 + 16 * x;
+                        const auto* at =
+                            reinterpret_cast<const uint8_t*>(base + row_at(a, p[x], i0 - fdiv(a.page, i0) * (int)a.page.d));
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
+                        for (int j = 0; j < 4; j++)
 #pragma unroll
-                        for (int vb = 0; vb < VB; vb++) {
-                            const auto* q = at + (uint32_t)(lane_at + (uint32_t)j * row_bytes + 256 * vb);
-                            if constexpr (VD == 4) {
-                                to[4 * x + j][vb] = *reinterpret_cast<const u32x4*>(q);
-                            } else {
-                                const u32x2 y = *reinterpret_cast<const u32x2*>(q);
-                                to[4 * x + j][vb] = u32x4{y[0], y[1], 0u, 0u};
+                            for (int vb = 0; vb < VB; vb++) {
+                                const auto* q = at + (uint32_t)(lane_at + (uint32_t)j * row_bytes + 256 * vb);
+                                using R = std::conditional_t<VD == 4, u32x4, u32x2>;
+                                const auto* r = reinterpret_cast<const R*>(q);
+                                R y;
+                                if constexpr (decltype(nt)::value) y = __builtin_nontemporal_load(r);
+                                else y = *r;
+#pragma unroll
+                                for (int d = 0; d < VD; d++) to[4 * x + j][vb][d] = y[d];
                             }
-                        }
+                    }
+                };
+                if (stream) {
+                    asm volatile("");  // keeps the two kinds of load from being merged into one
+                    get(std::true_type());
+                } else {
+                    get(std::false_type());
                 }
                 return;
             }
@@ -1281,10 +1296,10 @@ void launch_attn_paged(const Paged& a0, int cache_type, const void* q, int64_t q
     g.DT = padded(a.D);
     g.groups = 256;
     g.waves = kWaves;
-    // us of a CU: 64 keys x 256 rows of 128 by 8 waves (630 TFLOP/s), 32 keys of 128 (one CU alone draws 48 GB/s)
+    // us of a CU: 64 keys x 256 rows of 128 by 8 waves (630 TFLOP/s), 32 keys of 128 (a CU draws 34 GB/s beside the others)
     const int parts = q_type != BPD_T_F32 ? 1 : cache_type == BPD_T_BF16 ? 3 : 2;
     g.tile_cost = 3.4f * (float)(g.R * g.DT * parts) / (256.f * 128.f) * (g.DT == 256 ? 2.f : 1.f);
-    g.wave_cost = 0.35f * (float)g.DT / 128.f;
+    g.wave_cost = 0.48f * (float)g.DT / 128.f;
     g.planned = planned_way(a.q_start, g.G);
     const Sizes z = sizes(g.planned, a.B, a.T, g.G, a.hkv, g.R, g.DT, a.P);
     uint8_t* at = static_cast<uint8_t*>(ws);
