@@ -191,10 +191,10 @@ __device__ __forceinline__ void join_wave(Max& a) {
     for (int d = 1; d < 64; d <<= 1) join(a, __shfl_xor(a.top, d), __shfl_xor(a.low, d), __shfl_xor(a.n, d));
 }
 
-// ---- max: in every thread
+// ---- max: in every thread, and what the thread itself met
 // (visit(f) calls f(index, logit) for a thread's part of the elements)
 template <int THREADS, typename VISIT>
-__device__ __forceinline__ Max part_max(VISIT&& visit, Max* s_part) {
+__device__ __forceinline__ Max part_max(VISIT&& visit, Max* s_part, float& mine) {
     Max m = {-__builtin_inff(), __builtin_inff(), 0u};
     visit([&](int, float v) {
         const bool is = v > -__builtin_inff();
@@ -202,6 +202,7 @@ __device__ __forceinline__ Max part_max(VISIT&& visit, Max* s_part) {
         m.low = is ? fminf(m.low, v) : m.low;
         m.n += is;
     });
+    mine = m.top;
     join_wave(m);
     if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = m;
     __syncthreads();
@@ -547,10 +548,27 @@ __device__ __forceinline__ void search_row(const SampleArgs& g, int row, const X
     }
 }
 
-// Sorts n values of LDS, falling, by a bitonic network.  Up to 1024 each thread holds one, and partners less than 64
-// apart are asked by shuffles.
-__device__ __forceinline__ void sort_falling(u64* a, int n) {
+// Sorts n different values of LDS, falling.  Up to 256 find their places by counting those above them, four threads
+// each (1.6 us against 2.9); more go through a bitonic network: up to 1024 each thread holds one, and
+// partners less than 64 apart are asked by shuffles.
+__device__ __forceinline__ void sort_falling(u64* a, int n, uint32_t* s_rank) {
     const int tid = (int)threadIdx.x;
+    if (n <= kThreads / 4) {
+        const int e = tid & 255, j0 = (tid >> 8) * ((n + 3) >> 2), j1 = min(n, j0 + ((n + 3) >> 2));
+        if (tid < 256) s_rank[tid] = 0;
+        __syncthreads();
+        const u64 v = e < n ? a[e] : 0;
+        uint32_t rank = 0;
+        if ((e & ~63) < n) {
+#pragma unroll 8
+            for (int j = j0; j < j1; j++) rank += a[j] > v;
+        }
+        if (e < n && rank != 0) atomicAdd(&s_rank[e], rank);
+        __syncthreads();
+        if (tid < n) a[s_rank[tid]] = v;
+        __syncthreads();
+        return;
+    }
     if (n <= kThreads) {
         u64 v = tid < n ? a[tid] : 0;
         for (int k = 2; k < 2 * n; k <<= 1)
@@ -591,6 +609,7 @@ struct DrawLds {
     u64 list[kList];  // (key, ~index), later (~index, key)
     u64 part[kWaves];
     u64 slice[kSlices];
+    uint32_t rank[kThreads / 4];
     u64 before;
     uint32_t n, kept;
     int chosen;
@@ -603,7 +622,7 @@ __device__ __forceinline__ void draw_row(const SampleArgs& g, int row, const X* 
                                          const Pick& pick, const Sum* sums, int S, int len, uint32_t n_list, uint32_t n_stay,
                                          DrawLds& s) {
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    sort_falling(s.list, (int)n_list);  // by logit, equal ones by index
+    sort_falling(s.list, (int)n_list, s.rank);  // by logit, equal ones by index
     // how many of the list stay.  Every loop here is kept rolled: a row's workgroup runs through this code
     // once, and waits for its instructions more than for its data
     const int n_ranked = mode == kTopK ? min((int)n_list, set.k) : (int)n_list;
@@ -637,7 +656,7 @@ __device__ __forceinline__ void draw_row(const SampleArgs& g, int row, const X* 
             s.list[i] = e << 32 | e >> 32;
         }
         __syncthreads();
-        sort_falling(s.list, (int)kept_list);  // ~index falls
+        sort_falling(s.list, (int)kept_list, s.rank);  // ~index falls
         for (int pass = 0; pass < 2; pass++) {  // the total, then the place
             const u64 target = pass == 0 ? 0 : draw_target(set.u, total);
             run0 = 0;
@@ -780,7 +799,8 @@ __global__ __launch_bounds__(kThreads) void k_sample_row(SampleArgs g, int shift
             for (int j = 0; j < N; j++) f((c * kThreads + tid) * N + j, (float)held[c].v[j]);
         }
     };
-    const Max m = part_max<kThreads>(visit, s_max);
+    float mine;
+    const Max m = part_max<kThreads>(visit, s_max, mine);
     const Mode mode = mode_of(set, m);
     if (mode == kNone) {
         if (tid == 0) answer(g, row, -1, __builtin_nanf(""), 0);
@@ -792,7 +812,10 @@ __global__ __launch_bounds__(kThreads) void k_sample_row(SampleArgs g, int shift
     }
     const Row r = row_of(set, m, shift, table);
     if (mode != kSearch) {
-        part_hist(visit, r, mode, hw);
+        // top-k of few: where k threads' largest logits stand, k logits stand, so that these alone are counted (the
+        // histogram of all 32,000: 2.8 us)
+        if (mode == kTopK && 2 * set.k <= min(kThreads, g.V / N)) part_hist([&](auto&& f) { f(0, mine); }, r, mode, hw);
+        else part_hist(visit, r, mode, hw);
         const Pick pick = mode == kTopK ? find_buckets<kThreads>(reinterpret_cast<const uint32_t*>(hw), 0, 1, r, set, mode,
                                                                  reinterpret_cast<uint32_t*>(s_part),
                                                                  reinterpret_cast<uint32_t*>(&s_before), &s_bucket)
@@ -805,10 +828,12 @@ __global__ __launch_bounds__(kThreads) void k_sample_row(SampleArgs g, int shift
             const u64 at = scan_block<kThreads>((u64)n << 32 | (uint32_t)__popc(listed), both, s_part);
             n_stay = (uint32_t)(both >> 32);
             n_list = (uint32_t)both;
-            uint32_t to = (uint32_t)at;
-            for (; listed != 0 && n_list <= (uint32_t)kList; listed &= listed - 1) {
-                const int k = __builtin_ctz(listed), i = (k / N * kThreads + tid) * N + k % N;
-                s.draw.list[to++] = (u64)key_of((float)x[i]) << 32 | (uint32_t)~(uint32_t)i;
+            if (n_list <= (uint32_t)kList && listed != 0) {
+                uint32_t to = (uint32_t)at, bit = 1;
+                visit([&](int i, float v) {
+                    if (listed & bit) s.draw.list[to++] = (u64)key_of(v) << 32 | (uint32_t)~(uint32_t)i;
+                    bit <<= 1;
+                });
             }
         }
         __syncthreads();
@@ -844,7 +869,8 @@ __global__ __launch_bounds__(kSliceThreads) void k_max(SampleArgs g, Work w) {
     const int row = (int)(blockIdx.x / (unsigned)w.S), slice = (int)(blockIdx.x % (unsigned)w.S);
     const int lo = slice * w.len, hi = min(g.V, lo + w.len);
     const X* x = reinterpret_cast<const X*>(g.logits) + (int64_t)row * g.stride;
-    const Max m = part_max<kSliceThreads>([&](auto&& f) { each<X, kSliceThreads>(x, lo, hi, f); }, part);
+    float mine;
+    const Max m = part_max<kSliceThreads>([&](auto&& f) { each<X, kSliceThreads>(x, lo, hi, f); }, part, mine);
     if (threadIdx.x == 0) w.max[blockIdx.x] = m;
 }
 
