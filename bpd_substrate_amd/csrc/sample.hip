@@ -45,14 +45,14 @@ __device__ __forceinline__ void fill_table(double* table) {
 
 struct Row {
     float top;            // the largest logit
-    double per, off;      // log2(e) / temperature, -top times that
+    double max, per;      // top, log2(e) / temperature
     int shift;            // weights are multiples of 2^-shift
     float buckets;        // buckets per unit of logit
     const double* table;  // in LDS
-    // 2^((x - top) per + up) up to some units of 2^-52; 2^(up - 60) for what is less, -infinity and NaN, and for all
-    // but the largest where that is infinite
+    // 2^((x - top) per + up) up to some units of 2^-52, exactly 2^up for the largest; 2^(up - 60) for what is less,
+    // -infinity and NaN, and for all where the largest is infinite
     __device__ __forceinline__ double power(float x, int up) const {
-        const double y = __builtin_fmax(__builtin_fma((double)x, per, off), -60.0);
+        const double y = __builtin_fmax(((double)x - max) * per, -60.0);
         const double magic = 6755399441055744.0 / kTable;  // 1.5 2^52 / 64: leaves y in 64ths in the low bits
         const double t = y + magic, r = y - (t - magic);
         double p = __builtin_fma(r, 1.33335581464284434e-3, 9.61812910762847716e-3);  // ln2^5 / 120, ln2^4 / 24
@@ -64,8 +64,7 @@ struct Row {
         p *= table[k & (kTable - 1)];
         return __longlong_as_double(__double_as_longlong(p) + ((long long)((k >> 6) + up) << 52));
     }
-    // at most 2^44: adding 2^52 rounds to an integer and leaves it in the low bits.  The largest logit's is exactly
-    // 2^shift: its exponent is off by what off rounds to, 2^-53 of it
+    // at most 2^44: adding 2^52 rounds to an integer and leaves it in the low bits
     __device__ __forceinline__ u64 weight(float x) const {
         return (u64)__double_as_longlong(power(x, shift) + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
     }
@@ -76,7 +75,7 @@ struct Row {
     __device__ __forceinline__ bool passes(uint32_t key, float min_p) const {
         const float x = logit_of(key);
         return !(min_p > 0.f) || x == top || (min_p < 1.f && power(x, 0) >= (double)min_p && min_p > 0x1p-59f) ||
-               (min_p <= 0x1p-59f && exp2(__builtin_fma((double)x, per, off)) >= (double)min_p);
+               (min_p <= 0x1p-59f && exp2(((double)x - max) * per) >= (double)min_p);
     }
     // Distance from the largest logit, which is finite, in buckets: does not fall as logits do; NaN only for NaN
     __device__ __forceinline__ float distance(float x) const { return (top - x) * buckets; }
@@ -216,7 +215,7 @@ __device__ __forceinline__ Row row_of(const Set& set, const Max& m, int shift, c
     Row r;
     r.top = m.top;
     r.per = 1.4426950408889634074 / (double)set.t;
-    r.off = -(double)m.top * r.per;
+    r.max = (double)m.top;
     r.shift = shift;
     r.table = table;
     // 32 to a unit of (l - max) / t, which weighs nothing beyond kBuckets of them; a smaller range of logits
@@ -228,7 +227,7 @@ __device__ __forceinline__ Row row_of(const Set& set, const Max& m, int shift, c
 __device__ __forceinline__ Mode mode_of(const Set& s, const Max& m) {
     if (m.n == 0) return kNone;
     if (s.greedy) return kGreedy;
-    if (m.top == __builtin_inff()) return kSearch;
+    if (!(m.top - m.low < __builtin_inff())) return kSearch;  // no distance in binary32, or an infinite largest
     if (s.k > 0 && (uint32_t)s.k < m.n) return s.k > kList ? kSearch : kTopK;
     return kWeights;
 }

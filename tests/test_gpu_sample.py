@@ -85,6 +85,29 @@ def test_special_values(dev, f):
     run(dev, x.to(dev), u, **f)
 
 
+@pytest.mark.parametrize("t", [1e-38, 1e-20, 1e-12, 1e-5, 1e10, 1e38, float("inf")])
+@pytest.mark.parametrize("V", [700, 40000])
+def test_extreme_temperatures(dev, t, V):
+    """Some rows' ranges have no binary32 distance, some temperatures leave the largest logit alone."""
+    x = logits(8, 5, V).clone()
+    x[0] = x[0] * 1e4
+    x[1] = torch.from_numpy(np.linspace(-3e38, 3e38, V))
+    x[2] = x[2] * 1e-30
+    x[3, ::2] = -float("inf")
+    for f in ({}, {"p": 0.9}, {"k": 20, "p": 0.99}, {"m": 0.2}):
+        run(dev, x.to(dev), np.array([0.1, 0.4, 0.5, 0.9, 0.99], np.float32), t=t, **f)
+
+
+@pytest.mark.parametrize("V", [5000, 40000])
+def test_more_equal_logits_than_are_listed(dev, V):
+    x = torch.zeros(4, V)
+    x[1, 7] = 1.0
+    x[2, ::2] = -5.0
+    x[3, V // 2] = 12.0
+    for f in ({"k": 10}, {"p": 0.5}, {"k": 4500, "p": 0.3}, {"m": 0.9}, {"k": 4999, "m": 0.5, "p": 0.9}, {}):
+        run(dev, x.to(dev), np.array([0.2, 0.6, 0.0, 0.97], np.float32), **f)
+
+
 def test_random_numbers_at_the_borders(dev):
     x = torch.zeros(6, 8)
     tok, _, _ = run(dev, x.to(dev), np.array([0.0, 0.125, 0.124999, 0.875, 1 - 2.0 ** -24, 0.5], np.float32))
@@ -145,3 +168,28 @@ def test_sample_captured(dev):
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), i
+
+
+def test_no_rows_and_no_vocabulary(dev):
+    t, lp, k = serve.sample(torch.zeros(0, 10, device=dev), torch.zeros(0, device=dev))
+    assert t.shape == lp.shape == k.shape == (0,)
+    t, lp, k = serve.sample(torch.zeros(3, 0, device=dev), torch.zeros(3, device=dev))
+    assert t.tolist() == [-1] * 3 and k.tolist() == [0] * 3 and lp.isnan().all()
+
+
+@pytest.mark.parametrize("V", [16384, 16385, 32768, 32769, 40000])
+@pytest.mark.parametrize("k", [None, 40, 4096, 4097])
+def test_sizes_where_the_launches_change(dev, V, k):
+    run(dev, logits(V, 3, V).to(dev), np.array([0.1, 0.5, 0.9], np.float32), k=k, p=0.9)
+
+
+def test_equal_largest_threads(dev):
+    """The largest logits all next to each other, so few threads hold them; and every thread's largest equal."""
+    V = 32000
+    x = logits(6, 4, V)
+    x[0, :200] += 30
+    x[1, 31900:] += 30
+    x[2, ::4] = 9.0
+    x[3, ::32] = 9.0
+    for k in (1, 50, 500):
+        run(dev, x.to(dev), np.array([0.1, 0.5, 0.9, 0.99], np.float32), k=k, p=0.95)
