@@ -71,7 +71,7 @@ __device__ __forceinline__ void seq_tokens(const Paged& a, int b, int& t0, int& 
         return;
     }
     t0 = min(max(a.q_start[b], 0), a.T);
-    n = max(min(a.q_start[b + 1], a.T) - t0, 0);
+    n = max(min(max(a.q_start[b + 1], 0), a.T) - t0, 0);
 }
 
 template <int TYPE>

@@ -30,7 +30,7 @@ struct AppendArgs {
 // those rot/2 behind them, later ones pass N elements on; without, unit u is elements
 // [N u, N u + N), turned in pairs below rot.
 template <typename X, typename Y, int N, bool NEOX>
-__device__ __forceinline__ void turn(const X* __restrict__ x, Y* y, int u, int rot, const float2* __restrict__ cs) {
+__device__ __forceinline__ void turn(const X* x, Y* y, int u, int rot, const float2* __restrict__ cs) {
     using VX = Vec<X, N>;
     using VY = Vec<Y, N>;
     if constexpr (NEOX) {
@@ -83,16 +83,17 @@ __global__ __launch_bounds__(256) void k_rope_append(AppendArgs g) {
     __shared__ float2 cs[128];
     const Paged& a = g.a;
     const int t = (int)blockIdx.x;
-    int b = t, idx;
+    int b = t;
+    int64_t index;  // in the sequence's own part
     if (a.q_start != nullptr) {
         b = __builtin_amdgcn_readfirstlane(count_le(a.q_start, a.B + 1, t) - 1);
         if (b < 0 || b >= a.B) return;  // the whole workgroup: the token is no sequence's
-        idx = a.lens[b] - (a.q_start[b + 1] - a.q_start[b]) + (t - a.q_start[b]);
+        index = (int64_t)a.lens[b] - a.q_start[b + 1] + t;
     } else {
-        idx = a.lens[b] - 1;
+        index = (int64_t)a.lens[b] - 1;
     }
     for (int j = (int)threadIdx.x; j < (g.rot >> 1); j += 256) {
-        const double p = g.pos != nullptr ? (double)g.pos[t] : (double)a.P + (double)idx;
+        const double p = g.pos != nullptr ? (double)g.pos[t] : (double)(a.P + index);
         const double r = p * g.turns[j];
         const float f = (float)(2.0 * (r - __builtin_rint(r)));  // half revolutions in [-1, 1]
         float s, c;
@@ -101,9 +102,9 @@ __global__ __launch_bounds__(256) void k_rope_append(AppendArgs g) {
     }
     __syncthreads();
     C *kc = nullptr, *vc = nullptr;
-    if (g.k != nullptr && idx >= 0) {
-        const int pg = fdiv(a.page, idx);
-        const int page = pg < a.W ? a.table[(int64_t)b * a.table_stride + pg] : -1;
+    if (g.k != nullptr && index >= 0 && index < (int64_t)a.W * (int)a.page.d) {
+        const int idx = (int)index, pg = fdiv(a.page, idx);
+        const int page = a.table[(int64_t)b * a.table_stride + pg];
         if (page >= 0 && page < a.n_pages) {
             const int64_t at = (int64_t)page * a.page_stride + (int64_t)(idx - pg * (int)a.page.d) * a.row_stride;
             kc = reinterpret_cast<C*>(a.k) + at;

@@ -33,7 +33,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kKeys = 64;   // keys of a unit
-constexpr int kGroupsMax = 256;  // workgroups that share the units: one per CU
+constexpr int kGroups = 256;  // workgroups that share the units: one per CU
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -__builtin_inff();
 
@@ -1039,20 +1039,21 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs g) {
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int t = (int)blockIdx.x, h0 = ((int)blockIdx.y * 4 + wave) * HW;
     if (h0 >= g.H) return;
-    int b = t, i = 0;
+    int b = t;
     if (a.q_start != nullptr) {
         b = __builtin_amdgcn_readfirstlane(count_le(a.q_start, a.B + 1, t) - 1);
         if (b < 0 || b >= a.B) return;
-        i = t - a.q_start[b];
     }
+    int t0, n;
+    seq_tokens(a, b, t0, n);
+    const int i = t - t0;
+    if (i < 0 || i >= n) return;  // offsets that decrease: the token is not really the sequence's
     int2 wp = make_int2(0, 0), wo = make_int2(0, 0);  // this lane's head: packed results, the sequence's
     int rp = 0, ro = 0;
     bool done = lane >= HW || h0 + lane >= g.H;
     if (!done) {
         const int h = h0 + lane, head = fdiv(g.g, h), gq = h - head * g.G;
         if (g.planned) {
-            int t0, n;
-            seq_tokens(a, b, t0, n);
             const int nitems = g.p.info[0];
             const bool packed = a.P > 0 && !is_joint(g, n);
             const int at = packed ? g.p.place[t] : -1;
@@ -1219,7 +1220,7 @@ Sizes sizes(bool planned, int B, int T, int G, int HKV, int R, int DT, int P) {
     Sizes s = {};
     const int64_t per_rows = (int64_t)T * G / R + 1;
     s.items = planned ? 2 * per_rows + B : P > 0 ? per_rows : 0;
-    const int64_t slots = s.items > 0 ? kGroupsMax + s.items * HKV : 0;
+    const int64_t slots = s.items > 0 ? kGroups + s.items * HKV : 0;
     s.ints = planned ? up16(4 * (4 + (s.items + 1) + 2 * s.items + B + 2 * (int64_t)T)) : 0;
     s.part = slots * R * DT * 4;
     s.ml = up16(slots * R * 8);
@@ -1294,7 +1295,7 @@ void launch_attn_paged(const Paged& a0, int cache_type, const void* q, int64_t q
     g.scale = scale;
     g.R = rows_of(a.D, q_type == BPD_T_F32 ? 2 : 1);
     g.DT = padded(a.D);
-    g.groups = 256;
+    g.groups = kGroups;
     g.waves = kWaves;
     // us of a CU: 64 keys x 256 rows of 128 by 8 waves (630 TFLOP/s), 32 keys of 128 (a CU draws 34 GB/s beside the others)
     const int parts = q_type != BPD_T_F32 ? 1 : cache_type == BPD_T_BF16 ? 3 : 2;

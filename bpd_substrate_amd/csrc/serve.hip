@@ -66,6 +66,7 @@ void check_paged(Args& c, const bpd_paged_cache* kv, const bpd_paged_batch* b) {
     if (!c.ok) return;
     c.shape((int64_t)b->table_width * kv->page_size + b->prefix_len + b->n_tokens < INT_MAX,
             "prefix_len, the table's rows and n_tokens add up to 2^31 or more");
+    c.need(b->n_tokens <= 1 << 23, BPDQ_ERR_LIMIT, "n_tokens is above 2^23");  // a workgroup each
     c.shape(b->q_start != nullptr || b->n_tokens == b->n_seqs, "without q_start n_tokens has to be n_seqs");
     if (!c.ok || b->n_seqs == 0 || b->n_tokens == 0) return;
     if (b->table_width > 0) c.ptr(b->table, 4, "batch.table");
@@ -108,6 +109,36 @@ void* work_space(bpdq::WsLease& lease, void* ws, int64_t ws_bytes, int64_t need,
     return c.ok ? ws : nullptr;
 }
 
+// Whether rows of `row` bytes, n of them `as` and `bs` bytes apart, share a byte.  Rows of one stride may lie
+// between each other.
+bool overlap(const void* a, int64_t as, int64_t arow, const void* b, int64_t bs, int64_t brow, int n) {
+    const int64_t d = (int64_t)(reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a));
+    if (d >= (n - 1) * as + arow || -d >= (n - 1) * bs + brow) return false;
+    if (as != bs) return true;
+    const int64_t at = (d % as + as) % as;  // of b's rows behind a's
+    return at < arow || at + brow > as;
+}
+
+// What the attention's kernels index with 32 bits: heads of a launch, rows of a kv head, units, results.
+void check_attn(Args& c, const bpd_paged_cache& kv, const bpd_paged_batch& b, int n_heads) {
+    c.shape(n_heads >= 1 && n_heads % kv.n_kv_heads == 0, "n_heads is no multiple of n_kv_heads above 0");
+    c.need(n_heads <= 1 << 16, BPDQ_ERR_LIMIT, "n_heads is above 2^16");
+    if (!c.ok) return;
+    const int64_t rows = (int64_t)b.n_tokens * (n_heads / kv.n_kv_heads);
+    c.need(rows <= 1 << 26, BPDQ_ERR_LIMIT, "n_tokens times the heads of a kv head is above 2^26");
+    const int64_t items = 2 * (rows / 64 + 1) + b.n_seqs;  // of 64 rows at least, of 64 keys' units
+    const int64_t units = ((int64_t)b.table_width * kv.page_size + b.prefix_len) / (b.q_start != nullptr ? 64 : 32) + 2;
+    c.need(items <= INT_MAX / units && items <= INT_MAX / 2 / kv.n_kv_heads, BPDQ_ERR_LIMIT,
+           "sequences, tokens and their lengths multiply to 2^31 or more");
+}
+
+void check_sample(Args& c, int n_rows, int vocab) {
+    c.shape(n_rows >= 0, "n_rows is negative").shape(vocab >= 0, "vocab is negative");
+    c.need(vocab <= 1 << 22, BPDQ_ERR_LIMIT, "vocab is above 2^22");
+    // workgroups of a launch: a row's, or its slices' of 2048 logits at least, 16384 where they are many
+    c.need(n_rows < 1 << 22 && (int64_t)n_rows * (vocab / 16384 + 1) < 1 << 22, BPDQ_ERR_LIMIT, "n_rows is too large");
+}
+
 }  // namespace
 
 extern "C" {
@@ -140,6 +171,16 @@ void bpd_rope_append_paged_gpu(const bpd_paged_cache* kv, const bpd_paged_batch*
     if (rot > 0) c.ptr(rope->turns, 8, "rope.turns");
     if (pos != nullptr) c.ptr(pos, 4, "pos");
     if (!c.ok || (n_heads == 0 && k == nullptr)) return;
+    if (n_heads > 0) {
+        const int64_t row = (int64_t)es * n_heads * kv->head_dim, kv_row = (int64_t)es * kv->n_kv_heads * kv->head_dim;
+        c.shape((q == q_out && q_stride == q_out_stride) ||
+                    !overlap(q, es * q_stride, row, q_out, es * q_out_stride, row, b->n_tokens), "q_out overlaps q and is not q");
+        if (k != nullptr)
+            c.shape(!overlap(q_out, es * q_out_stride, row, k, es * k_stride, kv_row, b->n_tokens) &&
+                        !overlap(q_out, es * q_out_stride, row, v, es * v_stride, kv_row, b->n_tokens),
+                    "q_out overlaps k or v");
+        if (!c.ok) return;
+    }
     bpdq::launch_rope_append(paged(*kv, *b), kv->type, rot > 0 ? rope->turns : nullptr, rot,
                              rot > 0 && rope->neox == 1, pos, q, q_stride, k, k_stride, v, v_stride, q_out,
                              q_out_stride, x_type, n_heads, bpdq::abi_stream());
@@ -150,8 +191,7 @@ int64_t bpd_attn_paged_workspace(const bpd_paged_cache* kv, const bpd_paged_batc
     Args c("bpd_attn_paged_workspace");
     check_paged(c, kv, b);
     if (!c.ok) return -1;
-    c.shape(n_heads >= 1 && n_heads % kv->n_kv_heads == 0, "n_heads is no multiple of n_kv_heads above 0");
-    c.shape((int64_t)b->n_tokens * n_heads < INT_MAX, "n_tokens * n_heads is 2^31 or more");
+    check_attn(c, *kv, *b, n_heads);
     if (!c.ok) return -1;
     return bpdq::attn_paged_ws(b->q_start, b->n_seqs, b->n_tokens, n_heads, kv->n_kv_heads, kv->head_dim, b->prefix_len);
 }
@@ -164,13 +204,15 @@ void bpd_attn_paged_gpu(const bpd_paged_cache* kv, const bpd_paged_batch* b, con
     check_paged(c, kv, b);
     if (!c.ok) return;
     c.shape(q_type == BPD_T_F32 || q_type == kv->type, "q_type is neither fp32 nor the cache's type");
-    c.shape(n_heads >= 1 && n_heads % kv->n_kv_heads == 0, "n_heads is no multiple of n_kv_heads above 0");
-    c.shape((int64_t)b->n_tokens * n_heads < INT_MAX, "n_tokens * n_heads is 2^31 or more");
+    check_attn(c, *kv, *b, n_heads);
     if (!c.ok || b->n_seqs == 0 || b->n_tokens == 0) return;
     const int es = esize(q_type);
     const int64_t row = (int64_t)n_heads * kv->head_dim;
     c.ptr(q, 16, "q").stride(q_stride, row, es, "q_stride").ptr(out, 16, "out").stride(out_stride, row, es, "out_stride");
     if (lse != nullptr) c.ptr(lse, 4, "lse");
+    if (!c.ok) return;
+    // rows are written while others are still read
+    c.shape(!overlap(q, es * q_stride, es * row, out, es * out_stride, es * row, b->n_tokens), "q and out overlap");
     if (!c.ok) return;
     bpdq::WsLease lease;
     void* w = work_space(lease, ws, ws_bytes, bpdq::attn_paged_ws(b->q_start, b->n_seqs, b->n_tokens, n_heads, kv->n_kv_heads,
@@ -183,8 +225,7 @@ void bpd_attn_paged_gpu(const bpd_paged_cache* kv, const bpd_paged_batch* b, con
 
 int64_t bpd_sample_workspace(int n_rows, int vocab) {
     Args c("bpd_sample_workspace");
-    c.shape(n_rows >= 0, "n_rows is negative").shape(vocab >= 0, "vocab is negative").need(
-        vocab <= 1 << 22, BPDQ_ERR_LIMIT, "vocab is above 2^22");
+    check_sample(c, n_rows, vocab);
     return c.ok ? bpdq::sample_ws(n_rows, vocab) : -1;
 }
 
@@ -194,8 +235,7 @@ void bpd_sample_gpu(const void* logits, int type, int64_t row_stride, int n_rows
     const char* fn = "bpd_sample_gpu";
     Args c(fn);
     c.shape(type == BPD_T_F32 || type == BPD_T_F16 || type == BPD_T_BF16, "type is unknown");
-    c.shape(n_rows >= 0, "n_rows is negative").shape(vocab >= 0, "vocab is negative");
-    c.need(vocab <= 1 << 22, BPDQ_ERR_LIMIT, "vocab is above 2^22");
+    check_sample(c, n_rows, vocab);
     c.shape(row_stride >= vocab && row_stride <= kMaxStride, "row_stride is shorter than a row, or 2^30 or more");
     if (!c.ok || n_rows == 0) return;
     if (vocab > 0) c.ptr(logits, (uintptr_t)esize(type), "logits");

@@ -81,8 +81,8 @@ typedef struct {
  * [n_tokens]) or NULL: positions other than prefix_len + index.  q [n_tokens]
  * [n_heads][head_dim] and k, v [n_tokens][n_kv_heads][head_dim] of x_type, tokens
  * q_stride, k_stride and v_stride elements apart (the parts of one projection's
- * row, for instance); q_out of x_type, may be q itself; q may be NULL
- * with n_heads 0, k and v NULL together (nothing is appended).  Tensors and token
+ * row, for instance); q_out of x_type, may be q itself and overlaps it or k and v in no
+ * other way; q may be NULL with n_heads 0, k and v NULL together (nothing is appended).  Tensors and token
  * strides 16-byte aligned.  A row that two tokens write (one page in two
  * sequences' tables) holds elements of either. */
 void bpd_rope_append_paged_gpu(const bpd_paged_cache* cache, const bpd_paged_batch* batch, const bpd_rope* rope,
@@ -96,7 +96,10 @@ void bpd_rope_append_paged_gpu(const bpd_paged_cache* cache, const bpd_paged_bat
  * that sees no row gets zeros, and an lse of -infinity.  What stands in rows that a
  * token does not see (infinities and NaN too) does not reach its output.  q and out
  * [n_tokens][n_heads][head_dim] of q_type: the cache's type, or fp32, whose products
- * keep fp32's precision.  Tensors and token strides 16-byte aligned (lse 4).
+ * keep fp32's precision; rows of out and q do not overlap.  Tensors and token strides
+ * 16-byte aligned (lse 4).  n_heads a multiple of n_kv_heads, up to 2^16; n_tokens up to
+ * 2^23, times n_heads / n_kv_heads 2^26; beyond, and where the tokens' tiles times
+ * the table's rows pass 2^31 units, BPDQ_ERR_LIMIT.
  * ws: at least bpd_attn_paged_workspace() bytes, 16-byte aligned, for this call
  * alone until it has run, or NULL: the library's workspace of (device, stream). */
 void bpd_attn_paged_gpu(const bpd_paged_cache* cache, const bpd_paged_batch* batch, const void* q, int64_t q_stride,
@@ -105,8 +108,9 @@ void bpd_attn_paged_gpu(const bpd_paged_cache* cache, const bpd_paged_batch* bat
 int64_t bpd_attn_paged_workspace(const bpd_paged_cache* cache, const bpd_paged_batch* batch, int n_heads);
 
 /* One token per row of logits [n_rows][vocab] (type, rows row_stride elements
- * apart, aligned to an element; vocab up to 2^22, more is BPDQ_ERR_LIMIT).  In order, each over what the one before left, equal
- * logits ranked by index:
+ * apart, aligned to an element; vocab up to 2^22, n_rows and n_rows * vocab / 16384
+ * below 2^22, more is BPDQ_ERR_LIMIT).  In order, each over what the one before left,
+ * equal logits ranked by index:
  *   temperature  weights w_i = exp((l_i - max l) / temperature); not above 0: the
  *                largest logit alone
  *   top_k        the top_k largest; below 1: all

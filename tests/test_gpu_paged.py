@@ -173,6 +173,56 @@ def test_library_workspace_serves_callers_without_one(dev):
     assert torch.equal(out, want)
 
 
+def test_empty_batches_and_a_cache_without_pages(dev):
+    cache = serve.PagedCache.empty(0, 16, 2, 64, device=dev)
+    t = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev)  # noqa: E731
+    out, lse = serve.attention(cache, serve.PagedBatch(t(3, 2), t(3) + 20), torch.ones(3, 4, 64, dtype=torch.float16, device=dev),
+                               return_lse=True)
+    assert (out == 0).all() and (lse == -float("inf")).all()
+    none = serve.PagedBatch(t(0, 2), t(0))
+    assert serve.attention(cache, none, torch.ones(0, 4, 64, dtype=torch.float16, device=dev)).shape == (0, 4, 64)
+    full = serve.PagedCache.empty(2, 16, 2, 64, device=dev)
+    assert serve.attention(full, serve.PagedBatch(t(2, 0), t(2) + 5), torch.ones(2, 4, 64, dtype=torch.float16, device=dev)).sum() == 0
+    ragged = serve.PagedBatch(t(2, 1), t(2), q_start=t(3), n_tokens=4)      # four rows of no sequence
+    o = torch.full((4, 4, 64), 5.0, dtype=torch.float16, device=dev)
+    serve.attention(full, ragged, torch.ones(4, 4, 64, dtype=torch.float16, device=dev), out=o)
+    assert (o == 5.0).all()
+    q = torch.ones(4, 4, 64, dtype=torch.float32, device=dev)
+    o = torch.full((4, 4, 64), 5.0, device=dev)
+    serve.rope_append(full, ragged, q, q[:, :2], q[:, :2], rope=serve.Rope(64, device=dev), q_out=o)
+    assert (o == 5.0).all() and (full.k == 0).all()
+
+
+@pytest.mark.parametrize("q_start", [[0, 40, 8, 60], [60, 30, 10, 0], [-5, 20, -2 ** 31, 2 ** 31 - 1], [7, 2 ** 31 - 1, 3, 5],
+                                     [-2 ** 31, -2 ** 31, 60, 60], [0, 0, 0, 0]])
+@pytest.mark.parametrize("P", [0, 70])
+def test_offsets_that_decrease_stay_inside(dev, q_start, P):
+    """Which rows such a batch writes is open; the guards around out, lse and the cache are not."""
+    b = O.Batch(71, [20, 20, 20], [30, 90, 20], P, 4, 2, 64, "f16", "f16", 16)
+    cache, batch, q = b.device(dev)
+    batch.q_start.copy_(torch.tensor(q_start, dtype=torch.int32))
+    wide = torch.full((62, 4, 64), 7.0, dtype=torch.float16, device=dev)
+    bits = lambda: cache.k.contiguous().view(torch.int16).clone()  # noqa: E731
+    pages, table = bits(), batch.table.clone()
+    serve.attention(cache, batch, q, out=wide[1:61])
+    assert (wide[0] == 7).all() and (wide[61] == 7).all() and torch.equal(bits(), pages)
+    x = torch.randn(60, 2, 64, dtype=torch.float16, device=dev)
+    serve.rope_append(cache, batch, q, x, x, rope=serve.Rope(64, device=dev), q_out=wide[1:61])
+    assert (wide[0] == 7).all() and (wide[61] == 7).all() and torch.equal(batch.table, table)
+
+
+def test_attention_own_keys_beyond_the_last_cache(dev):
+    """Own keys and values of more than 256 MB, as the formula's size goes: they are read past the last-level cache."""
+    check_attention(O.Batch(60, [1] * 9, [8200, 1, 8192, 8191, 33, 0, 8200, 8000, 8100], 40, 8, 8, 128, "f16", "f16", 64,
+                            decode=True), dev)
+
+
+def test_attention_many_heads_and_one_kv_head_of_many(dev):
+    check_attention(O.Batch(57, [1, 1], [70, 3], 40, 64, 64, 64, "f16", "f16", 16, decode=True), dev)
+    check_attention(O.Batch(58, [1, 1], [70, 3], 40, 16, 1, 128, "bf16", "bf16", 16, decode=True), dev)
+    check_attention(O.Batch(59, [2, 1], [70, 3], 40, 130, 1, 64, "f16", "f16", 16), dev)
+
+
 # ---------------------------------------------------------------- append
 
 # new tokens, own rows, prefix, H, HKV, D, x, kv, page, heads_first, padding, rot, neox

@@ -76,12 +76,29 @@ def test_attention_refusals(L):
     for kw, code, text in ((dict(type=2), 2, "q_type"), (dict(H=3), 2, "n_heads"), (dict(H=0), 2, "n_heads"),
                            (dict(q=None), 1, "q is NULL"), (dict(out=0x40008), 3, "out is not 16-byte"),
                            (dict(qs=248), 2, "q_stride is shorter"), (dict(os=260), 3, "out_stride"),
-                           (dict(lse=0x42), 3, "lse"), (dict(n=0), 2, "ws_bytes"), (dict(ws=0x50008), 3, "ws")):
+                           (dict(lse=0x42), 3, "lse"), (dict(n=0), 2, "ws_bytes"), (dict(ws=0x50008), 3, "ws"),
+                           (dict(H=1 << 17), 7, "n_heads is above"), (dict(out=0x30000), 2, "q and out overlap"),
+                           (dict(out=0x30000 + 1008), 2, "overlap"), (dict(out=0x30000 - 1008), 2, "overlap"),
+                           (dict(out=0x30000 + 512, qs=512, os=504), 2, "overlap"),
+                           (dict(out=0x30000 + 496, qs=512, os=512), 2, "overlap"),
+                           (dict(out=0x30000 + 528, qs=512, os=512), 2, "overlap"),
+                           (dict(out=0x30000 + 512, qs=512, os=512, n=0), 2, "ws_bytes"),      # between q's rows
+                           (dict(out=0x30000 + 1024, n=0), 2, "ws_bytes"), (dict(out=0x30000 - 1024, n=0), 2, "ws_bytes")):
         attn(L, cache(), batch(), **kw)
         err(L, code, text)
     assert L.bpd_attn_paged_workspace(ctypes.addressof(cache()), ctypes.addressof(batch()), 3) == -1
     err(L, 2, "n_heads")
     assert L.bpd_attn_paged_workspace(ctypes.addressof(cache()), ctypes.addressof(batch()), 4) > 0
+    many = batch(n_seqs=1 << 20, n_tokens=1 << 20, table_width=1 << 20, table_stride=1 << 20)
+    assert L.bpd_attn_paged_workspace(ctypes.addressof(cache()), ctypes.addressof(many), 4) == -1
+    err(L, 7, "multiply to 2^31")
+    for f, kw in ((attn, dict(out=0x100000000000)), (append, dict(out=0x100000000000))):
+        f(L, cache(), batch(n_seqs=(1 << 23) + 1, n_tokens=(1 << 23) + 1), **kw)
+        err(L, 7, "n_tokens is above 2^23")
+    attn(L, cache(), batch(n_seqs=1 << 22, n_tokens=1 << 22), H=34, qs=2176, os=2176)
+    err(L, 7, "heads of a kv head")
+    assert L.bpd_sample_workspace(1, (1 << 22) + 1) == -1
+    err(L, 7, "2^22")
 
 
 def test_append_refusals(L):
@@ -91,7 +108,11 @@ def test_append_refusals(L):
                                  (None, dict(ks=64), 2, "k_stride is shorter"), (None, dict(vs=130), 3, "v_stride"),
                                  (None, dict(pos=0x3), 3, "pos"), (R(None, 64, 0), {}, 1, "rope.turns"),
                                  (R(0x1000, 65, 0), {}, 2, "rot_dim"), (R(0x1000, 128, 0), {}, 2, "rot_dim"),
-                                 (R(0x1000, 64, 2), {}, 2, "neox"), (R(0x1004, 64, 1), {}, 3, "rope.turns")):
+                                 (R(0x1000, 64, 2), {}, 2, "neox"), (R(0x1004, 64, 1), {}, 3, "rope.turns"),
+                                 (None, dict(out=0x30010), 2, "q_out overlaps q"),
+                                 (None, dict(out=0x30000, os=512), 2, "q_out overlaps q"),
+                                 (None, dict(out=0x60000 - 1024), 2, "q_out overlaps k"),
+                                 (None, dict(out=0x70000 + 512), 2, "q_out overlaps k or v")):
         append(L, cache(), batch(), rope, **kw)
         err(L, code, text)
 
@@ -102,7 +123,8 @@ def test_sample_refusals(L):
     for kw, code, text in ((dict(type=5), 2, "type"), (dict(B=-1), 2, "n_rows"), (dict(V=-1), 2, "vocab"),
                            (dict(stride=99), 2, "row_stride"), (dict(x=None), 1, "logits"), (dict(x=0x1002), 3, "logits"),
                            (dict(u=None), 1, "u is NULL"), (dict(tok=0x3001), 3, "token"), (dict(t=0x3), 3, "temperature"),
-                           (dict(n=0), 2, "ws_bytes")):
+                           (dict(n=0), 2, "ws_bytes"), (dict(V=(1 << 22) + 1, stride=1 << 23), 7, "2^22"),
+                           (dict(B=1 << 22), 7, "n_rows"), (dict(B=1 << 14, V=1 << 22, stride=1 << 22), 7, "n_rows")):
         call(**kw)
         err(L, code, text)
 
