@@ -693,51 +693,60 @@ __device__ __forceinline__ void draw_row(const SampleArgs& g, int row, const X* 
         }
     }
     __syncthreads();
-    // the place in the slice: by the waves' parts of it, then 64 at a time
+    // the place in the slice: a thread weighs some elements in a row, then a wave those of the thread that it falls to
     const u64 target = draw_target(set.u, total);
-    const int lo = s.chosen * len, hi = min(g.V, lo + len), seg = (min(len, g.V) + kWaves * 64 - 1) / (kWaves * 64) * 64;
-    const int wlo = lo + wave * seg, whi = min(hi, wlo + seg);
+    constexpr int N = 16 / (int)sizeof(X);
+    const int lo = s.chosen * len, hi = min(g.V, lo + len);
+    const int per = (min(len, g.V) + 8 * kThreads - 1) / (8 * kThreads) * 8;  // 32 at most
     const float first = (float)pick.first;
     auto weight_at = [&](float f, int i) -> u64 {
         const bool in = r.distance(f) < first || (cut != 0 && ((u64)key_of(f) << 32 | (uint32_t)~(uint32_t)i) >= cut);
         return in ? r.weight(f) : 0;
     };
+    const bool aligned = ((uintptr_t)(x + lo) & 15) == 0;
+    const int a0 = lo + tid * per;
     u64 mine = 0;
 #pragma unroll 1
-    for (int i0 = wlo + lane; i0 < whi; i0 += 8 * 64) {
-        float f[8];
+    for (int i0 = a0; i0 < min(hi, a0 + per); i0 += 16) {
+        Vec<X, N> v[16 / N];
 #pragma unroll
-        for (int j = 0; j < 8; j++) f[j] = i0 + 64 * j < whi ? (float)x[i0 + 64 * j] : -__builtin_inff();
+        for (int c = 0; c < 16 / N; c++) {
+            const int i = i0 + c * N, end = min(hi, a0 + per);
+            if (aligned && i + N <= end) {
+                v[c] = *reinterpret_cast<const Vec<X, N>*>(x + i);
+            } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const u64 v = weight_at(f[j], i0 + 64 * j);
-            mine += v;
+                for (int j = 0; j < N; j++) v[c].v[j] = i + j < end ? x[i + j] : (X)-__builtin_inff();
+            }
         }
+#pragma unroll
+        for (int c = 0; c < 16 / N; c++)
+#pragma unroll
+            for (int j = 0; j < N; j++) mine += weight_at((float)v[c].v[j], i0 + c * N + j);
     }
-    mine = wave_sum(mine);
+    auto up_to = [&](u64 sum) {  // over the lanes up to this one
+        for (int d = 1; d < 64; d <<= 1) {
+            const u64 o = __shfl_up(sum, d);
+            if (lane >= d) sum += o;
+        }
+        return sum;
+    };
+    const u64 run = up_to(mine);
     __syncthreads();
-    if (lane == 0) s.part[wave] = mine;
+    if (lane == 63) s.part[wave] = run;
     __syncthreads();
     u64 before = s.before;
     int chosen = 0;
     for (; chosen < kWaves - 1 && before + s.part[chosen] <= target; chosen++) before += s.part[chosen];
     if (wave != chosen) return;
-#pragma unroll 1
-    for (int i0 = wlo; i0 < whi; i0 += 64) {
-        const int i = i0 + lane;
-        const u64 v = i < whi ? weight_at((float)x[i], i) : 0;
-        u64 sum = v;
-        for (int d = 1; d < 64; d <<= 1) {
-            const u64 o = __shfl_up(sum, d);
-            if (lane >= d) sum += o;
-        }
-        const uint64_t over = __ballot(before + sum > target);
-        if (over != 0) {
-            if (lane == __builtin_ctzll(over)) answer(g, row, i, (float)log((double)v / (double)total), kept);
-            return;
-        }
-        before += __shfl(sum, 63);
-    }
+    const uint64_t past = __ballot(before + run > target);
+    if (past == 0) return;
+    const int who = __builtin_ctzll(past);
+    before += __shfl(run - mine, who);
+    const int i = lo + (wave * 64 + who) * per + lane;
+    const u64 v = lane < per && i < hi ? weight_at((float)x[i], i) : 0;
+    const uint64_t over = __ballot(before + up_to(v) > target);
+    if (over != 0 && lane == __builtin_ctzll(over)) answer(g, row, i, (float)log((double)v / (double)total), kept);
 }
 
 // The first index of the largest logit, which [lo, hi) holds.
