@@ -5,19 +5,32 @@
 //
 // in one pass over the keys: a row of a query head keeps a reference exponent r (base 2), its
 // sum l = sum 2^(s - r) and O = sum 2^(s - r) v in fp32.  Where a later part of the
-// keys has another reference, sums join as O 2^(r - r') + O' (k_attn_join).
+// keys has another reference, sums join as O 2^(r - r') + O' (k_attn_join).  Weights are rounded
+// to the cache's type for their product with v, as the matrix instructions take them (half a step each, relative to
+// the weight; with an fp32 q two or three parts keep 22 or 24 bits); l sums them unrounded.
 //
 // Work.  The query heads of one kv head share its keys, so a row is a (token, query head)
-// pair and a tile is R rows of one kv head against 64 keys at a time.  An item is a tile's
-// rows with all their keys:
+// pair.  Two kernels take the keys:
+//   - k_attn_tile: R rows against 64 keys at a time, through LDS.  The matrix units bound it.
+//   - k_attn_wave, for sequences with one new token and up to 16 heads on a kv head: a wave by itself
+//     streams a sequence's keys past one 16-row tile.  Memory bounds it.
+// With one token each (q_start NULL) the tokens' rows are packed against the prefix, which is so
+// read once for R / (heads per kv head) sequences, and the own keys are k_attn_wave's; k_attn_both runs the two
+// side by side.  Otherwise k_attn_plan lays out items, tile rows with all their keys, on the device, as the lengths are
+// there:
 //   - own items: the rows of one sequence against its own keys, causal, and where a
 //     sequence fills half a tile by itself, the prefix before them;
-//   - packed items: the rows of all other sequences together against the prefix, which is so
-//     read once for R / (heads per kv head) sequences.
-// Units of 64 keys, item by item, are dealt evenly to the workgroups, whose number does
-// not depend on the batch: a workgroup runs through its units, and where an item ends in the
-// middle leaves its O, r and l for k_attn_join, in a place of its own.  The plan (k_attn_plan) is
-// made on the device, as the lengths are there.
+//   - packed items: the rows of all other sequences together against the prefix.
+// Units of 64 keys (32 of k_attn_wave's), item by item, are dealt evenly to the workgroups, whose number
+// does not depend on the batch: a workgroup runs through its units, and where an item ends in
+// the middle leaves its O, r and l for k_attn_join, in a place of its own.
+//
+// Measured, bf16 unless said (H 32, 8 kv heads, D 128; calls back to back):
+//   8 chunks of 512 tokens over 4096 + up to 1024 keys    333 us   705 TFLOP/s (a 8192^3 product: 1256)
+//   32 sequences of up to 8192 own keys, 670 MB           113 us   5.9 TB/s (reads alone: 6.8)
+//   256 sequences behind 32,768 shared keys, 1024 own     243 us   140 GFLOP and 781 MB: 112 + 115 us
+//   64 sequences (f16) behind 8192 shared keys, 600 own    44 us   9 GFLOP and 130 MB: 14 + 19 us
+//   1 sequence of 300 keys, D 64                           14 us   two launches
 #include <type_traits>
 
 #include "bpdq_paged.h"
@@ -94,7 +107,7 @@ __device__ __forceinline__ int seen_rows(const Paged& a, int b, int n, int i, in
     return (int)(s < 0 ? 0 : s > own ? own : s);
 }
 
-// One workgroup lays out the items.  Sequences are taken 1024 at a time, a thread each, then their tiles
+// One workgroup lays out the items (6 us for 8 sequences of 512 tokens beside 330 us that follow: latency).  Sequences are taken 1024 at a time, a thread each, then their tiles
 // and tokens, a thread each.
 __global__ __launch_bounds__(1024) void k_attn_plan(AttnArgs g) {
     constexpr int N = 1024;
@@ -362,6 +375,11 @@ __device__ __forceinline__ u32x2 read_tr(const uint8_t* p) {
 // lane group g.  V's operand comes in that order from two transposing reads; row c of it is
 // element 16 e + c of the head in product e.
 // UNI: pages hold multiples of 16 rows, so the rows that a wave's lanes move at a time share a page.
+//
+// 8 waves of 32 rows: a half's K operands serve both row tiles of a wave, and 256 rows share what a unit brings to
+// LDS.  What bounds it at 705 TFLOP/s: a SIMD's two waves are both in their softmax for part of the time (matrix units
+// busy 33 % of the clocks, VALU 45 %).  Measured and left: K of the next half read behind P V (338 us against 334),
+// wave priorities around the products (no change).
 template <int QT, int CT, int NS, int DT, int MT, int NW, bool UNI>
 __device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w, int groups) {
     using M = Mfma<CT>;
@@ -703,6 +721,7 @@ __device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w,
 // its own: no barrier.  The shares of all waves are dealt as k_attn_tile's, in units of 32 keys.
 // UNI: pages hold multiples of 16 rows, which span less than 2^32 bytes, so the 16 rows of a score tile share
 // a page, its lookup and the high half of their addresses.
+// One read of every key and value: 5.9 TB/s for 670 MB, two units of loads in flight in each of 2048 waves.
 template <int QT, int CT, int NS, int DT, bool UNI>
 __device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT / 8], int w, int waves, int UH) {
     using M = Mfma<CT>;
@@ -1009,7 +1028,7 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_wave(AttnArgs g
 
 // One token per sequence behind a prefix: x of the workgroups take the prefix's tiles, which the matrix
 // units bound, the others the sequences' own keys, which memory bounds, at the same time.  x by
-// the time that a unit of each takes a CU: kTileCost (64 keys x R rows) against kWaveCost (32 keys x 16).
+// the time that a unit of each takes a CU: tile_cost (64 keys x R rows) against wave_cost (32 keys x 16).
 template <int QT, int CT, int NS, int DT, int MT, int NW, bool UNI>
 __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_both(AttnArgs g) {
     __shared__ union {
@@ -1032,6 +1051,7 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_both(AttnAr
 
 // Joins what was left of each (token, query head): its packed results, then its sequence's.  A
 // workgroup takes a token and HW heads for each of its 4 waves; a lane looks up one of the wave's heads.
+// Three dependent lookups and the results bound it: 8 us at 64 tokens of 32 heads, 12 at 256, 21 at 4096.
 template <int QT, int HW>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs g) {
     using Q = typename Elem<QT>::type;

@@ -14,6 +14,11 @@
 // k_sample_row takes them in turn with one workgroup for a row; k_max, k_hist and k_pick with one per
 // slice of a row, and k_cut and k_draw with one per row.  A row whose list is too long (thousands of equal
 // logits at the cut) is searched digit by digit instead.
+//
+// Measured (calls back to back): 1 row of 32,000, top-k and top-p, 18 us, one launch, latency; 64 rows of 128,256 (fp32,
+// mixed settings) 55 us; 256 rows of 128,256 (binary16, top-p) 97 us: max 16 (66 MB at 4.2 TB/s), hist 34 (21 vector
+// instructions and two LDS operations a logit), cut 8, pick 22, draw 25 (latency of a workgroup).  Left: a slice's first loads
+// ahead of its row's settings (their registers cost a workgroup of four per CU: hist 34 -> 37 us).
 #include "bpdq_paged.h"
 
 namespace bpdq {
@@ -25,7 +30,6 @@ constexpr int kRow = 32768;  // elements of a row that its workgroup holds in re
 constexpr int kSliceThreads = 512;
 constexpr int kBuckets = 1024;
 constexpr int kList = 4096;  // entries of a list that is sorted
-constexpr int kTable = 64;
 constexpr int kSlices = 256;  // at most: vocab up to 2^22
 typedef unsigned long long u64;
 
@@ -38,35 +42,41 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
     return __uint_as_float((key >> 31) ? key & 0x7FFFFFFFu : ~key);
 }
 
-// 2^(i / 64), for exp by table and polynomial (Tang 1989): 2^y = 2^e 2^(i/64) 2^r, y = e + i/64 + r.
-__device__ __forceinline__ void fill_table(double* table) {
-    if (threadIdx.x < kTable) table[threadIdx.x] = exp2((double)threadIdx.x / kTable);
-}
-
+// Buckets and weights go by the distance from the largest logit, d = (max - l) scale in binary64, b = d rounded:
+//   exp((l - max) / t) = exp(-b c) exp(-(d - b) c),  c = 1 / (scale t) <= 1 / 32,
+// the first from a table of the buckets (2^shift times it), the second by 6 terms of its series: 2^-54 of it is left out.
 struct Row {
     float top;            // the largest logit
-    double max, per;      // top, log2(e) / temperature
+    double max, scale;    // top, buckets per unit of logit
+    double k[6];          // (-c)^j / j!
+    double c, t;
     int shift;            // weights are multiples of 2^-shift
-    float buckets;        // buckets per unit of logit
-    const double* table;  // in LDS
-    // 2^((x - top) per + up) up to some units of 2^-52, exactly 2^up for the largest; 2^(up - 60) for what is less,
-    // -infinity and NaN, and for all where the largest is infinite
-    __device__ __forceinline__ double power(float x, int up) const {
-        const double y = __builtin_fmax(((double)x - max) * per, -60.0);
-        const double magic = 6755399441055744.0 / kTable;  // 1.5 2^52 / 64: leaves y in 64ths in the low bits
-        const double t = y + magic, r = y - (t - magic);
-        double p = __builtin_fma(r, 1.33335581464284434e-3, 9.61812910762847716e-3);  // ln2^5 / 120, ln2^4 / 24
-        p = __builtin_fma(r, p, 5.55041086648215800e-2);
-        p = __builtin_fma(r, p, 2.40226506959100712e-1);
-        p = __builtin_fma(r, p, 6.93147180559945309e-1);
+    const double* table;  // in LDS, kBuckets of them
+    // x up to max.  Grows as logits fall, up to the last bucket's, where only logits are that weigh nothing, -infinity and NaN
+    __device__ __forceinline__ double distance(double x) const { return __builtin_fmin((max - x) * scale, kBuckets - 0.6); }
+    __device__ __forceinline__ int bucket(double x) const {
+        return (int)(uint32_t)__double_as_longlong(distance(x) + 6755399441055744.0);  // 1.5 2^52: rounds, low bits
+    }
+    // 2^shift exp((x - top) / t) up to some units of 2^-52 of it, exactly 2^shift for the largest logit; 0 in
+    // the last bucket
+    __device__ __forceinline__ double power(float x, int& b) const {
+        const double magic = 6755399441055744.0, d = distance((double)x), to = d + magic, r = d - (to - magic);
+        b = (int)(uint32_t)__double_as_longlong(to);
+        double p = __builtin_fma(r, k[5], k[4]);
+        p = __builtin_fma(r, p, k[3]);
+        p = __builtin_fma(r, p, k[2]);
+        p = __builtin_fma(r, p, k[1]);
+        p = __builtin_fma(r, p, k[0]);
         p = __builtin_fma(r, p, 1.0);
-        const int k = (int)(uint32_t)__double_as_longlong(t);
-        p *= table[k & (kTable - 1)];
-        return __longlong_as_double(__double_as_longlong(p) + ((long long)((k >> 6) + up) << 52));
+        return p * table[b];
     }
     // at most 2^44: adding 2^52 rounds to an integer and leaves it in the low bits
+    __device__ __forceinline__ u64 weight(float x, int& b) const {
+        return (u64)__double_as_longlong(power(x, b) + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+    }
     __device__ __forceinline__ u64 weight(float x) const {
-        return (u64)__double_as_longlong(power(x, shift) + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+        int b;
+        return weight(x, b);
     }
     // where the largest may be infinite
     __device__ __forceinline__ u64 weight_of(uint32_t key) const {
@@ -74,12 +84,17 @@ struct Row {
     }
     __device__ __forceinline__ bool passes(uint32_t key, float min_p) const {
         const float x = logit_of(key);
-        return !(min_p > 0.f) || x == top || (min_p < 1.f && power(x, 0) >= (double)min_p && min_p > 0x1p-59f) ||
-               (min_p <= 0x1p-59f && exp2(((double)x - max) * per) >= (double)min_p);
+        if (!(min_p > 0.f) || x == top) return true;
+        if (!(min_p < 1.f)) return false;
+        if (!(min_p > 0x1p-45f)) return exp(((double)x - max) / t) >= (double)min_p;  // beyond the table
+        int b;
+        return power(x, b) >= (double)min_p * (double)(1ull << shift);
     }
-    // Distance from the largest logit, which is finite, in buckets: does not fall as logits do; NaN only for NaN
-    __device__ __forceinline__ float distance(float x) const { return (top - x) * buckets; }
-    __device__ __forceinline__ int bucket(float x) const { return (int)fminf(distance(x), (float)(kBuckets - 1)); }
+    template <int THREADS>
+    __device__ __forceinline__ void fill(double* to) const {
+        for (int b = (int)threadIdx.x; b < kBuckets; b += THREADS)
+            to[b] = b < kBuckets - 1 ? exp(-(double)b * c) * (double)(1ull << shift) : 0.0;
+    }
 };
 
 template <typename T>
@@ -139,10 +154,12 @@ struct Sum {
     u64 w;
     uint32_t n, list;
 };
-// The buckets [0, first) stay, [first, last] are listed; top-p: weight to be reached within the list.
+// The buckets [0, first) stay, logits from x1 on; those below from x2 on are listed; top-p: weight to be reached
+// within the list.
 struct Pick {
     u64 want;
-    int first, last;
+    int first;
+    float x1, x2;
 };
 struct Work {
     int S, len;  // slices, elements of one
@@ -160,6 +177,18 @@ template <typename X, int THREADS, typename F>
 __device__ __forceinline__ void each(const X* __restrict__ x, int lo, int hi, F&& f) {
     constexpr int N = 16 / (int)sizeof(X), STEP = THREADS * N;
     const bool aligned = ((uintptr_t)(x + lo) & 15) == 0;
+    if (aligned && (hi - lo) % (4 * STEP) == 0) {  // nothing to check
+        for (int i0 = lo; i0 < hi; i0 += 4 * STEP) {
+            Vec<X, N> v[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) v[c] = *reinterpret_cast<const Vec<X, N>*>(x + i0 + c * STEP + (int)threadIdx.x * N);
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+#pragma unroll
+                for (int j = 0; j < N; j++) f(i0 + c * STEP + (int)threadIdx.x * N + j, (float)v[c].v[j]);
+        }
+        return;
+    }
     for (int i0 = lo + (int)threadIdx.x * N; i0 < hi; i0 += 4 * STEP) {
         Vec<X, N> v[4];
 #pragma unroll
@@ -214,20 +243,27 @@ __device__ __forceinline__ Max part_max(VISIT&& visit, Max* s_part, float& mine)
 __device__ __forceinline__ Row row_of(const Set& set, const Max& m, int shift, const double* table) {
     Row r;
     r.top = m.top;
-    r.per = 1.4426950408889634074 / (double)set.t;
     r.max = (double)m.top;
+    r.t = (double)set.t;
+    // 32 to a unit of (l - max) / t, which weighs nothing beyond kBuckets of them; a smaller range of logits
+    // is cut finer, up to the bucket before the last
+    r.scale = __builtin_fmin(__builtin_fmax(32.0 / r.t, (kBuckets - 2) / (r.max - (double)m.low)), 1e300);
+    r.c = __builtin_fmin(1.0 / (r.scale * r.t), 1.0 / 32);
+    r.k[0] = -r.c;
+    r.k[1] = r.c * r.c * (1.0 / 2);
+    r.k[2] = r.k[1] * r.c * (-1.0 / 3);
+    r.k[3] = r.k[2] * r.c * (-1.0 / 4);
+    r.k[4] = r.k[3] * r.c * (-1.0 / 5);
+    r.k[5] = r.k[4] * r.c * (-1.0 / 6);
     r.shift = shift;
     r.table = table;
-    // 32 to a unit of (l - max) / t, which weighs nothing beyond kBuckets of them; a smaller range of logits
-    // is cut finer
-    r.buckets = fminf(fmaxf(32.f / set.t, 0.999f * (float)kBuckets / (m.top - m.low)), 1e30f);
     return r;
 }
 
 __device__ __forceinline__ Mode mode_of(const Set& s, const Max& m) {
     if (m.n == 0) return kNone;
     if (s.greedy) return kGreedy;
-    if (!(m.top - m.low < __builtin_inff())) return kSearch;  // no distance in binary32, or an infinite largest
+    if (m.top == __builtin_inff()) return kSearch;
     if (s.k > 0 && (uint32_t)s.k < m.n) return s.k > kList ? kSearch : kTopK;
     return kWeights;
 }
@@ -239,13 +275,14 @@ __device__ __forceinline__ void part_hist(VISIT&& visit, const Row& r, Mode mode
         uint32_t* hc = reinterpret_cast<uint32_t*>(hw);
         visit([&](int, float v) {
             // the last bucket's are what the others leave, and not asked for
-            const float d = r.distance(v);
-            if (d < (float)(kBuckets - 1)) atomicAdd(&hc[(int)d], 1u);
+            const int b = r.bucket((double)v);
+            if (b < kBuckets - 1) atomicAdd(&hc[b], 1u);
         });
     } else {
         visit([&](int, float v) {  // in the last bucket few weigh anything
-            const u64 w = r.weight(v);
-            if (w != 0) atomicAdd(&hw[r.bucket(v)], w);
+            int b;
+            const u64 w = r.weight(v, b);
+            if (w != 0) atomicAdd(&hw[b], w);
         });
     }
     __syncthreads();
@@ -258,67 +295,75 @@ __device__ __forceinline__ u64 reach(float p, u64 total) {
     return want == 0 ? 1 : want;
 }
 
-// ---- pick, first half: which buckets, from the row's histogram of S slices, `stride` apart (of T); every thread
-template <int THREADS, typename T>
+// The smallest finite logit in the buckets before `end`, 1 or more; the lowest of all at kBuckets.  The whole wave.
+__device__ __forceinline__ float lowest_before(const Row& r, int end) {
+    constexpr uint32_t kLowest = 0x00800000u;  // the key of -FLT_MAX
+    uint32_t lo = kLowest - 1, hi = end < kBuckets ? key_of(r.top) : kLowest;  // in (lo, hi]
+    while (hi - lo > 1) {
+        const uint32_t step = (hi - lo + 63) >> 6, k = lo + (((uint32_t)threadIdx.x & 63) + 1) * step;
+        const int l = __builtin_ctzll(__ballot(k >= hi || r.bucket((double)logit_of(k)) < end));  // the last lane's is
+        hi = min(hi, lo + (uint32_t)(l + 1) * step);
+        lo += (uint32_t)l * step;
+    }
+    return logit_of(hi);
+}
+
+// ---- pick, first half: which logits, from the row's histogram of S slices, `stride` apart (of T); every thread
+template <typename T>
+struct FindLds {
+    T part[kWaves], before;
+    int bucket;
+    float x[2];
+};
+template <typename T>
 __device__ __forceinline__ Pick find_buckets(const T* hist, int stride, int S, const Row& r, const Set& set, Mode mode,
-                                             T* s_part, T* s_before, int* s_bucket) {
-    constexpr int PER = kBuckets / THREADS;
+                                             FindLds<T>& s) {
+    static_assert(kBuckets == kThreads, "a thread for each");
     const int tid = (int)threadIdx.x;
-    T v[PER], mine = 0, total;
-#pragma unroll
-    for (int j = 0; j < PER; j++) v[j] = 0;
+    T v = 0, total;
 #pragma unroll 8
-    for (int s = 0; s < S; s++)
-#pragma unroll
-        for (int j = 0; j < PER; j++) v[j] += hist[(int64_t)s * stride + tid * PER + j];
-#pragma unroll
-    for (int j = 0; j < PER; j++) mine += v[j];
-    if (tid == 0) *s_bucket = kBuckets - 1;
-    const T before = scan_block<THREADS>(mine, total, s_part);
+    for (int i = 0; i < S; i++) v += hist[(int64_t)i * stride + tid];
+    if (tid == 0) s.bucket = kBuckets - 1;
+    const T before = scan_block<kThreads>(v, total, s.part);
     const bool by_p = mode == kWeights && set.p < 1.f;
     const T need = mode == kTopK ? (T)set.k : by_p ? (T)reach(set.p, (u64)total) : 0;
-    T at = before;
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-        if (at < need && at + v[j] >= need) *s_bucket = tid * PER + j;  // one thread's one bucket, or none's
-        at += v[j];
+    if (before < need && before + v >= need) s.bucket = tid;  // one thread, or none
+    __syncthreads();
+    Pick p = {~0ull, 0, __builtin_inff(), 0.f};
+    int last = s.bucket;
+    if (mode != kTopK) {
+        p.first = last = by_p ? last : kBuckets;
+        if (set.m > 0.f) {
+            // min-p's own cut lies between the logits x + off and x - off
+            const double x = r.max + log((double)fminf(set.m, 1.f)) * r.t;
+            const double off = 1e-6 * (__builtin_fabs(r.max) + __builtin_fabs(x)) + 1e-30;
+            p.first = min(p.first, r.bucket(__builtin_fmin(x + off, r.max)));
+            last = min(last, r.bucket(x - off));
+        }
+        if (by_p && tid == p.first) s.before = before;
+    }
+    if (tid < 128) {
+        const int end = __builtin_amdgcn_readfirstlane(tid < 64 ? p.first : last < kBuckets - 1 ? last + 1 : kBuckets);
+        const float x = end > 0 ? lowest_before(r, end) : __builtin_inff();
+        if ((tid & 63) == 0) s.x[tid >> 6] = x;
     }
     __syncthreads();
-    Pick p = {~0ull, 0, *s_bucket};
-    if (mode == kTopK) return p;
-    p.first = p.last = by_p ? p.last : kBuckets;
-    if (set.m > 0.f) {
-        // min-p's own cut lies between the logits hi and lo
-        const double x = (double)r.top + log((double)fminf(set.m, 1.f)) * (double)set.t;
-        const double off = 1e-6 * (__builtin_fabs((double)r.top) + __builtin_fabs(x)) + 1e-30;
-        p.first = min(p.first, max(r.bucket((float)(x + off)), 0));
-        p.last = min(p.last, max(r.bucket((float)(x - off)), 0));
-    }
-    if (by_p) {
-        at = before;
-#pragma unroll
-        for (int j = 0; j < PER; j++) {
-            if (tid * PER + j == p.first) *s_before = at;
-            at += v[j];
-        }
-        __syncthreads();
-        p.want = (u64)need - (u64)*s_before;
-    }
+    p.x1 = s.x[0];
+    p.x2 = s.x[1];
+    if (by_p) p.want = (u64)need - (u64)s.before;
     return p;
 }
 
 // ---- pick, second half: bit k of `listed` for the k-th element that visit shows the thread, 32 at most; returns
 // how many stay, by thread
 template <typename VISIT>
-__device__ __forceinline__ uint32_t part_pick(VISIT&& visit, const Row& r, const Pick& p, uint32_t& listed) {
-    const float first = (float)p.first, last = p.last < kBuckets - 1 ? (float)(p.last + 1) : __builtin_inff();
+__device__ __forceinline__ uint32_t part_pick(VISIT&& visit, const Pick& p, uint32_t& listed) {
     uint32_t n = 0, bit = 1;
     listed = 0;
     visit([&](int, float v) {
-        const float d = r.distance(v);
-        const bool stays = d < first;
+        const bool stays = v >= p.x1;
         n += stays;
-        if (!stays && (d < last || (last > (float)kBuckets && v > -__builtin_inff()))) listed |= bit;
+        listed |= v >= p.x2 && !stays ? bit : 0u;
         bit <<= 1;
     });
     return n;
@@ -698,9 +743,8 @@ __device__ __forceinline__ void draw_row(const SampleArgs& g, int row, const X* 
     constexpr int N = 16 / (int)sizeof(X);
     const int lo = s.chosen * len, hi = min(g.V, lo + len);
     const int per = (min(len, g.V) + 8 * kThreads - 1) / (8 * kThreads) * 8;  // 32 at most
-    const float first = (float)pick.first;
     auto weight_at = [&](float f, int i) -> u64 {
-        const bool in = r.distance(f) < first || (cut != 0 && ((u64)key_of(f) << 32 | (uint32_t)~(uint32_t)i) >= cut);
+        const bool in = f >= pick.x1 || (cut != 0 && ((u64)key_of(f) << 32 | (uint32_t)~(uint32_t)i) >= cut);
         return in ? r.weight(f) : 0;
     };
     const bool aligned = ((uintptr_t)(x + lo) & 15) == 0;
@@ -772,17 +816,19 @@ union RowLds {
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void k_sample_row(SampleArgs g, int shift) {
     using X = typename Elem<TYPE>::type;
-    __shared__ double table[kTable];
+    __shared__ double table[kBuckets];
     __shared__ u64 hw[kBuckets];
     __shared__ Max s_max[kWaves];
-    __shared__ u64 s_part[kWaves], s_before;
-    __shared__ int s_bucket;
+    __shared__ u64 s_part[kWaves];
+    __shared__ union {
+        FindLds<u64> w;
+        FindLds<uint32_t> n;
+    } s_find;
     __shared__ Sum s_sum;
     __shared__ RowLds s;
     const int row = (int)blockIdx.x, tid = (int)threadIdx.x;
     const Set set = settings(g, row);
     const X* x = reinterpret_cast<const X*>(g.logits) + (int64_t)row * g.stride;
-    fill_table(table);
     hw[tid] = 0;
     if (tid == 0) s.draw.n = s.draw.kept = 0;
     // the row's kRow elements at most stay in registers
@@ -819,19 +865,19 @@ __global__ __launch_bounds__(kThreads) void k_sample_row(SampleArgs g, int shift
         return;
     }
     const Row r = row_of(set, m, shift, table);
+    r.fill<kThreads>(table);
+    __syncthreads();
     if (mode != kSearch) {
         // top-k of few: where k threads' largest logits stand, k logits stand, so that these alone are counted (the
         // histogram of all 32,000: 2.8 us)
         if (mode == kTopK && 2 * set.k <= min(kThreads, g.V / N)) part_hist([&](auto&& f) { f(0, mine); }, r, mode, hw);
         else part_hist(visit, r, mode, hw);
-        const Pick pick = mode == kTopK ? find_buckets<kThreads>(reinterpret_cast<const uint32_t*>(hw), 0, 1, r, set, mode,
-                                                                 reinterpret_cast<uint32_t*>(s_part),
-                                                                 reinterpret_cast<uint32_t*>(&s_before), &s_bucket)
-                                        : find_buckets<kThreads>(hw, 0, 1, r, set, mode, s_part, &s_before, &s_bucket);
+        const Pick pick = mode == kTopK ? find_buckets(reinterpret_cast<const uint32_t*>(hw), 0, 1, r, set, mode, s_find.n)
+                                        : find_buckets(hw, 0, 1, r, set, mode, s_find.w);
         uint32_t n_stay = m.n, n_list = 0;
         if (pick.first < kBuckets) {
             uint32_t listed;
-            const uint32_t n = part_pick(visit, r, pick, listed);
+            const uint32_t n = part_pick(visit, pick, listed);
             u64 both;  // staying above, listed below
             const u64 at = scan_block<kThreads>((u64)n << 32 | (uint32_t)__popc(listed), both, s_part);
             n_stay = (uint32_t)(both >> 32);
@@ -885,39 +931,39 @@ __global__ __launch_bounds__(kSliceThreads) void k_max(SampleArgs g, Work w) {
 template <int TYPE>
 __global__ __launch_bounds__(kSliceThreads) void k_hist(SampleArgs g, Work w) {
     using X = typename Elem<TYPE>::type;
-    __shared__ double table[kTable];
+    __shared__ double table[kBuckets];
     __shared__ u64 hw[kBuckets];
     const int row = (int)(blockIdx.x / (unsigned)w.S), slice = (int)(blockIdx.x % (unsigned)w.S), tid = (int)threadIdx.x;
     const Set set = settings(g, row);
     const Max m = row_max(w, row);
     const Mode mode = mode_of(set, m);
     if (mode != kWeights && mode != kTopK) return;
-    fill_table(table);
+    const Row r = row_of(set, m, w.shift, table);
+    if (mode == kWeights) r.fill<kSliceThreads>(table);
     for (int i = tid; i < kBuckets; i += kSliceThreads) hw[i] = 0;
     __syncthreads();
     const int lo = slice * w.len, hi = min(g.V, lo + w.len);
     const X* x = reinterpret_cast<const X*>(g.logits) + (int64_t)row * g.stride;
-    part_hist([&](auto&& f) { each<X, kSliceThreads>(x, lo, hi, f); }, row_of(set, m, w.shift, table), mode, hw);
+    part_hist([&](auto&& f) { each<X, kSliceThreads>(x, lo, hi, f); }, r, mode, hw);
     const int64_t at = (int64_t)blockIdx.x * kBuckets;
     const int n = mode == kTopK ? kBuckets / 2 : kBuckets;
     for (int i = tid; i < n; i += kSliceThreads) w.weight[at + i] = hw[i];
 }
 
 __global__ __launch_bounds__(kThreads) void k_cut(SampleArgs g, Work w) {
-    __shared__ u64 s_part[kWaves], s_before;
-    __shared__ int s_bucket;
+    __shared__ union {
+        FindLds<u64> w;
+        FindLds<uint32_t> n;
+    } s;
     const int row = (int)blockIdx.x;
     const Set set = settings(g, row);
     const Max m = row_max(w, row);
     const Mode mode = mode_of(set, m);
     if (mode != kWeights && mode != kTopK) return;
-    const Row r = row_of(set, m, w.shift, nullptr);
+    const Row r = row_of(set, m, w.shift, nullptr);  // no weights here
     const int64_t at = (int64_t)row * w.S;
-    const Pick pick = mode == kTopK ? find_buckets<kThreads>(w.count + at * 2 * kBuckets, 2 * kBuckets, w.S, r, set, mode,
-                                                             reinterpret_cast<uint32_t*>(s_part),
-                                                             reinterpret_cast<uint32_t*>(&s_before), &s_bucket)
-                                    : find_buckets<kThreads>(w.weight + at * kBuckets, kBuckets, w.S, r, set, mode, s_part,
-                                                             &s_before, &s_bucket);
+    const Pick pick = mode == kTopK ? find_buckets(w.count + at * 2 * kBuckets, 2 * kBuckets, w.S, r, set, mode, s.n)
+                                    : find_buckets(w.weight + at * kBuckets, kBuckets, w.S, r, set, mode, s.w);
     if (threadIdx.x == 0) w.pick[row] = pick;
 }
 
@@ -931,7 +977,6 @@ __global__ __launch_bounds__(kSliceThreads) void k_pick(SampleArgs g, Work w) {
     const Max m = row_max(w, row);
     const Mode mode = mode_of(set, m);
     if (mode != kWeights && mode != kTopK) return;
-    const Row r = row_of(set, m, w.shift, nullptr);  // no weights here
     const Pick pick = w.pick[row];
     const int lo = slice * w.len, hi = min(g.V, lo + w.len);
     uint16_t* list = w.list + (int64_t)blockIdx.x * w.len;
@@ -939,7 +984,7 @@ __global__ __launch_bounds__(kSliceThreads) void k_pick(SampleArgs g, Work w) {
     if (pick.first < kBuckets) {
         const X* x = reinterpret_cast<const X*>(g.logits) + (int64_t)row * g.stride;
         uint32_t listed;
-        const uint32_t n = part_pick([&](auto&& f) { each<X, T>(x, lo, hi, f); }, r, pick, listed);
+        const uint32_t n = part_pick([&](auto&& f) { each<X, T>(x, lo, hi, f); }, pick, listed);
         u64 both;  // staying above, listed below
         const u64 at = scan_block<T>((u64)n << 32 | (uint32_t)__popc(listed), both, s_part);
         n_all = (uint32_t)(both >> 32);
@@ -959,7 +1004,7 @@ __global__ __launch_bounds__(kSliceThreads) void k_pick(SampleArgs g, Work w) {
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void k_draw(SampleArgs g, Work w) {
     using X = typename Elem<TYPE>::type;
-    __shared__ double table[kTable];
+    __shared__ double table[kBuckets];
     __shared__ RowLds s;
     const int row = (int)blockIdx.x, tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Set set = settings(g, row);
@@ -978,9 +1023,9 @@ __global__ __launch_bounds__(kThreads) void k_draw(SampleArgs g, Work w) {
         greedy_row(g, row, x, slice * w.len, min(g.V, (slice + 1) * w.len), m.top, &s.search.key);
         return;
     }
-    fill_table(table);
     if (tid == 0) s.draw.n = s.draw.kept = 0;
     const Row r = row_of(set, m, w.shift, table);
+    r.fill<kThreads>(table);
     const Sum* sums = w.sum + (int64_t)row * w.S;
     __syncthreads();
     uint32_t n_list = 0, n_stay = 0;
