@@ -26,10 +26,11 @@
 // the middle leaves its O, r and l for k_attn_join, in a place of its own.
 //
 // Measured, bf16 unless said (H 32, 8 kv heads, D 128; calls back to back):
-//   8 chunks of 512 tokens over 4096 + up to 1024 keys    333 us   705 TFLOP/s (a 8192^3 product: 1256)
+//   8 chunks of up to 512 tokens, 3,070 in all, over 4096
+//   shared and up to 1024 own keys                        333 us   705 TFLOP/s (an 8192^3 product: 1256)
 //   32 sequences of up to 8192 own keys, 670 MB           113 us   5.9 TB/s (reads alone: 6.8)
 //   256 sequences behind 32,768 shared keys, 1024 own     243 us   140 GFLOP and 781 MB: 112 + 115 us
-//   64 sequences (f16) behind 8192 shared keys, 600 own    44 us   9 GFLOP and 130 MB: 14 + 19 us
+//   64 sequences (f16) behind 8192 shared keys, 600 own    45 us   9 GFLOP and 130 MB: 14 + 19 us
 //   1 sequence of 300 keys, D 64                           14 us   two launches
 #include <type_traits>
 
@@ -84,7 +85,7 @@ struct AttnArgs {
     int2* where1;  // [head][sequence]
 };
 
-__host__ __device__ constexpr int round64(int v) { return (v + 63) / 64; }
+__host__ __device__ constexpr int units_of(int v) { return (v + 63) / 64; }
 // Units are numbered head by head, as a head's items may share keys (a prefix), which its neighbours in
 // the order then find in the L2 of their XCD.  [w U / n, (w + 1) U / n) go to share w of n = min(groups, U).
 // A share leaves at most one result per (head, item): share and pair never repeat together
@@ -107,15 +108,15 @@ __device__ __forceinline__ int seen_rows(const Paged& a, int b, int n, int i, in
     return (int)(s < 0 ? 0 : s > own ? own : s);
 }
 
-// One workgroup lays out the items (6 us for 8 sequences of 512 tokens beside 330 us that follow: latency).  Sequences are taken 1024 at a time, a thread each, then their tiles
-// and tokens, a thread each.
+// One workgroup lays out the items: sequences are taken 1024 at a time, a thread each, then their tiles and
+// tokens, a thread each.  Latency bounds it: 6 us for 3,070 tokens of 8 sequences, beside the 350 of what follows.
 __global__ __launch_bounds__(1024) void k_attn_plan(AttnArgs g) {
     constexpr int N = 1024;
     __shared__ int s_wave[N / 64];
     __shared__ int s_at[N];   // exclusive sums of a round
     const Paged& a = g.a;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int ntp = round64(a.P);
+    const int ntp = units_of(a.P);
     auto scan = [&](int v) {  // (exclusive sum, total) over the workgroup
         int x = v;
         for (int d = 1; d < 64; d <<= 1) {
@@ -194,7 +195,7 @@ __global__ __launch_bounds__(1024) void k_attn_plan(AttnArgs g) {
             int t0, n;
             seq_tokens(a, b, t0, n);
             const int last = min(n, ((r + 1) * g.R - 1) / g.G + 1) - 1;
-            mine = (is_joint(g, n) ? ntp : 0) + round64(seen_rows(a, b, n, last, own_rows(a, b)));
+            mine = (is_joint(g, n) ? ntp : 0) + units_of(seen_rows(a, b, n, last, own_rows(a, b)));
         }
         const int2 at = scan(mine);
         if (k < items) g.p.first[k] = units + at.x;
@@ -378,7 +379,7 @@ __device__ __forceinline__ u32x2 read_tr(const uint8_t* p) {
 //
 // 8 waves of 32 rows: a half's K operands serve both row tiles of a wave, and 256 rows share what a unit brings to
 // LDS.  What bounds it at 705 TFLOP/s: a SIMD's two waves are both in their softmax for part of the time (matrix units
-// busy 33 % of the clocks, VALU 45 %).  Measured and left: K of the next half read behind P V (338 us against 334),
+// busy 32 % of the clocks, vector units 42 %, no LDS conflicts).  Measured and left: K of the next half read behind P V (338 us against 334),
 // wave priorities around the products (no change).
 template <int QT, int CT, int NS, int DT, int MT, int NW, bool UNI>
 __device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w, int groups) {
@@ -394,7 +395,7 @@ __device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w,
     const Paged& a = g.a;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, lg = lane >> 4;
-    const int ntiles = round64(a.P);
+    const int ntiles = units_of(a.P);
     const int nitems = g.planned ? g.p.info[0] : (a.T * g.G + g.R - 1) / g.R;
     const int UH = g.planned ? g.p.info[1] : nitems * ntiles;
     const int64_t U = (int64_t)UH * a.hkv;
@@ -1037,7 +1038,7 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_both(AttnAr
     } s;
     const Paged& a = g.a;
     const int uw = wave_units(a), eighths = g.groups >> 3;
-    const float ct = (float)(((a.T * g.G + g.R - 1) / g.R) * round64(a.P)) * g.tile_cost, cw = (float)uw * g.wave_cost;
+    const float ct = (float)(((a.T * g.G + g.R - 1) / g.R) * units_of(a.P)) * g.tile_cost, cw = (float)uw * g.wave_cost;
     const int x8 = cw == 0.f ? eighths : max(1, min(eighths - 1, (int)((float)eighths * ct / (ct + cw) + 0.5f)));
     const int row = (int)blockIdx.x >> 3;
     if (row < x8) {
@@ -1051,7 +1052,7 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_both(AttnAr
 
 // Joins what was left of each (token, query head): its packed results, then its sequence's.  A
 // workgroup takes a token and HW heads for each of its 4 waves; a lane looks up one of the wave's heads.
-// Three dependent lookups and the results bound it: 8 us at 64 tokens of 32 heads, 12 at 256, 21 at 4096.
+// Three dependent lookups and the results bound it: 8 us at 64 tokens of 32 heads, 12 at 256, 21 at 3,070.
 template <int QT, int HW>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs g) {
     using Q = typename Elem<QT>::type;

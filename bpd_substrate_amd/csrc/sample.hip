@@ -16,8 +16,8 @@
 // logits at the cut) is searched digit by digit instead.
 //
 // Measured (calls back to back): 1 row of 32,000, top-k and top-p, 18 us, one launch, latency; 64 rows of 128,256 (fp32,
-// mixed settings) 55 us; 256 rows of 128,256 (binary16, top-p) 97 us: max 16 (66 MB at 4.2 TB/s), hist 34 (21 vector
-// instructions and two LDS operations a logit), cut 8, pick 22, draw 25 (latency of a workgroup).  Left: a slice's first loads
+// mixed settings) 55 us; 256 rows of 128,256 (binary16, top-p) 97 us: max 16 (66 MB at 4.2 TB/s), hist 34 (28 vector
+// instructions a logit, which keep their units busy 93 % of it), cut 8, pick 22, draw 25 (latency of a workgroup).  Left: a slice's first loads
 // ahead of its row's settings (their registers cost a workgroup of four per CU: hist 34 -> 37 us).
 #include "bpdq_paged.h"
 
