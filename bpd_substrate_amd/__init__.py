@@ -6,9 +6,10 @@ C ABI (include/bpdq.h, libbpdq_hip.so).
 Modules:
   formats  GGUF block layouts and byte counts
   gpu      host mirror of the reference GPU entry points (ctypes over the C ABI)
+  serve    many sequences at once: paged K/V append and attention, sampling (include/bpdq_serve.h)
   synth    deterministic synthetic tensors for the benchmark configurations
   build    in-tree build of the native libraries
 """
 from . import formats  # noqa: F401
 
-__all__ = ["formats", "gpu", "synth", "build"]
+__all__ = ["formats", "gpu", "serve", "synth", "build"]
