@@ -137,8 +137,10 @@ def rope_bound(x, rot, neox, dtype, ref):
 
 def check_sample(x, token, logprob, kept, u, t=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """One row's result against the definition.  Weights are multiples of 2^-44 (vocab up to 2^18) of the
-    largest, each off by at most 2^-45 + 2^-51 of itself: a border between cumulated sums may fall on
-    either side within `slack`, nothing else may differ."""
+    largest, each off by 2^-45, and before that by (3 y + 4) 2^-53 of itself, y = (max - l) / t: three
+    roundings of y and four of the exponential's parts.  As exp(-y) y <= 1 / e, that is at most 2^-45 + 2^-52 +
+    2^-51 of itself; a border between cumulated sums may fall on either side within `slack`, nothing else
+    may differ."""
     x = np.asarray(x, np.float64)
     x = np.where(np.isnan(x), -np.inf, x)
     V = len(x)
@@ -163,7 +165,8 @@ def check_sample(x, token, logprob, kept, u, t=1.0, top_k=0, top_p=1.0, min_p=0.
         hi = min(n, int(np.searchsorted(c, need + slack)) + 1)
     if min_p > 0:
         m = min(min_p, 1.0)
-        lo, hi = min(lo, max(1, int((w >= m * (1 + 2.0 ** -50)).sum()))), min(hi, max(1, int((w >= m * (1 - 2.0 ** -50)).sum())))
+        near = (3 * -np.log(m) + 4) * 2.0 ** -53     # where w is about min_p, y is about -log(min_p)
+        lo, hi = min(lo, max(1, int((w >= m * (1 + near)).sum()))), min(hi, max(1, int((w >= m * (1 - near)).sum())))
     assert lo <= kept <= hi, (kept, lo, hi)
     left = np.sort(order[:kept])
     place = {int(i): j for j, i in enumerate(order)}
