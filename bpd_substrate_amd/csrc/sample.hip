@@ -30,7 +30,9 @@ constexpr int kRow = 32768;  // elements of a row that its workgroup holds in re
 constexpr int kSliceThreads = 512;
 constexpr int kBuckets = 1024;
 constexpr int kList = 4096;  // entries of a list that is sorted
-constexpr int kSlices = 256;  // at most: vocab up to 2^22
+constexpr int kMaxSlice = 16384;  // elements of a slice at most: 32 for a thread, marked in one word
+constexpr int kSlices = 256;  // of a row at most
+static_assert((int64_t)kSlices * kMaxSlice >= 1 << 22, "the largest vocab");
 typedef unsigned long long u64;
 
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -1059,10 +1061,11 @@ int shift_of(int V) {
     return bits <= 18 ? 44 : 62 - bits;
 }
 
-// Elements of a slice: enough workgroups for the chip, up to 16384 (32 for a thread, marked in one word).
+// Elements of a slice: enough workgroups for the chip, but no more slices of a row than k_draw has sums for.
 int slice_len(int B, int V) {
-    int len = 16384;
-    while (len > 2048 && (int64_t)B * ((V + len - 1) / len) < 1024) len >>= 1;
+    auto slices = [&](int len) { return (V + len - 1) / len; };
+    int len = kMaxSlice;
+    while (len > 2048 && (int64_t)B * slices(len) < 1024 && slices(len / 2) <= kSlices) len >>= 1;
     return len;
 }
 
