@@ -64,8 +64,9 @@ void check_paged(Args& c, const bpd_paged_cache* kv, const bpd_paged_batch* b) {
     c.shape(b->table_width >= 0, "table_width is negative").shape(b->prefix_len >= 0, "prefix_len is negative");
     c.shape(b->table_stride >= b->table_width, "table_stride is shorter than table_width");
     if (!c.ok) return;
-    c.shape((int64_t)b->table_width * kv->page_size + b->prefix_len + b->n_tokens < INT_MAX,
-            "prefix_len, the table's rows and n_tokens add up to 2^31 or more");
+    // the kernels round rows up to units of 64 and name those of units that they ask for ahead, in 32 bits
+    c.shape((int64_t)b->table_width * kv->page_size + b->prefix_len + b->n_tokens <= INT_MAX - 1024,
+            "prefix_len, the table's rows and n_tokens add up to 2^31 - 1024 or more");
     c.need(b->n_tokens <= 1 << 23, BPDQ_ERR_LIMIT, "n_tokens is above 2^23");  // a workgroup each
     c.shape(b->q_start != nullptr || b->n_tokens == b->n_seqs, "without q_start n_tokens has to be n_seqs");
     if (!c.ok || b->n_seqs == 0 || b->n_tokens == 0) return;

@@ -54,7 +54,8 @@ typedef struct {
  * outside [q_start[0], q_start[n_seqs]) belong to no sequence: nothing is written
  * for them.  With q_start NULL every sequence has one new token
  * (n_tokens == n_seqs).  The prefix comes before every sequence's own part: row i is
- * row i % page_size of page prefix[i / page_size]. */
+ * row i % page_size of page prefix[i / page_size].  table_width * page_size, prefix_len
+ * and n_tokens add up to less than 2^31 - 1024. */
 typedef struct {
     const int32_t* table;
     int64_t table_stride;
