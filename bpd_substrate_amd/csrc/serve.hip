@@ -68,6 +68,7 @@ void check_paged(Args& c, const bpd_paged_cache* kv, const bpd_paged_batch* b) {
     c.shape((int64_t)b->table_width * kv->page_size + b->prefix_len + b->n_tokens <= INT_MAX - 1024,
             "prefix_len, the table's rows and n_tokens add up to 2^31 - 1024 or more");
     c.need(b->n_tokens <= 1 << 23, BPDQ_ERR_LIMIT, "n_tokens is above 2^23");  // a workgroup each
+    c.need(b->n_seqs <= 1 << 30, BPDQ_ERR_LIMIT, "n_seqs is above 2^30");  // the search takes up to 63 more, in 32 bits
     c.shape(b->q_start != nullptr || b->n_tokens == b->n_seqs, "without q_start n_tokens has to be n_seqs");
     if (!c.ok || b->n_seqs == 0 || b->n_tokens == 0) return;
     if (b->table_width > 0) c.ptr(b->table, 4, "batch.table");

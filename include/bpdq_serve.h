@@ -55,7 +55,7 @@ typedef struct {
  * for them.  With q_start NULL every sequence has one new token
  * (n_tokens == n_seqs).  The prefix comes before every sequence's own part: row i is
  * row i % page_size of page prefix[i / page_size].  table_width * page_size, prefix_len
- * and n_tokens add up to less than 2^31 - 1024. */
+ * and n_tokens add up to less than 2^31 - 1024; n_seqs up to 2^30 (BPDQ_ERR_LIMIT). */
 typedef struct {
     const int32_t* table;
     int64_t table_stride;

@@ -41,3 +41,11 @@ def test_rows_whose_units_would_pass_2_31_are_refused(L, f, split):
     else:
         f(L, c, b, pos=0x3)
         err(L, 3, "pos")
+
+
+@pytest.mark.parametrize("f", [attn, append])
+def test_sequences_beyond_the_search_are_refused(L, f):
+    """count_le looks through q_start's n_seqs + 1 values in 32 bits, 63 more for its rounding."""
+    for n in ((1 << 30) + 1, (1 << 31) - 1):
+        f(L, cache(), batch(n_seqs=n, q_start=0x9000, n_tokens=5))
+        err(L, 7, "n_seqs is above 2^30")
