@@ -107,6 +107,9 @@ HIP_SIGNATURES = {
     "bpd_attn_paged_workspace": (L, [P, P, I]),
     "bpd_sample_gpu": (None, [P, I, L, I, I, P, P, P, P, P, P, P, P, P, L]),
     "bpd_sample_workspace": (L, [I, I]),
+    "bpd_rope_append_paged_on_gpu": (None, [P, P, P, P, P, P, L, P, L, P, L, P, L, I, I]),
+    "bpd_attn_paged_on_gpu": (None, [P, P, P, P, L, P, L, P, I, I, F, P, L]),
+    "bpd_sample_on_gpu": (None, [P, P, I, L, I, I, P, P, P, P, P, P, P, P, P, L]),
 }
 
 SYNTH_SIGNATURES = {

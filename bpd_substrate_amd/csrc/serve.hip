@@ -101,9 +101,9 @@ bpdq::Paged paged(const bpd_paged_cache& kv, const bpd_paged_batch& b) {
 }
 
 // The caller's workspace or the library's; nullptr with the error recorded.
-void* work_space(bpdq::WsLease& lease, void* ws, int64_t ws_bytes, int64_t need, const char* fn) {
+void* work_space(bpdq::WsLease& lease, void* ws, int64_t ws_bytes, int64_t need, hipStream_t stream, const char* fn) {
     if (ws == nullptr) {
-        lease = bpdq::workspace((size_t)need, bpdq::abi_stream(), fn);
+        lease = bpdq::workspace((size_t)need, stream, fn);
         return lease.ptr;
     }
     Args c(fn);
@@ -145,11 +145,12 @@ void check_sample(Args& c, int n_rows, int vocab) {
 
 extern "C" {
 
-void bpd_rope_append_paged_gpu(const bpd_paged_cache* kv, const bpd_paged_batch* b, const bpd_rope* rope,
-                               const int32_t* pos, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
-                               const void* v, int64_t v_stride, void* q_out, int64_t q_out_stride, int x_type,
-                               int n_heads) {
+void bpd_rope_append_paged_on_gpu(void* hip_stream, const bpd_paged_cache* kv, const bpd_paged_batch* b,
+                                  const bpd_rope* rope, const int32_t* pos, const void* q, int64_t q_stride,
+                                  const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* q_out,
+                                  int64_t q_out_stride, int x_type, int n_heads) {
     const char* fn = "bpd_rope_append_paged_gpu";
+    const hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     Args c(fn);
     check_paged(c, kv, b);
     c.shape(x_type == BPD_T_F32 || x_type == BPD_T_F16 || x_type == BPD_T_BF16, "x_type is unknown");
@@ -185,8 +186,16 @@ void bpd_rope_append_paged_gpu(const bpd_paged_cache* kv, const bpd_paged_batch*
     }
     bpdq::launch_rope_append(paged(*kv, *b), kv->type, rot > 0 ? rope->turns : nullptr, rot,
                              rot > 0 && rope->neox == 1, pos, q, q_stride, k, k_stride, v, v_stride, q_out,
-                             q_out_stride, x_type, n_heads, bpdq::abi_stream());
+                             q_out_stride, x_type, n_heads, stream);
     bpdq::abi_hip_ok(hipGetLastError(), fn);
+}
+
+void bpd_rope_append_paged_gpu(const bpd_paged_cache* kv, const bpd_paged_batch* b, const bpd_rope* rope,
+                               const int32_t* pos, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                               const void* v, int64_t v_stride, void* q_out, int64_t q_out_stride, int x_type,
+                               int n_heads) {
+    bpd_rope_append_paged_on_gpu(bpdq::abi_stream(), kv, b, rope, pos, q, q_stride, k, k_stride, v, v_stride, q_out,
+                                 q_out_stride, x_type, n_heads);
 }
 
 int64_t bpd_attn_paged_workspace(const bpd_paged_cache* kv, const bpd_paged_batch* b, int n_heads) {
@@ -198,10 +207,11 @@ int64_t bpd_attn_paged_workspace(const bpd_paged_cache* kv, const bpd_paged_batc
     return bpdq::attn_paged_ws(b->q_start, b->n_seqs, b->n_tokens, n_heads, kv->n_kv_heads, kv->head_dim, b->prefix_len);
 }
 
-void bpd_attn_paged_gpu(const bpd_paged_cache* kv, const bpd_paged_batch* b, const void* q, int64_t q_stride,
-                        void* out, int64_t out_stride, float* lse, int q_type, int n_heads, float scale, void* ws,
-                        int64_t ws_bytes) {
+void bpd_attn_paged_on_gpu(void* hip_stream, const bpd_paged_cache* kv, const bpd_paged_batch* b, const void* q,
+                           int64_t q_stride, void* out, int64_t out_stride, float* lse, int q_type, int n_heads,
+                           float scale, void* ws, int64_t ws_bytes) {
     const char* fn = "bpd_attn_paged_gpu";
+    const hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     Args c(fn);
     check_paged(c, kv, b);
     if (!c.ok) return;
@@ -217,12 +227,20 @@ void bpd_attn_paged_gpu(const bpd_paged_cache* kv, const bpd_paged_batch* b, con
     c.shape(!overlap(q, es * q_stride, es * row, out, es * out_stride, es * row, b->n_tokens), "q and out overlap");
     if (!c.ok) return;
     bpdq::WsLease lease;
-    void* w = work_space(lease, ws, ws_bytes, bpdq::attn_paged_ws(b->q_start, b->n_seqs, b->n_tokens, n_heads, kv->n_kv_heads,
-                                                                  kv->head_dim, b->prefix_len), fn);
+    const int64_t need = bpdq::attn_paged_ws(b->q_start, b->n_seqs, b->n_tokens, n_heads, kv->n_kv_heads, kv->head_dim,
+                                             b->prefix_len);
+    void* w = work_space(lease, ws, ws_bytes, need, stream, fn);
     if (w == nullptr) return;
     bpdq::launch_attn_paged(paged(*kv, *b), kv->type, q, q_stride, out, out_stride, lse, q_type, n_heads, scale, w,
-                            bpdq::abi_stream());
+                            stream);
     bpdq::abi_hip_ok(hipGetLastError(), fn);
+}
+
+void bpd_attn_paged_gpu(const bpd_paged_cache* kv, const bpd_paged_batch* b, const void* q, int64_t q_stride,
+                        void* out, int64_t out_stride, float* lse, int q_type, int n_heads, float scale, void* ws,
+                        int64_t ws_bytes) {
+    bpd_attn_paged_on_gpu(bpdq::abi_stream(), kv, b, q, q_stride, out, out_stride, lse, q_type, n_heads, scale, ws,
+                          ws_bytes);
 }
 
 int64_t bpd_sample_workspace(int n_rows, int vocab) {
@@ -231,10 +249,11 @@ int64_t bpd_sample_workspace(int n_rows, int vocab) {
     return c.ok ? bpdq::sample_ws(n_rows, vocab) : -1;
 }
 
-void bpd_sample_gpu(const void* logits, int type, int64_t row_stride, int n_rows, int vocab, const float* temperature,
-                    const int32_t* top_k, const float* top_p, const float* min_p, const float* u, int32_t* token,
-                    float* logprob, int32_t* n_kept, void* ws, int64_t ws_bytes) {
+void bpd_sample_on_gpu(void* hip_stream, const void* logits, int type, int64_t row_stride, int n_rows, int vocab,
+                       const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                       const float* u, int32_t* token, float* logprob, int32_t* n_kept, void* ws, int64_t ws_bytes) {
     const char* fn = "bpd_sample_gpu";
+    const hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     Args c(fn);
     c.shape(type == BPD_T_F32 || type == BPD_T_F16 || type == BPD_T_BF16, "type is unknown");
     check_sample(c, n_rows, vocab);
@@ -250,11 +269,18 @@ void bpd_sample_gpu(const void* logits, int type, int64_t row_stride, int n_rows
     if (n_kept != nullptr) c.ptr(n_kept, 4, "n_kept");
     if (!c.ok) return;
     bpdq::WsLease lease;
-    void* w = work_space(lease, ws, ws_bytes, bpdq::sample_ws(n_rows, vocab), fn);
+    void* w = work_space(lease, ws, ws_bytes, bpdq::sample_ws(n_rows, vocab), stream, fn);
     if (w == nullptr) return;
     bpdq::launch_sample({logits, row_stride, n_rows, vocab, temperature, top_k, top_p, min_p, u, token, logprob, n_kept},
-                        type, w, bpdq::abi_stream());
+                        type, w, stream);
     bpdq::abi_hip_ok(hipGetLastError(), fn);
+}
+
+void bpd_sample_gpu(const void* logits, int type, int64_t row_stride, int n_rows, int vocab, const float* temperature,
+                    const int32_t* top_k, const float* top_p, const float* min_p, const float* u, int32_t* token,
+                    float* logprob, int32_t* n_kept, void* ws, int64_t ws_bytes) {
+    bpd_sample_on_gpu(bpdq::abi_stream(), logits, type, row_stride, n_rows, vocab, temperature, top_k, top_p, min_p, u,
+                      token, logprob, n_kept, ws, ws_bytes);
 }
 
 }  // extern "C"

@@ -19,7 +19,6 @@ in several captured graphs do not share one.
 import ctypes
 import functools
 import math
-import threading
 
 import torch
 
@@ -74,22 +73,16 @@ def _rows(t, what, shape, dtype, device):
     return s[0] if n > 1 else h * d
 
 
-# The library's launch stream is one for the process: a call sets it and launches under this lock,
-# so that calls of several threads on streams of their own do not take each other's.
-_lock = threading.Lock()
-
-
 def _launch(device, fn, *args):
-    """fn(*args), an entry point of the library, on torch's current stream of `device`."""
+    """fn(stream, *args), an entry point of the library, with torch's current stream of `device`.  The stream goes
+    with the call: bpd_gpu_set_stream()'s is one for the process, and other threads may choose it in between."""
     if device.type != "cuda":
         _bad(f"{fn.__name__}: the tensors are on {device}, not on a GPU")
     index = device.index
     if index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return _launch(device, fn, *args)
-    with _lock:
-        gpu._fn("bpd_gpu_set_stream")(torch._C._cuda_getCurrentRawStream(index))
-        fn(*args)
+    fn(torch._C._cuda_getCurrentRawStream(index), *args)
     gpu.check()
 
 
@@ -228,7 +221,7 @@ def rope_append(cache, batch, q, k, v, rope=None, pos=None, q_out=None):
         _tensor(pos, "pos", (torch.int32,), 1, dev, contiguous=True)
         if pos.shape[0] != T:
             _bad(f"pos has {pos.shape[0]} values for {T} tokens")
-    _launch(dev, gpu._fn("bpd_rope_append_paged_gpu"), cache._p, batch._p, None if rope is None else rope._p,
+    _launch(dev, gpu._fn("bpd_rope_append_paged_on_gpu"), cache._p, batch._p, None if rope is None else rope._p,
             None if pos is None else pos.data_ptr(), qp, qs, kp, ks, vp, vs, op, os_, TYPES[x.dtype], H)
     return q_out
 
@@ -252,7 +245,7 @@ def attention(cache, batch, q, scale=None, out=None, return_lse=False):
     lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
     n = batch._workspace(cache, H)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    _launch(dev, gpu._fn("bpd_attn_paged_gpu"), cache._p, batch._p, q.data_ptr(), qs, out.data_ptr(), os_,
+    _launch(dev, gpu._fn("bpd_attn_paged_on_gpu"), cache._p, batch._p, q.data_ptr(), qs, out.data_ptr(), os_,
             None if lse is None else lse.data_ptr(), TYPES[q.dtype], H, D ** -0.5 if scale is None else float(scale),
             ws.data_ptr(), n)
     return (out, lse) if return_lse else out
@@ -288,6 +281,6 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
     token, logprob, kept = res[0], res[1].view(torch.float32), res[2]
     n = _sample_workspace(B, V)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    _launch(dev, gpu._fn("bpd_sample_gpu"), logits.data_ptr(), TYPES[logits.dtype], logits.stride(0) if B > 1 else V, B, V,
+    _launch(dev, gpu._fn("bpd_sample_on_gpu"), logits.data_ptr(), TYPES[logits.dtype], logits.stride(0) if B > 1 else V, B, V,
             *ptrs, token.data_ptr(), logprob.data_ptr(), kept.data_ptr(), ws.data_ptr(), n)
     return token, logprob, kept

@@ -133,6 +133,20 @@ void bpd_sample_gpu(const void* logits, int type, int64_t row_stride, int n_rows
                     float* logprob, int32_t* n_kept, void* ws, int64_t ws_bytes);
 int64_t bpd_sample_workspace(int n_rows, int vocab);
 
+/* The same three on a stream of the current device given with the call (a hipStream_t; NULL = the null
+ * stream).  bpd_gpu_set_stream()'s stream is one for the process, and a call that takes it has to be kept apart from
+ * other threads' choices; these neither read nor change it. */
+void bpd_rope_append_paged_on_gpu(void* hip_stream, const bpd_paged_cache* cache, const bpd_paged_batch* batch,
+                                  const bpd_rope* rope, const int32_t* pos, const void* q, int64_t q_stride,
+                                  const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* q_out,
+                                  int64_t q_out_stride, int x_type, int n_heads);
+void bpd_attn_paged_on_gpu(void* hip_stream, const bpd_paged_cache* cache, const bpd_paged_batch* batch, const void* q,
+                           int64_t q_stride, void* out, int64_t out_stride, float* lse, int q_type, int n_heads,
+                           float scale, void* ws, int64_t ws_bytes);
+void bpd_sample_on_gpu(void* hip_stream, const void* logits, int type, int64_t row_stride, int n_rows, int vocab,
+                       const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                       const float* u, int32_t* token, float* logprob, int32_t* n_kept, void* ws, int64_t ws_bytes);
+
 #ifdef __cplusplus
 }
 #endif
