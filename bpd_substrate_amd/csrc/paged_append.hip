@@ -90,7 +90,10 @@ __global__ __launch_bounds__(256) void k_rope_append(AppendArgs g) {
     if (a.q_start != nullptr) {
         b = __builtin_amdgcn_readfirstlane(count_le(a.q_start, a.B + 1, t) - 1);
         if (b < 0 || b >= a.B) return;  // the whole workgroup: the token is no sequence's
-        index = (int64_t)a.lens[b] - a.q_start[b + 1] + t;
+        int t0, n;
+        seq_tokens(a, b, t0, n);
+        if (t < t0 || t >= t0 + n) return;  // offsets that decrease: not really the sequence's
+        index = (int64_t)a.lens[b] - n + (t - t0);
     } else {
         index = (int64_t)a.lens[b] - 1;
     }

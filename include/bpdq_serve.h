@@ -15,8 +15,8 @@
  * (lens, q_start, table, prefix) are read by the kernels, so a captured graph
  * follows their contents from replay to replay.  Whatever they hold, no access
  * leaves the tensors that the structs describe: a length is clamped to the
- * table, a token index to n_tokens, and a page index outside [0, n_pages) makes
- * its rows absent (not written by the append, not seen by the attention).
+ * table, a value of q_start to [0, n_tokens], and a page index outside [0, n_pages)
+ * makes its rows absent (not written by the append, not seen by the attention).
  */
 #ifndef BPDQ_SERVE_H
 #define BPDQ_SERVE_H
