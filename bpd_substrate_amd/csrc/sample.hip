@@ -84,9 +84,11 @@ struct Row {
     __device__ __forceinline__ u64 weight_of(uint32_t key) const {
         return logit_of(key) == top ? 1ull << shift : weight(logit_of(key));
     }
+    // min-p's rule; above 1 no weight reaches it, and the first of the largest logits is the caller's to keep
     __device__ __forceinline__ bool passes(uint32_t key, float min_p) const {
         const float x = logit_of(key);
-        if (!(min_p > 0.f) || x == top) return true;
+        if (!(min_p > 0.f)) return true;
+        if (x == top) return min_p <= 1.f;
         if (!(min_p < 1.f)) return false;
         if (!(min_p > 0x1p-45f)) return exp(((double)x - max) / t) >= (double)min_p;  // beyond the table
         int b;
@@ -504,7 +506,10 @@ __device__ __forceinline__ void search_row(const SampleArgs& g, int row, const X
             tie = num;
             kept = above + num;
         }
-        if (mf > 0.f) {  // weights fall with the key: the cut moves up to the last key at or above min_p
+        if (mf > 1.f) {  // the first of the largest alone
+            cut = key_of(r.top);
+            tie = kept = 1;
+        } else if (mf > 0.f) {  // weights fall with the key: the cut moves up to the last key at or above min_p
             __syncthreads();
             if (tid == 0) s_cnt = 0, s_key = 0xFFFFFFFFu;
             __syncthreads();
@@ -688,7 +693,8 @@ __device__ __forceinline__ void draw_row(const SampleArgs& g, int row, const X* 
         u64 all = 0, run = run0;
         if (want != ~0ull) run += scan_block<kThreads>(i < n_ranked ? r.weight_of(k) : 0, all, s.part);
         // what stands before it falls short of what is wanted
-        const uint64_t stay = __ballot(i < n_ranked && run < want && r.passes(k, set.m));
+        const bool largest = i == 0 && n_stay == 0;  // min-p leaves it in any case
+        const uint64_t stay = __ballot(i < n_ranked && run < want && (largest || r.passes(k, set.m)));
         if (lane == 0 && stay != 0) atomicAdd(&s.kept, (uint32_t)__popcll(stay));
         run0 += all;
     }

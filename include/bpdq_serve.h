@@ -118,7 +118,7 @@ int64_t bpd_attn_paged_workspace(const bpd_paged_cache* cache, const bpd_paged_b
  *   top_p        the fewest largest ones whose weights reach top_p of the sum, at
  *                least one; 1 or more: all
  *   min_p        those with w_i >= min_p (times the largest weight, which is 1), at
- *                least the largest
+ *                least the first of the largest, which above 1 is left alone
  * then token = the first index, in the vocabulary's order, at which the sum of the
  * weights left exceeds u times their total.  One value of each per row; a NULL array:
  * temperature 1, no filter.  u in [0, 1).  NaN and -infinity logits are never
