@@ -301,6 +301,12 @@ __device__ __forceinline__ int row_exponent(float (&x)[KS][8]) {
     return e2;
 }
 
+// What a score is multiplied by, the exponent put back.  Not 0: a row that is not there has a score of -infinity.
+__device__ __forceinline__ float score_scale(float scale2, int e2) {
+    const float s = ldexpf(scale2, e2);
+    return s < 0x1p-126f ? 0x1p-126f : s;  // scores of less than 2^-90 weigh 1
+}
+
 // The lane's elements of a row of O, of the first D, where row c of product 8 vb + e holds element
 // 128 vb + 2 VD c + e.
 template <typename Q, int VD, int VB>
@@ -466,7 +472,7 @@ __device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w,
         }
         float qscale[MT];
 #pragma unroll
-        for (int m = 0; m < MT; m++) qscale[m] = NS > 1 && CT == BPD_T_F16 ? ldexpf(scale2, e2[m]) : scale2;
+        for (int m = 0; m < MT; m++) qscale[m] = NS > 1 && CT == BPD_T_F16 ? score_scale(scale2, e2[m]) : scale2;
         const bool busy = __ballot(lim[0] >= 0) != 0;  // rows of a wave fill from its first
         f32x4 o[MT][NE];
         float ref[MT], l[MT];
@@ -892,7 +898,7 @@ __device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT
             const Q* q = reinterpret_cast<const Q*>(g.q) + b * g.qs + (int64_t)(head * g.G + (row ? col : 0)) * a.D;
             float x[KS][8];
             load_query<KS>(q, row, per, lg, sign, x);
-            if constexpr (NS > 1 && CT == BPD_T_F16) qscale = ldexpf(scale2, row_exponent<KS>(x));
+            if constexpr (NS > 1 && CT == BPD_T_F16) qscale = score_scale(scale2, row_exponent<KS>(x));
 #pragma unroll
             for (int k = 0; k < KS; k++) split8<CT, NS>(x[k], qf[k]);
         }

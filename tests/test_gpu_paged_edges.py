@@ -4,6 +4,7 @@ import torch
 
 import paged_oracle as O
 from bpd_substrate_amd import serve
+from test_gpu_paged import check_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +31,17 @@ def test_offsets_are_clamped_alike_by_append_and_attention(dev, start, same, x):
         got.append((cache.k.contiguous().view(torch.int16), cache.v.contiguous().view(torch.int16), r, out, lse))
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------- tiny scores, queries of infinities
+
+@pytest.mark.parametrize("kv", ["f16", "bf16"])
+@pytest.mark.parametrize("decode", [False, True])
+@pytest.mark.parametrize("exponent,scale", [(-110, 1e-20), (-126, 1e-38), (0, 2.0 ** -126), (-60, 2.0 ** -100)])
+def test_scores_that_vanish(dev, kv, decode, exponent, scale):
+    """Queries and scales so small that every score is next to 0: the mean of the values seen, none of the rows that are
+    not there."""
+    b = O.Batch(23, [1, 1] if decode else [1, 40], [21, 90], 70, 4, 2, 64, "f32", kv, 16, decode=decode)
+    b.table[1, 2] = -1
+    b.q = torch.ldexp(b.q, torch.tensor(exponent))
+    check_attention(b, dev, scale)
