@@ -1056,9 +1056,26 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_both(AttnAr
     }
 }
 
+// Whether a row that token i of n new ones of sequence b sees is there.  The whole wave.
+__device__ __forceinline__ bool sees_a_row(const Paged& a, int b, int n, int i) {
+    const int lane = (int)threadIdx.x & 63, own = seen_rows(a, b, n, i, own_rows(a, b));
+    auto any = [&](const int32_t* pages, int rows) {
+        const int used = rows > 0 ? fdiv(a.page, rows - 1) + 1 : 0;
+        for (int p0 = 0; p0 < used; p0 += 64) {
+            const int page = p0 + lane < used ? pages[p0 + lane] : -1;
+            if (__ballot(page >= 0 && page < a.n_pages) != 0) return true;
+        }
+        return false;
+    };
+    return any(a.prefix, a.P) || any(a.table + (int64_t)b * a.table_stride, own);
+}
+
 // Joins what was left of each (token, query head): its packed results, then its sequence's.  A
 // workgroup takes a token and HW heads for each of its 4 waves; a lane looks up one of the wave's heads.
 // Three dependent lookups and the results bound it: 8 us at 64 tokens of 32 heads, 12 at 256, 21 at 3,070.
+// A query with infinities or NaN has NaN for k_attn_tile's rows that are not there too (0 times infinity).  Where all are
+// absent the result is that of no row; that is looked for here, as a mask within the tiles' loop or at their items' ends took
+// 2 % of the prompt chunks' time.
 template <int QT, int HW>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs g) {
     using Q = typename Elem<QT>::type;
@@ -1111,6 +1128,14 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs g) {
     const float* part1 = g.planned ? g.part : g.part1;
     const float2* ml1 = g.planned ? g.ml : g.ml1;
     const int R1 = g.planned ? g.R : g.G;
+    if (g.planned) {  // results that were written, but are NaN
+        Q* out = reinterpret_cast<Q*>(g.out) + t * g.os + (int64_t)(h0 + lane) * a.D;
+        const bool odd = done && lane < HW && h0 + lane < g.H && (float)out[0] != (float)out[0];
+        if (__ballot(odd) != 0 && !sees_a_row(a, b, n, i) && odd) {
+            for (int d = 0; d < a.D; d++) out[d] = (Q)0.f;
+            if (g.lse != nullptr) g.lse[(int64_t)t * g.H + h0 + lane] = kNegInf;
+        }
+    }
     uint64_t todo = __ballot(!done);
     // a row of the head in 16-byte pieces by DT / 4 lanes: 64 / (DT / 4) results at a time
     const int lanes = g.DT >> 2, sub = lane / lanes, piece = lane - sub * lanes, step = 64 / lanes;
@@ -1131,6 +1156,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs g) {
             f[k] = x[k].x == kNegInf ? (x[k].y != 0.f ? x[k].y : 0.f) : __builtin_amdgcn_exp2f(x[k].x - m);
             l += x[k].y * f[k];
         }
+        if (__ballot(!done && l != l) != 0 && !sees_a_row(a, b, n, i)) l = 0.f;
         const bool any = l != 0.f;
         if (!done && g.lse != nullptr)
             g.lse[(int64_t)t * g.H + h0 + lane] = any ? (m + __builtin_log2f(l)) * kLn2 : kNegInf;
@@ -1203,6 +1229,10 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs g) {
         for (int d = lanes; d < 64; d <<= 1)
 #pragma unroll
             for (int c = 0; c < 4; c++) acc[c] += __shfl_xor(acc[c], d);
+        if (l != l && !sees_a_row(a, b, n, i)) {
+            l = 0.f;
+            acc = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
         const bool any = l != 0.f;
         const float inv = any ? 1.f / l : 0.f;
         const int h = h0 + j;

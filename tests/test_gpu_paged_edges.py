@@ -1,4 +1,5 @@
 """Edges of bpd_rope_append_paged_gpu and bpd_attn_paged_gpu that their other tests do not reach."""
+import numpy as np
 import pytest
 import torch
 
@@ -7,6 +8,8 @@ from bpd_substrate_amd import serve
 from test_gpu_paged import check_attention
 
 pytestmark = pytest.mark.gpu
+
+INF, NAN = float("inf"), float("nan")
 
 
 # ---------------------------------------------------------------- offsets beyond the tokens
@@ -45,3 +48,38 @@ def test_scores_that_vanish(dev, kv, decode, exponent, scale):
     b.table[1, 2] = -1
     b.q = torch.ldexp(b.q, torch.tensor(exponent))
     check_attention(b, dev, scale)
+
+
+@pytest.mark.parametrize("bad", [INF, -INF, NAN])
+@pytest.mark.parametrize("q", ["f32", "f16"])
+@pytest.mark.parametrize("form", ["chunks", "chunks without a prefix", "a chunk of its own tiles", "one token behind a prefix",
+                                  "one token", "rows split over many workgroups"])
+def test_a_query_of_infinities_that_sees_no_row(dev, bad, q, form):
+    """Every page outside the cache: zeros and -infinity, whatever the query holds."""
+    one = form.startswith("one")
+    new, lens, P = {"chunks": ([1, 40], [20, 90], 70), "chunks without a prefix": ([1, 40], [20, 90], 0),
+                    "a chunk of its own tiles": ([1, 150], [20, 190], 70), "one token": ([1, 1], [20, 90], 0),
+                    "one token behind a prefix": ([1, 1], [20, 90], 70),
+                    "rows split over many workgroups": ([1, 2], [20, 2500], 3000)}[form]
+    b = O.Batch(21, new, lens, P, 4, 2, 64, q, "f16", 16, decode=one)
+    b.table[:] = -1
+    b.prefix_pages[:] = b.kc.shape[0]
+    b.q[:, :, 3] = bad
+    cache, batch, qd = b.device(dev)
+    out, lse = serve.attention(cache, batch, qd, return_lse=True)
+    assert (out == 0).all() and (lse == -INF).all()
+
+
+@pytest.mark.parametrize("bad", [INF, NAN])
+def test_a_query_of_infinities_leaves_the_others_alone(dev, bad):
+    """Rows of one tile whose neighbour's scores are NaN, pages missing in between.  Their bits may change (the rows of a
+    wave move their reference exponents together), their bounds do not."""
+    b = O.Batch(22, [1, 40], [20, 90], 70, 4, 2, 64, "f16", "f16", 16)
+    b.table[1, 2], b.prefix_pages[1] = -1, 2 ** 30
+    cache, batch, qd = b.device(dev)
+    ref, rlse, eo, el = b.attention()
+    qd[5] = bad
+    out, lse = (O.f64(x) for x in serve.attention(cache, batch, qd, return_lse=True))
+    keep = np.arange(len(qd)) != 5
+    assert (np.abs(out - ref) <= eo)[keep].all() and (np.abs(lse - rlse) <= el)[keep].all()
+    assert np.isnan(out[5]).all() and np.isnan(lse[5]).all()
