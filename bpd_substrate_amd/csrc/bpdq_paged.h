@@ -8,22 +8,9 @@
 #include <stdint.h>
 
 #include "../../include/bpdq_serve.h"
+#include "bpdq_paged_plan.h"
 
 namespace bpdq {
-
-// n / d for 0 <= n < 2^31, d >= 1: with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1,
-// n / d = (mulhi(m, n) + n) >> s (division by an invariant integer, Granlund and Montgomery 1994).
-struct FastDiv {
-    uint32_t m, s, d;
-};
-inline FastDiv fast_div(int d) {
-    FastDiv f;
-    f.d = (uint32_t)d;
-    f.s = 0;
-    while ((1ull << f.s) < (uint64_t)d) f.s++;
-    f.m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << f.s) - (uint64_t)d)) / (uint64_t)d + 1);
-    return f;
-}
 
 struct Paged {
     uint8_t *k, *v;
@@ -41,10 +28,6 @@ struct Paged {
 };
 
 #ifdef __HIPCC__
-__device__ __forceinline__ int fdiv(FastDiv f, int n) {
-    return (int)((__umulhi(f.m, (uint32_t)n) + (uint32_t)n) >> f.s);
-}
-
 // How many of the values p[0..n), not decreasing, are <= t: a search over 64 places at a
 // time, one load for up to 64 values.  The whole wave calls it with the same arguments.
 // Values that do decrease give some number in 0..n.
@@ -70,8 +53,7 @@ __device__ __forceinline__ void seq_tokens(const Paged& a, int b, int& t0, int& 
         n = 1;
         return;
     }
-    t0 = min(max(a.q_start[b], 0), a.T);
-    n = max(min(max(a.q_start[b + 1], 0), a.T) - t0, 0);
+    clamp_tokens(a.q_start[b], a.q_start[b + 1], a.T, t0, n);
 }
 
 template <int TYPE>

@@ -46,8 +46,6 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kKeys = 64;   // keys of a unit
-constexpr int kGroups = 256;  // workgroups that share the units: one per CU
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -__builtin_inff();
 
@@ -85,22 +83,11 @@ struct AttnArgs {
     int2* where1;  // [head][sequence]
 };
 
-__host__ __device__ constexpr int units_of(int v) { return (v + 63) / 64; }
-// Units are numbered head by head, as a head's items may share keys (a prefix), which its neighbours in
-// the order then find in the L2 of their XCD.  [w U / n, (w + 1) U / n) go to share w of n = min(groups, U).
-// A share leaves at most one result per (head, item): share and pair never repeat together
-// in share + pair, as each step along the units raises one or both.
-__device__ __forceinline__ int64_t slot_of(int share, int item, int nitems, int h) {
-    return (int64_t)share + (int64_t)h * nitems + item;
-}
-__device__ __forceinline__ int64_t unit_of(int w, int64_t U, int n) { return w * U / n; }
-__device__ __forceinline__ int group_of(int64_t u, int64_t U, int n) { return (int)(((u + 1) * n - 1) / U); }
-
 // Rows of a sequence's own part that the table holds.
 __device__ __forceinline__ int own_rows(const Paged& a, int b) {
     return max(0, min(a.lens[b], a.W * (int)a.page.d));
 }
-__device__ __forceinline__ bool is_joint(const AttnArgs& g, int n) { return n * g.G * 2 >= g.R; }
+__device__ __forceinline__ bool is_joint(const AttnArgs& g, int n) { return bpdq::is_joint(n, g.G, g.R); }
 
 // Whole own rows that row `last` (token index within the sequence) of a tile can see.
 __device__ __forceinline__ int seen_rows(const Paged& a, int b, int n, int i, int own) {
@@ -1248,49 +1235,6 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs g) {
 
 // ---------------------------------------------------------------- host
 
-int padded(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
-// Waves of a workgroup and 16-row tiles of a wave: 8 waves of 32 rows where the accumulators and the
-// parts of the queries fit the 256 registers of two waves per SIMD.
-struct Tile {
-    int mt, nw;
-};
-Tile tile_of(int D, int parts) {
-    if (D <= 64) return {2, 8};
-    if (D <= 128) return {parts == 1 ? 2 : 1, 8};
-    return {1, 4};
-}
-
-int rows_of(int D, int parts) {
-    const Tile t = tile_of(D, parts);
-    return 16 * t.mt * t.nw;
-}
-
-int64_t up16(int64_t v) { return (v + 15) / 16 * 16; }
-
-constexpr int kWaves = 2048;  // k_attn_wave's: two per SIMD
-
-// The workspace of either way: planned, or one token per sequence by k_attn_wave with the prefix packed.
-struct Sizes {
-    int64_t items, ints, part, ml, where, part1, ml1, where1, total;
-};
-Sizes sizes(bool planned, int B, int T, int G, int HKV, int R, int DT, int P) {
-    Sizes s = {};
-    const int64_t per_rows = (int64_t)T * G / R + 1;
-    s.items = planned ? 2 * per_rows + B : P > 0 ? per_rows : 0;
-    const int64_t slots = s.items > 0 ? kGroups + s.items * HKV : 0;
-    s.ints = planned ? up16(4 * (4 + (s.items + 1) + 2 * s.items + B + 2 * (int64_t)T)) : 0;
-    s.part = slots * R * DT * 4;
-    s.ml = up16(slots * R * 8);
-    s.where = up16(s.items * HKV * 8);
-    if (!planned) {
-        const int64_t n = (kWaves + (int64_t)B * HKV) * G;
-        s.part1 = n * DT * 4;
-        s.ml1 = up16(n * 8);
-        s.where1 = up16((int64_t)B * HKV * 8);
-    }
-    s.total = s.ints + s.part + s.ml + s.where + s.part1 + s.ml1 + s.where1;
-    return s;
-}
 bool planned_way(const int32_t* q_start, int G) { return q_start != nullptr || G > 16; }
 
 template <int QT, int CT, int NS, int DT, int MT, int NW, bool UNI>
@@ -1353,7 +1297,7 @@ void launch_attn_paged(const Paged& a0, int cache_type, const void* q, int64_t q
     g.R = rows_of(a.D, q_type == BPD_T_F32 ? 2 : 1);
     g.DT = padded(a.D);
     g.groups = kGroups;
-    g.waves = kWaves;
+    g.waves = kStreamWaves;
     // us of a CU: 64 keys x 256 rows of 128 by 8 waves (630 TFLOP/s), 32 keys of 128 (a CU draws 34 GB/s beside the others)
     const int parts = q_type != BPD_T_F32 ? 1 : cache_type == BPD_T_BF16 ? 3 : 2;
     g.tile_cost = 3.4f * (float)(g.R * g.DT * parts) / (256.f * 128.f) * (g.DT == 256 ? 2.f : 1.f);
