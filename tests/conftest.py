@@ -25,8 +25,9 @@ def dev():
 
 
 # Tests that capture a torch sum.  torch splits it over workgroups that count themselves in memory cleared by
-# hipMemsetAsync, which becomes a memset node of the graph, and on replays after the first such nodes have left the counts as
-# they were: no workgroup was the last, and the sum of the replay before stayed.  They get the same sum from additions alone.
+# hipMemsetAsync, which becomes a memset node of the graph, and on replays after the first such nodes have left the
+# counts as they were: no workgroup was the last, and the sum of the replay before stayed.  They get the same sum from
+# additions alone.
 SUMS_IN_GRAPHS = {"test_decode_steps_together_in_a_graph"}
 
 

@@ -12,8 +12,8 @@ INF = float("inf")
 @pytest.mark.parametrize("V", [2, 9, 3001, 5000, 32768, 32769, 60000])
 @pytest.mark.parametrize("f", [{}, {"k": 10}, {"p": 0.7}, {"k": 4097}, {"k": 3, "p": 0.5, "t": 0.3}])
 def test_min_p_above_1_leaves_the_first_of_the_largest(dev, V, f):
-    """No weight is above 1, so the largest logit alone is left: of equal ones the first, as they rank by index.  At 1 all
-    that equal the largest stay."""
+    """No weight is above 1, so the largest logit alone is left: of equal ones the first, as they rank by index.  At 1
+    all that equal the largest stay."""
     x = torch.zeros(5, V)
     x[1, ::2] = -3.0                   # half of them the largest, from index 1 on
     x[2] = torch.linspace(-4, 0, V)    # one, the last

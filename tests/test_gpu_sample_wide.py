@@ -12,8 +12,8 @@ pytestmark = pytest.mark.gpu
 
 
 def check_row(x, token, logprob, kept, u, t=1.0, top_k=0, top_p=1.0, min_p=0.0):
-    """Weights are multiples of s = 2^-(62 - bits) of the largest, bits = ceil(log2 V), each off by s / 2 and by 2^-50 of
-    itself: a cumulated sum over V of them by V s / 2 + 2^-50 of the sum, which is how far a border may lie."""
+    """Weights are multiples of s = 2^-(62 - bits) of the largest, bits = ceil(log2 V), each off by s / 2 and by 2^-50
+    of itself: a cumulated sum over V of them by V s / 2 + 2^-50 of the sum, which is how far a border may lie."""
     x = np.asarray(x, np.float64)
     V = len(x)
     if not t > 0:
@@ -62,7 +62,8 @@ def test_wide_rows(dev, V, B, f):
     full = lambda v, dt=torch.float32: torch.full((B,), v, dtype=dt, device=dev)  # noqa: E731
     got = serve.sample(x.to(dev), u.to(dev), temperature=full(f["t"]) if "t" in f else None,
                        top_k=full(f["top_k"], torch.int32) if "top_k" in f else None,
-                       top_p=full(f["top_p"]) if "top_p" in f else None, min_p=full(f["min_p"]) if "min_p" in f else None)
+                       top_p=full(f["top_p"]) if "top_p" in f else None,
+                       min_p=full(f["min_p"]) if "min_p" in f else None)
     tok, lp, kept = (a.cpu().numpy() for a in got)
     f = {k: float(np.float32(v)) if k in ("top_p", "min_p") else v for k, v in f.items()}
     for b in range(B):

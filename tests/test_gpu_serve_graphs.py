@@ -37,15 +37,16 @@ def nodes(graph):
                                             ("chunks", 40000, 1 + 3 + 5)])
 def test_a_captured_step_is_kernels_one_after_the_other(dev, form, V, kernels):
     """No memset or copy among them: on replays after the first, memset nodes have not done their work."""
-    b = O.Batch(5, [1, 20] if form == "chunks" else [1, 1], [90, 40], 70 if form == "behind a prefix" else 0, 4, 2, 64, "f16",
-                "f16", 16, decode=form != "chunks")
+    new, P = [1, 20] if form == "chunks" else [1, 1], 70 if form == "behind a prefix" else 0
+    b = O.Batch(5, new, [90, 40], P, 4, 2, 64, "f16", "f16", 16, decode=form != "chunks")
     cache, batch, q = b.device(dev)
     rope, T = serve.Rope(64, device=dev), b.T
     k = torch.randn(T, 2, 64, device=dev).half()
     logits, u = torch.randn(T, V, device=dev), torch.rand(T, device=dev)
 
     def step():
-        return serve.attention(cache, batch, serve.rope_append(cache, batch, q, k, k, rope=rope)), serve.sample(logits, u)
+        r = serve.rope_append(cache, batch, q, k, k, rope=rope)
+        return serve.attention(cache, batch, r), serve.sample(logits, u)
 
     step()
     torch.cuda.synchronize()

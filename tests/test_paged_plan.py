@@ -42,7 +42,8 @@ def C(tmp_path_factory):
     src, so = os.path.join(d, "plan.cpp"), os.path.join(d, "plan.so")
     with open(src, "w") as f:
         f.write(SRC)
-    subprocess.run([build.CXX, "-std=c++17", "-O2", "-Wall", "-fPIC", "-shared", "-I", build.CSRC, "-o", so, src], check=True)
+    subprocess.run([build.CXX, "-std=c++17", "-O2", "-Wall", "-fPIC", "-shared", "-I", build.CSRC, "-o", so, src],
+                   check=True)
     lib = ctypes.CDLL(so)
     for name in ("t_slot", "t_unit"):
         getattr(lib, name).restype = ctypes.c_longlong
@@ -88,8 +89,8 @@ def test_shares(C, U, groups):
         assert 0 <= w < n and start[w] <= u < start[w + 1]
 
 
-@pytest.mark.parametrize("s,e,T", [(0, 5, 5), (-7, 2, 5), (2, 50, 5), (2, 2 ** 31 - 1, 5), (-2 ** 31, 2 ** 31 - 1, 9), (4, 2, 5),
-                                   (9, 12, 5), (2 ** 31 - 1, -2 ** 31, 3), (3, 3, 5), (0, 0, 0)])
+@pytest.mark.parametrize("s,e,T", [(0, 5, 5), (-7, 2, 5), (2, 50, 5), (2, 2 ** 31 - 1, 5), (-2 ** 31, 2 ** 31 - 1, 9),
+                                   (4, 2, 5), (9, 12, 5), (2 ** 31 - 1, -2 ** 31, 3), (3, 3, 5), (0, 0, 0)])
 def test_tokens_are_clamped(C, s, e, T):
     lo, hi = (min(max(x, 0), T) for x in (s, e))
     t0, n = clamp(C, s, e, T)
@@ -152,7 +153,8 @@ def test_a_planned_batch_fits_its_workspace(C, seed):
     assert slots * R * 8 <= z["ml"] and len(nk) * HKV * 8 <= z["where"]
     replay(C, nk, HKV, C.t_groups(), slots)
     asked = library_asks(B, T, G, HKV, D, P, planned=True)
-    assert asked == max(sizes(C, 1, B, T, G, HKV, C.t_rows(D, x), DT, P)["total"] for x in (1, 2)) and asked >= z["total"]
+    assert asked == max(sizes(C, 1, B, T, G, HKV, C.t_rows(D, x), DT, P)["total"] for x in (1, 2))
+    assert asked >= z["total"]
 
 
 def library_asks(B, T, G, HKV, D, P, planned):

@@ -14,7 +14,8 @@ def launched(tmp_path_factory):
 
 
 def sample_launches(launched, B, V, type=0):
-    return launched("bpd_sample_gpu", A, type, V, B, V, None, None, None, None, 2 * A, 3 * A, None, None, 4 * A, 1 << 40)
+    none = [None] * 4
+    return launched("bpd_sample_gpu", A, type, V, B, V, *none, 2 * A, 3 * A, None, None, 4 * A, 1 << 40)
 
 
 def slice_of(launched, B, V):
