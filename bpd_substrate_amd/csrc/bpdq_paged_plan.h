@@ -1,5 +1,5 @@
-// bpdq_paged_plan.h — the index arithmetic of the paged kernels that needs neither a GPU nor its intrinsics: divisions by
-// the page size, which share takes which units, places of results, tiles and the workspace.  The kernels and their
+// bpdq_paged_plan.h — the index arithmetic of the paged kernels that needs neither a GPU nor its intrinsics: divisions
+// by the page size, which share takes which units, places of results, tiles and the workspace.  The kernels and their
 // launchers include it as the CPU's tests do.
 #pragma once
 #include <stdint.h>
@@ -48,7 +48,9 @@ BPDQ_BOTH constexpr int units_of(int v) { return (v + 63) / 64; }
 // the order then find in the L2 of their XCD.  [w U / n, (w + 1) U / n) go to share w of n = min(groups, U).
 // A share leaves at most one result per (head, item): share and pair never repeat together
 // in share + pair, as each step along the units raises one or both.
-BPDQ_BOTH int64_t slot_of(int share, int item, int nitems, int h) { return (int64_t)share + (int64_t)h * nitems + item; }
+BPDQ_BOTH int64_t slot_of(int share, int item, int nitems, int h) {
+    return (int64_t)share + (int64_t)h * nitems + item;
+}
 BPDQ_BOTH int64_t unit_of(int w, int64_t U, int n) { return w * U / n; }
 BPDQ_BOTH int group_of(int64_t u, int64_t U, int n) { return (int)(((u + 1) * n - 1) / U); }
 // Whether a sequence's n tokens of G heads fill half a tile by themselves: then it takes the prefix's keys too.

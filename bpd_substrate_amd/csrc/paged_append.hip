@@ -7,8 +7,9 @@
 // position 2^20 that leaves 2^-33 revolutions, below fp32's rounding of the sine.
 // Everything is read and written once.  One workgroup per token: its rot/2 sines
 // are taken once and serve every head, and its row of the cache is looked up once.  Bound by
-// memory where there are many tokens: 6,343 of 32 + 2 x 8 heads of 128, 156 MB in and out, 31 us = 5.0 TB/s, what a copy
-// reaches; a few tokens take the latency of lengths, sines and rows, 4.5 us.
+// memory where there are many tokens: 6,343 of 32 + 2 x 8 heads of 128, 156 MB in and out, 31 us = 5.0 TB/s, what a
+// copy reaches; a few tokens take the latency of lengths, sines and rows one after the other, 4.5 us, and 1,740 (20 + 2
+// x 5 heads of 96, 48 turning) 9.3 us where their bytes take 4: q waits for the sines, k and v for the page as well.
 #include "bpdq_paged.h"
 
 namespace bpdq {

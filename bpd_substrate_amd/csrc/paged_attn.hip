@@ -27,10 +27,11 @@
 //
 // Measured, bf16 unless said (H 32, 8 kv heads, D 128; calls back to back):
 //   8 chunks of up to 512 tokens, 3,070 in all, over 4096
-//   shared and up to 1024 own keys                        333 us   705 TFLOP/s (an 8192^3 product: 1256)
+//   shared and up to 1024 own keys                        332 us   705 TFLOP/s (an 8192^3 product: 1256)
+//   the same with fp32 queries, f16 / bf16 pages          586 / 682 us
 //   32 sequences of up to 8192 own keys, 670 MB           113 us   5.9 TB/s (reads alone: 6.8)
 //   256 sequences behind 32,768 shared keys, 1024 own     243 us   140 GFLOP and 781 MB: 112 + 115 us
-//   64 sequences (f16) behind 8192 shared keys, 600 own    45 us   9 GFLOP and 130 MB: 14 + 19 us
+//   64 sequences (f16) behind 8192 shared keys, 600 own    46 us   9 GFLOP and 130 MB: 14 + 19 us
 //   1 sequence of 300 keys, D 64                           14 us   two launches
 #include <type_traits>
 
@@ -255,7 +256,8 @@ __device__ __forceinline__ float xor_max(float x) {
 
 // Elements 8 (4 k + lg) .. + 7 of a query, in binary32; zeros behind its end and for a row that is none.
 template <int KS, typename Q>
-__device__ __forceinline__ void load_query(const Q* __restrict__ q, bool row, int per, int lg, float sign, float (&x)[KS][8]) {
+__device__ __forceinline__ void load_query(const Q* __restrict__ q, bool row, int per, int lg, float sign,
+                                           float (&x)[KS][8]) {
 #pragma unroll
     for (int k = 0; k < KS; k++) {
         const int c = 4 * k + lg;
@@ -347,7 +349,8 @@ struct Lds {
 // Bit 15 of each half: that 16-bit value is an infinity or NaN (the exponent's carry).
 template <int CT>
 __device__ __forceinline__ uint32_t not_finite(uint32_t d) {
-    constexpr uint32_t e = CT == BPD_T_F16 ? 0x7C007C00u : 0x7F807F80u, one = CT == BPD_T_F16 ? 0x04000400u : 0x00800080u;
+    constexpr uint32_t e = CT == BPD_T_F16 ? 0x7C007C00u : 0x7F807F80u;
+    constexpr uint32_t one = CT == BPD_T_F16 ? 0x04000400u : 0x00800080u;
     return ((d & e) + one) & 0x80008000u;
 }
 template <int CT>
@@ -372,8 +375,9 @@ __device__ __forceinline__ u32x2 read_tr(const uint8_t* p) {
 //
 // 8 waves of 32 rows: a half's K operands serve both row tiles of a wave, and 256 rows share what a unit brings to
 // LDS.  What bounds it at 705 TFLOP/s: a SIMD's two waves are both in their softmax for part of the time (matrix units
-// busy 32 % of the clocks, vector units 42 %, no LDS conflicts).  Measured and left: K of the next half read behind P V (338 us against 334),
-// wave priorities around the products (no change).
+// busy 32 % of the clocks, vector units 42 %, no LDS conflicts), and registers: all 256, with 9-11 vector and 87-143
+// scalar ones of the 16-bit form kept aside.  Measured and left: K of the next half read behind P V (338 us against
+// 334), wave priorities around the products (no change).
 template <int QT, int CT, int NS, int DT, int MT, int NW, bool UNI>
 __device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w, int groups) {
     using M = Mfma<CT>;
@@ -450,8 +454,8 @@ __device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w,
             const int i = query_of(m, tok, hq);
             lim[m] = tok < 0 ? -1 : b >= 0 ? seen_rows(a, b, n, i, own) : 0;
             float x[KS][8];
-            load_query<KS>(reinterpret_cast<const Q*>(g.q) + max(tok, 0) * g.qs + (int64_t)hq * a.D, tok >= 0, per, lg, sign,
-                           x);
+            load_query<KS>(reinterpret_cast<const Q*>(g.q) + max(tok, 0) * g.qs + (int64_t)hq * a.D, tok >= 0, per, lg,
+                           sign, x);
             e2[m] = 0;
             if constexpr (NS > 1 && CT == BPD_T_F16) e2[m] = row_exponent<KS>(x);
 #pragma unroll
@@ -505,7 +509,8 @@ __device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w,
                 key_of(t, j, i, top);
                 const bool there = pg[j] >= 0 && pg[j] < a.n_pages;
                 const int64_t at = 2 * row_at(a, pg[j], i - fdiv(a.page, i) * (int)a.page.d);
-                const auto *kp = reinterpret_cast<const uint4*>(kthread + at), *vp = reinterpret_cast<const uint4*>(vthread + at);
+                const auto* kp = reinterpret_cast<const uint4*>(kthread + at);
+                const auto* vp = reinterpret_cast<const uint4*>(vthread + at);
                 if (UNI && there && i + LR <= top && per == CPR) {  // all lanes
                     rin[j] = true;
                     rk[j] = *kp;
@@ -563,7 +568,8 @@ __device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w,
                             for (int m = 0; m < MT; m++)
 #pragma unroll
                                 for (int x = 0; x < NS; x++)
-                                    sc4[kk][m] = M::go(kf[kk][k], qf[m][k][x], k == 0 && x == 0 ? bias[kk] : sc4[kk][m]);
+                                    sc4[kk][m] = M::go(kf[kk][k], qf[m][k][x],
+                                                       k == 0 && x == 0 ? bias[kk] : sc4[kk][m]);
                     u32x4 vf[NE];
 #pragma unroll
                     for (int e = 0; e < NE; e++)
@@ -601,7 +607,8 @@ __device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w,
 #pragma unroll
                         for (int e = 0; e < 8; e++)
                             p[m][e] = __builtin_amdgcn_exp2f(fmaf(sc4[e >> 2][m][e & 3], qscale[m], -base));
-                        s8[m] = ((p[m][0] + p[m][1]) + (p[m][2] + p[m][3])) + ((p[m][4] + p[m][5]) + (p[m][6] + p[m][7]));
+                        s8[m] = ((p[m][0] + p[m][1]) + (p[m][2] + p[m][3])) +
+                                ((p[m][4] + p[m][5]) + (p[m][6] + p[m][7]));
                     };
                     bool over = fresh;
 #pragma unroll
@@ -698,7 +705,8 @@ __device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w,
                     store_row4<Q, NE>(reinterpret_cast<Q*>(g.out) + tok * g.os + (int64_t)hq * a.D, a.D, lg, o[m],
                                          l[m] != 0.f ? 1.f / l[m] : 0.f);
                     if (g.lse != nullptr && lg == 0)
-                        g.lse[(int64_t)tok * g.H + hq] = l[m] != 0.f ? (ref[m] + __builtin_log2f(l[m])) * kLn2 : kNegInf;
+                        g.lse[(int64_t)tok * g.H + hq] =
+                            l[m] != 0.f ? (ref[m] + __builtin_log2f(l[m])) * kLn2 : kNegInf;
                 } else {
                     const int64_t row = slot * g.R + (wave * MT + m) * 16 + col;
                     store_row4<float, NE>(g.part + row * DT, DT, lg, o[m], 1.f);
@@ -722,7 +730,8 @@ __device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT
     using T = typename M::T;
     using Q = typename Elem<QT>::type;
     constexpr int KS = DT / 32, NE = DT / 16, VD = DT < 128 ? 2 : 4, VB = DT < 128 ? 1 : DT / 128;
-    constexpr int BUF = UNI && (DT == 64 || (DT == 128 && NS == 1)) ? 2 : 1;  // units in flight: what 256 registers hold
+    // units in flight: what 256 registers hold
+    constexpr int BUF = UNI && (DT == 64 || (DT == 128 && NS == 1)) ? 2 : 1;
     const Paged& a = g.a;
     const int lane = (int)threadIdx.x & 63, col = lane & 15, lg = lane >> 4;
     const int per = a.D / 8;
@@ -804,15 +813,15 @@ __device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT
             }
         };
         auto load = [&](u32x4 (&to)[8][VB], uint32_t& oks, const T* base, const int (&p)[2], int t) {
+            // a whole unit: two scalar bases, the lane's part the same for each
             if (UNI && all_lanes && t * 32 + 32 <= own && (uint32_t)p[0] < (uint32_t)a.n_pages &&
-                (uint32_t)p[1] < (uint32_t)a.n_pages) {  // a whole unit: two scalar bases, the lane's part the same for each
+                (uint32_t)p[1] < (uint32_t)a.n_pages) {
                 oks = 255u;
                 auto get = [&](auto nt) {
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
-                        const int i0 = t * 32 + 16 * x;
-                        const auto* at =
-                            reinterpret_cast<const uint8_t*>(base + row_at(a, p[x], i0 - fdiv(a.page, i0) * (int)a.page.d));
+                        const int i0 = t * 32 + 16 * x, in_page = i0 - fdiv(a.page, i0) * (int)a.page.d;
+                        const auto* at = reinterpret_cast<const uint8_t*>(base + row_at(a, p[x], in_page));
 #pragma unroll
                         for (int j = 0; j < 4; j++)
 #pragma unroll
@@ -905,7 +914,8 @@ __device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT
                     if constexpr (VD == 4)
                         *reinterpret_cast<u32x4*>(&ks[row][k_slot<DT>(row, vb * 16 + col)]) = n.k[j][vb];
                     else
-                        reinterpret_cast<u32x2*>(&ks[row][k_slot<DT>(row, col >> 1)])[col & 1] = u32x2{n.k[j][vb][0], n.k[j][vb][1]};
+                        reinterpret_cast<u32x2*>(&ks[row][k_slot<DT>(row, col >> 1)])[col & 1] =
+                            u32x2{n.k[j][vb][0], n.k[j][vb][1]};
                 }
             const uint32_t ok = n.ok;
             const bool more = t + BUF < k1;
@@ -984,7 +994,8 @@ __device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT
                 const float inv = l != 0.f ? 1.f / l : 0.f;
                 Q* out = reinterpret_cast<Q*>(g.out) + b * g.os + (int64_t)h * a.D;
                 store_row<Q, VD, VB>(out, a.D, lg, o, inv);
-                if (g.lse != nullptr && lg == 0) g.lse[(int64_t)b * g.H + h] = l != 0.f ? (ref + __builtin_log2f(l)) * kLn2 : kNegInf;
+                if (g.lse != nullptr && lg == 0)
+                    g.lse[(int64_t)b * g.H + h] = l != 0.f ? (ref + __builtin_log2f(l)) * kLn2 : kNegInf;
             } else {
                 store_row<float, VD, VB>(g.part1 + (slot * g.G + col) * DT, DT, lg, o, 1.f);
                 if (lg == 0) g.ml1[slot * g.G + col] = make_float2(ref, l);
@@ -1060,9 +1071,9 @@ __device__ __forceinline__ bool sees_a_row(const Paged& a, int b, int n, int i) 
 // Joins what was left of each (token, query head): its packed results, then its sequence's.  A
 // workgroup takes a token and HW heads for each of its 4 waves; a lane looks up one of the wave's heads.
 // Three dependent lookups and the results bound it: 8 us at 64 tokens of 32 heads, 12 at 256, 21 at 3,070.
-// A query with infinities or NaN has NaN for k_attn_tile's rows that are not there too (0 times infinity).  Where all are
-// absent the result is that of no row; that is looked for here, as a mask within the tiles' loop or at their items' ends took
-// 2 % of the prompt chunks' time.
+// A query with infinities or NaN has NaN for k_attn_tile's rows that are not there too (0 times infinity).  Where all
+// are absent the result is that of no row; that is looked for here, as a mask within the tiles' loop or at their items'
+// ends took 2 % of the prompt chunks' time.
 template <int QT, int HW>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs g) {
     using Q = typename Elem<QT>::type;
@@ -1135,7 +1146,8 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs g) {
 #pragma unroll
         for (int k = 0; k < FEW; k++) {
             x[k] = make_float2(kNegInf, 0.f);
-            if (!done && k < wp.y + wo.y) x[k] = k < wp.y ? g.ml[sp + (int64_t)k * g.R] : ml1[so + (int64_t)(k - wp.y) * R1];
+            if (!done && k < wp.y + wo.y)
+                x[k] = k < wp.y ? g.ml[sp + (int64_t)k * g.R] : ml1[so + (int64_t)(k - wp.y) * R1];
             m = fmaxf(m, x[k].x);
         }
 #pragma unroll
@@ -1160,14 +1172,16 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs g) {
             for (int k = 0; k < FEW; k++) {
                 const float fk = __shfl(f[k], j);
                 if (skip || k >= n || fk == 0.f) continue;  // nothing, or what is not there
-                const float* p = k < np ? g.part + (p0 + (int64_t)k * g.R) * g.DT : part1 + (p1 + (int64_t)(k - np) * R1) * g.DT;
+                const float* p = k < np ? g.part + (p0 + (int64_t)k * g.R) * g.DT
+                                        : part1 + (p1 + (int64_t)(k - np) * R1) * g.DT;
                 acc += *reinterpret_cast<const f32x4*>(p + 4 * piece) * fk;
             }
             if (!skip && 4 * piece < a.D) {
                 Vec<Q, 4> v;
 #pragma unroll
                 for (int c = 0; c < 4; c++) v.v[c] = (Q)acc[c];
-                *reinterpret_cast<Vec<Q, 4>*>(reinterpret_cast<Q*>(g.out) + t * g.os + (int64_t)(h0 + j) * a.D + 4 * piece) = v;
+                Q* to = reinterpret_cast<Q*>(g.out) + t * g.os + (int64_t)(h0 + j) * a.D + 4 * piece;
+                *reinterpret_cast<Vec<Q, 4>*>(to) = v;
             }
         }
         return;
@@ -1176,7 +1190,8 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs g) {
         const int j = __builtin_ctzll(todo);
         todo &= todo - 1;
         const int np = __shfl(wp.y, j), no = __shfl(wo.y, j);
-        const int64_t sp = (int64_t)__shfl(wp.x, j) * g.R + __shfl(rp, j), so = (int64_t)__shfl(wo.x, j) * R1 + __shfl(ro, j);
+        const int64_t sp = (int64_t)__shfl(wp.x, j) * g.R + __shfl(rp, j);
+        const int64_t so = (int64_t)__shfl(wo.x, j) * R1 + __shfl(ro, j);
         auto ml_at = [&](int k) {
             return k < np ? g.ml[sp + (int64_t)k * g.R] : ml1[so + (int64_t)(k - np) * R1];
         };
@@ -1229,7 +1244,8 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs g) {
             for (int c = 0; c < 4; c++) v.v[c] = (Q)(acc[c] * inv);
             *reinterpret_cast<Vec<Q, 4>*>(reinterpret_cast<Q*>(g.out) + t * g.os + (int64_t)h * a.D + 4 * piece) = v;
         }
-        if (g.lse != nullptr && lane == 0) g.lse[(int64_t)t * g.H + h] = any ? (m + __builtin_log2f(l)) * kLn2 : kNegInf;
+        if (g.lse != nullptr && lane == 0)
+            g.lse[(int64_t)t * g.H + h] = any ? (m + __builtin_log2f(l)) * kLn2 : kNegInf;
     }
 }
 
@@ -1266,7 +1282,8 @@ void launch_types(const AttnArgs& g, hipStream_t s) {
     if ((int64_t)g.a.T * g.H <= 32768)
         hipLaunchKernelGGL((k_attn_join<QT, 1>), dim3((unsigned)g.a.T, (unsigned)((g.H + 3) / 4)), dim3(256), 0, s, g);
     else
-        hipLaunchKernelGGL((k_attn_join<QT, 8>), dim3((unsigned)g.a.T, (unsigned)((g.H + 31) / 32)), dim3(256), 0, s, g);
+        hipLaunchKernelGGL((k_attn_join<QT, 8>), dim3((unsigned)g.a.T, (unsigned)((g.H + 31) / 32)), dim3(256), 0, s,
+                           g);
 }
 
 }  // namespace
@@ -1298,7 +1315,8 @@ void launch_attn_paged(const Paged& a0, int cache_type, const void* q, int64_t q
     g.DT = padded(a.D);
     g.groups = kGroups;
     g.waves = kStreamWaves;
-    // us of a CU: 64 keys x 256 rows of 128 by 8 waves (630 TFLOP/s), 32 keys of 128 (a CU draws 34 GB/s beside the others)
+    // us of a CU: 64 keys x 256 rows of 128 by 8 waves (630 TFLOP/s), 32 keys of 128 (a CU draws 34 GB/s beside the
+    // others)
     const int parts = q_type != BPD_T_F32 ? 1 : cache_type == BPD_T_BF16 ? 3 : 2;
     g.tile_cost = 3.4f * (float)(g.R * g.DT * parts) / (256.f * 128.f) * (g.DT == 256 ? 2.f : 1.f);
     g.wave_cost = 0.48f * (float)g.DT / 128.f;

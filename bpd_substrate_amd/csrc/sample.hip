@@ -15,10 +15,12 @@
 // slice of a row, and k_cut and k_draw with one per row.  A row whose list is too long (thousands of equal
 // logits at the cut) is searched digit by digit instead.
 //
-// Measured (calls back to back): 1 row of 32,000, top-k and top-p, 18 us, one launch, latency; 64 rows of 128,256 (fp32,
-// mixed settings) 55 us; 256 rows of 128,256 (binary16, top-p) 97 us: max 16 (66 MB at 4.2 TB/s), hist 34 (28 vector
-// instructions a logit, which keep their units busy 93 % of it), cut 8, pick 22, draw 25 (latency of a workgroup).  Left: a slice's first loads
-// ahead of its row's settings (their registers cost a workgroup of four per CU: hist 34 -> 37 us).
+// Measured (calls back to back): 1 row of 32,000, top-k and top-p, 18 us, one launch, latency; 64 rows of 128,256
+// (fp32, mixed settings) 51-54 us; 256 rows of 128,256 (binary16, top-p) 97 us, and of 128,257, whose rows lie at no
+// 16-byte border and are read by element, 145.  Traced apart the five launches of those 256 rows take 101 us: max 15 (66
+// MB at 4.4 TB/s), hist 32 (28 vector instructions a logit, which keep their units busy 93 % of it), cut 8, pick 22, draw
+// 25 (latency of a workgroup).  Left: a slice's first loads ahead of its row's settings (their registers cost a
+// workgroup of four per CU: hist 34 -> 37 us).
 #include "bpdq_paged.h"
 
 namespace bpdq {
@@ -46,7 +48,8 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
 
 // Buckets and weights go by the distance from the largest logit, d = (max - l) scale in binary64, b = d rounded:
 //   exp((l - max) / t) = exp(-b c) exp(-(d - b) c),  c = 1 / (scale t) <= 1 / 32,
-// the first from a table of the buckets (2^shift times it), the second by 6 terms of its series: 2^-54 of it is left out.
+// the first from a table of the buckets (2^shift times it), the second by 6 terms of its series: 2^-54 of it is left
+// out.
 struct Row {
     float top;            // the largest logit
     double max, scale;    // top, buckets per unit of logit
@@ -54,8 +57,11 @@ struct Row {
     double c, t;
     int shift;            // weights are multiples of 2^-shift
     const double* table;  // in LDS, kBuckets of them
-    // x up to max.  Grows as logits fall, up to the last bucket's, where only logits are that weigh nothing, -infinity and NaN
-    __device__ __forceinline__ double distance(double x) const { return __builtin_fmin((max - x) * scale, kBuckets - 0.6); }
+    // x up to max.  Grows as logits fall, up to the last bucket's, where only logits are that weigh nothing, -infinity
+    // and NaN
+    __device__ __forceinline__ double distance(double x) const {
+        return __builtin_fmin((max - x) * scale, kBuckets - 0.6);
+    }
     __device__ __forceinline__ int bucket(double x) const {
         return (int)(uint32_t)__double_as_longlong(distance(x) + 6755399441055744.0);  // 1.5 2^52: rounds, low bits
     }
@@ -185,7 +191,8 @@ __device__ __forceinline__ void each(const X* __restrict__ x, int lo, int hi, F&
         for (int i0 = lo; i0 < hi; i0 += 4 * STEP) {
             Vec<X, N> v[4];
 #pragma unroll
-            for (int c = 0; c < 4; c++) v[c] = *reinterpret_cast<const Vec<X, N>*>(x + i0 + c * STEP + (int)threadIdx.x * N);
+            for (int c = 0; c < 4; c++)
+                v[c] = *reinterpret_cast<const Vec<X, N>*>(x + i0 + c * STEP + (int)threadIdx.x * N);
 #pragma unroll
             for (int c = 0; c < 4; c++)
 #pragma unroll
@@ -403,8 +410,8 @@ struct SearchLds {
     u64 w;
 };
 template <typename X>
-__device__ __forceinline__ void search_row(const SampleArgs& g, int row, const X* x, const Row& r, const Set& set, uint32_t n,
-                                           SearchLds& s) {
+__device__ __forceinline__ void search_row(const SampleArgs& g, int row, const X* x, const Row& r, const Set& set,
+                                           uint32_t n, SearchLds& s) {
     auto& hc = s.hc;
     auto& ties = s.ties;
     auto& hw = s.hw;
@@ -669,9 +676,9 @@ struct DrawLds {
 // ---- draw: from the list (n_list entries, in LDS), n_stay logits that stay whatever it says and the slices'
 // weights of those; S slices of len elements.  kThreads threads.
 template <typename X>
-__device__ __forceinline__ void draw_row(const SampleArgs& g, int row, const X* x, const Row& r, const Set& set, Mode mode,
-                                         const Pick& pick, const Sum* sums, int S, int len, uint32_t n_list, uint32_t n_stay,
-                                         DrawLds& s) {
+__device__ __forceinline__ void draw_row(const SampleArgs& g, int row, const X* x, const Row& r, const Set& set,
+                                         Mode mode, const Pick& pick, const Sum* sums, int S, int len, uint32_t n_list,
+                                         uint32_t n_stay, DrawLds& s) {
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     sort_falling(s.list, (int)n_list, s.rank);  // by logit, equal ones by index
     // how many of the list stay.  Every loop here is kept rolled: a row's workgroup runs through this code
@@ -720,7 +727,8 @@ __device__ __forceinline__ void draw_row(const SampleArgs& g, int row, const X* 
                 const u64 run = run0 + scan_block<kThreads>(v, all, s.part);
                 run0 += all;
                 if (pass == 0 && kept_list > (uint32_t)kThreads) continue;
-                const u64 t = kept_list > (uint32_t)kThreads ? target : draw_target(set.u, all), sum = pass == 0 ? all : total;
+                const u64 t = kept_list > (uint32_t)kThreads ? target : draw_target(set.u, all);
+                const u64 sum = pass == 0 ? all : total;
                 if (run <= t && run + v > t)
                     answer(g, row, (int)~(uint32_t)(e >> 32), (float)log((double)v / (double)sum), kept);
             }
@@ -803,7 +811,8 @@ __device__ __forceinline__ void draw_row(const SampleArgs& g, int row, const X* 
 
 // The first index of the largest logit, which [lo, hi) holds.
 template <typename X>
-__device__ __forceinline__ void greedy_row(const SampleArgs& g, int row, const X* x, int lo, int hi, float top, uint32_t* s_at) {
+__device__ __forceinline__ void greedy_row(const SampleArgs& g, int row, const X* x, int lo, int hi, float top,
+                                           uint32_t* s_at) {
     if (threadIdx.x == 0) *s_at = 0xFFFFFFFFu;
     __syncthreads();
     uint32_t at = 0xFFFFFFFFu;
@@ -880,7 +889,8 @@ __global__ __launch_bounds__(kThreads) void k_sample_row(SampleArgs g, int shift
         // histogram of all 32,000: 2.8 us)
         if (mode == kTopK && 2 * set.k <= min(kThreads, g.V / N)) part_hist([&](auto&& f) { f(0, mine); }, r, mode, hw);
         else part_hist(visit, r, mode, hw);
-        const Pick pick = mode == kTopK ? find_buckets(reinterpret_cast<const uint32_t*>(hw), 0, 1, r, set, mode, s_find.n)
+        const uint32_t* hc = reinterpret_cast<const uint32_t*>(hw);
+        const Pick pick = mode == kTopK ? find_buckets(hc, 0, 1, r, set, mode, s_find.n)
                                         : find_buckets(hw, 0, 1, r, set, mode, s_find.w);
         uint32_t n_stay = m.n, n_list = 0;
         if (pick.first < kBuckets) {
@@ -941,7 +951,8 @@ __global__ __launch_bounds__(kSliceThreads) void k_hist(SampleArgs g, Work w) {
     using X = typename Elem<TYPE>::type;
     __shared__ double table[kBuckets];
     __shared__ u64 hw[kBuckets];
-    const int row = (int)(blockIdx.x / (unsigned)w.S), slice = (int)(blockIdx.x % (unsigned)w.S), tid = (int)threadIdx.x;
+    const int row = (int)(blockIdx.x / (unsigned)w.S), slice = (int)(blockIdx.x % (unsigned)w.S);
+    const int tid = (int)threadIdx.x;
     const Set set = settings(g, row);
     const Max m = row_max(w, row);
     const Mode mode = mode_of(set, m);
@@ -980,7 +991,8 @@ __global__ __launch_bounds__(kSliceThreads) void k_pick(SampleArgs g, Work w) {
     using X = typename Elem<TYPE>::type;
     constexpr int T = kSliceThreads;
     __shared__ u64 s_part[T / 64];
-    const int row = (int)(blockIdx.x / (unsigned)w.S), slice = (int)(blockIdx.x % (unsigned)w.S), tid = (int)threadIdx.x;
+    const int row = (int)(blockIdx.x / (unsigned)w.S), slice = (int)(blockIdx.x % (unsigned)w.S);
+    const int tid = (int)threadIdx.x;
     const Set set = settings(g, row);
     const Max m = row_max(w, row);
     const Mode mode = mode_of(set, m);
@@ -1075,8 +1087,8 @@ int slice_len(int B, int V) {
     return len;
 }
 
-// Whether rows take one workgroup each or one per slice: as long as a workgroup holds them.  Measured at 32,000 logits: 1
-// row 29 us against 33, with top-k 18 against 29; 256 rows 37 against 55.
+// Whether rows take one workgroup each or one per slice: as long as a workgroup holds them.  Measured at 32,000 logits:
+// 1 row 29 us against 33, with top-k 18 against 29; 256 rows 37 against 55.
 bool by_row(int V) { return V <= kRow; }
 
 struct Layout {

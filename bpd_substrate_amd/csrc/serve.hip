@@ -177,7 +177,8 @@ void bpd_rope_append_paged_on_gpu(void* hip_stream, const bpd_paged_cache* kv, c
     if (n_heads > 0) {
         const int64_t row = (int64_t)es * n_heads * kv->head_dim, kv_row = (int64_t)es * kv->n_kv_heads * kv->head_dim;
         c.shape((q == q_out && q_stride == q_out_stride) ||
-                    !overlap(q, es * q_stride, row, q_out, es * q_out_stride, row, b->n_tokens), "q_out overlaps q and is not q");
+                    !overlap(q, es * q_stride, row, q_out, es * q_out_stride, row, b->n_tokens),
+                "q_out overlaps q and is not q");
         if (k != nullptr)
             c.shape(!overlap(q_out, es * q_out_stride, row, k, es * k_stride, kv_row, b->n_tokens) &&
                         !overlap(q_out, es * q_out_stride, row, v, es * v_stride, kv_row, b->n_tokens),
@@ -204,7 +205,8 @@ int64_t bpd_attn_paged_workspace(const bpd_paged_cache* kv, const bpd_paged_batc
     if (!c.ok) return -1;
     check_attn(c, *kv, *b, n_heads);
     if (!c.ok) return -1;
-    return bpdq::attn_paged_ws(b->q_start, b->n_seqs, b->n_tokens, n_heads, kv->n_kv_heads, kv->head_dim, b->prefix_len);
+    return bpdq::attn_paged_ws(b->q_start, b->n_seqs, b->n_tokens, n_heads, kv->n_kv_heads, kv->head_dim,
+                               b->prefix_len);
 }
 
 void bpd_attn_paged_on_gpu(void* hip_stream, const bpd_paged_cache* kv, const bpd_paged_batch* b, const void* q,
@@ -220,7 +222,8 @@ void bpd_attn_paged_on_gpu(void* hip_stream, const bpd_paged_cache* kv, const bp
     if (!c.ok || b->n_seqs == 0 || b->n_tokens == 0) return;
     const int es = esize(q_type);
     const int64_t row = (int64_t)n_heads * kv->head_dim;
-    c.ptr(q, 16, "q").stride(q_stride, row, es, "q_stride").ptr(out, 16, "out").stride(out_stride, row, es, "out_stride");
+    c.ptr(q, 16, "q").stride(q_stride, row, es, "q_stride");
+    c.ptr(out, 16, "out").stride(out_stride, row, es, "out_stride");
     if (lse != nullptr) c.ptr(lse, 4, "lse");
     if (!c.ok) return;
     // rows are written while others are still read
@@ -271,8 +274,8 @@ void bpd_sample_on_gpu(void* hip_stream, const void* logits, int type, int64_t r
     bpdq::WsLease lease;
     void* w = work_space(lease, ws, ws_bytes, bpdq::sample_ws(n_rows, vocab), stream, fn);
     if (w == nullptr) return;
-    bpdq::launch_sample({logits, row_stride, n_rows, vocab, temperature, top_k, top_p, min_p, u, token, logprob, n_kept},
-                        type, w, stream);
+    bpdq::launch_sample({logits, row_stride, n_rows, vocab, temperature, top_k, top_p, min_p, u, token, logprob,
+                         n_kept}, type, w, stream);
     bpdq::abi_hip_ok(hipGetLastError(), fn);
 }
 

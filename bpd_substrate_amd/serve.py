@@ -107,7 +107,8 @@ class PagedCache:
 
     @classmethod
     def empty(cls, n_pages, page_size, n_kv_heads, head_dim, dtype=torch.float16, device="cuda"):
-        make = lambda: torch.zeros(n_pages, n_kv_heads, page_size, head_dim, dtype=dtype, device=device).transpose(1, 2)  # noqa: E731
+        def make():
+            return torch.zeros(n_pages, n_kv_heads, page_size, head_dim, dtype=dtype, device=device).transpose(1, 2)
         return cls(make(), make())
 
 
@@ -228,7 +229,8 @@ def rope_append(cache, batch, q, k, v, rope=None, pos=None, q_out=None):
 
 def attention(cache, batch, q, scale=None, out=None, return_lse=False):
     """softmax(scale q k^T) v of every new token over the prefix's rows and its sequence's own up to
-    its own (bpd_attn_paged_gpu).  q [n_tokens, heads, head_dim], of the cache's type or float32, as is out.
+    its own (bpd_attn_paged_gpu).  q [n_tokens, heads, head_dim], of the cache's type or float32, as is out.  With q of
+    the cache's type the weights are rounded to it before they meet v; with a float32 q they keep 22 bits or more.
     scale: head_dim ** -0.5 unless given.  return_lse: also the float32 [n_tokens, heads] logarithm of each
     softmax's denominator.  Rows of a padded batch that belong to no sequence are left as they are
     in out; in a new tensor they are arbitrary."""
@@ -281,6 +283,6 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
     token, logprob, kept = res[0], res[1].view(torch.float32), res[2]
     n = _sample_workspace(B, V)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    _launch(dev, gpu._fn("bpd_sample_on_gpu"), logits.data_ptr(), TYPES[logits.dtype], logits.stride(0) if B > 1 else V, B, V,
-            *ptrs, token.data_ptr(), logprob.data_ptr(), kept.data_ptr(), ws.data_ptr(), n)
+    _launch(dev, gpu._fn("bpd_sample_on_gpu"), logits.data_ptr(), TYPES[logits.dtype], logits.stride(0) if B > 1 else V,
+            B, V, *ptrs, token.data_ptr(), logprob.data_ptr(), kept.data_ptr(), ws.data_ptr(), n)
     return token, logprob, kept

@@ -96,8 +96,11 @@ void bpd_rope_append_paged_gpu(const bpd_paged_cache* cache, const bpd_paged_bat
  * lse[t][h] (fp32, may be NULL) = log sum_i exp(scale * q . k_i).  A token
  * that sees no row gets zeros, and an lse of -infinity.  What stands in rows that a
  * token does not see (infinities and NaN too) does not reach its output.  q and out
- * [n_tokens][n_heads][head_dim] of q_type: the cache's type, or fp32, whose products
- * keep fp32's precision; rows of out and q do not overlap.  Tensors and token strides
+ * [n_tokens][n_heads][head_dim] of q_type: the cache's type, or fp32; rows of out and q do
+ * not overlap.  Scores, statistics and sums are fp32 for either.  With q of the cache's type
+ * the softmax's weights are rounded to that type once before they meet v (half a step of each,
+ * 2^-11 or 2^-8; the denominator sums them unrounded); with fp32 q they keep 22 bits (f16 pages)
+ * or 24 (bf16), as the queries do.  Tensors and token strides
  * 16-byte aligned (lse 4).  n_heads a multiple of n_kv_heads, up to 2^16; n_tokens up to
  * 2^23, times n_heads / n_kv_heads 2^26; beyond, and where the tokens' tiles times
  * the table's rows pass 2^31 units, BPDQ_ERR_LIMIT.
