@@ -189,7 +189,8 @@ class Rope:
 
 def rope_append(cache, batch, q, k, v, rope=None, pos=None, q_out=None):
     """Rotates q [n_tokens, heads, head_dim] and k, and writes k and v [n_tokens, n_kv_heads, head_dim]
-    into the new tokens' rows of the cache; returns the rotated q (q_out, which may be q itself).
+    into the new tokens' rows of the cache; returns the rotated q (q_out, which may be q itself).  Rows of a padded
+    batch that belong to no sequence are left as they are in q_out; in a new tensor they are arbitrary.
     q or both of k and v may be None.  rope None: nothing rotates.  pos int32 [n_tokens]: positions
     other than prefix_len + the token's index.  Token strides of q, k and v are free, so the
     parts of a fused projection's rows will do."""

@@ -27,7 +27,7 @@ def test_serving_calls_leave_the_launch_stream_alone(dev):
         gpu.call("bpd_gpu_set_stream", mine.cuda_stream)
         try:
             with torch.cuda.stream(mine):
-                torch.cuda._sleep(100_000_000)
+                torch.cuda._sleep(500_000_000)
             call()
             gpu.call("bpd_expf_gpu", x, y, 64)     # on `mine`, behind the sleep
             with torch.cuda.stream(other):
