@@ -81,9 +81,20 @@ struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Vec {
 void launch_rope_append(const Paged& a, int cache_type, const double* turns, int rot, bool neox, const int32_t* pos,
                         const void* q, int64_t qs, const void* k, int64_t ks, const void* v, int64_t vs, void* qo,
                         int64_t qos, int x_type, int H, hipStream_t s);
+struct HeadNorm {
+    const void *q, *k;
+    int type;
+    int64_t q_stride, k_stride;
+    float eps;
+};
+void launch_norm_append(const Paged& a, int cache_type, const HeadNorm& n, const double* turns, int rot, bool neox,
+                        const int32_t* pos, const void* q, int64_t qs, const void* k, int64_t ks, const void* v, int64_t vs,
+                        void* qo, int64_t qos, int x_type, int H, hipStream_t s);
 int64_t attn_paged_ws(const int32_t* q_start, int B, int T, int H, int HKV, int D, int P);
 void launch_attn_paged(const Paged& a, int cache_type, const void* q, int64_t qs, void* out, int64_t os, float* lse,
                        int q_type, int H, float scale, void* ws, hipStream_t s);
+void launch_attn_window(const Paged& a, int cache_type, const void* q, int64_t qs, void* out, int64_t os, float* lse,
+                        int q_type, int H, float scale, int window, int sinks, void* ws, hipStream_t s);
 int64_t sample_ws(int n_rows, int vocab);
 struct SampleArgs {
     const void* logits;
@@ -97,5 +108,45 @@ struct SampleArgs {
     int32_t* kept;
 };
 void launch_sample(const SampleArgs& a, int type, void* ws, hipStream_t s);
+struct AdjustArgs {
+    const void* x;
+    int64_t xs;
+    void* y;
+    int64_t ys;
+    int B, V;
+    const int32_t* tokens;
+    int64_t token_stride;
+    int width;
+    const int32_t *lens, *prompt;
+    const float *repetition, *frequency, *presence;
+    const int32_t *bias_start, *bias_token;
+    const float* bias_value;
+    int n_bias;
+    const int32_t* mask;
+    int64_t mask_stride;
+    int n_masks;
+    const int32_t* mask_row;
+    int slice, slices;  // the launcher's
+};
+void launch_adjust(const AdjustArgs& a, int type, int out_type, hipStream_t s);
+struct PoolArgs {
+    int32_t* table;
+    int64_t table_stride;
+    int W;
+    int32_t *lens, *gone, *free_pages, *n_free;
+    int n_rows, n_pages;
+    FastDiv page;
+    const int32_t *rows, *add, *keep;
+    int B, T;
+    int32_t* table_out;
+    int64_t table_out_stride;
+    int32_t *lens_out, *q_start, *slots, *pos, *refused;
+    int prefix_len, window, sinks;
+    int4* plan;  // [B + 1]
+    int parts;   // the launcher's
+};
+int64_t pages_ws(int B);
+void launch_pages_extend(const PoolArgs& a, hipStream_t s);
+void launch_pages_release(const PoolArgs& a, hipStream_t s);
 
 }  // namespace bpdq

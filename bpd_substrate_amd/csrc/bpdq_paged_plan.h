@@ -56,6 +56,41 @@ BPDQ_BOTH int group_of(int64_t u, int64_t U, int n) { return (int)(((u + 1) * n 
 // Whether a sequence's n tokens of G heads fill half a tile by themselves: then it takes the prefix's keys too.
 BPDQ_BOTH bool is_joint(int n, int G, int R) { return n * G * 2 >= R; }
 
+// The units of U rows that hold a row which tokens at positions `first` and later see through a window of W
+// positions or among the first S ones: of the prefix's P rows units [0, a1) and [b0, b1), of the own ones, `seen`
+// of them seen by the last token, [0, c1) and [d0, d1).  Positions of own rows begin at P.
+struct Span {
+    int a1, b0, b1, c1, d0, d1;
+};
+BPDQ_BOTH int64_t window_low(int64_t p, int W) { return p - W + 1 > 0 ? p - W + 1 : 0; }
+BPDQ_BOTH Span span_of(int64_t first, int W, int S, int P, int seen, int U) {
+    const int64_t low = window_low(first, W);
+    const int sp = S < P ? S : P, so = S - sp < seen ? S - sp : seen;  // of the first S rows
+    const int lp = low < P ? (int)low : P;                             // where the window begins
+    const int64_t lo64 = low < P ? 0 : low - P;
+    const int lo = lo64 < seen ? (int)lo64 : seen;
+    Span r;
+    r.a1 = (sp + U - 1) / U;
+    r.b1 = (P + U - 1) / U;
+    r.b0 = lp < P ? lp / U : r.b1;
+    if (r.b0 < r.a1) r.b0 = r.a1;
+    r.c1 = (so + U - 1) / U;
+    r.d1 = (seen + U - 1) / U;
+    r.d0 = lo < seen ? lo / U : r.d1;
+    if (r.d0 < r.c1) r.d0 = r.c1;
+    return r;
+}
+BPDQ_BOTH int prefix_units(const Span& r) { return r.a1 + r.b1 - r.b0; }
+BPDQ_BOTH int own_units(const Span& r) { return r.c1 + r.d1 - r.d0; }
+// Which unit of the prefix (pre) or of the own rows is the t-th of a span.
+BPDQ_BOTH int unit_at(const Span& r, int t, bool& pre) {
+    const int n = prefix_units(r);
+    pre = t < n;
+    if (pre) return t < r.a1 ? t : t - r.a1 + r.b0;
+    t -= n;
+    return t < r.c1 ? t : t - r.c1 + r.d0;
+}
+
 inline int padded(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 // Waves of a workgroup and 16-row tiles of a wave: 8 waves of 32 rows where the accumulators and the
 // parts of the queries fit the 256 registers of two waves per SIMD.

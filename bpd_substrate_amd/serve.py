@@ -7,7 +7,16 @@
     out   = serve.attention(cache, batch, q)
     token, logprob, kept = serve.sample(logits, u, temperature=t, top_k=k, top_p=p, min_p=m)
 
-PagedCache, PagedBatch and Rope describe tensors that the program owns: page tables,
+and around them what a serving loop does on the device from step to step:
+
+    pool  = serve.PagePool.empty(n_pages, 64, n_rows, width, windowed=True, device="cuda")
+    step  = pool.extend(new, n_tokens, rows=rows)                   # pages, tables, slots, positions
+    q     = serve.rope_append(cache, step.batch(), q, k, v, rope=rope, q_norm=wq, k_norm=wk)
+    out   = serve.attention(cache, step.batch(), q, window=1024, sinks=4)
+    logits = serve.adjust_logits(logits, tokens=t, lens=n, repetition=r, bias=b, mask=m)
+    pool.release(keep, rows=rows, window=1024, sinks=4)
+
+PagedCache, PagedBatch, PagePool and Rope describe tensors that the program owns: page tables,
 lengths and offsets stay on the device and may be changed in place between calls (and between
 the replays of a captured graph), their shapes may not.
 
@@ -42,6 +51,27 @@ class _Batch(ctypes.Structure):    # bpd_paged_batch
 
 class _Rope(ctypes.Structure):     # bpd_rope
     _fields_ = [("turns", ctypes.c_void_p), ("rot_dim", ctypes.c_int), ("neox", ctypes.c_int)]
+
+
+class _Pool(ctypes.Structure):     # bpd_page_pool
+    _fields_ = [("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int),
+                ("lens", ctypes.c_void_p), ("gone", ctypes.c_void_p), ("free_pages", ctypes.c_void_p),
+                ("n_free", ctypes.c_void_p), ("n_rows", ctypes.c_int), ("n_pages", ctypes.c_int),
+                ("page_size", ctypes.c_int)]
+
+
+class _Norm(ctypes.Structure):     # bpd_head_norm
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("type", ctypes.c_int), ("q_stride", ctypes.c_int64),
+                ("k_stride", ctypes.c_int64), ("eps", ctypes.c_float)]
+
+
+class _Rules(ctypes.Structure):    # bpd_logit_rules
+    _fields_ = [("tokens", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("token_width", ctypes.c_int),
+                ("lens", ctypes.c_void_p), ("prompt", ctypes.c_void_p), ("repetition", ctypes.c_void_p),
+                ("frequency", ctypes.c_void_p), ("presence", ctypes.c_void_p), ("bias_start", ctypes.c_void_p),
+                ("bias_token", ctypes.c_void_p), ("bias_value", ctypes.c_void_p), ("n_bias", ctypes.c_int),
+                ("mask", ctypes.c_void_p), ("mask_stride", ctypes.c_int64), ("n_masks", ctypes.c_int),
+                ("mask_row", ctypes.c_void_p)]
 
 
 def _bad(what):
@@ -159,12 +189,15 @@ class PagedBatch:
             _bad(f"prefix_len {self.prefix_len} is more than its pages hold")
 
 
-    def _workspace(self, cache, heads):
+    def _workspace(self, cache, heads, window, sinks):
         """Bytes that an attention call needs, which go by shapes alone."""
-        key = (heads, cache.n_kv_heads, cache.head_dim)
+        key = (heads, cache.n_kv_heads, cache.head_dim, window, sinks)
         n = self._bytes.get(key)
         if n is None:
-            n = gpu.call("bpd_attn_paged_workspace", cache._p, self._p, heads)
+            if window is None:
+                n = gpu.call("bpd_attn_paged_workspace", cache._p, self._p, heads)
+            else:
+                n = gpu.call("bpd_attn_window_paged_workspace", cache._p, self._p, heads, window, sinks)
             self._bytes[key] = n
         return n
 
@@ -187,13 +220,153 @@ class Rope:
         self._p = ctypes.addressof(self.c)
 
 
-def rope_append(cache, batch, q, k, v, rope=None, pos=None, q_out=None):
+class PageStep:
+    """What PagePool.extend gives: for n_seqs sequences and n_tokens new tokens, int32 on the device,
+
+    table    [n_seqs, width]: their pages, -1 behind them (the pool's own table where rows is None)
+    lens     [n_seqs]: their rows, the new ones' included
+    q_start  [n_seqs + 1]: first new token of each; q_start[n_seqs] of the n_tokens are granted
+    slots    [n_tokens]: every new token's row of the cache, page * page_size + row in it; -1 behind the last
+    pos      [n_tokens]: its position; -1 behind the last
+    refused  [n_seqs]: 0, or why a sequence got nothing: 1 no row, a row named twice or a negative number, 2 the
+             table's width, 3 pages, 4 n_tokens
+    """
+
+    def __init__(self, table, lens, q_start, slots, pos, refused, n_tokens, prefix_len):
+        self.table, self.lens, self.q_start, self.slots, self.pos, self.refused = table, lens, q_start, slots, pos, refused
+        self.n_tokens, self.prefix_len = n_tokens, prefix_len
+        self._batch = None
+
+    def batch(self, prefix=None):
+        """The PagedBatch of these sequences and tokens, behind the pages `prefix` of extend's prefix_len rows."""
+        if self._batch is None or self._batch.prefix is not prefix:
+            self._batch = PagedBatch(self.table, self.lens, q_start=self.q_start, n_tokens=self.n_tokens, prefix=prefix,
+                                     prefix_len=self.prefix_len)
+        return self._batch
+
+
+class PagePool:
+    """Pages that sequences take and give back on the device (bpd_page_pool).
+
+    table    int32 [n_rows, width]: the pages of each row's sequence, -1 where there is none
+    lens     int32 [n_rows]: its rows
+    free     int32 [n_pages]: in its first n_free[0] places the pages that no sequence holds
+    n_free   int32 [2]: their number, and a 0
+    gone     int32 [n_rows, 2] or None: the pages that slid out of a window; needed to release by window
+    """
+
+    def __init__(self, table, lens, free, n_free, page_size, gone=None):
+        i32 = (torch.int32,)
+        _tensor(table, "table", i32, 2)
+        self.device, (R, W) = table.device, table.shape
+        if W > 1 and table.stride(1) != 1 or R > 1 and table.stride(0) < W:
+            _bad("table's rows are not contiguous, or overlap")
+        for t, what, shape in ((lens, "lens", (R,)), (free, "free", None), (n_free, "n_free", (2,)), (gone, "gone", (R, 2))):
+            if t is None and what == "gone":
+                continue
+            _tensor(t, what, i32, 2 if what == "gone" else 1, self.device, contiguous=True)
+            if shape is not None and t.shape != shape:
+                _bad(f"{what} is {list(t.shape)}, not {list(shape)}")
+        self.table, self.lens, self.free, self.n_free, self.gone = table, lens, free, n_free, gone
+        self.n_rows, self.width, self.n_pages, self.page_size = R, W, free.shape[0], page_size
+        self.c = _Pool(table.data_ptr(), table.stride(0) if R > 1 else W, W, lens.data_ptr(),
+                       None if gone is None else gone.data_ptr(), free.data_ptr(), n_free.data_ptr(), R, free.shape[0],
+                       page_size)
+        self._p = ctypes.addressof(self.c)
+
+    @classmethod
+    def empty(cls, n_pages, page_size, n_rows, width, reserved=0, windowed=False, device="cuda"):
+        """A pool of n_pages pages of which the first `reserved` (a prefix's) are never handed out."""
+        if not 0 <= reserved <= n_pages:
+            _bad(f"reserved {reserved} is not in 0..{n_pages}")
+        z = lambda *s: torch.zeros(s, dtype=torch.int32, device=device)  # noqa: E731
+        free, n_free = z(n_pages), z(2)
+        free[:n_pages - reserved] = torch.arange(n_pages - 1, reserved - 1, -1, dtype=torch.int32, device=device)
+        n_free[0] = n_pages - reserved
+        return cls(z(n_rows, width) - 1, z(n_rows), free, n_free, page_size, z(n_rows, 2) if windowed else None)
+
+    def _rows(self, rows, t, what):
+        """How many sequences a call names, and where."""
+        if rows is not None:
+            _tensor(rows, "rows", (torch.int32,), 1, self.device, contiguous=True)
+        if t is not None:
+            _tensor(t, what, (torch.int32,), 1, self.device, contiguous=True)
+            if rows is not None and rows.shape != t.shape:
+                _bad(f"{what} has {t.shape[0]} values and rows {rows.shape[0]}")
+        n = t.shape[0] if t is not None else rows.shape[0] if rows is not None else self.n_rows
+        return n, None if rows is None else rows.data_ptr(), None if t is None else t.data_ptr()
+
+    def extend(self, new, n_tokens, rows=None, prefix_len=0):
+        """Sequence b, row rows[b] of the pool (None: row b), grows by new[b] rows (int32, on the device): a PageStep.
+        n_tokens: room for new tokens, the sum of new or more (bpd_pages_extend_gpu)."""
+        if new is None:
+            _bad("new is None")
+        B, rp, np_ = self._rows(rows, new, "new")
+        dev, T, W = self.device, n_tokens, self.width
+        if T < 0:
+            _bad("n_tokens is negative")
+        sizes = (B, B + 1, T, T, B, 0 if rows is None else B * W)
+        out = torch.empty(sum(sizes), dtype=torch.int32, device=dev)
+        lens, q_start, slots, pos, refused, table = out.split(sizes)
+        if B == 0:
+            q_start.zero_()
+            slots.fill_(-1)
+            pos.fill_(-1)
+        table = self.table[:B] if rows is None else table.view(B, W)
+        n = _pages_workspace(B)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        _launch(dev, gpu._fn("bpd_pages_extend_on_gpu"), self._p, rp, np_, B, T, prefix_len,
+                None if rows is None else table.data_ptr(), W, lens.data_ptr(), q_start.data_ptr(), slots.data_ptr(),
+                pos.data_ptr(), refused.data_ptr(), ws.data_ptr(), n)
+        return PageStep(table, lens, q_start, slots, pos, refused, T, prefix_len)
+
+    def release(self, keep=None, rows=None, window=None, sinks=0, prefix_len=0):
+        """Sequence b keeps its first keep[b] rows (int32, on the device; None: all) and gives its other pages back; with a
+        window also those that neither the tokens to come see through it nor hold one of the first `sinks` positions, of
+        which the first prefix_len are a shared prefix's (bpd_pages_release_gpu).  rows and keep None: every row."""
+        B, rp, kp = self._rows(rows, keep, "keep")
+        if window is not None and window < 1:
+            _bad(f"window {window} is below 1")
+        if sinks < 0 or prefix_len < 0:
+            _bad("sinks or prefix_len is negative")
+        n = _pages_workspace(B)
+        ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+        _launch(self.device, gpu._fn("bpd_pages_release_on_gpu"), self._p, rp, kp, B, 0 if window is None else window,
+                max(0, sinks - prefix_len), ws.data_ptr(), n)
+
+
+@functools.lru_cache(maxsize=256)
+def _pages_workspace(n_seqs):
+    return gpu.call("bpd_pages_workspace", n_seqs)
+
+
+def _head_norm(q_norm, k_norm, eps, x, heads, kv_heads, D):
+    """bpd_head_norm of weights [head_dim] or [heads, head_dim], fp32 or of x's type."""
+    one = q_norm if q_norm is not None else k_norm
+    ptrs, strides = [], []
+    for w, what, h in ((q_norm, "q_norm", heads), (k_norm, "k_norm", kv_heads)):
+        if w is None:
+            ptrs.append(None)
+            strides.append(0)
+            continue
+        if w.dtype not in (torch.float32, x.dtype) or w.dtype != one.dtype or w.device != x.device:
+            _bad(f"{what} is {w.dtype} on {w.device}, not float32 or {x.dtype} on {x.device}, alike for q and k")
+        if w.shape != (D,) and w.shape != (h, D) or not w.is_contiguous():
+            _bad(f"{what} is not a contiguous [{D}] or [{h}, {D}]")
+        ptrs.append(w.data_ptr())
+        strides.append(0 if w.dim() == 1 else D)
+    return _Norm(*ptrs, TYPES[one.dtype], *strides, eps)
+
+
+def rope_append(cache, batch, q, k, v, rope=None, pos=None, q_out=None, q_norm=None, k_norm=None, eps=1e-6):
     """Rotates q [n_tokens, heads, head_dim] and k, and writes k and v [n_tokens, n_kv_heads, head_dim]
     into the new tokens' rows of the cache; returns the rotated q (q_out, which may be q itself).  Rows of a padded
     batch that belong to no sequence are left as they are in q_out; in a new tensor they are arbitrary.
     q or both of k and v may be None.  rope None: nothing rotates.  pos int32 [n_tokens]: positions
     other than prefix_len + the token's index.  Token strides of q, k and v are free, so the
-    parts of a fused projection's rows will do."""
+    parts of a fused projection's rows will do.
+    q_norm, k_norm: weights [head_dim] or [heads, head_dim], float32 or of q's type: every head of q or k becomes
+    x / sqrt(mean x^2 + eps) * weight before it turns (bpd_norm_rope_append_paged_gpu)."""
     batch._check(cache)
     T, D, dev = batch.n_tokens, cache.head_dim, cache.device
     x = q if q is not None else k
@@ -223,21 +396,30 @@ def rope_append(cache, batch, q, k, v, rope=None, pos=None, q_out=None):
         _tensor(pos, "pos", (torch.int32,), 1, dev, contiguous=True)
         if pos.shape[0] != T:
             _bad(f"pos has {pos.shape[0]} values for {T} tokens")
-    _launch(dev, gpu._fn("bpd_rope_append_paged_on_gpu"), cache._p, batch._p, None if rope is None else rope._p,
-            None if pos is None else pos.data_ptr(), qp, qs, kp, ks, vp, vs, op, os_, TYPES[x.dtype], H)
+    args = (None if rope is None else rope._p, None if pos is None else pos.data_ptr(), qp, qs, kp, ks, vp, vs, op, os_,
+            TYPES[x.dtype], H)
+    if q_norm is None and k_norm is None:
+        _launch(dev, gpu._fn("bpd_rope_append_paged_on_gpu"), cache._p, batch._p, *args)
+    else:
+        norm = _head_norm(q_norm, k_norm, eps, x, H, cache.n_kv_heads, D)
+        _launch(dev, gpu._fn("bpd_norm_rope_append_paged_on_gpu"), cache._p, batch._p, ctypes.addressof(norm), *args)
     return q_out
 
 
-def attention(cache, batch, q, scale=None, out=None, return_lse=False):
+def attention(cache, batch, q, scale=None, out=None, return_lse=False, window=None, sinks=0):
     """softmax(scale q k^T) v of every new token over the prefix's rows and its sequence's own up to
     its own (bpd_attn_paged_gpu).  q [n_tokens, heads, head_dim], of the cache's type or float32, as is out.  With q of
     the cache's type the weights are rounded to it before they meet v; with a float32 q they keep 22 bits or more.
     scale: head_dim ** -0.5 unless given.  return_lse: also the float32 [n_tokens, heads] logarithm of each
     softmax's denominator.  Rows of a padded batch that belong to no sequence are left as they are
-    in out; in a new tensor they are arbitrary."""
+    in out; in a new tensor they are arbitrary.
+    window: a token at position p (the prefix's rows are the first) sees positions p - window + 1 .. p alone, and of those
+    before them the first `sinks` (bpd_attn_window_paged_gpu); table entries of pages that none sees may be -1."""
     batch._check(cache)
     if q.dim() != 3:
         _bad(f"q has {q.dim()} dimensions, not 3")
+    if window is None and sinks != 0:
+        _bad("sinks without a window")
     T, H, D, dev = batch.n_tokens, q.shape[1], cache.head_dim, cache.device
     if q.dtype not in (cache.dtype, torch.float32):
         _bad(f"q is {q.dtype}, neither float32 nor the cache's {cache.dtype}")
@@ -246,11 +428,14 @@ def attention(cache, batch, q, scale=None, out=None, return_lse=False):
         out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
     os_ = _rows(out, "out", (T, H, D), q.dtype, dev)
     lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
-    n = batch._workspace(cache, H)
+    n = batch._workspace(cache, H, window, sinks)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    _launch(dev, gpu._fn("bpd_attn_paged_on_gpu"), cache._p, batch._p, q.data_ptr(), qs, out.data_ptr(), os_,
-            None if lse is None else lse.data_ptr(), TYPES[q.dtype], H, D ** -0.5 if scale is None else float(scale),
-            ws.data_ptr(), n)
+    args = (cache._p, batch._p, q.data_ptr(), qs, out.data_ptr(), os_, None if lse is None else lse.data_ptr(),
+            TYPES[q.dtype], H, D ** -0.5 if scale is None else float(scale))
+    if window is None:
+        _launch(dev, gpu._fn("bpd_attn_paged_on_gpu"), *args, ws.data_ptr(), n)
+    else:
+        _launch(dev, gpu._fn("bpd_attn_window_paged_on_gpu"), *args, window, sinks, ws.data_ptr(), n)
     return (out, lse) if return_lse else out
 
 
@@ -287,3 +472,71 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
     _launch(dev, gpu._fn("bpd_sample_on_gpu"), logits.data_ptr(), TYPES[logits.dtype], logits.stride(0) if B > 1 else V,
             B, V, *ptrs, token.data_ptr(), logprob.data_ptr(), kept.data_ptr(), ws.data_ptr(), n)
     return token, logprob, kept
+
+
+def adjust_logits(logits, tokens=None, lens=None, prompt=None, repetition=None, frequency=None, presence=None, bias=None,
+                  mask=None, mask_row=None, out=None, dtype=None):
+    """Rows of logits [rows, vocab] under penalties, biases and masks (bpd_adjust_logits_gpu), in that order.
+
+    tokens     int32 [rows, width]: every row's history, of which the first lens[row] (None: all) count, the first
+               prompt[row] of them (None: none) as its prompt
+    repetition float32 [rows]: l / r above 0, else l * r, of every token in the history
+    frequency  float32 [rows]: times how often a token stands behind the prompt, taken off; presence: once
+    bias       (start int32 [rows + 1], token int32 [n], value float32 [n]): added; a token's last entry counts
+    mask       int32 [masks, ceil(vocab / 32) or more] of bits: a token whose bit is 0 becomes -infinity; mask_row int32
+               [rows]: each row's mask, -1 none (None: mask `row`)
+    out        may be logits itself; else a new tensor of dtype, the logits' unless float32"""
+    if logits.dtype not in TYPES:
+        _bad(f"logits are {logits.dtype}, not float32, float16 or bfloat16")
+    if logits.dim() != 2:
+        _bad(f"logits have {logits.dim()} dimensions, not 2")
+    B, V = logits.shape
+    dev = logits.device
+    if out is None:
+        out = torch.empty((B, V), dtype=logits.dtype if dtype is None else dtype, device=dev)
+    if out.dtype not in (logits.dtype, torch.float32) or dtype not in (None, out.dtype) or out.shape != (B, V) \
+            or out.device != dev:
+        _bad(f"out is {out.dtype} {list(out.shape)} on {out.device}, not {logits.dtype} or float32 {[B, V]} on {dev}")
+    for t, what in ((logits, "logits"), (out, "out")):
+        if V > 1 and t.stride(1) != 1 or B > 1 and t.stride(0) < V:
+            _bad(f"rows of {what} are not contiguous, or overlap")
+    if tokens is None and (lens is not None or prompt is not None):
+        _bad("lens or prompt without tokens")
+    if mask is None and mask_row is not None:
+        _bad("mask_row without mask")
+    i32, f32, r = torch.int32, torch.float32, _Rules()
+    for t, what, dt in ((lens, "lens", i32), (prompt, "prompt", i32), (repetition, "repetition", f32),
+                        (frequency, "frequency", f32), (presence, "presence", f32), (mask_row, "mask_row", i32)):
+        if t is None:
+            continue
+        if t.dtype is not dt or t.shape != (B,) or t.device != dev or not t.is_contiguous():
+            _bad(f"{what} is not a contiguous {dt} [{B}] on {dev}")
+        setattr(r, what, t.data_ptr())
+    for t, what, n in ((tokens, "tokens", B), (mask, "mask", None)):
+        if t is None:
+            continue
+        _tensor(t, what, (i32,), 2, dev)
+        h, w = t.shape
+        if n is not None and h != n:
+            _bad(f"{what} has {h} rows and logits {n}")
+        if w > 1 and t.stride(1) != 1 or h > 1 and t.stride(0) < w:
+            _bad(f"rows of {what} are not contiguous, or overlap")
+        if what == "tokens":
+            r.tokens, r.token_stride, r.token_width = t.data_ptr(), t.stride(0) if h > 1 else w, w
+        else:
+            if w < (V + 31) // 32:
+                _bad(f"mask has {w} words a row for {V} tokens")
+            r.mask, r.mask_stride, r.n_masks = t.data_ptr(), t.stride(0) if h > 1 else w, h
+    if bias is not None:
+        start, token, value = bias
+        _tensor(start, "bias's start", (i32,), 1, dev, contiguous=True)
+        _tensor(token, "bias's token", (i32,), 1, dev, contiguous=True)
+        _tensor(value, "bias's value", (f32,), 1, dev, contiguous=True)
+        if start.shape[0] != B + 1 or token.shape != value.shape:
+            _bad(f"bias has {start.shape[0]} offsets for {B} rows, or {token.shape[0]} tokens and {value.shape[0]} values")
+        r.bias_start, r.bias_token, r.bias_value, r.n_bias = (start.data_ptr(), token.data_ptr(), value.data_ptr(),
+                                                              token.shape[0])
+    _launch(dev, gpu._fn("bpd_adjust_logits_on_gpu"), logits.data_ptr(), TYPES[logits.dtype],
+            logits.stride(0) if B > 1 else V, out.data_ptr(), TYPES[out.dtype], out.stride(0) if B > 1 else V, B, V,
+            ctypes.addressof(r))
+    return out

@@ -9,6 +9,12 @@
  *                              sequences may share a prefix
  *   bpd_sample_gpu             one token per row of logits: temperature, top-k,
  *                              top-p, min-p, from given random numbers
+ *   bpd_pages_extend_gpu       pages from a pool for sequences that grow, with their
+ *                              tables, and every new token's slot and position
+ *   bpd_pages_release_gpu      pages back to the pool
+ *   bpd_norm_rope_append_paged_gpu  the append, every head of q and k normed first
+ *   bpd_attn_window_paged_gpu  the attention over a sliding window and the first rows
+ *   bpd_adjust_logits_gpu      penalties, biases and masks on logits
  *
  * The structs are host memory, read during the call; the pointers in them and
  * every other tensor argument are device memory.  Sizes that live on the device
@@ -136,7 +142,110 @@ void bpd_sample_gpu(const void* logits, int type, int64_t row_stride, int n_rows
                     float* logprob, int32_t* n_kept, void* ws, int64_t ws_bytes);
 int64_t bpd_sample_workspace(int n_rows, int vocab);
 
-/* The same three on a stream of the current device given with the call (a hipStream_t; NULL = the null
+/* A pool of n_pages pages of page_size rows, and the sequences that hold them, a row of table each.
+ * Entries [0, ceil(lens[r] / page_size)) of row r are its pages, in order; -1 one that it gave
+ * back.  free_pages[0 .. n_free[0]) are the pages that no sequence holds.  gone (may be NULL, without windows):
+ * pages [gone[2 r], gone[2 r + 1]) of row r have slid out of its window and were given back.  All of it is
+ * device memory that the caller fills once (tables -1, lens, gone and n_free[1] 0) and the two calls below keep.
+ * Pages that are no part of the pool (a shared prefix's) are left out of free_pages.  n_pages and table_width times
+ * page_size stay below 2^31; n_rows up to 16384 (BPDQ_ERR_LIMIT). */
+typedef struct {
+    int32_t* table;
+    int64_t table_stride;
+    int table_width;
+    int32_t* lens;
+    int32_t* gone;
+    int32_t* free_pages;
+    int32_t* n_free; /* [2]: how many, and a counter of the calls' own */
+    int n_rows, n_pages, page_size;
+} bpd_page_pool;
+
+/* Sequence b = 0 .. n_seqs - 1 (n_seqs up to n_rows), row rows[b] of the pool (rows NULL: row b), grows by
+ * n_new[b] rows, 0 or more.  In that order each is granted what it asks for, or nothing; refused[b] says
+ * which: 0 granted; 1 no row of the pool, one that an earlier sequence names, or n_new below 0; 2 more rows than
+ * its table holds; 3 the pages asked for by it and all before it are more than the pool has (a sequence that needs no
+ * page is not refused for that); 4 with the tokens of it and of those before it that pages were there for they would be
+ * more than n_tokens.  Pages come from the end of free_pages.  lens and table of the pool follow.
+ * Outputs, device memory that overlaps nothing else of the call (with n_seqs 0 nothing is written): lens_out[b] the sequence's rows, q_start[n_seqs + 1] the running sum of tokens granted,
+ * slots[t] and pos[t] of every new token its row of the cache, page * page_size + row in it (-1 where its
+ * page is outside the pool), and its position, prefix_len + index; -1 of tokens behind the last.  table_out
+ * (may be NULL) [n_seqs][table_width]: the sequences' tables, -1 behind their pages.  With these a bpd_paged_batch
+ * describes the step.  n_tokens up to 2^23, with prefix_len and a table's rows below 2^31 - 1024.
+ * ws: as above, at least bpd_pages_workspace() bytes. */
+void bpd_pages_extend_gpu(const bpd_page_pool* pool, const int32_t* rows, const int32_t* n_new, int n_seqs, int n_tokens,
+                          int prefix_len, int32_t* table_out, int64_t table_out_stride, int32_t* lens_out,
+                          int32_t* q_start, int32_t* slots, int32_t* pos, int32_t* refused, void* ws, int64_t ws_bytes);
+
+/* Sequence b keeps its first keep[b] rows (NULL, or more than it has: all), and of those, with a window above 0
+ * (gone not NULL), the pages that hold one of the first `sinks` rows or a row that a token at index keep[b] or
+ * later sees through the window: those from keep[b] - window + 1 on.  sinks counts rows of the sequence's own part and is the
+ * same from call to call.  The other pages go to the end of free_pages, the first sequence's first page last, so that an
+ * extension which is taken back leaves the pool as it was; their entries become -1.  Rows that are not the pool's, and all
+ * but the first sequence that names a row, are passed over. */
+void bpd_pages_release_gpu(const bpd_page_pool* pool, const int32_t* rows, const int32_t* keep, int n_seqs, int window,
+                           int sinks, void* ws, int64_t ws_bytes);
+int64_t bpd_pages_workspace(int n_seqs);
+
+/* bpd_rope_append_paged_gpu with every head of q and k normed before it turns:
+ *   y_i = x_i / sqrt(mean over the head of x^2 + eps) * w_i
+ * q and k: [head_dim] weights of all heads (stride 0), or of each, a head's q_stride / k_stride elements behind
+ * the one before (multiples of 8, head_dim at least); of `type`, fp32 or x's.  NULL: not normed.  The sum of
+ * squares, the scale and the rotation are binary32 (a head whose squares add up beyond it becomes 0), and
+ * the result is rounded once. */
+typedef struct {
+    const void *q, *k;
+    int type;
+    int64_t q_stride, k_stride;
+    float eps; /* not below 0 */
+} bpd_head_norm;
+void bpd_norm_rope_append_paged_gpu(const bpd_paged_cache* cache, const bpd_paged_batch* batch, const bpd_head_norm* norm,
+                                    const bpd_rope* rope, const int32_t* pos, const void* q, int64_t q_stride,
+                                    const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* q_out,
+                                    int64_t q_out_stride, int x_type, int n_heads);
+
+/* bpd_attn_paged_gpu over a window: of the rows that it lets a token at position p (prefix_len + index) see, those at
+ * positions j > p - window or j < sinks, the prefix's rows being the first.  window at least 1, sinks 0 or more.
+ * Pages without a row that a new token sees are not read: their entries of the table may be -1.  The same rules and
+ * limits otherwise; ws: at least bpd_attn_window_paged_workspace() bytes. */
+void bpd_attn_window_paged_gpu(const bpd_paged_cache* cache, const bpd_paged_batch* batch, const void* q,
+                               int64_t q_stride, void* out, int64_t out_stride, float* lse, int q_type, int n_heads,
+                               float scale, int window, int sinks, void* ws, int64_t ws_bytes);
+int64_t bpd_attn_window_paged_workspace(const bpd_paged_cache* cache, const bpd_paged_batch* batch, int n_heads,
+                                        int window, int sinks);
+
+/* What happens to a row of logits before it is sampled, in this order, in binary32:
+ *   history    tokens[row][0 .. lens[row]) (lens NULL: width), the first prompt[row] of them the prompt's (NULL:
+ *              none).  A token that stands there has l = l > 0 ? l / repetition : l * repetition; one that stands
+ *              behind the prompt, n times, then l - n * frequency - presence
+ *   bias       entries bias_start[row] .. bias_start[row + 1] of a list: l + bias_value of its bias_token; of a token with
+ *              several entries the last one counts
+ *   mask       bit t % 32 of word t / 32 of mask row mask_row[row] (NULL: row `row`): where it is 0, l =
+ *              -infinity whatever it was.  A row outside [0, n_masks): none
+ * One repetition, frequency and presence per row; NULL: 1, 0, 0.  Lengths are clamped to the arrays
+ * (bias_start to [0, n_bias]), and tokens outside [0, vocab) passed over, so rows may be padded with them. */
+typedef struct {
+    const int32_t* tokens; /* NULL: no history */
+    int64_t token_stride;
+    int token_width;
+    const int32_t *lens, *prompt;
+    const float *repetition, *frequency, *presence;
+    const int32_t* bias_start; /* NULL: no biases */
+    const int32_t* bias_token;
+    const float* bias_value;
+    int n_bias;
+    const int32_t* mask; /* NULL: no masks */
+    int64_t mask_stride; /* words, ceil(vocab / 32) at least */
+    int n_masks;
+    const int32_t* mask_row;
+} bpd_logit_rules;
+
+/* out [n_rows][vocab] (out_type: that of the logits, or fp32) = the logits under the rules, rounded once; rows
+ * row_stride and out_stride elements apart, aligned to an element.  out may be the logits themselves, and overlaps them in
+ * no other way.  vocab and n_rows as in bpd_sample_gpu. */
+void bpd_adjust_logits_gpu(const void* logits, int type, int64_t row_stride, void* out, int out_type, int64_t out_stride,
+                           int n_rows, int vocab, const bpd_logit_rules* rules);
+
+/* The same on a stream of the current device given with the call (a hipStream_t; NULL = the null
  * stream).  bpd_gpu_set_stream()'s stream is one for the process, and a call that takes it has to be kept apart from
  * other threads' choices; these neither read nor change it. */
 void bpd_rope_append_paged_on_gpu(void* hip_stream, const bpd_paged_cache* cache, const bpd_paged_batch* batch,
@@ -149,6 +258,21 @@ void bpd_attn_paged_on_gpu(void* hip_stream, const bpd_paged_cache* cache, const
 void bpd_sample_on_gpu(void* hip_stream, const void* logits, int type, int64_t row_stride, int n_rows, int vocab,
                        const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                        const float* u, int32_t* token, float* logprob, int32_t* n_kept, void* ws, int64_t ws_bytes);
+void bpd_pages_extend_on_gpu(void* hip_stream, const bpd_page_pool* pool, const int32_t* rows, const int32_t* n_new,
+                             int n_seqs, int n_tokens, int prefix_len, int32_t* table_out, int64_t table_out_stride,
+                             int32_t* lens_out, int32_t* q_start, int32_t* slots, int32_t* pos, int32_t* refused, void* ws,
+                             int64_t ws_bytes);
+void bpd_pages_release_on_gpu(void* hip_stream, const bpd_page_pool* pool, const int32_t* rows, const int32_t* keep,
+                              int n_seqs, int window, int sinks, void* ws, int64_t ws_bytes);
+void bpd_norm_rope_append_paged_on_gpu(void* hip_stream, const bpd_paged_cache* cache, const bpd_paged_batch* batch,
+                                       const bpd_head_norm* norm, const bpd_rope* rope, const int32_t* pos, const void* q,
+                                       int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                                       void* q_out, int64_t q_out_stride, int x_type, int n_heads);
+void bpd_attn_window_paged_on_gpu(void* hip_stream, const bpd_paged_cache* cache, const bpd_paged_batch* batch,
+                                  const void* q, int64_t q_stride, void* out, int64_t out_stride, float* lse, int q_type,
+                                  int n_heads, float scale, int window, int sinks, void* ws, int64_t ws_bytes);
+void bpd_adjust_logits_on_gpu(void* hip_stream, const void* logits, int type, int64_t row_stride, void* out, int out_type,
+                              int64_t out_stride, int n_rows, int vocab, const bpd_logit_rules* rules);
 
 #ifdef __cplusplus
 }

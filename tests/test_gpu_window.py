@@ -1,0 +1,150 @@
+"""bpd_attn_window_paged_gpu against a plain float64 form (window_oracle)."""
+import numpy as np
+import pytest
+import torch
+
+import paged_oracle as O
+from bpd_substrate_amd import serve
+from window_oracle import Batch
+
+pytestmark = pytest.mark.gpu
+
+
+def check(b, dev, window, sinks, scale=None):
+    cache, batch, q = b.device(dev)
+    out = torch.full(q.shape, 7.0, dtype=q.dtype, device=dev)
+    got, lse = serve.attention(cache, batch, q, scale=scale, out=out, return_lse=True, window=window, sinks=sinks)
+    ref, rlse, eo, el = b.attention(scale, window, sinks)
+    got, lse = O.f64(got), O.f64(lse)
+    none = np.isnan(ref[:, 0, 0])
+    assert (got[none] == 7.0).all(), "rows of no sequence were written"
+    assert np.isfinite(got[~none]).all()
+    over = np.abs(got - ref)[~none] - eo[~none]
+    assert over.max(initial=-1) <= 0, (over.max(), np.unravel_index(over.argmax(), over.shape))
+    empty = rlse == -np.inf
+    assert np.array_equal(lse[~none] == -np.inf, empty[~none])
+    m = ~none[:, None] & ~empty
+    assert (np.abs(lse[m] - rlse[m]) <= el[m]).all(), (np.abs(lse[m] - rlse[m]) - el[m]).max()
+
+
+# new tokens, own rows, prefix, H, HKV, D, q, kv, page, heads_first, padding rows; window, sinks
+CASES = [
+    (([1], [1], 0, 1, 1, 8, "f16", "f16", 1, True, 0), (1, 0)),
+    (([1], [0], 0, 2, 2, 64, "f16", "f16", 16, True, 0), (5, 3)),                     # nothing to see
+    (([1], [0], 5, 2, 1, 64, "f32", "bf16", 16, True, 0), (3, 1)),                    # the prefix alone
+    (([1, 1, 1], [300, 1, 17], 0, 8, 2, 64, "f16", "f16", 16, True, 0), (64, 4)),
+    (([1, 1, 1], [300, 33, 97], 0, 8, 2, 64, "f16", "f16", 16, True, 0), (1, 0)),     # itself alone
+    (([1] * 5, [33, 64, 1, 129, 95], 77, 8, 8, 128, "bf16", "bf16", 16, False, 0), (100, 10)),   # windows into the prefix
+    (([1] * 3, [40, 500, 7], 130, 32, 8, 128, "f32", "f16", 32, False, 0), (60, 140)),           # sinks behind the prefix
+    (([1] * 3, [40, 500, 7], 130, 32, 8, 128, "f32", "bf16", 64, True, 0), (31, 33)),
+    (([1] * 2, [100, 31], 61, 5, 1, 80, "f16", "f16", 21, True, 0), (50, 2)),         # pages that end inside every unit
+    (([1] * 2, [100, 31], 61, 12, 4, 96, "f32", "f16", 3, False, 0), (37, 65)),
+    (([1] * 2, [150, 31], 200, 6, 2, 256, "bf16", "bf16", 64, True, 0), (33, 5)),
+    (([1] * 2, [700, 66], 0, 40, 1, 64, "f16", "f16", 16, True, 0), (65, 1)),         # more than 16 heads a kv head
+    (([3, 0, 20, 1], [10, 4, 20, 90], 0, 4, 2, 64, "f16", "f16", 16, True, 3), (7, 2)),
+    (([3, 0, 70, 1], [10, 0, 170, 90], 50, 8, 2, 128, "bf16", "bf16", 64, True, 2), (64, 0)),
+    (([130], [330], 33, 4, 4, 128, "f32", "f16", 16, False, 0), (100, 40)),
+    (([150, 9], [400, 9], 90, 4, 2, 96, "f16", "f16", 48, False, 1), (128, 3)),
+    (([150], [700], 0, 4, 2, 64, "bf16", "bf16", 16, True, 0), (200, 64)),
+    (([5, 5], [3, 5], 0, 2, 2, 64, "f16", "f16", 16, True, 0), (2, 1)),               # more new tokens than rows
+    (([40, 33], [45, 200], 64, 4, 2, 256, "f32", "bf16", 32, True, 0), (30, 65)),
+    (([200], [200], 0, 2, 1, 64, "f16", "f16", 16, True, 0), (1000, 5)),              # a window beyond everything
+    (([200], [300], 70, 2, 1, 64, "f16", "f16", 16, True, 0), (2 ** 31 - 1, 0)),
+    (([9], [300], 70, 2, 1, 64, "f16", "f16", 16, True, 0), (4, 2 ** 31 - 1)),        # every row a sink
+]
+
+
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_window(dev, case):
+    args, win = CASES[case]
+    check(Batch(300 + case, *args), dev, *win)
+
+
+@pytest.mark.parametrize("case", [c for c in range(len(CASES)) if set(CASES[c][0][0]) == {1} and not CASES[c][0][10]])
+def test_one_token_each(dev, case):
+    args, win = CASES[case]
+    check(Batch(400 + case, *args, decode=True), dev, *win)
+
+
+@pytest.mark.parametrize("decode", [True, False])
+@pytest.mark.parametrize("case", [3, 6, 8, 9, 10])
+def test_pages_behind_the_window_are_not_read(dev, case, decode):
+    """Their entries are -1, and infinities and NaN stand in every row that no token sees."""
+    args, (window, sinks) = CASES[case]
+    b = Batch(500 + case, *args, decode=decode)
+    b.slide(window, sinks)
+    check(b, dev, window, sinks)
+
+
+@pytest.mark.parametrize("case", [12, 13, 14, 15, 16, 18])
+def test_chunks_beside_poisoned_rows(dev, case):
+    args, (window, sinks) = CASES[case]
+    b = Batch(600 + case, *args)
+    b.slide(window, sinks)
+    check(b, dev, window, sinks)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("P", [0, 70])
+def test_a_bad_row_reaches_the_tokens_that_see_it_alone(dev, bad, P):
+    """One row of infinities or NaN in v: tokens whose window holds it are not finite, the others as without it."""
+    W, S, n, own, at = 40, 3, 100, 160, 90
+    b = Batch(7, [n], [own], P, 2, 1, 64, "f16", "f16", 16)
+    ref = b.attention(None, W, S)
+    b.vc[b.table[0, at // 16], at % 16] = bad
+    cache, batch, q = b.device(dev)
+    got = O.f64(serve.attention(cache, batch, q, window=W, sinks=S))
+    i = own - n + np.arange(n)
+    sees = (at <= i) & (at > i - W)
+    assert sees.any() and not sees.all()
+    assert (~np.isfinite(got[sees])).all()
+    assert (np.abs(got - ref[0])[~sees] <= ref[2][~sees]).all()
+
+
+def test_scales(dev):
+    for s in (0.0, -0.3, 3.0):
+        check(Batch(8, [1, 20], [90, 120], 30, 4, 2, 64, "f16", "f16", 16), dev, 50, 5, s)
+
+
+def test_a_window_of_everything_is_the_attention_without(dev):
+    for decode in (True, False):
+        b = Batch(9, [1, 1, 1], [90, 1, 300], 0, 8, 2, 128, "bf16", "bf16", 16, decode=decode)
+        cache, batch, q = b.device(dev)
+        a, la = serve.attention(cache, batch, q, return_lse=True)
+        w, lw = serve.attention(cache, batch, q, return_lse=True, window=1000)
+        assert torch.equal(a, w) and torch.equal(la, lw)
+
+
+@pytest.mark.parametrize("lens", [[2 ** 31 - 1, 5], [-3, 70], [1000, 10]])
+@pytest.mark.parametrize("decode", [True, False])
+def test_lengths_of_any_kind_stay_inside(dev, lens, decode):
+    b = Batch(10, [1, 1], [70, 70], 40, 4, 2, 64, "f16", "f16", 16, decode=decode)
+    cache, batch, q = b.device(dev)
+    batch.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+    out = serve.attention(cache, batch, q, window=30, sinks=4)
+    torch.cuda.synchronize()
+    assert out.shape == q.shape
+
+
+def test_pages_of_any_kind_are_absent(dev):
+    b = Batch(11, [1, 30], [200, 150], 40, 4, 2, 64, "f16", "f16", 16)
+    b.table[0, 11], b.table[1, 4], b.prefix_pages[0] = -5, 2 ** 31 - 1, 10 ** 6
+    check(b, dev, 100, 20)
+
+
+def test_a_replayed_graph_follows_the_lengths(dev):
+    b = Batch(12, [1] * 4, [120, 60, 200, 90], 20, 4, 2, 64, "f16", "f16", 16, decode=True)
+    cache, batch, q = b.device(dev)
+    f = lambda: serve.attention(cache, batch, q, window=48, sinks=6, return_lse=True)  # noqa: E731
+    f()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        out, lse = f()
+    for lens in ([120, 60, 200, 90], [100, 1, 7, 33], [113, 59, 160, 64]):
+        batch.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, wl = f()
+        assert torch.equal(out, want) and torch.equal(lse, wl)
+        torch.cuda.synchronize()
