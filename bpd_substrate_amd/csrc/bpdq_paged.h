@@ -142,10 +142,8 @@ struct PoolArgs {
     int64_t table_out_stride;
     int32_t *lens_out, *q_start, *slots, *pos, *refused;
     int prefix_len, window, sinks;
-    int4* plan;  // [B + 1]
-    int parts;   // the launcher's
+    int parts;  // the launcher's
 };
-int64_t pages_ws(int B);
 void launch_pages_extend(const PoolArgs& a, hipStream_t s);
 void launch_pages_release(const PoolArgs& a, hipStream_t s);
 

@@ -274,7 +274,7 @@ void check_pool(Args& c, const bpd_page_pool* p, const int32_t* rows, int n_seqs
     if (rows != nullptr) c.ptr(rows, 4, "rows");
 }
 
-bpdq::PoolArgs pool_args(const bpd_page_pool& p, const int32_t* rows, int n_seqs, void* ws) {
+bpdq::PoolArgs pool_args(const bpd_page_pool& p, const int32_t* rows, int n_seqs) {
     bpdq::PoolArgs a = {};
     a.table = p.table;
     a.table_stride = p.table_stride;
@@ -288,7 +288,6 @@ bpdq::PoolArgs pool_args(const bpd_page_pool& p, const int32_t* rows, int n_seqs
     a.page = bpdq::fast_div(p.page_size);
     a.rows = rows;
     a.B = n_seqs;
-    a.plan = static_cast<int4*>(ws);
     return a;
 }
 
@@ -421,16 +420,9 @@ void bpd_sample_gpu(const void* logits, int type, int64_t row_stride, int n_rows
                       token, logprob, n_kept, ws, ws_bytes);
 }
 
-int64_t bpd_pages_workspace(int n_seqs) {
-    Args c("bpd_pages_workspace");
-    c.shape(n_seqs >= 0, "n_seqs is negative").need(n_seqs <= kPoolRows, BPDQ_ERR_LIMIT, "n_seqs is above 2^14");
-    return c.ok ? bpdq::pages_ws(n_seqs) : -1;
-}
-
 void bpd_pages_extend_on_gpu(void* hip_stream, const bpd_page_pool* pool, const int32_t* rows, const int32_t* n_new,
                              int n_seqs, int n_tokens, int prefix_len, int32_t* table_out, int64_t table_out_stride,
-                             int32_t* lens_out, int32_t* q_start, int32_t* slots, int32_t* pos, int32_t* refused, void* ws,
-                             int64_t ws_bytes) {
+                             int32_t* lens_out, int32_t* q_start, int32_t* slots, int32_t* pos, int32_t* refused) {
     const char* fn = "bpd_pages_extend_gpu";
     const hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     Args c(fn);
@@ -446,10 +438,7 @@ void bpd_pages_extend_on_gpu(void* hip_stream, const bpd_page_pool* pool, const 
         c.ptr(table_out, 4, "table_out").shape(table_out_stride >= pool->table_width,
                                                "table_out_stride is shorter than table_width");
     if (!c.ok) return;
-    bpdq::WsLease lease;
-    void* w = work_space(lease, ws, ws_bytes, bpdq::pages_ws(n_seqs), stream, fn);
-    if (w == nullptr) return;
-    bpdq::PoolArgs a = pool_args(*pool, rows, n_seqs, w);
+    bpdq::PoolArgs a = pool_args(*pool, rows, n_seqs);
     a.add = n_new;
     a.T = n_tokens;
     a.prefix_len = prefix_len;
@@ -466,13 +455,13 @@ void bpd_pages_extend_on_gpu(void* hip_stream, const bpd_page_pool* pool, const 
 
 void bpd_pages_extend_gpu(const bpd_page_pool* pool, const int32_t* rows, const int32_t* n_new, int n_seqs, int n_tokens,
                           int prefix_len, int32_t* table_out, int64_t table_out_stride, int32_t* lens_out,
-                          int32_t* q_start, int32_t* slots, int32_t* pos, int32_t* refused, void* ws, int64_t ws_bytes) {
+                          int32_t* q_start, int32_t* slots, int32_t* pos, int32_t* refused) {
     bpd_pages_extend_on_gpu(bpdq::abi_stream(), pool, rows, n_new, n_seqs, n_tokens, prefix_len, table_out,
-                            table_out_stride, lens_out, q_start, slots, pos, refused, ws, ws_bytes);
+                            table_out_stride, lens_out, q_start, slots, pos, refused);
 }
 
 void bpd_pages_release_on_gpu(void* hip_stream, const bpd_page_pool* pool, const int32_t* rows, const int32_t* keep,
-                              int n_seqs, int window, int sinks, void* ws, int64_t ws_bytes) {
+                              int n_seqs, int window, int sinks) {
     const char* fn = "bpd_pages_release_gpu";
     const hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     Args c(fn);
@@ -482,10 +471,7 @@ void bpd_pages_release_on_gpu(void* hip_stream, const bpd_page_pool* pool, const
     if (!c.ok || n_seqs == 0) return;
     if (keep != nullptr) c.ptr(keep, 4, "keep");
     if (!c.ok) return;
-    bpdq::WsLease lease;
-    void* w = work_space(lease, ws, ws_bytes, bpdq::pages_ws(n_seqs), stream, fn);
-    if (w == nullptr) return;
-    bpdq::PoolArgs a = pool_args(*pool, rows, n_seqs, w);
+    bpdq::PoolArgs a = pool_args(*pool, rows, n_seqs);
     a.keep = keep;
     a.window = window;
     a.sinks = sinks;
@@ -494,8 +480,8 @@ void bpd_pages_release_on_gpu(void* hip_stream, const bpd_page_pool* pool, const
 }
 
 void bpd_pages_release_gpu(const bpd_page_pool* pool, const int32_t* rows, const int32_t* keep, int n_seqs, int window,
-                           int sinks, void* ws, int64_t ws_bytes) {
-    bpd_pages_release_on_gpu(bpdq::abi_stream(), pool, rows, keep, n_seqs, window, sinks, ws, ws_bytes);
+                           int sinks) {
+    bpd_pages_release_on_gpu(bpdq::abi_stream(), pool, rows, keep, n_seqs, window, sinks);
 }
 
 void bpd_adjust_logits_on_gpu(void* hip_stream, const void* logits, int type, int64_t row_stride, void* out, int out_type,

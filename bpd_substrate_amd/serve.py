@@ -313,11 +313,9 @@ class PagePool:
             slots.fill_(-1)
             pos.fill_(-1)
         table = self.table[:B] if rows is None else table.view(B, W)
-        n = _pages_workspace(B)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
         _launch(dev, gpu._fn("bpd_pages_extend_on_gpu"), self._p, rp, np_, B, T, prefix_len,
                 None if rows is None else table.data_ptr(), W, lens.data_ptr(), q_start.data_ptr(), slots.data_ptr(),
-                pos.data_ptr(), refused.data_ptr(), ws.data_ptr(), n)
+                pos.data_ptr(), refused.data_ptr())
         return PageStep(table, lens, q_start, slots, pos, refused, T, prefix_len)
 
     def release(self, keep=None, rows=None, window=None, sinks=0, prefix_len=0):
@@ -329,15 +327,8 @@ class PagePool:
             _bad(f"window {window} is below 1")
         if sinks < 0 or prefix_len < 0:
             _bad("sinks or prefix_len is negative")
-        n = _pages_workspace(B)
-        ws = torch.empty(n, dtype=torch.uint8, device=self.device)
         _launch(self.device, gpu._fn("bpd_pages_release_on_gpu"), self._p, rp, kp, B, 0 if window is None else window,
-                max(0, sinks - prefix_len), ws.data_ptr(), n)
-
-
-@functools.lru_cache(maxsize=256)
-def _pages_workspace(n_seqs):
-    return gpu.call("bpd_pages_workspace", n_seqs)
+                max(0, sinks - prefix_len))
 
 
 def _head_norm(q_norm, k_norm, eps, x, heads, kv_heads, D):

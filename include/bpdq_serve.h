@@ -170,11 +170,10 @@ typedef struct {
  * slots[t] and pos[t] of every new token its row of the cache, page * page_size + row in it (-1 where its
  * page is outside the pool), and its position, prefix_len + index; -1 of tokens behind the last.  table_out
  * (may be NULL) [n_seqs][table_width]: the sequences' tables, -1 behind their pages.  With these a bpd_paged_batch
- * describes the step.  n_tokens up to 2^23, with prefix_len and a table's rows below 2^31 - 1024.
- * ws: as above, at least bpd_pages_workspace() bytes. */
+ * describes the step.  n_tokens up to 2^23, with prefix_len and a table's rows below 2^31 - 1024. */
 void bpd_pages_extend_gpu(const bpd_page_pool* pool, const int32_t* rows, const int32_t* n_new, int n_seqs, int n_tokens,
                           int prefix_len, int32_t* table_out, int64_t table_out_stride, int32_t* lens_out,
-                          int32_t* q_start, int32_t* slots, int32_t* pos, int32_t* refused, void* ws, int64_t ws_bytes);
+                          int32_t* q_start, int32_t* slots, int32_t* pos, int32_t* refused);
 
 /* Sequence b keeps its first keep[b] rows (NULL, or more than it has: all), and of those, with a window above 0
  * (gone not NULL), the pages that hold one of the first `sinks` rows or a row that a token at index keep[b] or
@@ -183,8 +182,7 @@ void bpd_pages_extend_gpu(const bpd_page_pool* pool, const int32_t* rows, const 
  * extension which is taken back leaves the pool as it was; their entries become -1.  Rows that are not the pool's, and all
  * but the first sequence that names a row, are passed over. */
 void bpd_pages_release_gpu(const bpd_page_pool* pool, const int32_t* rows, const int32_t* keep, int n_seqs, int window,
-                           int sinks, void* ws, int64_t ws_bytes);
-int64_t bpd_pages_workspace(int n_seqs);
+                           int sinks);
 
 /* bpd_rope_append_paged_gpu with every head of q and k normed before it turns:
  *   y_i = x_i / sqrt(mean over the head of x^2 + eps) * w_i
@@ -260,10 +258,9 @@ void bpd_sample_on_gpu(void* hip_stream, const void* logits, int type, int64_t r
                        const float* u, int32_t* token, float* logprob, int32_t* n_kept, void* ws, int64_t ws_bytes);
 void bpd_pages_extend_on_gpu(void* hip_stream, const bpd_page_pool* pool, const int32_t* rows, const int32_t* n_new,
                              int n_seqs, int n_tokens, int prefix_len, int32_t* table_out, int64_t table_out_stride,
-                             int32_t* lens_out, int32_t* q_start, int32_t* slots, int32_t* pos, int32_t* refused, void* ws,
-                             int64_t ws_bytes);
+                             int32_t* lens_out, int32_t* q_start, int32_t* slots, int32_t* pos, int32_t* refused);
 void bpd_pages_release_on_gpu(void* hip_stream, const bpd_page_pool* pool, const int32_t* rows, const int32_t* keep,
-                              int n_seqs, int window, int sinks, void* ws, int64_t ws_bytes);
+                              int n_seqs, int window, int sinks);
 void bpd_norm_rope_append_paged_on_gpu(void* hip_stream, const bpd_paged_cache* cache, const bpd_paged_batch* batch,
                                        const bpd_head_norm* norm, const bpd_rope* rope, const int32_t* pos, const void* q,
                                        int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,

@@ -124,6 +124,16 @@ def test_more_sequences_than_a_workgroup_has_threads(dev):
     b.release()
 
 
+def test_the_largest_pool(dev):
+    b = Both(dev, 20000, 4, 16384, 3)
+    r = np.random.default_rng(6)
+    rows = [int(x) for x in r.permutation(16384)[:700]]
+    b.extend([int(x) for x in r.integers(0, 9, 700)], 5000, rows)
+    b.release([int(x) for x in r.integers(0, 5, 700)], rows)
+    b.extend([1] * 16384, 16384)
+    b.release([0] * 16384)
+
+
 def test_one_long_sequence_and_empty_calls(dev):
     b = Both(dev, 5000, 16, 3, 4400)
     b.extend([0, 70000, 1], 70001, [2, 1, 0])
