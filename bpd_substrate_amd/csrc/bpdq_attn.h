@@ -51,6 +51,7 @@ struct AttnArgs {
     float2* ml1;
     int2* where1;  // [head][sequence]
     int window, sinks;  // of the WIN forms
+    bool past_mall;     // k_attn_head: keys and values are read past the MALL
 };
 
 // Rows of a sequence's own part that the table holds.
@@ -477,6 +478,22 @@ __device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w,
 #pragma unroll
         for (int m = 0; m < MT; m++) qscale[m] = NS > 1 && CT == BPD_T_F16 ? score_scale(scale2, e2[m]) : scale2;
         const bool busy = __ballot(lim[0] >= 0) != 0;  // rows of a wave fill from its first
+        // WIN: every row of the wave sees own rows below lim_all, and positions from low_all on
+        int lim_all = 0, low_all = 0;
+        if constexpr (WIN) {
+            int x = 1 << 30, y = 0;
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                if (lim[m] >= 0) x = min(x, lim[m]);
+                y = max(y, low[m]);
+            }
+            for (int d = 1; d < 16; d <<= 1) {
+                x = min(x, __shfl_xor(x, d));
+                y = max(y, __shfl_xor(y, d));
+            }
+            lim_all = __builtin_amdgcn_readfirstlane(x);
+            low_all = __builtin_amdgcn_readfirstlane(y);
+        }
         f32x4 o[MT][NE];
         float ref[MT], l[MT];
         int mend0 = 1 << 30, mend1 = 0;
@@ -606,13 +623,8 @@ __device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w,
                     __builtin_amdgcn_sched_barrier(0);  // V's reads run behind the softmax
                     bool diag = false;
                     if constexpr (WIN) {
-                        // a row's first key in the half that is there, and the last behind it, among the first ones or not
-                        const int k = key0 + half * 32, end = min(own, k + 32);
-                        bool d = false;
-#pragma unroll
-                        for (int m = 0; m < MT; m++)
-                            d |= lim[m] >= 0 && ((kt >= ntp && lim[m] < end) || (a.P + k < low[m] && a.P + k + 32 > g.sinks));
-                        diag = __ballot(d) != 0;
+                        const int k = key0 + half * 32;
+                        diag = (kt >= ntp && lim_all < min(own, k + 32)) || (a.P + k < low_all && a.P + k + 32 > g.sinks);
                     } else if (kt >= ntp && b >= 0) {
                         bool d = false;
 #pragma unroll
@@ -766,8 +778,12 @@ __device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w,
 // a page, its lookup and the high half of their addresses.
 // One read of every key and value: 5.9 TB/s for 670 MB, two units of loads in flight in each of 2048 waves.
 // WIN: the sequence's units are those of the prefix and of its own rows that the token sees.
+//
+// This is a wave's share of one (sequence, head): its units [kt, k1), kt below k1.  o, l: sums with weights 2^(score - ref).
 template <int QT, int CT, int NS, int DT, bool UNI, bool WIN>
-__device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT / 8], int w, int waves, int UH) {
+__device__ __forceinline__ void wave_range(const AttnArgs& g, uint4 (&ks)[32][DT / 8], int b, int head, int own,
+                                           const Span& span, int low, int kt, int k1, bool stream, f32x4 (&o)[DT / 16],
+                                           float& ref, float& l) {
     using M = Mfma<CT>;
     using T = typename M::T;
     using Q = typename Elem<QT>::type;
@@ -777,6 +793,249 @@ __device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT
     const Paged& a = g.a;
     const int lane = (int)threadIdx.x & 63, col = lane & 15, lg = lane >> 4;
     const int per = a.D / 8;
+    const float sign = g.scale > 0.f ? 1.f : g.scale < 0.f ? -1.f : 0.f;
+    const float scale2 = (g.scale == 0.f ? 1.f : __builtin_fabsf(g.scale)) * kLog2e;
+    const int32_t* table = a.table + (int64_t)b * a.table_stride;
+    const int64_t hoff = (int64_t)head * a.head_stride;
+    const T* kbase = reinterpret_cast<const T*>(a.k) + hoff;
+    const T* vbase = reinterpret_cast<const T*>(a.v) + hoff;
+
+    // the rows of units in flight: row 16 (j / 4) + 4 lg + j % 4, 16 lanes across it
+    struct Unit {
+        u32x4 k[8][VB], v[8][VB];
+        uint32_t ok;  // bit j: row j is there
+    };
+    Unit un[BUF];
+    constexpr int NP = UNI ? 2 : 8;  // pages of a unit: of 16 rows each, or of the lane's rows
+    int pg[BUF][NP];
+    const uint32_t row_bytes = 2u * (uint32_t)a.row_stride, lane_at = 4u * lg * row_bytes + 4u * VD * col;
+    const bool all_lanes = a.D == DT;
+    // rows, pages and number of rows of the part that unit t is in
+    struct Part {
+        int row, rows;
+        bool pre;
+        const int32_t* pages;
+    };
+    auto part_of = [&](int t) {
+        Part r = {t * 32, own, false, table};
+        if constexpr (WIN) {
+            r.row = unit_at(span, t, r.pre) * 32;
+            r.rows = r.pre ? a.P : own;
+            r.pages = r.pre ? a.prefix : table;
+        }
+        return r;
+    };
+    // whether rows [i, i + n) of a part are all seen
+    auto seen = [&](const Part& r, int i, int n) {
+        if constexpr (!WIN) return true;
+        const int at = i + (r.pre ? 0 : a.P);
+        return at >= low || at + n <= g.sinks;
+    };
+    auto look = [&](int (&p)[NP], int t) {
+        const Part r = part_of(t);
+#pragma unroll
+        for (int x = 0; x < NP; x++) {
+            if constexpr (UNI) {
+                const int i = r.row + 16 * x;
+                p[x] = t < k1 && i < r.rows ? load_uniform(r.pages + fdiv(a.page, i)) : -1;
+            } else {
+                const int i = r.row + 16 * (x >> 2) + 4 * lg + (x & 3);
+                p[x] = -1;
+                if (t < k1 && i < r.rows) p[x] = r.pages[fdiv(a.page, i)];
+            }
+        }
+    };
+    auto load = [&](u32x4 (&to)[8][VB], uint32_t& oks, const T* base, const int (&p)[NP], int t) {
+        const Part r = part_of(t);
+        // a whole unit: two scalar bases, the lane's part the same for each
+        if (UNI && all_lanes && r.row + 32 <= r.rows && (uint32_t)p[0] < (uint32_t)a.n_pages &&
+            (uint32_t)p[1] < (uint32_t)a.n_pages && seen(r, r.row, 32)) {
+            oks = 255u;
+            auto get = [&](auto nt) {
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const int i0 = r.row + 16 * x, in_page = i0 - fdiv(a.page, i0) * (int)a.page.d;
+                    const auto* at = reinterpret_cast<const uint8_t*>(base + row_at(a, p[x], in_page));
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int vb = 0; vb < VB; vb++) {
+                            const auto* q = at + (uint32_t)(lane_at + (uint32_t)j * row_bytes + 256 * vb);
+                            using R = std::conditional_t<VD == 4, u32x4, u32x2>;
+                            const auto* from = reinterpret_cast<const R*>(q);
+                            R y;
+                            if constexpr (decltype(nt)::value) y = __builtin_nontemporal_load(from);
+                            else y = *from;
+#pragma unroll
+                            for (int d = 0; d < VD; d++) to[4 * x + j][vb][d] = y[d];
+                        }
+                }
+            };
+            if (stream) {
+                asm volatile("");  // keeps the two kinds of load from being merged into one
+                get(std::true_type());
+            } else {
+                get(std::false_type());
+            }
+            return;
+        }
+        oks = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int x = j >> 2, i0 = r.row + 16 * x, i = i0 + 4 * lg + (j & 3);
+            const int page = p[UNI ? x : j], in_page = i - fdiv(a.page, UNI ? i0 : i) * (int)a.page.d;
+            const bool ok = page >= 0 && page < a.n_pages && i < r.rows && seen(r, i, 1);
+            oks |= ok ? 1u << j : 0u;
+            const int64_t at = row_at(a, page, in_page);
+#pragma unroll
+            for (int vb = 0; vb < VB; vb++) {
+                const int d = vb * 128 + 2 * VD * col;
+                to[j][vb] = u32x4{0u, 0u, 0u, 0u};
+                if (ok && d < a.D) {
+                    if constexpr (VD == 4) {
+                        to[j][vb] = *reinterpret_cast<const u32x4*>(base + at + d);
+                    } else {
+                        const u32x2 y = *reinterpret_cast<const u32x2*>(base + at + d);
+                        to[j][vb][0] = y[0];
+                        to[j][vb][1] = y[1];
+                    }
+                }
+            }
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < BUF; i++) look(pg[i], kt + i);
+#pragma unroll
+    for (int i = 0; i < BUF; i++) {
+        if (kt + i >= k1) break;
+        load(un[i].k, un[i].ok, kbase, pg[i], kt + i);
+        load(un[i].v, un[i].ok, vbase, pg[i], kt + i);
+    }
+
+    // the queries
+    u32x4 qf[KS][NS];
+    float qscale = scale2;
+    {
+        const bool row = col < g.G;
+        const Q* q = reinterpret_cast<const Q*>(g.q) + b * g.qs + (int64_t)(head * g.G + (row ? col : 0)) * a.D;
+        float x[KS][8];
+        load_query<KS>(q, row, per, lg, sign, x);
+        if constexpr (NS > 1 && CT == BPD_T_F16) qscale = score_scale(scale2, row_exponent<KS>(x));
+#pragma unroll
+        for (int k = 0; k < KS; k++) split8<CT, NS>(x[k], qf[k]);
+    }
+#pragma unroll
+    for (int e = 0; e < NE; e++) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    ref = kNegInf;
+    l = 0.f;
+    // unit t, held in n; then the unit BUF further on is asked for
+    auto step = [&](Unit& n, int (&p)[NP], int t) {
+        // K's rows through the wave's own LDS into the order of the product's operand: read from memory as
+        // the operand takes them, 16 lanes would meet 16 rows at a time
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+#pragma unroll
+            for (int vb = 0; vb < VB; vb++) {
+                const int row = 16 * (j >> 2) + 4 * lg + (j & 3);
+                if constexpr (VD == 4)
+                    *reinterpret_cast<u32x4*>(&ks[row][k_slot<DT>(row, vb * 16 + col)]) = n.k[j][vb];
+                else
+                    reinterpret_cast<u32x2*>(&ks[row][k_slot<DT>(row, col >> 1)])[col & 1] =
+                        u32x2{n.k[j][vb][0], n.k[j][vb][1]};
+            }
+        const uint32_t ok = n.ok;
+        const bool more = t + BUF < k1;
+        int pn[NP];
+#pragma unroll
+        for (int x = 0; x < NP; x++) pn[x] = p[x];
+        if (more) {
+            load(n.k, n.ok, kbase, pn, t + BUF);
+            look(p, t + 2 * BUF);
+        }
+        u32x4 kf[2][KS];
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+                kf[x][k] = __builtin_bit_cast(u32x4, ks[16 * x + col][k_slot<DT>(col, 4 * k + lg)]);
+        f32x4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int y = 0; y < NS; y++) sc[x] = M::go(kf[x][k], qf[k][y], sc[x]);
+        // keys that are not there: the lane's scores are those of the rows that it read
+        if (__ballot(ok != 255u) != 0) {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (!((ok >> e) & 1u)) sc[e >> 2][e & 3] = kNegInf;
+        }
+        const float top = xor_max(fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                                        fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])))) * qscale;
+        if (__ballot(top - 15.f > ref) != 0) {
+            const float nr = top - 15.f > ref ? top - 12.f : ref;
+            const float f = nr == ref ? 1.f : __builtin_amdgcn_exp2f(ref - nr);
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < NE; e++) o[e] *= f;
+            ref = nr;
+        }
+        const float base = ref == kNegInf ? 0.f : ref;
+        float w8[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) w8[e] = __builtin_amdgcn_exp2f(fmaf(sc[e >> 2][e & 3], qscale, -base));
+        l += ((w8[0] + w8[1]) + (w8[2] + w8[3])) + ((w8[4] + w8[5]) + (w8[6] + w8[7]));
+        u32x4 pf[NS];
+        split8<CT, NS>(w8, pf);
+#pragma unroll
+        for (int vb = 0; vb < VB; vb++)
+#pragma unroll
+            for (int e = 0; e < 2 * VD; e++) {
+                const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+                u32x4 vf;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    vf[j] = __builtin_amdgcn_perm(n.v[2 * j + 1][vb][e >> 1], n.v[2 * j][vb][e >> 1], sel);
+#pragma unroll
+                for (int x = 0; x < NS; x++) o[vb * 8 + e] = M::go(vf, pf[x], o[vb * 8 + e]);
+            }
+        if (more) load(n.v, n.ok, vbase, pn, t + BUF);
+    };
+    // the pages of the units behind those in flight
+#pragma unroll
+    for (int i = 0; i < BUF; i++) look(pg[i], kt + BUF + i);
+    while (true) {
+#pragma unroll
+        for (int i = 0; i < BUF; i++) {
+            if (kt + i >= k1) break;
+            step(un[i], pg[i], kt + i);
+        }
+        kt += BUF;
+        if (kt >= k1) break;
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+}
+
+// The first position that sequence b's token sees through the window, and the units.
+template <bool WIN>
+__device__ __forceinline__ int wave_rows(const AttnArgs& g, int b, int own, Span& span, int& low) {
+    if constexpr (WIN) {
+        span = wave_span(g, b);
+        low = (int)min(window_low(position(g.a, b, 1, 0), g.window), (int64_t)g.a.P + own);
+        return prefix_units(span) + own_units(span);
+    }
+    return (own + 31) >> 5;
+}
+
+// A wave's share of all sequences' units.
+template <int QT, int CT, int NS, int DT, bool UNI, bool WIN>
+__device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT / 8], int w, int waves, int UH) {
+    using Q = typename Elem<QT>::type;
+    constexpr int NE = DT / 16, VD = DT < 128 ? 2 : 4, VB = DT < 128 ? 1 : DT / 128;
+    const Paged& a = g.a;
+    const int lane = (int)threadIdx.x & 63, col = lane & 15, lg = lane >> 4;
     const int64_t U = (int64_t)UH * a.hkv;
     const int n_waves = (int)(U < waves ? U : waves);
     if (w >= n_waves) return;
@@ -804,8 +1063,6 @@ __device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT
         b = __builtin_amdgcn_readfirstlane(b);
         before = __builtin_amdgcn_readfirstlane(before);
     }
-    const float sign = g.scale > 0.f ? 1.f : g.scale < 0.f ? -1.f : 0.f;
-    const float scale2 = (g.scale == 0.f ? 1.f : __builtin_fabsf(g.scale)) * kLog2e;
     // keys and values beyond the 256 MB of the MALL are read past it (128 -> 114 us for 670 MB); fewer may be there
     // from the call before (27.4 us for 74 MB, 30 read past it)
     const bool stream = U * 32 * a.D * 4 > (int64_t)256 << 20;
@@ -813,12 +1070,8 @@ __device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT
     while (u < u1) {
         const int own = own_rows(a, b);
         Span span = {};
-        int nk = (own + 31) >> 5, low = 0;
-        if constexpr (WIN) {
-            span = wave_span(g, b);
-            nk = prefix_units(span) + own_units(span);
-            low = (int)min(window_low(position(a, b, 1, 0), g.window), (int64_t)a.P + own);
-        }
+        int low = 0;
+        const int nk = wave_rows<WIN>(g, b, own, span, low);
         const int in = (int)(u - (int64_t)head * UH);
         if (in >= before + nk) {  // the next sequence, or the next head's first
             before += nk;
@@ -838,228 +1091,9 @@ __device__ __forceinline__ void wave_share(const AttnArgs& g, uint4 (&ks)[32][DT
             const int64_t ue = (int64_t)head * UH + before + nk - 1;
             g.where1[(int64_t)head * a.B + b] = make_int2((int)slot, last_word ? 0 : group_of(ue, U, n_waves) - w + 1);
         }
-        const int32_t* table = a.table + (int64_t)b * a.table_stride;
-        const int64_t hoff = (int64_t)head * a.head_stride;
-        const T* kbase = reinterpret_cast<const T*>(a.k) + hoff;
-        const T* vbase = reinterpret_cast<const T*>(a.v) + hoff;
-
-        // the rows of units in flight: row 16 (j / 4) + 4 lg + j % 4, 16 lanes across it
-        struct Unit {
-            u32x4 k[8][VB], v[8][VB];
-            uint32_t ok;  // bit j: row j is there
-        };
-        Unit un[BUF];
-        int pg[BUF][2];
-        const uint32_t row_bytes = 2u * (uint32_t)a.row_stride, lane_at = 4u * lg * row_bytes + 4u * VD * col;
-        const bool all_lanes = a.D == DT;
-        // rows, pages and number of rows of the part that unit t is in
-        struct Part {
-            int row, rows;
-            bool pre;
-            const int32_t* pages;
-        };
-        auto part_of = [&](int t) {
-            Part r = {t * 32, own, false, table};
-            if constexpr (WIN) {
-                r.row = unit_at(span, t, r.pre) * 32;
-                r.rows = r.pre ? a.P : own;
-                r.pages = r.pre ? a.prefix : table;
-            }
-            return r;
-        };
-        // whether rows [i, i + n) of a part are all seen
-        auto seen = [&](const Part& r, int i, int n) {
-            if constexpr (!WIN) return true;
-            const int at = i + (r.pre ? 0 : a.P);
-            return at >= low || at + n <= g.sinks;
-        };
-        auto look = [&](int (&p)[2], int t) {
-            if constexpr (UNI) {
-                const Part r = part_of(t);
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const int i = r.row + 16 * x;
-                    p[x] = t < k1 && i < r.rows ? load_uniform(r.pages + fdiv(a.page, i)) : -1;
-                }
-            }
-        };
-        auto load = [&](u32x4 (&to)[8][VB], uint32_t& oks, const T* base, const int (&p)[2], int t) {
-            const Part r = part_of(t);
-            // a whole unit: two scalar bases, the lane's part the same for each
-            if (UNI && all_lanes && r.row + 32 <= r.rows && (uint32_t)p[0] < (uint32_t)a.n_pages &&
-                (uint32_t)p[1] < (uint32_t)a.n_pages && seen(r, r.row, 32)) {
-                oks = 255u;
-                auto get = [&](auto nt) {
-#pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        const int i0 = r.row + 16 * x, in_page = i0 - fdiv(a.page, i0) * (int)a.page.d;
-                        const auto* at = reinterpret_cast<const uint8_t*>(base + row_at(a, p[x], in_page));
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-#pragma unroll
-                            for (int vb = 0; vb < VB; vb++) {
-                                const auto* q = at + (uint32_t)(lane_at + (uint32_t)j * row_bytes + 256 * vb);
-                                using R = std::conditional_t<VD == 4, u32x4, u32x2>;
-                                const auto* from = reinterpret_cast<const R*>(q);
-                                R y;
-                                if constexpr (decltype(nt)::value) y = __builtin_nontemporal_load(from);
-                                else y = *from;
-#pragma unroll
-                                for (int d = 0; d < VD; d++) to[4 * x + j][vb][d] = y[d];
-                            }
-                    }
-                };
-                if (stream) {
-                    asm volatile("");  // keeps the two kinds of load from being merged into one
-                    get(std::true_type());
-                } else {
-                    get(std::false_type());
-                }
-                return;
-            }
-            oks = 0;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int x = j >> 2, i0 = r.row + 16 * x, i = i0 + 4 * lg + (j & 3);
-                int page, in_page;
-                if constexpr (UNI) {
-                    page = p[x];
-                    in_page = i - fdiv(a.page, i0) * (int)a.page.d;
-                } else {
-                    const int at = fdiv(a.page, i);
-                    page = i < r.rows ? r.pages[at] : -1;
-                    in_page = i - at * (int)a.page.d;
-                }
-                const bool ok = page >= 0 && page < a.n_pages && i < r.rows && seen(r, i, 1);
-                oks |= ok ? 1u << j : 0u;
-                const int64_t at = row_at(a, page, in_page);
-#pragma unroll
-                for (int vb = 0; vb < VB; vb++) {
-                    const int d = vb * 128 + 2 * VD * col;
-                    to[j][vb] = u32x4{0u, 0u, 0u, 0u};
-                    if (ok && d < a.D) {
-                        if constexpr (VD == 4) {
-                            to[j][vb] = *reinterpret_cast<const u32x4*>(base + at + d);
-                        } else {
-                            const u32x2 y = *reinterpret_cast<const u32x2*>(base + at + d);
-                            to[j][vb][0] = y[0];
-                            to[j][vb][1] = y[1];
-                        }
-                    }
-                }
-            }
-        };
-#pragma unroll
-        for (int i = 0; i < BUF; i++) look(pg[i], kt + i);
-#pragma unroll
-        for (int i = 0; i < BUF; i++) {
-            if (kt + i >= k1) break;
-            load(un[i].k, un[i].ok, kbase, pg[i], kt + i);
-            load(un[i].v, un[i].ok, vbase, pg[i], kt + i);
-        }
-
-        // the queries
-        u32x4 qf[KS][NS];
-        float qscale = scale2;
-        {
-            const bool row = col < g.G;
-            const Q* q = reinterpret_cast<const Q*>(g.q) + b * g.qs + (int64_t)(head * g.G + (row ? col : 0)) * a.D;
-            float x[KS][8];
-            load_query<KS>(q, row, per, lg, sign, x);
-            if constexpr (NS > 1 && CT == BPD_T_F16) qscale = score_scale(scale2, row_exponent<KS>(x));
-#pragma unroll
-            for (int k = 0; k < KS; k++) split8<CT, NS>(x[k], qf[k]);
-        }
         f32x4 o[NE];
-#pragma unroll
-        for (int e = 0; e < NE; e++) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float ref = kNegInf, l = 0.f;
-        // unit t, held in n; then the unit BUF further on is asked for
-        auto step = [&](Unit& n, int (&p)[2], int t) {
-            // K's rows through the wave's own LDS into the order of the product's operand: read from memory as
-            // the operand takes them, 16 lanes would meet 16 rows at a time
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-#pragma unroll
-                for (int vb = 0; vb < VB; vb++) {
-                    const int row = 16 * (j >> 2) + 4 * lg + (j & 3);
-                    if constexpr (VD == 4)
-                        *reinterpret_cast<u32x4*>(&ks[row][k_slot<DT>(row, vb * 16 + col)]) = n.k[j][vb];
-                    else
-                        reinterpret_cast<u32x2*>(&ks[row][k_slot<DT>(row, col >> 1)])[col & 1] =
-                            u32x2{n.k[j][vb][0], n.k[j][vb][1]};
-                }
-            const uint32_t ok = n.ok;
-            const bool more = t + BUF < k1;
-            int pn[2] = {p[0], p[1]};
-            if (more) {
-                load(n.k, n.ok, kbase, pn, t + BUF);
-                look(p, t + 2 * BUF);
-            }
-            u32x4 kf[2][KS];
-#pragma unroll
-            for (int x = 0; x < 2; x++)
-#pragma unroll
-                for (int k = 0; k < KS; k++)
-                    kf[x][k] = __builtin_bit_cast(u32x4, ks[16 * x + col][k_slot<DT>(col, 4 * k + lg)]);
-            f32x4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-            for (int k = 0; k < KS; k++)
-#pragma unroll
-                for (int x = 0; x < 2; x++)
-#pragma unroll
-                    for (int y = 0; y < NS; y++) sc[x] = M::go(kf[x][k], qf[k][y], sc[x]);
-            // keys that are not there: the lane's scores are those of the rows that it read
-            if (__ballot(ok != 255u) != 0) {
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (!((ok >> e) & 1u)) sc[e >> 2][e & 3] = kNegInf;
-            }
-            const float top = xor_max(fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
-                                            fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])))) * qscale;
-            if (__ballot(top - 15.f > ref) != 0) {
-                const float nr = top - 15.f > ref ? top - 12.f : ref;
-                const float f = nr == ref ? 1.f : __builtin_amdgcn_exp2f(ref - nr);
-                l *= f;
-#pragma unroll
-                for (int e = 0; e < NE; e++) o[e] *= f;
-                ref = nr;
-            }
-            const float base = ref == kNegInf ? 0.f : ref;
-            float w8[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) w8[e] = __builtin_amdgcn_exp2f(fmaf(sc[e >> 2][e & 3], qscale, -base));
-            l += ((w8[0] + w8[1]) + (w8[2] + w8[3])) + ((w8[4] + w8[5]) + (w8[6] + w8[7]));
-            u32x4 pf[NS];
-            split8<CT, NS>(w8, pf);
-#pragma unroll
-            for (int vb = 0; vb < VB; vb++)
-#pragma unroll
-                for (int e = 0; e < 2 * VD; e++) {
-                    const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
-                    u32x4 vf;
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        vf[j] = __builtin_amdgcn_perm(n.v[2 * j + 1][vb][e >> 1], n.v[2 * j][vb][e >> 1], sel);
-#pragma unroll
-                    for (int x = 0; x < NS; x++) o[vb * 8 + e] = M::go(vf, pf[x], o[vb * 8 + e]);
-                }
-            if (more) load(n.v, n.ok, vbase, pn, t + BUF);
-        };
-        // the pages of the units behind those in flight
-#pragma unroll
-        for (int i = 0; i < BUF; i++) look(pg[i], kt + BUF + i);
-        while (true) {
-#pragma unroll
-            for (int i = 0; i < BUF; i++) {
-                if (kt + i >= k1) break;
-                step(un[i], pg[i], kt + i);
-            }
-            kt += BUF;
-            if (kt >= k1) break;
-        }
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
+        float ref, l;
+        wave_range<QT, CT, NS, DT, UNI, WIN>(g, ks, b, head, own, span, low, kt, k1, stream, o, ref, l);
         if (col < g.G) {
             const int h = head * g.G + col;
             if (last_word) {
@@ -1102,6 +1136,59 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_wave(AttnArgs g
     __shared__ uint4 ks[4][32][DT / 8];
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     wave_share<QT, CT, NS, DT, UNI, WIN>(g, ks[wave], (int)blockIdx.x * 4 + wave, g.waves, wave_units<WIN>(g));
+}
+
+// The same with a workgroup for each (sequence, head), whose waves share its units and add up what they have in LDS:
+// one launch, for batches of which the host knows that the shares are about even.
+template <int QT, int CT, int NS, int DT, bool UNI, int NW>
+__global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_head(AttnArgs g) {
+    using Q = typename Elem<QT>::type;
+    constexpr int NE = DT / 16, VD = DT < 128 ? 2 : 4, VB = DT < 128 ? 1 : DT / 128;
+    __shared__ uint4 ks[NW][32][DT / 8];  // then the waves' sums, 16 rows of DT
+    __shared__ float2 ml[NW][16];
+    const Paged& a = g.a;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int b = (int)blockIdx.x / a.hkv, head = (int)blockIdx.x - b * a.hkv;
+    const int own = own_rows(a, b);
+    Span span = {};
+    int low = 0;
+    const int nk = wave_rows<true>(g, b, own, span, low);
+    const int k0 = (int)((int64_t)nk * wave / NW), k1 = (int)((int64_t)nk * (wave + 1) / NW);
+    f32x4 o[NE];
+    float ref = kNegInf, l = 0.f;
+    if (k0 < k1) {
+        wave_range<QT, CT, NS, DT, UNI, true>(g, ks[wave], b, head, own, span, low, k0, k1, g.past_mall, o, ref, l);
+        const int col = lane & 15;
+        float* to = reinterpret_cast<float*>(&ks[wave][0][0]) + col * DT;
+        if (col < g.G) store_row<float, VD, VB>(to, a.D, lane >> 4, o, 1.f);
+    }
+    if (lane < 16) ml[wave][lane] = make_float2(ref, l);
+    __syncthreads();
+    const int pieces = a.D >> 2;  // of 4 elements of a row
+    for (int i = tid; i < g.G * (DT / 4); i += 64 * NW) {
+        const int row = i / (DT / 4), piece = i % (DT / 4), h = head * g.G + row;
+        if (piece >= pieces) continue;
+        float m = kNegInf, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) m = fmaxf(m, ml[w][row].x);
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float2 x = ml[w][row];
+            // a wave that met no row (-inf, 0) weighs nothing; one of NaN scores alone keeps its NaN
+            const float f = x.x == kNegInf ? (x.y != 0.f ? x.y : 0.f) : __builtin_amdgcn_exp2f(x.x - m);
+            if (f == 0.f) continue;
+            sum += x.y * f;
+            acc += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(&ks[w][0][0]) + row * DT + 4 * piece) * f;
+        }
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
+        Vec<Q, 4> v;
+#pragma unroll
+        for (int c = 0; c < 4; c++) v.v[c] = (Q)(acc[c] * inv);
+        *reinterpret_cast<Vec<Q, 4>*>(reinterpret_cast<Q*>(g.out) + (int64_t)b * g.os + (int64_t)h * a.D + 4 * piece) = v;
+        if (g.lse != nullptr && piece == 0)
+            g.lse[(int64_t)b * g.H + h] = sum != 0.f ? (m + __builtin_log2f(sum)) * kLn2 : kNegInf;
+    }
 }
 
 // One token per sequence behind a prefix: x of the workgroups take the prefix's tiles, which the matrix

@@ -10,12 +10,40 @@ namespace bpdq {
 
 namespace {
 
+bool whole_pages(const AttnArgs& g) { return g.a.page.d % 16 == 0 && g.a.row_stride < 1 << 26; }
+
+// Waves of a workgroup for each (sequence, head), or 0: the units dealt to all waves of the chip, and a second launch.
+// `rows` is what a token sees at most, `items` sequences times kv heads.  One launch spares the dealing and the join, 6 to
+// 9 us, and costs where few items with many rows leave CUs idle.  Measured (us, one launch with 8 and with 4 waves,
+// two launches; 8 kv heads of 128, bf16):
+//   8 items, 132 / 2,052 / 4,100 rows      7.7, 8.3, 13.1 / 19.2, 25.5, 20.4 / 31.9, 45.4, 29.7
+//   128, 1,028 / 4,100                     18.1, 19.5, 27.1 / 62.7, 66.6, 68.6
+//   512, 1,028 / 4,100                     52.0, 46.6, 64.6 / 172.7, 170.5, 182.8
+// Waves with one unit in flight (`single`: fp32 queries, pages that are no multiple of 16 rows) take more than twice as
+// long for a row (5 heads of 96, page 21, 5 items, 516 / 1,028 rows: 14.7, 18.4, 14.2 / 21.7, 30.0, 15.8; 320 items:
+// 30.8, 23.8, 27.8 / 49.0, 41.6, 40.5).  Heads of 256 fill the registers with 4 waves (2 heads, 2 items, 516 / 1,028 rows:
+// -, 17.0, 17.8 / -, 24.0, 21.0; 128 items: -, 21.3, 43.6 / -, 37.0, 56.0).
+int head_waves(int DT, bool single, int64_t items, int64_t rows) {
+    if (DT == 256) return items >= 128 || rows <= 640 ? 4 : 0;
+    if (single ? rows > 640 : items < 128 && rows > 2304) return 0;
+    return items <= 256 ? 8 : 4;
+}
+
+template <int QT, int CT, int NS, int DT, bool UNI, int NW>
+void launch_head(const AttnArgs& g, hipStream_t s) {
+    hipLaunchKernelGGL((k_attn_head<QT, CT, NS, DT, UNI, NW>), dim3((unsigned)(g.a.B * g.a.hkv)), dim3(64 * NW), 0, s, g);
+}
+
 template <int QT, int CT, int NS, int DT, int MT, int NW, bool UNI>
 void launch_dim(const AttnArgs& g, hipStream_t s) {
     if (g.planned)
         hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, DT, MT, NW, UNI, true>), dim3((unsigned)g.groups), dim3(64 * NW), 0, s,
                            g);
-    else if (g.a.W > 0 || g.a.P > 0)
+    else if (DT < 256 && g.waves == 8)
+        launch_head<QT, CT, NS, DT, UNI, DT < 256 ? 8 : 4>(g, s);
+    else if (g.waves == 4)
+        launch_head<QT, CT, NS, DT, UNI, 4>(g, s);
+    else
         hipLaunchKernelGGL((k_attn_wave<QT, CT, NS, DT, UNI, true>), dim3((unsigned)(g.waves / 4)), dim3(256), 0, s, g);
 }
 
@@ -29,8 +57,9 @@ void launch_uni(const AttnArgs& g, hipStream_t s) {
 template <int QT, int CT, int NS>
 void launch_types(const AttnArgs& g, hipStream_t s) {
     if (g.planned) hipLaunchKernelGGL(k_attn_plan<true>, dim3(1), dim3(1024), 0, s, g);
-    if (g.a.page.d % 16 == 0 && g.a.row_stride < 1 << 26) launch_uni<QT, CT, NS, true>(g, s);
+    if (whole_pages(g)) launch_uni<QT, CT, NS, true>(g, s);
     else launch_uni<QT, CT, NS, false>(g, s);
+    if (!g.planned && g.waves <= 8) return;  // the workgroups have joined their waves
     // one head per wave while that fills the chip twice at most, more where most rows are done
     if ((int64_t)g.a.T * g.H <= 32768)
         hipLaunchKernelGGL((k_attn_join<QT, 1, true>), dim3((unsigned)g.a.T, (unsigned)((g.H + 3) / 4)), dim3(256), 0, s, g);
@@ -46,6 +75,14 @@ void launch_attn_window(const Paged& a, int cache_type, const void* q, int64_t q
     AttnArgs g = attn_args(a, cache_type, q, qs, out, os, lse, q_type, H, scale, 0, ws);
     g.window = window;
     g.sinks = sinks;
+    if (!g.planned) {
+        const int64_t all = (int64_t)g.a.W * g.a.page.d + g.a.P, seen = (int64_t)window + sinks, rows = seen < all ? seen : all;
+        const int64_t items = (int64_t)a.B * a.hkv;
+        const bool single = !whole_pages(g) || (q_type == BPD_T_F32 && g.DT > 64);
+        const int n = items <= INT32_MAX ? head_waves(g.DT, single, items, rows) : 0;
+        if (n > 0) g.waves = n;
+        g.past_mall = items * rows * a.D * 4 > (int64_t)256 << 20;  // as k_attn_wave's
+    }
     const bool bf = cache_type == BPD_T_BF16;
     if (q_type == BPD_T_F32 && bf) launch_types<BPD_T_F32, BPD_T_BF16, 3>(g, s);
     else if (q_type == BPD_T_F32) launch_types<BPD_T_F32, BPD_T_F16, 2>(g, s);

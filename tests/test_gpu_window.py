@@ -107,12 +107,15 @@ def test_scales(dev):
 
 
 def test_a_window_of_everything_is_the_attention_without(dev):
+    """Each is within the bound of the same exact value, as their sums may be split in other places: their difference is
+    within twice that."""
     for decode in (True, False):
         b = Batch(9, [1, 1, 1], [90, 1, 300], 0, 8, 2, 128, "bf16", "bf16", 16, decode=decode)
         cache, batch, q = b.device(dev)
         a, la = serve.attention(cache, batch, q, return_lse=True)
         w, lw = serve.attention(cache, batch, q, return_lse=True, window=1000)
-        assert torch.equal(a, w) and torch.equal(la, lw)
+        _, _, eo, el = b.attention(None, 1000, 0)
+        assert (np.abs(O.f64(a) - O.f64(w)) <= 2 * eo).all() and (np.abs(O.f64(la) - O.f64(lw)) <= 2 * el).all()
 
 
 @pytest.mark.parametrize("lens", [[2 ** 31 - 1, 5], [-3, 70], [1000, 10]])
