@@ -95,6 +95,7 @@ void launch_attn_paged(const Paged& a, int cache_type, const void* q, int64_t qs
                        int q_type, int H, float scale, void* ws, hipStream_t s);
 void launch_attn_window(const Paged& a, int cache_type, const void* q, int64_t qs, void* out, int64_t os, float* lse,
                         int q_type, int H, float scale, int window, int sinks, void* ws, hipStream_t s);
+int64_t attn_window_ws(const Paged& a, int q_type, int H, int window, int sinks);
 int64_t sample_ws(int n_rows, int vocab);
 struct SampleArgs {
     const void* logits;

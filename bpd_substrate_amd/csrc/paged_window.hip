@@ -10,7 +10,7 @@ namespace bpdq {
 
 namespace {
 
-bool whole_pages(const AttnArgs& g) { return g.a.page.d % 16 == 0 && g.a.row_stride < 1 << 26; }
+bool whole_pages(const Paged& a) { return a.page.d % 16 == 0 && a.row_stride < 1 << 26; }
 
 // Waves of a workgroup for each (sequence, head), or 0: the units dealt to all waves of the chip, and a second launch.
 // `rows` is what a token sees at most, `items` sequences times kv heads.  One launch spares the dealing and the join, 6 to
@@ -27,6 +27,19 @@ int head_waves(int DT, bool single, int64_t items, int64_t rows) {
     if (DT == 256) return items >= 128 || rows <= 640 ? 4 : 0;
     if (single ? rows > 640 : items < 128 && rows > 2304) return 0;
     return items <= 256 ? 8 : 4;
+}
+
+// Rows that a token sees at most.
+int64_t rows_seen(const Paged& a, int window, int sinks) {
+    const int64_t all = (int64_t)a.W * a.page.d + a.P, seen = (int64_t)window + sinks;
+    return seen < all ? seen : all;
+}
+// head_waves of a call, 0 where a plan has to be laid out.
+int waves_of(const Paged& a, int q_type, int G, int window, int sinks) {
+    const int DT = padded(a.D);
+    const int64_t items = (int64_t)a.B * a.hkv;
+    if (planned_way(a.q_start, G) || items > INT32_MAX) return 0;
+    return head_waves(DT, !whole_pages(a) || (q_type == BPD_T_F32 && DT > 64), items, rows_seen(a, window, sinks));
 }
 
 template <int QT, int CT, int NS, int DT, bool UNI, int NW>
@@ -57,7 +70,7 @@ void launch_uni(const AttnArgs& g, hipStream_t s) {
 template <int QT, int CT, int NS>
 void launch_types(const AttnArgs& g, hipStream_t s) {
     if (g.planned) hipLaunchKernelGGL(k_attn_plan<true>, dim3(1), dim3(1024), 0, s, g);
-    if (whole_pages(g)) launch_uni<QT, CT, NS, true>(g, s);
+    if (whole_pages(g.a)) launch_uni<QT, CT, NS, true>(g, s);
     else launch_uni<QT, CT, NS, false>(g, s);
     if (!g.planned && g.waves <= 8) return;  // the workgroups have joined their waves
     // one head per wave while that fills the chip twice at most, more where most rows are done
@@ -70,19 +83,21 @@ void launch_types(const AttnArgs& g, hipStream_t s) {
 
 }  // namespace
 
+int64_t attn_window_ws(const Paged& a, int q_type, int H, int window, int sinks) {
+    const int G = H / a.hkv, DT = padded(a.D);
+    if (waves_of(a, q_type, G, window, sinks) > 0) return 0;
+    return sizes(planned_way(a.q_start, G), a.B, a.T, G, a.hkv, rows_of(a.D, q_type == BPD_T_F32 ? 2 : 1), DT, 0).total;
+}
+
 void launch_attn_window(const Paged& a, int cache_type, const void* q, int64_t qs, void* out, int64_t os, float* lse,
                         int q_type, int H, float scale, int window, int sinks, void* ws, hipStream_t s) {
     AttnArgs g = attn_args(a, cache_type, q, qs, out, os, lse, q_type, H, scale, 0, ws);
     g.window = window;
     g.sinks = sinks;
-    if (!g.planned) {
-        const int64_t all = (int64_t)g.a.W * g.a.page.d + g.a.P, seen = (int64_t)window + sinks, rows = seen < all ? seen : all;
-        const int64_t items = (int64_t)a.B * a.hkv;
-        const bool single = !whole_pages(g) || (q_type == BPD_T_F32 && g.DT > 64);
-        const int n = items <= INT32_MAX ? head_waves(g.DT, single, items, rows) : 0;
-        if (n > 0) g.waves = n;
-        g.past_mall = items * rows * a.D * 4 > (int64_t)256 << 20;  // as k_attn_wave's
-    }
+    const int n = waves_of(g.a, q_type, g.G, window, sinks);
+    if (n > 0) g.waves = n;
+    // as k_attn_wave's
+    g.past_mall = (int64_t)a.B * a.hkv * rows_seen(g.a, window, sinks) * a.D * 4 > (int64_t)256 << 20;
     const bool bf = cache_type == BPD_T_BF16;
     if (q_type == BPD_T_F32 && bf) launch_types<BPD_T_F32, BPD_T_BF16, 3>(g, s);
     else if (q_type == BPD_T_F32) launch_types<BPD_T_F32, BPD_T_F16, 2>(g, s);

@@ -216,9 +216,9 @@ void check_window(Args& c, int window, int sinks) {
     c.shape(window >= 1, "window is below 1").shape(sinks >= 0, "sinks is negative");
 }
 
-int64_t attn_ws(const bpd_paged_cache& kv, const bpd_paged_batch& b, int n_heads, int window) {
-    return bpdq::attn_paged_ws(b.q_start, b.n_seqs, b.n_tokens, n_heads, kv.n_kv_heads, kv.head_dim,
-                               window > 0 ? 0 : b.prefix_len);
+int64_t attn_ws(const bpd_paged_cache& kv, const bpd_paged_batch& b, int q_type, int n_heads, int window, int sinks) {
+    if (window > 0) return bpdq::attn_window_ws(paged(kv, b), q_type, n_heads, window, sinks);
+    return bpdq::attn_paged_ws(b.q_start, b.n_seqs, b.n_tokens, n_heads, kv.n_kv_heads, kv.head_dim, b.prefix_len);
 }
 
 // The attention, over a window where that is above 0.
@@ -242,8 +242,9 @@ void attention(const char* fn, void* hip_stream, const bpd_paged_cache* kv, cons
     c.shape(!overlap(q, es * q_stride, es * row, out, es * out_stride, es * row, b->n_tokens), "q and out overlap");
     if (!c.ok) return;
     bpdq::WsLease lease;
-    void* w = work_space(lease, ws, ws_bytes, attn_ws(*kv, *b, n_heads, window), stream, fn);
-    if (w == nullptr) return;
+    const int64_t need = attn_ws(*kv, *b, q_type, n_heads, window, sinks);
+    void* w = need > 0 ? work_space(lease, ws, ws_bytes, need, stream, fn) : nullptr;
+    if (need > 0 && w == nullptr) return;
     if (window > 0)
         bpdq::launch_attn_window(paged(*kv, *b), kv->type, q, q_stride, out, out_stride, lse, q_type, n_heads, scale, window,
                                  sinks, w, stream);
@@ -336,7 +337,7 @@ int64_t bpd_attn_paged_workspace(const bpd_paged_cache* kv, const bpd_paged_batc
     check_paged(c, kv, b);
     if (!c.ok) return -1;
     check_attn(c, *kv, *b, n_heads);
-    return c.ok ? attn_ws(*kv, *b, n_heads, 0) : -1;
+    return c.ok ? attn_ws(*kv, *b, BPD_T_F32, n_heads, 0, 0) : -1;
 }
 
 void bpd_attn_paged_on_gpu(void* hip_stream, const bpd_paged_cache* kv, const bpd_paged_batch* b, const void* q,
@@ -346,14 +347,15 @@ void bpd_attn_paged_on_gpu(void* hip_stream, const bpd_paged_cache* kv, const bp
               ws_bytes);
 }
 
-int64_t bpd_attn_window_paged_workspace(const bpd_paged_cache* kv, const bpd_paged_batch* b, int n_heads, int window,
-                                        int sinks) {
+int64_t bpd_attn_window_paged_workspace(const bpd_paged_cache* kv, const bpd_paged_batch* b, int q_type, int n_heads,
+                                        int window, int sinks) {
     Args c("bpd_attn_window_paged_workspace");
     check_paged(c, kv, b);
     if (!c.ok) return -1;
     check_attn(c, *kv, *b, n_heads);
     check_window(c, window, sinks);
-    return c.ok ? attn_ws(*kv, *b, n_heads, window) : -1;
+    c.shape(q_type == BPD_T_F32 || q_type == kv->type, "q_type is neither fp32 nor the cache's type");
+    return c.ok ? attn_ws(*kv, *b, q_type, n_heads, window, sinks) : -1;
 }
 
 void bpd_attn_window_paged_on_gpu(void* hip_stream, const bpd_paged_cache* kv, const bpd_paged_batch* b, const void* q,

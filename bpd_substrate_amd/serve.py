@@ -133,6 +133,7 @@ class PagedCache:
         self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = k.shape
         s = [0 if n == 1 else st for n, st in zip(k.shape, k.stride())]   # of one page, row or head: never used
         self.c = _Cache(k.data_ptr(), v.data_ptr(), TYPES[k.dtype], *k.shape, s[0], s[1], s[2])
+        self._geometry = (k.shape[1:], s[1])   # what a workspace goes by
         self._p = ctypes.addressof(self.c)
 
     @classmethod
@@ -189,15 +190,15 @@ class PagedBatch:
             _bad(f"prefix_len {self.prefix_len} is more than its pages hold")
 
 
-    def _workspace(self, cache, heads, window, sinks):
+    def _workspace(self, cache, dtype, heads, window, sinks):
         """Bytes that an attention call needs, which go by shapes alone."""
-        key = (heads, cache.n_kv_heads, cache.head_dim, window, sinks)
+        key = (heads, cache._geometry, dtype, window, sinks)
         n = self._bytes.get(key)
         if n is None:
             if window is None:
                 n = gpu.call("bpd_attn_paged_workspace", cache._p, self._p, heads)
             else:
-                n = gpu.call("bpd_attn_window_paged_workspace", cache._p, self._p, heads, window, sinks)
+                n = gpu.call("bpd_attn_window_paged_workspace", cache._p, self._p, TYPES[dtype], heads, window, sinks)
             self._bytes[key] = n
         return n
 
@@ -307,7 +308,7 @@ class PagePool:
             _bad("n_tokens is negative")
         sizes = (B, B + 1, T, T, B, 0 if rows is None else B * W)
         out = torch.empty(sum(sizes), dtype=torch.int32, device=dev)
-        lens, q_start, slots, pos, refused, table = out.split(sizes)
+        lens, q_start, slots, pos, refused, table = out.split_with_sizes(sizes)
         if B == 0:
             q_start.zero_()
             slots.fill_(-1)
@@ -419,14 +420,15 @@ def attention(cache, batch, q, scale=None, out=None, return_lse=False, window=No
         out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
     os_ = _rows(out, "out", (T, H, D), q.dtype, dev)
     lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
-    n = batch._workspace(cache, H, window, sinks)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    n = batch._workspace(cache, q.dtype, H, window, sinks)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    wp = None if ws is None else ws.data_ptr()
     args = (cache._p, batch._p, q.data_ptr(), qs, out.data_ptr(), os_, None if lse is None else lse.data_ptr(),
             TYPES[q.dtype], H, D ** -0.5 if scale is None else float(scale))
     if window is None:
-        _launch(dev, gpu._fn("bpd_attn_paged_on_gpu"), *args, ws.data_ptr(), n)
+        _launch(dev, gpu._fn("bpd_attn_paged_on_gpu"), *args, wp, n)
     else:
-        _launch(dev, gpu._fn("bpd_attn_window_paged_on_gpu"), *args, window, sinks, ws.data_ptr(), n)
+        _launch(dev, gpu._fn("bpd_attn_window_paged_on_gpu"), *args, window, sinks, wp, n)
     return (out, lse) if return_lse else out
 
 

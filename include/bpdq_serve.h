@@ -204,12 +204,12 @@ void bpd_norm_rope_append_paged_gpu(const bpd_paged_cache* cache, const bpd_page
 /* bpd_attn_paged_gpu over a window: of the rows that it lets a token at position p (prefix_len + index) see, those at
  * positions j > p - window or j < sinks, the prefix's rows being the first.  window at least 1, sinks 0 or more.
  * Pages without a row that a new token sees are not read: their entries of the table may be -1.  The same rules and
- * limits otherwise; ws: at least bpd_attn_window_paged_workspace() bytes. */
+ * limits otherwise; ws: at least bpd_attn_window_paged_workspace() bytes, which may be 0 (then ws is not looked at). */
 void bpd_attn_window_paged_gpu(const bpd_paged_cache* cache, const bpd_paged_batch* batch, const void* q,
                                int64_t q_stride, void* out, int64_t out_stride, float* lse, int q_type, int n_heads,
                                float scale, int window, int sinks, void* ws, int64_t ws_bytes);
-int64_t bpd_attn_window_paged_workspace(const bpd_paged_cache* cache, const bpd_paged_batch* batch, int n_heads,
-                                        int window, int sinks);
+int64_t bpd_attn_window_paged_workspace(const bpd_paged_cache* cache, const bpd_paged_batch* batch, int q_type,
+                                        int n_heads, int window, int sinks);
 
 /* What happens to a row of logits before it is sampled, in this order, in binary32:
  *   history    tokens[row][0 .. lens[row]) (lens NULL: width), the first prompt[row] of them the prompt's (NULL:
