@@ -789,7 +789,7 @@ __device__ __forceinline__ void wave_range(const AttnArgs& g, uint4 (&ks)[32][DT
     using Q = typename Elem<QT>::type;
     constexpr int KS = DT / 32, NE = DT / 16, VD = DT < 128 ? 2 : 4, VB = DT < 128 ? 1 : DT / 128;
     // units in flight: what 256 registers hold
-    constexpr int BUF = UNI && (DT == 64 || (DT == 128 && NS == 1)) ? 2 : 1;
+    constexpr int BUF = DT == 64 || (UNI && DT == 128 && NS == 1) ? 2 : 1;
     const Paged& a = g.a;
     const int lane = (int)threadIdx.x & 63, col = lane & 15, lg = lane >> 4;
     const int per = a.D / 8;
@@ -804,6 +804,7 @@ __device__ __forceinline__ void wave_range(const AttnArgs& g, uint4 (&ks)[32][DT
     struct Unit {
         u32x4 k[8][VB], v[8][VB];
         uint32_t ok;  // bit j: row j is there
+        int64_t at[UNI ? 1 : 8];  // where, for pages of any length
     };
     Unit un[BUF];
     constexpr int NP = UNI ? 2 : 8;  // pages of a unit: of 16 rows each, or of the lane's rows
@@ -831,8 +832,21 @@ __device__ __forceinline__ void wave_range(const AttnArgs& g, uint4 (&ks)[32][DT
         const int at = i + (r.pre ? 0 : a.P);
         return at >= low || at + n <= g.sinks;
     };
+    // page of a table and row in it; those of the row behind
+    auto place = [&](int i, int& pg, int& in) {
+        pg = fdiv(a.page, i);
+        in = i - pg * (int)a.page.d;
+    };
+    auto next = [&](int& pg, int& in) {
+        in++;
+        if (in == (int)a.page.d) {
+            in = 0;
+            pg++;
+        }
+    };
     auto look = [&](int (&p)[NP], int t) {
         const Part r = part_of(t);
+        [[maybe_unused]] int pg, in;
 #pragma unroll
         for (int x = 0; x < NP; x++) {
             if constexpr (UNI) {
@@ -840,12 +854,54 @@ __device__ __forceinline__ void wave_range(const AttnArgs& g, uint4 (&ks)[32][DT
                 p[x] = t < k1 && i < r.rows ? load_uniform(r.pages + fdiv(a.page, i)) : -1;
             } else {
                 const int i = r.row + 16 * (x >> 2) + 4 * lg + (x & 3);
+                if ((x & 3) == 0) place(i, pg, in);
                 p[x] = -1;
-                if (t < k1 && i < r.rows) p[x] = r.pages[fdiv(a.page, i)];
+                if (t < k1 && i < r.rows) p[x] = r.pages[pg];
+                next(pg, in);
             }
         }
     };
-    auto load = [&](u32x4 (&to)[8][VB], uint32_t& oks, const T* base, const int (&p)[NP], int t) {
+    // the lane's part of a row, or zeros
+    auto get_row = [&](u32x4 (&to)[VB], const T* row, bool ok) {
+#pragma unroll
+        for (int vb = 0; vb < VB; vb++) {
+            const int d = vb * 128 + 2 * VD * col;
+            to[vb] = u32x4{0u, 0u, 0u, 0u};
+            if (ok && d < a.D) {
+                if constexpr (VD == 4) {
+                    to[vb] = *reinterpret_cast<const u32x4*>(row + d);
+                } else {
+                    const u32x2 y = *reinterpret_cast<const u32x2*>(row + d);
+                    to[vb][0] = y[0];
+                    to[vb][1] = y[1];
+                }
+            }
+        }
+    };
+    auto load = [&](Unit& n, auto key, const int (&p)[NP], int t) {
+        constexpr bool K = decltype(key)::value;  // the keys, or the values of the same rows afterwards
+        u32x4(&to)[8][VB] = K ? n.k : n.v;
+        const T* base = K ? kbase : vbase;
+        uint32_t& oks = n.ok;
+        if constexpr (!UNI) {
+            if constexpr (K) {
+                const Part r = part_of(t);
+                int pg, in;
+                oks = 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int i = r.row + 16 * (j >> 2) + 4 * lg + (j & 3);
+                    if ((j & 3) == 0) place(i, pg, in);
+                    const bool ok = (uint32_t)p[j] < (uint32_t)a.n_pages && i < r.rows && seen(r, i, 1);
+                    oks |= ok ? 1u << j : 0u;
+                    n.at[j] = row_at(a, p[j], in);
+                    next(pg, in);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) get_row(to[j], base + n.at[j], (oks >> j) & 1u);
+            return;
+        }
         const Part r = part_of(t);
         // a whole unit: two scalar bases, the lane's part the same for each
         if (UNI && all_lanes && r.row + 32 <= r.rows && (uint32_t)p[0] < (uint32_t)a.n_pages &&
@@ -883,24 +939,10 @@ __device__ __forceinline__ void wave_range(const AttnArgs& g, uint4 (&ks)[32][DT
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int x = j >> 2, i0 = r.row + 16 * x, i = i0 + 4 * lg + (j & 3);
-            const int page = p[UNI ? x : j], in_page = i - fdiv(a.page, UNI ? i0 : i) * (int)a.page.d;
+            const int page = p[UNI ? x : 0], in_page = i - fdiv(a.page, i0) * (int)a.page.d;
             const bool ok = page >= 0 && page < a.n_pages && i < r.rows && seen(r, i, 1);
             oks |= ok ? 1u << j : 0u;
-            const int64_t at = row_at(a, page, in_page);
-#pragma unroll
-            for (int vb = 0; vb < VB; vb++) {
-                const int d = vb * 128 + 2 * VD * col;
-                to[j][vb] = u32x4{0u, 0u, 0u, 0u};
-                if (ok && d < a.D) {
-                    if constexpr (VD == 4) {
-                        to[j][vb] = *reinterpret_cast<const u32x4*>(base + at + d);
-                    } else {
-                        const u32x2 y = *reinterpret_cast<const u32x2*>(base + at + d);
-                        to[j][vb][0] = y[0];
-                        to[j][vb][1] = y[1];
-                    }
-                }
-            }
+            get_row(to[j], base + row_at(a, page, in_page), ok);
         }
     };
 #pragma unroll
@@ -908,8 +950,8 @@ __device__ __forceinline__ void wave_range(const AttnArgs& g, uint4 (&ks)[32][DT
 #pragma unroll
     for (int i = 0; i < BUF; i++) {
         if (kt + i >= k1) break;
-        load(un[i].k, un[i].ok, kbase, pg[i], kt + i);
-        load(un[i].v, un[i].ok, vbase, pg[i], kt + i);
+        load(un[i], std::true_type(), pg[i], kt + i);
+        load(un[i], std::false_type(), pg[i], kt + i);
     }
 
     // the queries
@@ -949,7 +991,7 @@ __device__ __forceinline__ void wave_range(const AttnArgs& g, uint4 (&ks)[32][DT
 #pragma unroll
         for (int x = 0; x < NP; x++) pn[x] = p[x];
         if (more) {
-            load(n.k, n.ok, kbase, pn, t + BUF);
+            load(n, std::true_type(), pn, t + BUF);
             look(p, t + 2 * BUF);
         }
         u32x4 kf[2][KS];
@@ -1000,7 +1042,7 @@ __device__ __forceinline__ void wave_range(const AttnArgs& g, uint4 (&ks)[32][DT
 #pragma unroll
                 for (int x = 0; x < NS; x++) o[vb * 8 + e] = M::go(vf, pf[x], o[vb * 8 + e]);
             }
-        if (more) load(n.v, n.ok, vbase, pn, t + BUF);
+        if (more) load(n, std::false_type(), pn, t + BUF);
     };
     // the pages of the units behind those in flight
 #pragma unroll
