@@ -112,13 +112,13 @@ HIP_SIGNATURES = {
     "bpd_sample_on_gpu": (None, [P, P, I, L, I, I, P, P, P, P, P, P, P, P, P, L]),
     "bpd_pages_extend_gpu": (None, [P, P, P, I, I, I, P, L, P, P, P, P, P]),
     "bpd_pages_release_gpu": (None, [P, P, P, I, I, I]),
-    "bpd_norm_rope_append_paged_gpu": (None, [P, P, P, P, P, P, L, P, L, P, L, P, L, I, I]),
+    "bpd_norm_rope_append_paged_gpu": (None, [P, P, P, L, P, L, I, F, P, P, P, L, P, L, P, L, P, L, I, I]),
     "bpd_attn_window_paged_gpu": (None, [P, P, P, L, P, L, P, I, I, F, I, I, P, L]),
     "bpd_attn_window_paged_workspace": (L, [P, P, I, I, I, I]),
     "bpd_adjust_logits_gpu": (None, [P, I, L, P, I, L, I, I, P]),
     "bpd_pages_extend_on_gpu": (None, [P, P, P, P, I, I, I, P, L, P, P, P, P, P]),
     "bpd_pages_release_on_gpu": (None, [P, P, P, P, I, I, I]),
-    "bpd_norm_rope_append_paged_on_gpu": (None, [P, P, P, P, P, P, P, L, P, L, P, L, P, L, I, I]),
+    "bpd_norm_rope_append_paged_on_gpu": (None, [P, P, P, P, L, P, L, I, F, P, P, P, L, P, L, P, L, P, L, I, I]),
     "bpd_attn_window_paged_on_gpu": (None, [P, P, P, P, L, P, L, P, I, I, F, I, I, P, L]),
     "bpd_adjust_logits_on_gpu": (None, [P, P, I, L, P, I, L, I, I, P]),
 }

@@ -152,7 +152,7 @@ void check_weights(Args& c, int64_t s, int64_t D, const char* name) {
 
 // The append, with its heads normed where norm is given.
 void append(const char* fn, void* hip_stream, const bpd_paged_cache* kv, const bpd_paged_batch* b,
-            const bpd_head_norm* norm, const bpd_rope* rope, const int32_t* pos, const void* q, int64_t q_stride,
+            const bpdq::HeadNorm* norm, const bpd_rope* rope, const int32_t* pos, const void* q, int64_t q_stride,
             const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* q_out, int64_t q_out_stride, int x_type,
             int n_heads) {
     const hipStream_t stream = static_cast<hipStream_t>(hip_stream);
@@ -168,16 +168,16 @@ void append(const char* fn, void* hip_stream, const bpd_paged_cache* kv, const b
                 "rot_dim is negative, odd or above head_dim").shape(rope->neox == 0 || rope->neox == 1,
                                                                      "neox is neither 0 nor 1");
     if (norm != nullptr) {
-        c.shape(norm->type == BPD_T_F32 || norm->type == x_type, "the norm's type is neither fp32 nor x_type");
+        c.shape(norm->type == BPD_T_F32 || norm->type == x_type, "w_type is neither fp32 nor x_type");
         c.shape(norm->eps >= 0.f, "eps is below 0 or no number");
         const int64_t D = kv->head_dim;
-        if (norm->q != nullptr) check_weights(c, norm->q_stride, D, "norm.q_stride");
-        if (norm->k != nullptr) check_weights(c, norm->k_stride, D, "norm.k_stride");
+        if (norm->q != nullptr) check_weights(c, norm->q_stride, D, "q_norm_stride");
+        if (norm->k != nullptr) check_weights(c, norm->k_stride, D, "k_norm_stride");
     }
     if (!c.ok || b->n_seqs == 0 || b->n_tokens == 0) return;
     const int es = esize(x_type);
-    if (norm != nullptr && norm->q != nullptr) c.ptr(norm->q, 16, "norm.q");
-    if (norm != nullptr && norm->k != nullptr) c.ptr(norm->k, 16, "norm.k");
+    if (norm != nullptr && norm->q != nullptr) c.ptr(norm->q, 16, "q_norm");
+    if (norm != nullptr && norm->k != nullptr) c.ptr(norm->k, 16, "k_norm");
     if (n_heads > 0)
         c.ptr(q, 16, "q").ptr(q_out, 16, "q_out").stride(q_stride, (int64_t)n_heads * kv->head_dim, es, "q_stride")
             .stride(q_out_stride, (int64_t)n_heads * kv->head_dim, es, "q_out_stride");
@@ -202,9 +202,7 @@ void append(const char* fn, void* hip_stream, const bpd_paged_cache* kv, const b
     const double* turns = rot > 0 ? rope->turns : nullptr;
     const bool neox = rot > 0 && rope->neox == 1;
     if (norm != nullptr && (norm->q != nullptr || norm->k != nullptr))
-        bpdq::launch_norm_append(paged(*kv, *b), kv->type,
-                                 {norm->q, norm->k, norm->type, norm->q_stride, norm->k_stride, norm->eps}, turns, rot, neox,
-                                 pos, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, x_type, n_heads, stream);
+        bpdq::launch_norm_append(paged(*kv, *b), kv->type, *norm, turns, rot, neox, pos, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, x_type, n_heads, stream);
     else
         bpdq::launch_rope_append(paged(*kv, *b), kv->type, turns, rot, neox, pos, q, q_stride, k, k_stride, v, v_stride,
                                  q_out, q_out_stride, x_type, n_heads, stream);
@@ -305,23 +303,24 @@ void bpd_rope_append_paged_on_gpu(void* hip_stream, const bpd_paged_cache* kv, c
 }
 
 void bpd_norm_rope_append_paged_on_gpu(void* hip_stream, const bpd_paged_cache* kv, const bpd_paged_batch* b,
-                                       const bpd_head_norm* norm, const bpd_rope* rope, const int32_t* pos, const void* q,
-                                       int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
-                                       void* q_out, int64_t q_out_stride, int x_type, int n_heads) {
-    const char* fn = "bpd_norm_rope_append_paged_gpu";
-    Args c(fn);
-    c.need(norm != nullptr, BPDQ_ERR_NULL, "norm is NULL");
-    if (!c.ok) return;
-    append(fn, hip_stream, kv, b, norm, rope, pos, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, x_type,
-           n_heads);
+                                       const void* q_norm, int64_t q_norm_stride, const void* k_norm,
+                                       int64_t k_norm_stride, int w_type, float eps, const bpd_rope* rope,
+                                       const int32_t* pos, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                                       const void* v, int64_t v_stride, void* q_out, int64_t q_out_stride, int x_type,
+                                       int n_heads) {
+    const bpdq::HeadNorm norm = {q_norm, k_norm, w_type, q_norm_stride, k_norm_stride, eps};
+    append("bpd_norm_rope_append_paged_gpu", hip_stream, kv, b, &norm, rope, pos, q, q_stride, k, k_stride, v, v_stride,
+           q_out, q_out_stride, x_type, n_heads);
 }
 
-void bpd_norm_rope_append_paged_gpu(const bpd_paged_cache* kv, const bpd_paged_batch* b, const bpd_head_norm* norm,
-                                    const bpd_rope* rope, const int32_t* pos, const void* q, int64_t q_stride,
+void bpd_norm_rope_append_paged_gpu(const bpd_paged_cache* kv, const bpd_paged_batch* b, const void* q_norm,
+                                    int64_t q_norm_stride, const void* k_norm, int64_t k_norm_stride, int w_type,
+                                    float eps, const bpd_rope* rope, const int32_t* pos, const void* q, int64_t q_stride,
                                     const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* q_out,
                                     int64_t q_out_stride, int x_type, int n_heads) {
-    bpd_norm_rope_append_paged_on_gpu(bpdq::abi_stream(), kv, b, norm, rope, pos, q, q_stride, k, k_stride, v, v_stride,
-                                      q_out, q_out_stride, x_type, n_heads);
+    bpd_norm_rope_append_paged_on_gpu(bpdq::abi_stream(), kv, b, q_norm, q_norm_stride, k_norm, k_norm_stride, w_type, eps,
+                                      rope, pos, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, x_type,
+                                      n_heads);
 }
 
 void bpd_rope_append_paged_gpu(const bpd_paged_cache* kv, const bpd_paged_batch* b, const bpd_rope* rope,

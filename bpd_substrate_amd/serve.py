@@ -60,11 +60,6 @@ class _Pool(ctypes.Structure):     # bpd_page_pool
                 ("page_size", ctypes.c_int)]
 
 
-class _Norm(ctypes.Structure):     # bpd_head_norm
-    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("type", ctypes.c_int), ("q_stride", ctypes.c_int64),
-                ("k_stride", ctypes.c_int64), ("eps", ctypes.c_float)]
-
-
 class _Rules(ctypes.Structure):    # bpd_logit_rules
     _fields_ = [("tokens", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("token_width", ctypes.c_int),
                 ("lens", ctypes.c_void_p), ("prompt", ctypes.c_void_p), ("repetition", ctypes.c_void_p),
@@ -332,22 +327,15 @@ class PagePool:
                 max(0, sinks - prefix_len))
 
 
-def _head_norm(q_norm, k_norm, eps, x, heads, kv_heads, D):
-    """bpd_head_norm of weights [head_dim] or [heads, head_dim], fp32 or of x's type."""
-    one = q_norm if q_norm is not None else k_norm
-    ptrs, strides = [], []
-    for w, what, h in ((q_norm, "q_norm", heads), (k_norm, "k_norm", kv_heads)):
-        if w is None:
-            ptrs.append(None)
-            strides.append(0)
-            continue
-        if w.dtype not in (torch.float32, x.dtype) or w.dtype != one.dtype or w.device != x.device:
-            _bad(f"{what} is {w.dtype} on {w.device}, not float32 or {x.dtype} on {x.device}, alike for q and k")
-        if w.shape != (D,) and w.shape != (h, D) or not w.is_contiguous():
-            _bad(f"{what} is not a contiguous [{D}] or [{h}, {D}]")
-        ptrs.append(w.data_ptr())
-        strides.append(0 if w.dim() == 1 else D)
-    return _Norm(*ptrs, TYPES[one.dtype], *strides, eps)
+def _weights(w, what, x, heads, D):
+    """Address and stride of a norm's weights [head_dim] or [heads, head_dim], float32 or of x's type."""
+    if w is None:
+        return None, 0
+    if w.dtype is not torch.float32 and w.dtype is not x.dtype or w.device != x.device:
+        _bad(f"{what} is {w.dtype} on {w.device}, not float32 or {x.dtype} on {x.device}")
+    if w.shape != (D,) and w.shape != (heads, D) or not w.is_contiguous():
+        _bad(f"{what} is not a contiguous [{D}] or [{heads}, {D}]")
+    return w.data_ptr(), 0 if w.dim() == 1 else D
 
 
 def rope_append(cache, batch, q, k, v, rope=None, pos=None, q_out=None, q_norm=None, k_norm=None, eps=1e-6):
@@ -373,8 +361,9 @@ def rope_append(cache, batch, q, k, v, rope=None, pos=None, q_out=None, q_norm=N
         H = q.shape[1]
         qs = _rows(q, "q", (T, H, D), x.dtype, dev)
         if q_out is None:
-            q_out = torch.empty((T, H, D), dtype=x.dtype, device=dev)
-        os_ = _rows(q_out, "q_out", (T, H, D), x.dtype, dev)
+            q_out, os_ = torch.empty((T, H, D), dtype=x.dtype, device=dev), H * D
+        else:
+            os_ = _rows(q_out, "q_out", (T, H, D), x.dtype, dev)
         qp, op = q.data_ptr(), q_out.data_ptr()
     kp = vp = None
     ks = vs = 0
@@ -393,8 +382,12 @@ def rope_append(cache, batch, q, k, v, rope=None, pos=None, q_out=None, q_norm=N
     if q_norm is None and k_norm is None:
         _launch(dev, gpu._fn("bpd_rope_append_paged_on_gpu"), cache._p, batch._p, *args)
     else:
-        norm = _head_norm(q_norm, k_norm, eps, x, H, cache.n_kv_heads, D)
-        _launch(dev, gpu._fn("bpd_norm_rope_append_paged_on_gpu"), cache._p, batch._p, ctypes.addressof(norm), *args)
+        qw, qws = _weights(q_norm, "q_norm", x, H, D)
+        kw, kws = _weights(k_norm, "k_norm", x, cache.n_kv_heads, D)
+        wt = (k_norm if q_norm is None else q_norm).dtype
+        if q_norm is not None and k_norm is not None and k_norm.dtype is not wt:
+            _bad(f"q_norm is {wt} and k_norm {k_norm.dtype}")
+        _launch(dev, gpu._fn("bpd_norm_rope_append_paged_on_gpu"), cache._p, batch._p, qw, qws, kw, kws, TYPES[wt], eps, *args)
     return q_out
 
 
@@ -417,8 +410,9 @@ def attention(cache, batch, q, scale=None, out=None, return_lse=False, window=No
         _bad(f"q is {q.dtype}, neither float32 nor the cache's {cache.dtype}")
     qs = _rows(q, "q", (T, H, D), q.dtype, dev)
     if out is None:
-        out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
-    os_ = _rows(out, "out", (T, H, D), q.dtype, dev)
+        out, os_ = torch.empty((T, H, D), dtype=q.dtype, device=dev), H * D
+    else:
+        os_ = _rows(out, "out", (T, H, D), q.dtype, dev)
     lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
     n = batch._workspace(cache, q.dtype, H, window, sinks)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
@@ -467,6 +461,15 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
     return token, logprob, kept
 
 
+def _pitch(t, what):
+    """Elements from a row of a 2-D tensor to the next."""
+    n, w = t.shape
+    s = t.stride()
+    if w > 1 and s[1] != 1 or n > 1 and s[0] < w:
+        _bad(f"rows of {what} are not contiguous, or overlap")
+    return s[0] if n > 1 else w
+
+
 def adjust_logits(logits, tokens=None, lens=None, prompt=None, repetition=None, frequency=None, presence=None, bias=None,
                   mask=None, mask_row=None, out=None, dtype=None):
     """Rows of logits [rows, vocab] under penalties, biases and masks (bpd_adjust_logits_gpu), in that order.
@@ -485,51 +488,56 @@ def adjust_logits(logits, tokens=None, lens=None, prompt=None, repetition=None, 
         _bad(f"logits have {logits.dim()} dimensions, not 2")
     B, V = logits.shape
     dev = logits.device
+    xs = _pitch(logits, "logits")
     if out is None:
-        out = torch.empty((B, V), dtype=logits.dtype if dtype is None else dtype, device=dev)
-    if out.dtype not in (logits.dtype, torch.float32) or dtype not in (None, out.dtype) or out.shape != (B, V) \
-            or out.device != dev:
-        _bad(f"out is {out.dtype} {list(out.shape)} on {out.device}, not {logits.dtype} or float32 {[B, V]} on {dev}")
-    for t, what in ((logits, "logits"), (out, "out")):
-        if V > 1 and t.stride(1) != 1 or B > 1 and t.stride(0) < V:
-            _bad(f"rows of {what} are not contiguous, or overlap")
+        if dtype is not None and dtype is not torch.float32 and dtype is not logits.dtype:
+            _bad(f"dtype is {dtype}, neither float32 nor the logits' {logits.dtype}")
+        out, ys = torch.empty((B, V), dtype=logits.dtype if dtype is None else dtype, device=dev), V
+    else:
+        if out.dtype not in (logits.dtype, torch.float32) or dtype not in (None, out.dtype) or out.shape != (B, V) \
+                or out.device != dev:
+            _bad(f"out is {out.dtype} {list(out.shape)} on {out.device}, not {logits.dtype} or float32 {[B, V]} on {dev}")
+        ys = _pitch(out, "out")
     if tokens is None and (lens is not None or prompt is not None):
         _bad("lens or prompt without tokens")
     if mask is None and mask_row is not None:
         _bad("mask_row without mask")
-    i32, f32, r = torch.int32, torch.float32, _Rules()
-    for t, what, dt in ((lens, "lens", i32), (prompt, "prompt", i32), (repetition, "repetition", f32),
-                        (frequency, "frequency", f32), (presence, "presence", f32), (mask_row, "mask_row", i32)):
+    if tokens is None and not (repetition is frequency is presence is None):
+        _bad("penalties without tokens")
+    i32, r = (torch.int32,), _Rules()
+
+    def per_row(t, what, dt):
         if t is None:
-            continue
+            return None
         if t.dtype is not dt or t.shape != (B,) or t.device != dev or not t.is_contiguous():
             _bad(f"{what} is not a contiguous {dt} [{B}] on {dev}")
-        setattr(r, what, t.data_ptr())
-    for t, what, n in ((tokens, "tokens", B), (mask, "mask", None)):
-        if t is None:
-            continue
-        _tensor(t, what, (i32,), 2, dev)
-        h, w = t.shape
-        if n is not None and h != n:
-            _bad(f"{what} has {h} rows and logits {n}")
-        if w > 1 and t.stride(1) != 1 or h > 1 and t.stride(0) < w:
-            _bad(f"rows of {what} are not contiguous, or overlap")
-        if what == "tokens":
-            r.tokens, r.token_stride, r.token_width = t.data_ptr(), t.stride(0) if h > 1 else w, w
-        else:
-            if w < (V + 31) // 32:
-                _bad(f"mask has {w} words a row for {V} tokens")
-            r.mask, r.mask_stride, r.n_masks = t.data_ptr(), t.stride(0) if h > 1 else w, h
+        return t.data_ptr()
+
+    if tokens is not None:
+        _tensor(tokens, "tokens", i32, 2, dev)
+        h, w = tokens.shape
+        if h != B:
+            _bad(f"tokens has {h} rows and logits {B}")
+        r.tokens, r.token_stride, r.token_width = tokens.data_ptr(), _pitch(tokens, "tokens"), w
+        r.lens, r.prompt = per_row(lens, "lens", torch.int32), per_row(prompt, "prompt", torch.int32)
+        r.repetition = per_row(repetition, "repetition", torch.float32)
+        r.frequency = per_row(frequency, "frequency", torch.float32)
+        r.presence = per_row(presence, "presence", torch.float32)
+    if mask is not None:
+        _tensor(mask, "mask", i32, 2, dev)
+        if mask.shape[1] < (V + 31) // 32:
+            _bad(f"mask has {mask.shape[1]} words a row for {V} tokens")
+        r.mask, r.mask_stride, r.n_masks = mask.data_ptr(), _pitch(mask, "mask"), mask.shape[0]
+        r.mask_row = per_row(mask_row, "mask_row", torch.int32)
     if bias is not None:
         start, token, value = bias
-        _tensor(start, "bias's start", (i32,), 1, dev, contiguous=True)
-        _tensor(token, "bias's token", (i32,), 1, dev, contiguous=True)
-        _tensor(value, "bias's value", (f32,), 1, dev, contiguous=True)
+        _tensor(start, "bias's start", i32, 1, dev, contiguous=True)
+        _tensor(token, "bias's token", i32, 1, dev, contiguous=True)
+        _tensor(value, "bias's value", (torch.float32,), 1, dev, contiguous=True)
         if start.shape[0] != B + 1 or token.shape != value.shape:
             _bad(f"bias has {start.shape[0]} offsets for {B} rows, or {token.shape[0]} tokens and {value.shape[0]} values")
         r.bias_start, r.bias_token, r.bias_value, r.n_bias = (start.data_ptr(), token.data_ptr(), value.data_ptr(),
                                                               token.shape[0])
-    _launch(dev, gpu._fn("bpd_adjust_logits_on_gpu"), logits.data_ptr(), TYPES[logits.dtype],
-            logits.stride(0) if B > 1 else V, out.data_ptr(), TYPES[out.dtype], out.stride(0) if B > 1 else V, B, V,
-            ctypes.addressof(r))
+    _launch(dev, gpu._fn("bpd_adjust_logits_on_gpu"), logits.data_ptr(), TYPES[logits.dtype], xs, out.data_ptr(),
+            TYPES[out.dtype], ys, B, V, ctypes.addressof(r))
     return out

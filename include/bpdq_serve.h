@@ -186,18 +186,13 @@ void bpd_pages_release_gpu(const bpd_page_pool* pool, const int32_t* rows, const
 
 /* bpd_rope_append_paged_gpu with every head of q and k normed before it turns:
  *   y_i = x_i / sqrt(mean over the head of x^2 + eps) * w_i
- * q and k: [head_dim] weights of all heads (stride 0), or of each, a head's q_stride / k_stride elements behind
- * the one before (multiples of 8, head_dim at least); of `type`, fp32 or x's.  NULL: not normed.  The sum of
- * squares, the scale and the rotation are binary32 (a head whose squares add up beyond it becomes 0), and
- * the result is rounded once. */
-typedef struct {
-    const void *q, *k;
-    int type;
-    int64_t q_stride, k_stride;
-    float eps; /* not below 0 */
-} bpd_head_norm;
-void bpd_norm_rope_append_paged_gpu(const bpd_paged_cache* cache, const bpd_paged_batch* batch, const bpd_head_norm* norm,
-                                    const bpd_rope* rope, const int32_t* pos, const void* q, int64_t q_stride,
+ * q_norm and k_norm: [head_dim] weights of all heads (stride 0), or of each, a head's stride elements
+ * behind the one before (multiples of 8, head_dim at least); of w_type, fp32 or x_type.  NULL: not normed.  eps is not
+ * below 0.  The sum of squares, the scale and the rotation are binary32 (a head whose squares add up beyond it
+ * becomes 0), and the result is rounded once. */
+void bpd_norm_rope_append_paged_gpu(const bpd_paged_cache* cache, const bpd_paged_batch* batch, const void* q_norm,
+                                    int64_t q_norm_stride, const void* k_norm, int64_t k_norm_stride, int w_type,
+                                    float eps, const bpd_rope* rope, const int32_t* pos, const void* q, int64_t q_stride,
                                     const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* q_out,
                                     int64_t q_out_stride, int x_type, int n_heads);
 
@@ -262,9 +257,11 @@ void bpd_pages_extend_on_gpu(void* hip_stream, const bpd_page_pool* pool, const 
 void bpd_pages_release_on_gpu(void* hip_stream, const bpd_page_pool* pool, const int32_t* rows, const int32_t* keep,
                               int n_seqs, int window, int sinks);
 void bpd_norm_rope_append_paged_on_gpu(void* hip_stream, const bpd_paged_cache* cache, const bpd_paged_batch* batch,
-                                       const bpd_head_norm* norm, const bpd_rope* rope, const int32_t* pos, const void* q,
-                                       int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
-                                       void* q_out, int64_t q_out_stride, int x_type, int n_heads);
+                                       const void* q_norm, int64_t q_norm_stride, const void* k_norm,
+                                       int64_t k_norm_stride, int w_type, float eps, const bpd_rope* rope,
+                                       const int32_t* pos, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                                       const void* v, int64_t v_stride, void* q_out, int64_t q_out_stride, int x_type,
+                                       int n_heads);
 void bpd_attn_window_paged_on_gpu(void* hip_stream, const bpd_paged_cache* cache, const bpd_paged_batch* batch,
                                   const void* q, int64_t q_stride, void* out, int64_t out_stride, float* lse, int q_type,
                                   int n_heads, float scale, int window, int sinks, void* ws, int64_t ws_bytes);
