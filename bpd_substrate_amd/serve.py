@@ -319,8 +319,8 @@ class PagePool:
         window also those that neither the tokens to come see through it nor hold one of the first `sinks` positions, of
         which the first prefix_len are a shared prefix's (bpd_pages_release_gpu).  rows and keep None: every row."""
         B, rp, kp = self._rows(rows, keep, "keep")
-        if window is not None and window < 1:
-            _bad(f"window {window} is below 1")
+        if window is not None and (window < 1 or self.gone is None):
+            _bad(f"window {window} is below 1, or the pool is without gone")
         if sinks < 0 or prefix_len < 0:
             _bad("sinks or prefix_len is negative")
         _launch(self.device, gpu._fn("bpd_pages_release_on_gpu"), self._p, rp, kp, B, 0 if window is None else window,
