@@ -70,11 +70,11 @@ __device__ __forceinline__ int seen_rows(const Paged& a, int b, int n, int i, in
 __device__ __forceinline__ int64_t position(const Paged& a, int b, int n, int i) {
     return (int64_t)a.P + a.lens[b] - n + i;
 }
-// The units that the tokens of tile r of sequence b's rows see through the window.
-__device__ __forceinline__ Span item_span(const AttnArgs& g, int b, int n, int r) {
+// The units of U rows that the tokens of tile r, of R rows, of sequence b's see through the window.
+__device__ __forceinline__ Span item_span(const AttnArgs& g, int b, int n, int r, int R, int U) {
     const Paged& a = g.a;
-    const int first = (int)((int64_t)r * g.R / g.G), last = min(n, ((r + 1) * g.R - 1) / g.G + 1) - 1;
-    return span_of(position(a, b, n, first), g.window, g.sinks, a.P, seen_rows(a, b, n, last, own_rows(a, b)), kKeys);
+    const int first = fdiv(g.g, r * R), last = min(n, fdiv(g.g, (r + 1) * R - 1) + 1) - 1;
+    return span_of(position(a, b, n, first), g.window, g.sinks, a.P, seen_rows(a, b, n, last, own_rows(a, b)), U);
 }
 // The units of 32 rows that sequence b's one token sees.
 __device__ __forceinline__ Span wave_span(const AttnArgs& g, int b) {
@@ -179,7 +179,7 @@ __global__ __launch_bounds__(1024) void k_attn_plan(AttnArgs g) {
             int t0, n;
             seq_tokens(a, b, t0, n);
             if constexpr (WIN) {
-                const Span x = item_span(g, b, n, r);
+                const Span x = item_span(g, b, n, r, g.R, kKeys);
                 mine = prefix_units(x) + own_units(x);
             } else {
                 const int last = min(n, ((r + 1) * g.R - 1) / g.G + 1) - 1;
@@ -423,7 +423,7 @@ __device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w,
                 seq_tokens(a, b, t0, n);
                 own = own_rows(a, b);
                 if constexpr (WIN) {
-                    span = item_span(g, b, n, rt);
+                    span = item_span(g, b, n, rt, g.R, kKeys);
                     ntp = prefix_units(span);
                 } else {
                     if (!is_joint(g, n)) ntp = 0;
@@ -780,10 +780,15 @@ __device__ __forceinline__ void tile_share(const AttnArgs& g, Lds<DT>& s, int w,
 // WIN: the sequence's units are those of the prefix and of its own rows that the token sees.
 //
 // This is a wave's share of one (sequence, head): its units [kt, k1), kt below k1.  o, l: sums with weights 2^(score - ref).
-template <int QT, int CT, int NS, int DT, bool UNI, bool WIN>
+// ROWS: the columns are 16 of the rows of several tokens, `own` and `low` what the last and the first of them see; units
+// that some do not see whole are masked, as k_attn_tile masks them.
+struct Rows {
+    int t0, n, tile;  // the sequence's first token, its tokens, which 16 rows of theirs
+};
+template <int QT, int CT, int NS, int DT, bool UNI, bool WIN, bool ROWS = false>
 __device__ __forceinline__ void wave_range(const AttnArgs& g, uint4 (&ks)[32][DT / 8], int b, int head, int own,
                                            const Span& span, int low, int kt, int k1, bool stream, f32x4 (&o)[DT / 16],
-                                           float& ref, float& l) {
+                                           float& ref, float& l, Rows rows = {}) {
     using M = Mfma<CT>;
     using T = typename M::T;
     using Q = typename Elem<QT>::type;
@@ -957,9 +962,26 @@ __device__ __forceinline__ void wave_range(const AttnArgs& g, uint4 (&ks)[32][DT
     // the queries
     u32x4 qf[KS][NS];
     float qscale = scale2;
+    [[maybe_unused]] int lim_c = 0, low_c = 0, lim_all = 0, low_all = 0;  // ROWS: what the lane's row sees, and what all do
+    [[maybe_unused]] int mend0 = 1 << 30, mend1 = 0;
     {
-        const bool row = col < g.G;
+        bool row = col < g.G;
         const Q* q = reinterpret_cast<const Q*>(g.q) + b * g.qs + (int64_t)(head * g.G + (row ? col : 0)) * a.D;
+        if constexpr (ROWS) {
+            const int r = rows.tile * 16 + col, i = fdiv(g.g, r);
+            row = i < rows.n;
+            q = reinterpret_cast<const Q*>(g.q) + (int64_t)(rows.t0 + (row ? i : 0)) * g.qs +
+                (int64_t)(head * g.G + r - i * g.G) * a.D;
+            lim_c = row ? seen_rows(a, b, rows.n, i, own_rows(a, b)) : own;
+            low_c = row ? (int)min(window_low(position(a, b, rows.n, i), g.window), (int64_t)a.P + own) : 0;
+            int x = lim_c, y = low_c;
+            for (int d = 1; d < 16; d <<= 1) {
+                x = min(x, __shfl_xor(x, d));
+                y = max(y, __shfl_xor(y, d));
+            }
+            lim_all = __builtin_amdgcn_readfirstlane(x);
+            low_all = __builtin_amdgcn_readfirstlane(y);
+        }
         float x[KS][8];
         load_query<KS>(q, row, per, lg, sign, x);
         if constexpr (NS > 1 && CT == BPD_T_F16) qscale = score_scale(scale2, row_exponent<KS>(x));
@@ -1013,6 +1035,36 @@ __device__ __forceinline__ void wave_range(const AttnArgs& g, uint4 (&ks)[32][DT
             for (int e = 0; e < 8; e++)
                 if (!((ok >> e) & 1u)) sc[e >> 2][e & 3] = kNegInf;
         }
+        if constexpr (ROWS) {
+            const Part r = part_of(t);
+            const int at = r.row + (r.pre ? 0 : a.P);
+            if ((!r.pre && lim_all < min(own, r.row + 32)) || (at < low_all && at + 32 > g.sinks)) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int k = 16 * (e >> 2) + 4 * lg + (e & 3);
+                    if ((!r.pre && r.row + k >= lim_c) || (at + k < low_c && at + k >= g.sinks)) sc[e >> 2][e & 3] = kNegInf;
+                }
+                // an infinity or NaN in a row that some columns do not see counts as 0 here, and is added to those that
+                // do see it at the end
+                uint32_t x = 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++)
+#pragma unroll
+                        for (int d = 0; d < VD; d++) x |= not_finite<CT>(n.v[j][vb][d]);
+                if (__ballot(x != 0) != 0) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+#pragma unroll
+                        for (int vb = 0; vb < VB; vb++)
+#pragma unroll
+                            for (int d = 0; d < VD; d++) n.v[j][vb][d] = finite_or_0<CT>(n.v[j][vb][d]);
+                    mend0 = min(mend0, at - a.P);
+                    mend1 = at - a.P + 32;
+                }
+            }
+        }
         const float top = xor_max(fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                                         fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])))) * qscale;
         if (__ballot(top - 15.f > ref) != 0) {
@@ -1058,6 +1110,28 @@ __device__ __forceinline__ void wave_range(const AttnArgs& g, uint4 (&ks)[32][DT
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
+    if constexpr (ROWS) {
+        for (int key = mend0; key < min(mend1, own); key++) {  // own rows; row P + key of the prefix below 0
+            const bool pre = key < 0;
+            const int row = pre ? a.P + key : key, pgi = fdiv(a.page, row), page = pre ? a.prefix[pgi] : table[pgi];
+            if (page < 0 || page >= a.n_pages) continue;
+            if ((!pre && key >= lim_c) || (a.P + key < low_c && a.P + key >= g.sinks)) continue;
+            const T* v = vbase + row_at(a, page, row - pgi * (int)a.page.d);
+#pragma unroll
+            for (int vb = 0; vb < VB; vb++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int d = vb * 128 + 2 * VD * (4 * lg + r);
+                    if (d >= a.D) continue;
+                    const Vec<T, 2 * VD> x = *reinterpret_cast<const Vec<T, 2 * VD>*>(v + d);
+#pragma unroll
+                    for (int e = 0; e < 2 * VD; e++) {
+                        const float y = (float)x.v[e];
+                        if (!(__builtin_fabsf(y) < -kNegInf)) o[vb * 8 + e][r] += y;
+                    }
+                }
+        }
+    }
 }
 
 // The first position that sequence b's token sees through the window, and the units.
@@ -1180,9 +1254,38 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_wave(AttnArgs g
     wave_share<QT, CT, NS, DT, UNI, WIN>(g, ks[wave], (int)blockIdx.x * 4 + wave, g.waves, wave_units<WIN>(g));
 }
 
-// The same with a workgroup for each (sequence, head), whose waves share its units and add up what they have in LDS:
-// one launch, for batches of which the host knows that the shares are about even.
-template <int QT, int CT, int NS, int DT, bool UNI, int NW>
+// The sequence that the j-th tile of 16 rows is of, and which of its; false: there are fewer.  The whole wave.
+__device__ __forceinline__ bool tile_at(const AttnArgs& g, int j, int& b, Rows& rows) {
+    const int lane = (int)threadIdx.x & 63;
+    int before = 0;
+    for (int b0 = 0; b0 < g.a.B; b0 += 64) {
+        int t0 = 0, n = 0;
+        if (b0 + lane < g.a.B) seq_tokens(g.a, b0 + lane, t0, n);
+        const int mine = (n * g.G + 15) >> 4;
+        int x = mine;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(x, d);
+            if (lane >= d) x += o;
+        }
+        const uint64_t over = __ballot(before + x > j);
+        if (over != 0) {
+            const int at = __builtin_ctzll(over);
+            b = __builtin_amdgcn_readfirstlane(b0 + at);
+            rows.t0 = __builtin_amdgcn_readfirstlane(__shfl(t0, at));
+            rows.n = __builtin_amdgcn_readfirstlane(__shfl(n, at));
+            rows.tile = __builtin_amdgcn_readfirstlane(j - before - __shfl(x - mine, at));
+            return true;
+        }
+        // tiles of offsets that decrease may add up beyond those of n_tokens: the sum stops there, far below 2^31
+        before = min(before + __shfl(x, 63), 1 << 28);
+    }
+    return false;
+}
+
+// The same with a workgroup for each (sequence, head), or with ROWS for each 16 rows of a sequence's tokens, whose waves
+// share its units and add up what they have in LDS: one launch, for batches of which the host knows that the shares are
+// about even.
+template <int QT, int CT, int NS, int DT, bool UNI, int NW, bool ROWS>
 __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_head(AttnArgs g) {
     using Q = typename Elem<QT>::type;
     constexpr int NE = DT / 16, VD = DT < 128 ? 2 : 4, VB = DT < 128 ? 1 : DT / 128;
@@ -1190,25 +1293,36 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_head(AttnAr
     __shared__ float2 ml[NW][16];
     const Paged& a = g.a;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int b = (int)blockIdx.x / a.hkv, head = (int)blockIdx.x - b * a.hkv;
-    const int own = own_rows(a, b);
+    const int item = (int)(blockIdx.x / (unsigned)a.hkv), head = (int)blockIdx.x - item * a.hkv;
+    int b = item, own, low = 0, nk;
     Span span = {};
-    int low = 0;
-    const int nk = wave_rows<true>(g, b, own, span, low);
+    Rows rows = {item, 1, 0};
+    if constexpr (ROWS) {
+        if (!tile_at(g, item, b, rows)) return;  // the whole workgroup
+        const int first = fdiv(g.g, rows.tile * 16), last = min(rows.n, fdiv(g.g, rows.tile * 16 + 15) + 1) - 1;
+        own = seen_rows(a, b, rows.n, last, own_rows(a, b));
+        span = item_span(g, b, rows.n, rows.tile, 16, 32);
+        low = (int)min(window_low(position(a, b, rows.n, first), g.window), (int64_t)a.P + own);
+        nk = prefix_units(span) + own_units(span);
+    } else {
+        own = own_rows(a, b);
+        nk = wave_rows<true>(g, b, own, span, low);
+    }
     const int k0 = (int)((int64_t)nk * wave / NW), k1 = (int)((int64_t)nk * (wave + 1) / NW);
     f32x4 o[NE];
     float ref = kNegInf, l = 0.f;
     if (k0 < k1) {
-        wave_range<QT, CT, NS, DT, UNI, true>(g, ks[wave], b, head, own, span, low, k0, k1, g.past_mall, o, ref, l);
+        wave_range<QT, CT, NS, DT, UNI, true, ROWS>(g, ks[wave], b, head, own, span, low, k0, k1, g.past_mall, o, ref, l,
+                                                    rows);
         const int col = lane & 15;
         float* to = reinterpret_cast<float*>(&ks[wave][0][0]) + col * DT;
-        if (col < g.G) store_row<float, VD, VB>(to, a.D, lane >> 4, o, 1.f);
+        if (ROWS || col < g.G) store_row<float, VD, VB>(to, a.D, lane >> 4, o, 1.f);
     }
     if (lane < 16) ml[wave][lane] = make_float2(ref, l);
     __syncthreads();
-    const int pieces = a.D >> 2;  // of 4 elements of a row
-    for (int i = tid; i < g.G * (DT / 4); i += 64 * NW) {
-        const int row = i / (DT / 4), piece = i % (DT / 4), h = head * g.G + row;
+    const int pieces = a.D >> 2, used = ROWS ? min(16, rows.n * g.G - rows.tile * 16) : g.G;  // of 4 elements; rows
+    for (int i = tid; i < used * (DT / 4); i += 64 * NW) {
+        const int row = i / (DT / 4), piece = i % (DT / 4);
         if (piece >= pieces) continue;
         float m = kNegInf, sum = 0.f;
 #pragma unroll
@@ -1224,12 +1338,15 @@ __global__ __launch_bounds__(64 * NW, DT == 256 ? 1 : 2) void k_attn_head(AttnAr
             acc += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(&ks[w][0][0]) + row * DT + 4 * piece) * f;
         }
         const float inv = sum != 0.f ? 1.f / sum : 0.f;
+        const int r = rows.tile * 16 + row, tok = ROWS ? fdiv(g.g, r) : 0;
+        const int64_t t = rows.t0 + tok;
+        const int h = head * g.G + r - tok * g.G;
         Vec<Q, 4> v;
 #pragma unroll
         for (int c = 0; c < 4; c++) v.v[c] = (Q)(acc[c] * inv);
-        *reinterpret_cast<Vec<Q, 4>*>(reinterpret_cast<Q*>(g.out) + (int64_t)b * g.os + (int64_t)h * a.D + 4 * piece) = v;
+        *reinterpret_cast<Vec<Q, 4>*>(reinterpret_cast<Q*>(g.out) + t * g.os + (int64_t)h * a.D + 4 * piece) = v;
         if (g.lse != nullptr && piece == 0)
-            g.lse[(int64_t)b * g.H + h] = sum != 0.f ? (m + __builtin_log2f(sum)) * kLn2 : kNegInf;
+            g.lse[t * g.H + h] = sum != 0.f ? (m + __builtin_log2f(sum)) * kLn2 : kNegInf;
     }
 }
 

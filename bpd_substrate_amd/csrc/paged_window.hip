@@ -34,28 +34,61 @@ int64_t rows_seen(const Paged& a, int window, int sinks) {
     const int64_t all = (int64_t)a.W * a.page.d + a.P, seen = (int64_t)window + sinks;
     return seen < all ? seen : all;
 }
-// head_waves of a call, 0 where a plan has to be laid out.
+// Tiles of R rows that the tokens make at most, and where every sequence has as many of them.
+int64_t tiles_of(const Paged& a, int G, int R) { return (int64_t)a.T * G / R + a.B; }
+int64_t even_tiles(const Paged& a, int G, int R) {
+    const int64_t n = a.B > 0 ? ((int64_t)a.T + a.B - 1) / a.B : 0, even = a.B * ((n * G + R - 1) / R);
+    return even < tiles_of(a, G, R) ? even : tiles_of(a, G, R);
+}
+
+// The same for several tokens of a sequence, whose rows go 16 to a workgroup or by k_attn_plan, k_attn_tile and k_attn_join.
+// Those have 40 us of launches and uneven shares, and read the keys once for R rows; the cost of a unit, all CUs working,
+// is in ns.  Measured (us, 16 rows to a workgroup / tiles; 8 kv heads of 128, 4 query heads each, bf16):
+//   64 sequences, 516 rows, 2 / 4 / 8 / 16 / 32 tokens    35, 81 / 36, 83 / 54, 90 / 82, 106 / 142, 109
+//   64, 2,052 rows, 4 / 8 / 16                            92, 172 / 152, 180 / 238, 196
+//   8, 516 and 2,052 rows, 64                             35, 57 and 86, 74
+//   1, 2,052 rows, 128                                    20, 42
+// heads of 64 (5 to a kv head), 64 sequences, 2,052 rows, 8 / 32: 103, 135 / 240, 149; of 256 (2 kv heads, 8 each), 4 / 8:
+// 76, 98 / 147, 104.
+int rows_waves(const Paged& a, int G, int R, int64_t rows) {
+    const int DT = padded(a.D);
+    const double head = DT == 64 ? 0.95 : DT == 128 ? 1.6 : 4.2, tile = DT == 64 ? 6 : DT == 128 ? 9 : 14;
+    const int64_t items = even_tiles(a, G, 16) * a.hkv;
+    const double one = head * (double)items * (double)((rows + 63) / 32);
+    const double plan = 40e3 + tile * (double)(even_tiles(a, G, R) * a.hkv) * (double)((rows + 127) / 64);
+    if (one >= plan) return 0;
+    return DT == 256 || items > 256 ? 4 : 8;
+}
+
+// head_waves or rows_waves of a call.
 int waves_of(const Paged& a, int q_type, int G, int window, int sinks) {
     const int DT = padded(a.D);
+    const int64_t rows = rows_seen(a, window, sinks);
+    if (planned_way(a.q_start, G)) return rows_waves(a, G, rows_of(a.D, q_type == BPD_T_F32 ? 2 : 1), rows);
     const int64_t items = (int64_t)a.B * a.hkv;
-    if (planned_way(a.q_start, G) || items > INT32_MAX) return 0;
-    return head_waves(DT, !whole_pages(a) || (q_type == BPD_T_F32 && DT > 64), items, rows_seen(a, window, sinks));
+    if (items > INT32_MAX) return 0;
+    return head_waves(DT, !whole_pages(a) || (q_type == BPD_T_F32 && DT > 64), items, rows);
 }
 
 template <int QT, int CT, int NS, int DT, bool UNI, int NW>
 void launch_head(const AttnArgs& g, hipStream_t s) {
-    hipLaunchKernelGGL((k_attn_head<QT, CT, NS, DT, UNI, NW>), dim3((unsigned)(g.a.B * g.a.hkv)), dim3(64 * NW), 0, s, g);
+    const dim3 block(64 * NW);
+    if (g.planned)
+        hipLaunchKernelGGL((k_attn_head<QT, CT, NS, DT, UNI, NW, true>),
+                           dim3((unsigned)(tiles_of(g.a, g.G, 16) * g.a.hkv)), block, 0, s, g);
+    else
+        hipLaunchKernelGGL((k_attn_head<QT, CT, NS, DT, UNI, NW, false>), dim3((unsigned)(g.a.B * g.a.hkv)), block, 0, s, g);
 }
 
 template <int QT, int CT, int NS, int DT, int MT, int NW, bool UNI>
 void launch_dim(const AttnArgs& g, hipStream_t s) {
-    if (g.planned)
-        hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, DT, MT, NW, UNI, true>), dim3((unsigned)g.groups), dim3(64 * NW), 0, s,
-                           g);
-    else if (DT < 256 && g.waves == 8)
+    if (DT < 256 && g.waves == 8)
         launch_head<QT, CT, NS, DT, UNI, DT < 256 ? 8 : 4>(g, s);
     else if (g.waves == 4)
         launch_head<QT, CT, NS, DT, UNI, 4>(g, s);
+    else if (g.planned)
+        hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, DT, MT, NW, UNI, true>), dim3((unsigned)g.groups), dim3(64 * NW), 0, s,
+                           g);
     else
         hipLaunchKernelGGL((k_attn_wave<QT, CT, NS, DT, UNI, true>), dim3((unsigned)(g.waves / 4)), dim3(256), 0, s, g);
 }
@@ -69,10 +102,11 @@ void launch_uni(const AttnArgs& g, hipStream_t s) {
 
 template <int QT, int CT, int NS>
 void launch_types(const AttnArgs& g, hipStream_t s) {
-    if (g.planned) hipLaunchKernelGGL(k_attn_plan<true>, dim3(1), dim3(1024), 0, s, g);
+    const bool one = g.waves <= 8;  // one launch: the workgroups join their waves
+    if (g.planned && !one) hipLaunchKernelGGL(k_attn_plan<true>, dim3(1), dim3(1024), 0, s, g);
     if (whole_pages(g.a)) launch_uni<QT, CT, NS, true>(g, s);
     else launch_uni<QT, CT, NS, false>(g, s);
-    if (!g.planned && g.waves <= 8) return;  // the workgroups have joined their waves
+    if (one) return;
     // one head per wave while that fills the chip twice at most, more where most rows are done
     if ((int64_t)g.a.T * g.H <= 32768)
         hipLaunchKernelGGL((k_attn_join<QT, 1, true>), dim3((unsigned)g.a.T, (unsigned)((g.H + 3) / 4)), dim3(256), 0, s, g);

@@ -54,6 +54,46 @@ CASES = [
 ]
 
 
+# the same for batches that k_attn_plan lays out, whose tiles k_attn_tile takes
+TILES = [
+    (([900], [1100], 0, 32, 8, 64, "f16", "f16", 16, True, 0), (2000, 0)),
+    (([800, 300, 1, 0, 400], [900, 700, 60, 9, 700], 77, 32, 8, 64, "bf16", "bf16", 16, False, 3), (700, 100)),
+    (([600, 500], [600, 900], 130, 32, 8, 128, "bf16", "bf16", 64, True, 0), (401, 140)),
+    (([500, 611], [700, 800], 61, 40, 8, 96, "f16", "f16", 21, True, 1), (377, 4)),     # pages that end inside every unit
+    (([450, 550], [760, 900], 40, 32, 8, 128, "f32", "bf16", 32, True, 0), (700, 0)),
+    (([500, 490], [800, 900], 0, 32, 8, 80, "f32", "f16", 16, False, 0), (900, 33)),
+    (([300, 500], [700, 900], 50, 32, 4, 256, "f16", "f16", 16, True, 0), (840, 7)),
+]
+# one token each, too many rows for a workgroup: units dealt to all waves, and a join
+DEALT = [
+    (([1] * 2, [2700, 1200], 0, 8, 2, 128, "bf16", "bf16", 64, True, 0), (2400, 4)),
+    (([1] * 3, [2600, 40, 1000], 90, 8, 2, 64, "f16", "f16", 16, True, 0), (2500, 95)),
+    (([1] * 3, [900, 700, 33], 61, 12, 4, 96, "f32", "f16", 21, False, 0), (700, 3)),
+    (([1] * 2, [900, 120], 200, 6, 2, 256, "bf16", "bf16", 64, True, 0), (650, 5)),
+    (([1] * 2, [800, 300], 30, 6, 2, 128, "f32", "bf16", 32, True, 0), (700, 0)),
+]
+
+
+@pytest.mark.parametrize("slide", [False, True])
+@pytest.mark.parametrize("case", range(len(TILES)))
+def test_tiles(dev, case, slide):
+    args, win = TILES[case]
+    b = Batch(800 + case, *args)
+    if slide:
+        b.slide(*win)
+    check(b, dev, *win)
+
+
+@pytest.mark.parametrize("slide", [False, True])
+@pytest.mark.parametrize("case", range(len(DEALT)))
+def test_dealt_units(dev, case, slide):
+    args, win = DEALT[case]
+    b = Batch(820 + case, *args, decode=True)
+    if slide:
+        b.slide(*win)
+    check(b, dev, *win)
+
+
 @pytest.mark.parametrize("case", range(len(CASES)))
 def test_window(dev, case):
     args, win = CASES[case]
@@ -86,10 +126,12 @@ def test_chunks_beside_poisoned_rows(dev, case):
 
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
 @pytest.mark.parametrize("P", [0, 70])
-def test_a_bad_row_reaches_the_tokens_that_see_it_alone(dev, bad, P):
+@pytest.mark.parametrize("n,H,HKV", [(100, 2, 1), (1000, 32, 8)])     # 16 rows to a workgroup, and tiles
+def test_a_bad_row_reaches_the_tokens_that_see_it_alone(dev, bad, P, n, H, HKV):
     """One row of infinities or NaN in v: tokens whose window holds it are not finite, the others as without it."""
-    W, S, n, own, at = 40, 3, 100, 160, 90
-    b = Batch(7, [n], [own], P, 2, 1, 64, "f16", "f16", 16)
+    S, own, at = 3, n + 60, n - 10
+    W = 40 if n == 100 else 900
+    b = Batch(7, [n], [own], P, H, HKV, 64, "f16", "f16", 16)
     ref = b.attention(None, W, S)
     b.vc[b.table[0, at // 16], at % 16] = bad
     cache, batch, q = b.device(dev)
