@@ -1254,32 +1254,32 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void k_attn_wave(AttnArgs g
     wave_share<QT, CT, NS, DT, UNI, WIN>(g, ks[wave], (int)blockIdx.x * 4 + wave, g.waves, wave_units<WIN>(g));
 }
 
-// The sequence that the j-th tile of 16 rows is of, and which of its; false: there are fewer.  The whole wave.
+// The sequence whose tiles of 16 rows the j-th workgroup's is among, and which; false: none's.  The whole wave.
 __device__ __forceinline__ bool tile_at(const AttnArgs& g, int j, int& b, Rows& rows) {
+    const Paged& a = g.a;
     const int lane = (int)threadIdx.x & 63;
-    int before = 0;
-    for (int b0 = 0; b0 < g.a.B; b0 += 64) {
-        int t0 = 0, n = 0;
-        if (b0 + lane < g.a.B) seq_tokens(g.a, b0 + lane, t0, n);
-        const int mine = (n * g.G + 15) >> 4;
-        int x = mine;
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(x, d);
-            if (lane >= d) x += o;
+    auto first = [&](int i) {  // of sequence i: they do not decrease where the offsets do not
+        int t0 = i, n = 1;
+        if (a.q_start != nullptr) clamp_tokens(a.q_start[i], a.q_start[i], a.T, t0, n);
+        return first_tile(t0, i, g.G);
+    };
+    int lo = 0, hi = a.B;  // count_le's search for how many begin at j or before
+    while (lo < hi) {
+        const int step = (hi - lo + 63) >> 6, i = lo + lane * step;
+        const int c = __popcll(__ballot(i < hi && first(i < hi ? i : lo) <= j));
+        if (c == 0) break;
+        if (step == 1) {
+            lo += c;
+            break;
         }
-        const uint64_t over = __ballot(before + x > j);
-        if (over != 0) {
-            const int at = __builtin_ctzll(over);
-            b = __builtin_amdgcn_readfirstlane(b0 + at);
-            rows.t0 = __builtin_amdgcn_readfirstlane(__shfl(t0, at));
-            rows.n = __builtin_amdgcn_readfirstlane(__shfl(n, at));
-            rows.tile = __builtin_amdgcn_readfirstlane(j - before - __shfl(x - mine, at));
-            return true;
-        }
-        // tiles of offsets that decrease may add up beyond those of n_tokens: the sum stops there, far below 2^31
-        before = min(before + __shfl(x, 63), 1 << 28);
+        hi = min(hi, lo + c * step);
+        lo = lo + (c - 1) * step + 1;
     }
-    return false;
+    b = __builtin_amdgcn_readfirstlane(lo - 1);
+    if (b < 0) return false;
+    seq_tokens(a, b, rows.t0, rows.n);
+    rows.tile = j - first_tile(rows.t0, b, g.G);
+    return rows.tile >= 0 && rows.tile * 16 < rows.n * g.G;
 }
 
 // The same with a workgroup for each (sequence, head), or with ROWS for each 16 rows of a sequence's tokens, whose waves

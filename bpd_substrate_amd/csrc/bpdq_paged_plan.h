@@ -56,6 +56,10 @@ BPDQ_BOTH int group_of(int64_t u, int64_t U, int n) { return (int)(((u + 1) * n 
 // Whether a sequence's n tokens of G heads fill half a tile by themselves: then it takes the prefix's keys too.
 BPDQ_BOTH bool is_joint(int n, int G, int R) { return n * G * 2 >= R; }
 
+// Where the tiles of 16 rows of sequence b begin, whose first token is t0: each sequence has a place for the tile that
+// its rows may share with the one before, so ceil(n G / 16) tiles end before the next sequence's begin.
+BPDQ_BOTH int first_tile(int t0, int b, int G) { return (int)((int64_t)t0 * G / 16) + b; }
+
 // The units of U rows that hold a row which tokens at positions `first` and later see through a window of W
 // positions or among the first S ones: of the prefix's P rows units [0, a1) and [b0, b1), of the own ones, `seen`
 // of them seen by the last token, [0, c1) and [d0, d1).  Positions of own rows begin at P.

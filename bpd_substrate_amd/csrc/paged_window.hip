@@ -10,6 +10,8 @@ namespace bpdq {
 
 namespace {
 
+constexpr int64_t kMostItems = 1 << 22;  // workgroups of 512 threads in a launch
+
 bool whole_pages(const Paged& a) { return a.page.d % 16 == 0 && a.row_stride < 1 << 26; }
 
 // Waves of a workgroup for each (sequence, head), or 0: the units dealt to all waves of the chip, and a second launch.
@@ -56,7 +58,7 @@ int rows_waves(const Paged& a, int G, int R, int64_t rows) {
     const int64_t items = even_tiles(a, G, 16) * a.hkv;
     const double one = head * (double)items * (double)((rows + 63) / 32);
     const double plan = 40e3 + tile * (double)(even_tiles(a, G, R) * a.hkv) * (double)((rows + 127) / 64);
-    if (one >= plan) return 0;
+    if (one >= plan || tiles_of(a, G, 16) * a.hkv > kMostItems) return 0;
     return DT == 256 || items > 256 ? 4 : 8;
 }
 
@@ -66,7 +68,7 @@ int waves_of(const Paged& a, int q_type, int G, int window, int sinks) {
     const int64_t rows = rows_seen(a, window, sinks);
     if (planned_way(a.q_start, G)) return rows_waves(a, G, rows_of(a.D, q_type == BPD_T_F32 ? 2 : 1), rows);
     const int64_t items = (int64_t)a.B * a.hkv;
-    if (items > INT32_MAX) return 0;
+    if (items > kMostItems) return 0;
     return head_waves(DT, !whole_pages(a) || (q_type == BPD_T_F32 && DT > 64), items, rows);
 }
 

@@ -494,6 +494,8 @@ void bpd_adjust_logits_on_gpu(void* hip_stream, const void* logits, int type, in
     c.shape(type == BPD_T_F32 || type == BPD_T_F16 || type == BPD_T_BF16, "type is unknown");
     c.shape(out_type == BPD_T_F32 || out_type == type, "out_type is neither fp32 nor the logits' type");
     check_sample(c, n_rows, vocab);
+    // workgroups of a launch, one for each slice of 8192
+    c.need((int64_t)n_rows * (vocab / 8192 + 1) < 1 << 22, BPDQ_ERR_LIMIT, "n_rows is too large");
     c.shape(row_stride >= vocab && row_stride <= kMaxStride, "row_stride is shorter than a row, or 2^30 or more");
     c.shape(out_stride >= vocab && out_stride <= kMaxStride, "out_stride is shorter than a row, or 2^30 or more");
     if (!c.ok) return;

@@ -405,6 +405,8 @@ def attention(cache, batch, q, scale=None, out=None, return_lse=False, window=No
         _bad(f"q has {q.dim()} dimensions, not 3")
     if window is None and sinks != 0:
         _bad("sinks without a window")
+    if window is not None:   # beyond these limits every position is seen
+        window, sinks = min(window, 0x7FFFFFFF), min(sinks, 0x7FFFFFFF)
     T, H, D, dev = batch.n_tokens, q.shape[1], cache.head_dim, cache.device
     if q.dtype not in (cache.dtype, torch.float32):
         _bad(f"q is {q.dtype}, neither float32 nor the cache's {cache.dtype}")

@@ -147,6 +147,7 @@ int64_t bpd_sample_workspace(int n_rows, int vocab);
  * back.  free_pages[0 .. n_free[0]) are the pages that no sequence holds.  gone (may be NULL, without windows):
  * pages [gone[2 r], gone[2 r + 1]) of row r have slid out of its window and were given back.  All of it is
  * device memory that the caller fills once (tables -1, lens, gone and n_free[1] 0) and the two calls below keep.
+ * Calls on one pool follow each other, on one stream or by events.
  * Pages that are no part of the pool (a shared prefix's) are left out of free_pages.  n_pages and table_width times
  * page_size stay below 2^31; n_rows up to 16384 (BPDQ_ERR_LIMIT). */
 typedef struct {
@@ -166,7 +167,7 @@ typedef struct {
  * its table holds; 3 the pages asked for by it and all before it are more than the pool has (a sequence that needs no
  * page is not refused for that); 4 with the tokens of it and of those before it that pages were there for they would be
  * more than n_tokens.  Pages come from the end of free_pages.  lens and table of the pool follow.
- * Outputs, device memory that overlaps nothing else of the call (with n_seqs 0 nothing is written): lens_out[b] the sequence's rows, q_start[n_seqs + 1] the running sum of tokens granted,
+ * Outputs, device memory that overlaps nothing else of the call (with n_seqs 0 nothing is written): lens_out[b] the sequence's rows (0 without a row of the pool), q_start[n_seqs + 1] the running sum of tokens granted,
  * slots[t] and pos[t] of every new token its row of the cache, page * page_size + row in it (-1 where its
  * page is outside the pool), and its position, prefix_len + index; -1 of tokens behind the last.  table_out
  * (may be NULL) [n_seqs][table_width]: the sequences' tables, -1 behind their pages.  With these a bpd_paged_batch
@@ -234,7 +235,7 @@ typedef struct {
 
 /* out [n_rows][vocab] (out_type: that of the logits, or fp32) = the logits under the rules, rounded once; rows
  * row_stride and out_stride elements apart, aligned to an element.  out may be the logits themselves, and overlaps them in
- * no other way.  vocab and n_rows as in bpd_sample_gpu. */
+ * no other way.  vocab as in bpd_sample_gpu, n_rows * (vocab / 8192 + 1) below 2^22 (BPDQ_ERR_LIMIT). */
 void bpd_adjust_logits_gpu(const void* logits, int type, int64_t row_stride, void* out, int out_type, int64_t out_stride,
                            int n_rows, int vocab, const bpd_logit_rules* rules);
 

@@ -171,6 +171,30 @@ def test_lengths_of_any_kind_stay_inside(dev, lens, decode):
     assert out.shape == q.shape
 
 
+@pytest.mark.parametrize("offsets", [[0, 90, 3, 40, 60], [-5, 2 ** 31 - 1, -2 ** 31, 7, 10 ** 6], [60, 50, 40, 2, 0]])
+@pytest.mark.parametrize("D,HKV,lens", [(64, 2, 200), (256, 16, 3000)])
+def test_offsets_of_any_kind_stay_inside(dev, offsets, D, HKV, lens):
+    """Rows of the output that they do not name stay as they were, the others are some sequence's."""
+    cache = serve.PagedCache.empty(50, 64, HKV, D, torch.float16, device=dev)
+    cache.v.fill_(1.0)
+    table = torch.arange(50, dtype=torch.int32, device=dev).repeat(4, 1)
+    batch = serve.PagedBatch(table, torch.full((4,), lens, dtype=torch.int32, device=dev),
+                             q_start=torch.tensor(offsets, dtype=torch.int64).clamp(-2 ** 31, 2 ** 31 - 1).int().to(dev), n_tokens=64)
+    q = torch.randn(64, 2 * HKV, D, device=dev).half()
+    wide = torch.full((66, 2 * HKV, D), 7.0, dtype=torch.float16, device=dev)
+    out = wide[1:65]
+    serve.attention(cache, batch, q, window=2000, sinks=3, out=out)
+    torch.cuda.synchronize()
+    assert (wide[0] == 7.0).all() and (wide[65] == 7.0).all()
+    assert ((out == 7.0) | (out == 1.0) | (out == 0.0)).all()
+
+
+def test_many_sequences_of_few_tokens(dev):
+    """More than a wave's search looks at in one step."""
+    n = [i % 3 for i in range(700)]
+    check(Batch(13, n, [i % 40 + k for i, k in enumerate(n)], 0, 4, 1, 64, "f16", "f16", 16), dev, 20, 2)
+
+
 def test_pages_of_any_kind_are_absent(dev):
     b = Batch(11, [1, 30], [200, 150], 40, 4, 2, 64, "f16", "f16", 16)
     b.table[0, 11], b.table[1, 4], b.prefix_pages[0] = -5, 2 ** 31 - 1, 10 ** 6

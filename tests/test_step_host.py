@@ -120,13 +120,15 @@ def test_window_refusals(L):
                            (dict(lse=0x42), 3, "lse"), (dict(H=1 << 17), 7, "n_heads is above")):
         window(L, cache(), batch(), **kw)
         err(L, code, text)
-    chunk = batch(q_start=0x8000, n_tokens=50)
-    window(L, cache(), chunk, n=0)
+    chunk = batch(q_start=0x8000, n_tokens=4000, table_width=1000, table_stride=1000)
+    far = dict(out=0x40000000, W=9000)
+    window(L, cache(), chunk, n=0, **far)
     err(L, 2, "ws_bytes")
-    window(L, cache(), chunk, ws=0x50008)
+    window(L, cache(), chunk, ws=0x50008, **far)
     err(L, 3, "ws")
     need = lambda c, b, t=1, W=10, S=2, H=4: L.bpd_attn_window_paged_workspace(A(c), A(b), t, H, W, S)  # noqa: E731
-    assert need(cache(), batch()) == 0 and need(cache(), chunk) > 0
+    assert need(cache(), batch()) == 0 and need(cache(), batch(q_start=0x8000, n_tokens=50)) == 0
+    assert need(cache(), chunk, W=9000) > 0
     wide = batch(table_width=1000, table_stride=1000)                         # few sequences, many rows: two launches
     assert need(cache(), wide, W=10) == 0 and need(cache(), wide, W=9000) > 0
     for a in (dict(W=0), dict(S=-1), dict(t=2), dict(H=3)):
@@ -153,6 +155,7 @@ def test_adjust_refusals(L):
                            (dict(xs=99), 2, "row_stride"), (dict(os=99), 2, "out_stride"), (dict(x=None), 1, "logits"),
                            (dict(x=0x10001), 3, "logits"), (dict(out=None), 1, "out"), (dict(out=0x20001), 3, "out"),
                            (dict(V=(1 << 22) + 1, xs=1 << 23, os=1 << 23), 7, "2^22"), (dict(B=1 << 22), 7, "n_rows"),
+                           (dict(B=1 << 20, V=32767, xs=32767, os=32767), 7, "n_rows"),
                            (dict(out=0x10000 + 200), 2, "overlaps"), (dict(out=0x10000, ot=0), 2, "overlaps"),
                            (dict(out=0x10000, xs=200), 2, "overlaps")):
         adjust(L, rules(), **kw)

@@ -18,6 +18,7 @@ void t_span(long long first, int W, int S, int P, int seen, int U, int* out) {
     const int v[] = {s.a1, s.b0, s.b1, s.c1, s.d0, s.d1, prefix_units(s), own_units(s)};
     for (int i = 0; i < 8; i++) out[i] = v[i];
 }
+int t_first_tile(int t0, int b, int G) { return first_tile(t0, b, G); }
 int t_unit_at(long long first, int W, int S, int P, int seen, int U, int t, int* pre) {
     bool p;
     const int r = unit_at(span_of(first, W, S, P, seen, U), t, p);
@@ -68,6 +69,23 @@ def test_units_are_those_with_a_row_that_is_seen(C, seed):
         assert got == sorted(set(got)), "units in order, each once"
         want = {(j >= P, (j if j < P else j - P) // U) for j in range(P + own) if j >= low or j < S}
         assert set(got) == want
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_tiles_of_sequences_lie_behind_each_other(C, seed):
+    """Every sequence's ceil(n G / 16) tiles have places of their own, within the launch's T G / 16 + B."""
+    r = np.random.default_rng(seed)
+    B, G = int(r.integers(1, 300)), int(r.choice([1, 2, 3, 5, 8, 16, 40, 64]))
+    n = [int(x) for x in r.choice([0, 0, 1, 1, 2, 7, 64, 333], B)]
+    start = np.concatenate([[int(r.integers(0, 5))], n]).cumsum()
+    T, end = int(start[-1] + r.integers(0, 5)), 0
+    for b in range(B):
+        at = C.t_first_tile(int(start[b]), b, G)
+        assert at >= end
+        end = at + -(-n[b] * G // 16)
+        assert b + 1 == B or end <= C.t_first_tile(int(start[b + 1]), b + 1, G)
+    assert end <= T * G // 16 + B
+    assert C.t_first_tile(1 << 23, (1 << 23) - 1, 8) == (1 << 22) + (1 << 23) - 1
 
 
 def test_extreme_positions_and_lengths(C):
