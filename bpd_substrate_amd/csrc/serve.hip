@@ -27,19 +27,21 @@ struct Args {
         return *this;
     }
     Args& shape(bool good, const char* what) { return need(good, BPDQ_ERR_SHAPE, what); }
-    Args& ptr(const void* p, uintptr_t align, const char* name) {
+    // what failed is put into words only where it did: a call checks a dozen pointers and strides
+    Args& text(bool good, int code, const char* form, const char* name, int n = 0) {
+        if (!ok || good) return *this;
         char buf[96];
-        std::snprintf(buf, sizeof buf, "%s is NULL", name);
-        need(p != nullptr, BPDQ_ERR_NULL, buf);
-        std::snprintf(buf, sizeof buf, "%s is not %d-byte aligned", name, (int)align);
-        return need((reinterpret_cast<uintptr_t>(p) & (align - 1)) == 0, BPDQ_ERR_ALIGN, buf);
+        std::snprintf(buf, sizeof buf, form, name, n);
+        return need(false, code, buf);
+    }
+    Args& ptr(const void* p, uintptr_t align, const char* name) {
+        return text(p != nullptr, BPDQ_ERR_NULL, "%s is NULL", name)
+            .text((reinterpret_cast<uintptr_t>(p) & (align - 1)) == 0, BPDQ_ERR_ALIGN, "%s is not %d-byte aligned", name,
+                  (int)align);
     }
     Args& stride(int64_t s, int64_t row, int esize, const char* name) {
-        char buf[96];
-        std::snprintf(buf, sizeof buf, "%s is shorter than a token's row, or 2^30 or more", name);
-        shape(s >= row && s <= kMaxStride, buf);
-        std::snprintf(buf, sizeof buf, "%s is no multiple of 16 bytes", name);
-        return need(s * esize % 16 == 0, BPDQ_ERR_ALIGN, buf);
+        return text(s >= row && s <= kMaxStride, BPDQ_ERR_SHAPE, "%s is shorter than a token's row, or 2^30 or more", name)
+            .text(s * esize % 16 == 0, BPDQ_ERR_ALIGN, "%s is no multiple of 16 bytes", name);
     }
 };
 
@@ -143,11 +145,8 @@ void check_sample(Args& c, int n_rows, int vocab) {
 
 // A head's weights of `D` elements, one row for all heads or a row each.
 void check_weights(Args& c, int64_t s, int64_t D, const char* name) {
-    char buf[96];
-    std::snprintf(buf, sizeof buf, "%s is neither 0 nor head_dim or more, or 2^30 or more", name);
-    c.shape(s == 0 || (s >= D && s <= kMaxStride), buf);
-    std::snprintf(buf, sizeof buf, "%s is no multiple of 8 elements", name);
-    c.need(s % 8 == 0, BPDQ_ERR_ALIGN, buf);
+    c.text(s == 0 || (s >= D && s <= kMaxStride), BPDQ_ERR_SHAPE, "%s is neither 0 nor head_dim or more, or 2^30 or more",
+           name).text(s % 8 == 0, BPDQ_ERR_ALIGN, "%s is no multiple of 8 elements", name);
 }
 
 // The append, with its heads normed where norm is given.
