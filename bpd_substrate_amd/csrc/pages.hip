@@ -5,6 +5,10 @@
 // the L2, and spares a launch (or a grid-wide wait) between deciding and doing.  Of each 256 it then takes its parts: the
 // sequences' tables, their new tokens' slots and positions, or the pages that they put back onto the stack.  The
 // pool's lengths and counts, which all of them read, are written by the workgroup that is done last.
+// Latency bounds both: the names, the lengths, the sums, the table or the stack, the count of workgroups, one after the
+// other: 8.2 us for 256 sequences of up to 513 pages that grow by up to 4 rows each, 7.3 us back (a megabyte of tables, 0.2 us
+// of memory); 64 prompts of up to 2,048 rows 7.8 and 5.2.  In two and three launches the two calls took 24 us, in one
+// with a fence before the count 19, without 15.4.
 #include "bpdq_paged.h"
 
 namespace bpdq {

@@ -178,9 +178,10 @@ void bpd_pages_extend_gpu(const bpd_page_pool* pool, const int32_t* rows, const 
 
 /* Sequence b keeps its first keep[b] rows (NULL, or more than it has: all), and of those, with a window above 0
  * (gone not NULL), the pages that hold one of the first `sinks` rows or a row that a token at index keep[b] or
- * later sees through the window: those from keep[b] - window + 1 on.  sinks counts rows of the sequence's own part and is the
- * same from call to call.  The other pages go to the end of free_pages, the first sequence's first page last, so that an
- * extension which is taken back leaves the pool as it was; their entries become -1.  Rows that are not the pool's, and all
+ * later sees through the window: those from keep[b] - window + 1 on.  sinks counts rows of the sequence's own part and
+ * is the same from call to call.  A page that slid out stays out, also where its sequence is cut back behind it later.
+ * The other pages go to the end of free_pages, the first sequence's first page last, so that an extension which is
+ * taken back leaves the pool as it was; their entries become -1.  Rows that are not the pool's, and all
  * but the first sequence that names a row, are passed over. */
 void bpd_pages_release_gpu(const bpd_page_pool* pool, const int32_t* rows, const int32_t* keep, int n_seqs, int window,
                            int sinks);
