@@ -189,8 +189,8 @@ void bpd_pages_release_gpu(const bpd_page_pool* pool, const int32_t* rows, const
 /* bpd_rope_append_paged_gpu with every head of q and k normed before it turns:
  *   y_i = x_i / sqrt(mean over the head of x^2 + eps) * w_i
  * q_norm and k_norm: [head_dim] weights of all heads (stride 0), or of each, a head's stride elements
- * behind the one before (multiples of 8, head_dim at least); of w_type, fp32 or x_type.  NULL: not normed.  eps is not
- * below 0.  The sum of squares, the scale and the rotation are binary32 (a head whose squares add up beyond it
+ * behind the one before (multiples of 8, head_dim at least); of w_type, fp32 or x_type, 16-byte aligned.  NULL: not
+ * normed.  eps is not below 0.  The sum of squares, the scale and the rotation are binary32 (a head whose squares add up beyond it
  * becomes 0), and the result is rounded once. */
 void bpd_norm_rope_append_paged_gpu(const bpd_paged_cache* cache, const bpd_paged_batch* batch, const void* q_norm,
                                     int64_t q_norm_stride, const void* k_norm, int64_t k_norm_stride, int w_type,

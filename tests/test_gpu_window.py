@@ -217,3 +217,32 @@ def test_a_replayed_graph_follows_the_lengths(dev):
         want, wl = f()
         assert torch.equal(out, want) and torch.equal(lse, wl)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("decode", [True, False])
+def test_pages_beyond_32_bits(dev, decode):
+    """Pages 2^30 - 8 elements apart: the third begins at byte 2^32 - 32.  The append with norms writes its rows there, the
+    attention reads them, as with pages side by side."""
+    far, HKV, D, page = (1 << 30) - 8, 2, 64, 16
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 17 GB")
+    new = [1, 1] if decode else [20, 3]
+    lens, T = [45, 9], sum(new)
+    buf = [torch.empty(3 * far + 4096, dtype=torch.float16, device=dev) for _ in range(2)]
+    wide = [x.as_strided((4, page, HKV, D), (far, D, page * D, 1)) for x in buf]
+    near = [torch.zeros(4, HKV, page, D, dtype=torch.float16, device=dev).transpose(1, 2) for _ in range(2)]
+    g = torch.Generator(device=dev).manual_seed(1)
+    for a, b in zip(wide, near):
+        b.copy_(torch.randn(b.shape, generator=g, device=dev))
+        a.copy_(b)
+    table = torch.tensor([[3, 0, 2], [1, -1, -1]], dtype=torch.int32, device=dev)   # no page is two sequences'
+    n = torch.tensor(lens, dtype=torch.int32, device=dev)
+    start = None if decode else torch.tensor([0, new[0], T], dtype=torch.int32, device=dev)
+    x = torch.randn(T, 8, D, generator=g, device=dev).half()
+    w, rope = torch.ones(D, device=dev), serve.Rope(D, device=dev)
+    got = []
+    for k, v in (wide, near):
+        cache, batch = serve.PagedCache(k, v), serve.PagedBatch(table, n, q_start=start, n_tokens=T)
+        q = serve.rope_append(cache, batch, x[:, :4], x[:, 4:6], x[:, 6:], rope=rope, q_norm=w, k_norm=w)
+        got.append((serve.attention(cache, batch, q, window=30, sinks=2), k.contiguous(), v.contiguous()))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
