@@ -67,8 +67,23 @@ __global__ __launch_bounds__(kThreads) void k_adjust(AdjustArgs g) {
         const int i = 8 * (tid + k * kThreads);
         keep[k] = i < n && bits != nullptr ? bits[(lo + i) >> 3] : 255u;  // lo is a multiple of 8
     }
-    if (history) clear(count, n);
-    // the logits are on their way while the history is counted
+    // the history's first tokens and the logits are on their way while the counts are cleared
+    constexpr int A = 4;  // vectors of tokens under way
+    const int32_t* t = g.tokens + (int64_t)b * g.token_stride;
+    const int whole = len & ~3;
+    i32x4 w[A];
+    auto ask = [&](int i0) {
+#pragma unroll
+        for (int k = 0; k < A; k++) {
+            const int i = i0 + 4 * k * kThreads;
+            w[k] = i32x4{-1, -1, -1, -1};  // no token
+            if (i < whole) w[k] = *reinterpret_cast<const i32x4*>(t + i);
+        }
+    };
+    if (history) {
+        ask(4 * tid);
+        clear(count, n);
+    }
     VX v[kVecs];
 #pragma unroll
     for (int k = 0; k < kVecs; k++) {
@@ -78,23 +93,14 @@ __global__ __launch_bounds__(kThreads) void k_adjust(AdjustArgs g) {
     }
     if (history) {
         __syncthreads();
-        const int32_t* t = g.tokens + (int64_t)b * g.token_stride;
         auto met = [&](int token, int i) {
             const uint32_t at = (uint32_t)token - (uint32_t)lo;
             if (at >= (uint32_t)n) return;
             if (i < prompt) atomicOr(&count[at], kMet);
             else atomicAdd(&count[at], 1u);
         };
-        constexpr int A = 4;  // vectors under way
-        const int whole = len & ~3;
         for (int i0 = 4 * tid; i0 < whole; i0 += 4 * A * kThreads) {
-            i32x4 w[A];
-#pragma unroll
-            for (int k = 0; k < A; k++) {
-                const int i = i0 + 4 * k * kThreads;
-                w[k] = i32x4{-1, -1, -1, -1};  // no token
-                if (i < whole) w[k] = *reinterpret_cast<const i32x4*>(t + i);
-            }
+            if (i0 != 4 * tid) ask(i0);
 #pragma unroll
             for (int k = 0; k < A; k++)
 #pragma unroll
