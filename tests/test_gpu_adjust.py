@@ -96,7 +96,7 @@ def check(dev, x, k, out_dtype=None, in_place=False):
         assert torch.equal(xd.cpu(), x)
 
 
-SIZES = [(1, 1), (1, 7), (3, 33), (2, 1000), (2, 1024), (1, 8193), (5, 32001), (2, 128256), (70, 4099)]
+SIZES = [(1, 1), (1, 7), (3, 33), (2, 1000), (2, 1024), (1, 8193), (5, 32001), (2, 128256), (70, 4099), (1, 1 << 22)]
 TYPES = [("f32", None), ("f16", None), ("bf16", None), ("f16", "f32"), ("bf16", "f32")]
 
 

@@ -84,6 +84,17 @@ CASES = [  # new, lens, P, H, HKV, D, x, kv, page, heads_first, pad, rot, neox, 
     ([4], [400], 0, 3, 1, 200, "bf16", "bf16", 64, False, 0, 0, False, "bf16"),   # none do
     ([5], [3], 9, 2, 2, 64, "f32", "f16", 16, True, 0, 64, False, "f32"),         # more new tokens than rows
 ]
+MANY = [  # more tokens than take four waves each: two waves, and one where a token has few heads
+    ([600, 1, 505], [600, 9, 700], 5, 16, 2, 128, "bf16", "bf16", 16, True, 3, 64, True, "f32"),
+    ([1100], [1100], 0, 15, 3, 80, "f16", "f16", 21, False, 0, 40, True, "f16"),
+    ([700, 400], [800, 400], 0, 7, 1, 64, "f32", "f16", 16, True, 1, 64, False, "f32"),
+]
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("case", range(len(MANY)))
+def test_many_tokens(dev, case, in_place):
+    run(dev, 795 + case, *MANY[case], per_head=case == 1, in_place=in_place)
 
 
 @pytest.mark.parametrize("case", range(len(CASES)))

@@ -5,6 +5,7 @@ import ctypes
 import pytest
 
 from launches import Recorder
+from test_gpu_norm_append import MANY
 from test_gpu_window import CASES, DEALT, TILES
 from test_serve_host import batch, cache
 from test_step_host import pool, rules
@@ -62,7 +63,8 @@ def test_a_workgroup_for_each_sequence_and_head(launched):
 
 def test_slices_of_logits(launched):
     for B, V in ((1, 7), (1, 32000), (64, 128256), (4000, 1000), (1, 1 << 22), (255, 1 << 22)):
-        (one,) = launched("bpd_adjust_logits_gpu", 1 << 40, 0, V, 1 << 50, 0, V, B, V, A(rules(mask_stride=1 << 20)))
+        r = rules(mask_stride=1 << 20)
+        (one,) = launched("bpd_adjust_logits_gpu", 1 << 40, 0, V, 1 << 50, 0, V, B, V, A(r))
         assert one.kernel == "k_adjust" and one.grid[0] % B == 0 and one.lds == 0
         S = one.grid[0] // B
         assert any(S == -(-V // n) for n in (1024, 2048, 4096, 8192)) and one.grid[0] < 1 << 31
@@ -80,8 +82,20 @@ def test_the_pool_takes_one_launch_a_call(launched):
 
 def test_waves_of_a_token(launched):
     c = cache(n_kv_heads=8, head_dim=128, page_stride=16 * 8 * 128, row_stride=128, head_stride=16 * 128)
-    for n, H, waves in ((1, 32, 4), (1024, 32, 4), (1025, 32, 2), (5000, 4, 2), (5000, 1, 2)):
+    for n, H, waves in ((1, 32, 4), (1024, 32, 4), (1025, 32, 2), (5000, 4, 2)):
         b = batch(n_seqs=n, n_tokens=n)
         (one,) = launched("bpd_norm_rope_append_paged_gpu", A(c), A(b), 0x80000, 0, 0x90000, 0, 0, 1e-6, None, None, 1 << 40,
                           H * 128, 1 << 41, 1024, 1 << 42, 1024, 1 << 43, H * 128, 1, H)
         assert one.kernel == "k_norm_append" and one.grid[0] == n and one.block[0] == 64 * waves
+
+
+@pytest.mark.parametrize("case,waves", [(0, 2), (1, 2), (2, 1)])
+def test_waves_of_many_tokens(launched, case, waves):
+    new, lens, P, H, HKV, D, x, kv, page, hf, pad, rot, neox, w = MANY[case]
+    n = sum(new) + pad
+    c = cache(type=T[kv], page_size=page, n_kv_heads=HKV, head_dim=D, page_stride=page * HKV * D, row_stride=D,
+              head_stride=page * D)
+    b = batch(n_seqs=2, n_tokens=n, q_start=0x8000)
+    (one,) = launched("bpd_norm_rope_append_paged_gpu", A(c), A(b), 0x80000, 0, 0x90000, 0, T[w], 1e-6, None, None, 1 << 40,
+                      H * D, 1 << 41, HKV * D, 1 << 42, HKV * D, 1 << 43, H * D, T[x], H)
+    assert one.kernel == "k_norm_append" and one.block[0] == 64 * waves
