@@ -149,9 +149,9 @@ __global__ __launch_bounds__(kThreads) void k_adjust(AdjustArgs g) {
         if (history) __syncthreads();
         clear(count, n);
         __syncthreads();
-        for (int i = e0 + tid; i < e1; i += kThreads) {
+        for (unsigned i = (unsigned)(e0 + tid); i < (unsigned)e1; i += kThreads) {
             const uint32_t at = (uint32_t)g.bias_token[i] - (uint32_t)lo;
-            if (at < (uint32_t)n) atomicMax(&count[at], (uint32_t)i + 1u);
+            if (at < (uint32_t)n) atomicMax(&count[at], i + 1u);
         }
         __syncthreads();
 #pragma unroll

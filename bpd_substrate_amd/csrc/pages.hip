@@ -154,25 +154,26 @@ __global__ __launch_bounds__(N) void k_extend(PoolArgs g) {
             const Grant x = grant[at];
             const int had = pages_of(g, x.old), has = pages_of(g, x.old + x.add);
             int32_t* table = x.row >= 0 ? g.table + (int64_t)x.row * g.table_stride : nullptr;
+            // the counters have 64 bits: a step past the end of the longest tables is beyond 2^31
             auto entry = [&](int i) { return i < had ? table[i] : g.free_pages[n_free - 1 - x.page0 - (i - had)]; };
             if (g.table_out != nullptr) {
                 int32_t* out = g.table_out + (int64_t)(b0 + at) * g.table_out_stride;
-                for (int i = i0; i < g.W; i += step) {
-                    const int page = x.row >= 0 && i < has ? entry(i) : -1;
+                for (int64_t i = i0; i < g.W; i += step) {
+                    const int page = x.row >= 0 && i < has ? entry((int)i) : -1;
                     out[i] = page;
                     if (x.row >= 0 && i >= had && i < has) table[i] = page;
                 }
             } else {
-                for (int i = had + i0; i < has; i += step) table[i] = entry(i);
+                for (int64_t i = (int64_t)had + i0; i < has; i += step) table[i] = entry((int)i);
             }
-            for (int i = i0; i < x.add; i += step) {
-                const int index = x.old + i, pg = fdiv(g.page, index), in = index - pg * (int)g.page.d, page = entry(pg);
+            for (int64_t i = i0; i < x.add; i += step) {
+                const int index = x.old + (int)i, pg = fdiv(g.page, index), in = index - pg * (int)g.page.d, page = entry(pg);
                 g.slots[x.t0 + i] = page >= 0 && page < g.n_pages ? page * (int)g.page.d + in : -1;
                 g.pos[x.t0 + i] = g.prefix_len + index;
             }
         }
     }
-    for (int i = tokens + (int)blockIdx.x * N + tid; i < g.T; i += (int)gridDim.x * N) g.slots[i] = g.pos[i] = -1;
+    for (int64_t i = (int64_t)tokens + blockIdx.x * N + tid; i < g.T; i += gridDim.x * N) g.slots[i] = g.pos[i] = -1;
     const int taken = pages;
     if (blockIdx.x == 0 && tid == 0) g.q_start[g.B] = tokens;
     if (!last_here(g)) return;
@@ -264,12 +265,12 @@ __global__ __launch_bounds__(N) void k_release(PoolArgs g) {
             if (where[at].x < 0) continue;
             int32_t* table = g.table + (int64_t)where[at].x * g.table_stride;
             const int64_t top = (int64_t)n_free + total - 1 - where[at].y;
-            auto give = [&](int i, int k) {  // page i of the table, the k-th that the sequence gives
+            auto give = [&](int64_t i, int64_t k) {  // page i of the table, the k-th that the sequence gives
                 if (top - k >= 0 && top - k < g.n_pages) g.free_pages[top - k] = table[i];
                 table[i] = -1;
             };
-            for (int i = r.k0 + i0; i < r.k1; i += step) give(i, i - r.k0);
-            for (int i = r.kept + i0; i < r.used; i += step)
+            for (int64_t i = (int64_t)r.k0 + i0; i < r.k1; i += step) give(i, i - r.k0);
+            for (int64_t i = (int64_t)r.kept + i0; i < r.used; i += step)
                 if (i < r.lo || i >= r.hi) give(i, r.k1 - r.k0 + i - r.kept - (i >= r.hi ? r.hi - r.lo : 0));
         }
     }

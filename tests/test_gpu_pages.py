@@ -144,6 +144,24 @@ def test_one_long_sequence_and_empty_calls(dev):
     b.same()
 
 
+def test_the_widest_table(dev):
+    """A step of the threads past its end is beyond 2^31."""
+    n_tokens = 4
+    W = 2 ** 31 - 1025 - n_tokens
+    pool = serve.PagePool.empty(100, 1, 1, W, device=dev)
+    step = pool.extend(i32([n_tokens], dev), n_tokens, rows=i32([0], dev))
+    assert step.refused.tolist() == [0] and step.pos.tolist() == list(range(n_tokens))
+    for table in (step.table, pool.table):
+        assert table[0, :n_tokens].tolist() == step.slots.tolist() and sorted(set(step.slots.tolist())) == sorted(step.slots.tolist())
+        assert int(table[0, n_tokens:].max()) == -1 and int(table[0, n_tokens:].min()) == -1
+    pool.release(i32([0], dev))
+    assert pool.n_free.tolist() == [100, 0] and sorted(pool.free.tolist()) == list(range(100))
+    assert int(pool.table.max()) == -1
+    pool.lens.fill_(W)   # more than the pool has: the whole table is gone through
+    pool.release(i32([0], dev))
+    assert pool.n_free.tolist() == [100, 0] and pool.lens.tolist() == [0] and int(pool.table.max()) == -1
+
+
 def test_pools_of_any_content_stay_inside(dev):
     """Lengths, counts and pages that no pool has: every access stays in the tensors."""
     big = 2 ** 31 - 1
