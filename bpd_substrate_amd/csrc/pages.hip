@@ -1,21 +1,21 @@
 // pages.hip — bpd_pages_extend_gpu and bpd_pages_release_gpu: pages handed to sequences that grow, and taken back.
 //
-// One launch each.  Every workgroup goes through all sequences, 256 at a time, a thread each: running sums of the pages
+// One launch each.  Every workgroup goes through all sequences, one round of a thread each up to 1,024: running sums of the pages
 // and tokens that they ask for say who is served and from which place of the free stack.  That is a few kilobytes out of
-// the L2, and spares a launch (or a grid-wide wait) between deciding and doing.  Of each 256 it then takes its parts: the
+// the L2, and spares a launch (or a grid-wide wait) between deciding and doing.  Of each round it then takes its parts: the
 // sequences' tables, their new tokens' slots and positions, or the pages that they put back onto the stack.  The
 // pool's lengths and counts, which all of them read, are written by the workgroup that is done last.
 // Latency bounds both: the names, the lengths, the sums, the table or the stack, the count of workgroups, one after the
-// other: 8.2 us for 256 sequences of up to 513 pages that grow by up to 4 rows each, 7.3 us back (a megabyte of tables, 0.2 us
-// of memory); 64 prompts of up to 2,048 rows 7.8 and 5.2.  In two and three launches the two calls took 24 us, in one
-// with a fence before the count 19, without 15.4.
+// other: 7.8 us for 256 sequences of up to 513 pages that grow by up to 4 rows each, 6.2 us back (a megabyte of tables, 0.2 us
+// of memory); 64 prompts of up to 2,048 rows 8.0 and 5.3.  In two and three launches the two calls took 24 us, in one
+// with a fence before the count 19, without 15.4, with 128 workgroups 13.6.
 #include "bpdq_paged.h"
 
 namespace bpdq {
 
 namespace {
 
-constexpr int N = 256;
+constexpr int kAhead = 4;  // places of a table under way
 
 // A pair of numbers; its sums over the threads before this one, and over all.
 struct Two {
@@ -24,6 +24,7 @@ struct Two {
 struct Sums {
     Two before, all;
 };
+template <int N>  // threads
 struct Scan {
     Two wave[2][N / 64];  // of this sum, and of the one before
     __device__ __forceinline__ Sums go(int64_t a, int64_t b, int& turn) {
@@ -61,6 +62,7 @@ __device__ __forceinline__ int pages_of(const PoolArgs& g, int rows) {  // rows 
 
 // Which sequence is the first to name each row; then the row that sequence b names, or -1: none, or one that an earlier
 // sequence names.
+template <int N>
 __device__ __forceinline__ void claim_rows(const PoolArgs& g, int* claim) {
     if (g.rows == nullptr) return;
     for (int i = (int)threadIdx.x; i < g.n_rows; i += N) claim[i] = g.B;
@@ -97,13 +99,14 @@ struct Grant {
     int row, old, add, t0, page0;
 };
 
+template <int N>
 __global__ __launch_bounds__(N) void k_extend(PoolArgs g) {
     extern __shared__ int claim[];
-    __shared__ Scan s;
+    __shared__ Scan<N> s;
     __shared__ Grant grant[N];
     const int tid = (int)threadIdx.x, most = g.W * (int)g.page.d;  // rows of a table
     const int n_free = clamp(g.n_free[0], 0, g.n_pages);
-    claim_rows(g, claim);
+    claim_rows<N>(g, claim);
     int turn = 0;
     int64_t asked = 0, wanted = 0;  // pages by all before, tokens by those of them who can be paid
     int tokens = 0, pages = 0;      // granted to those before
@@ -158,10 +161,19 @@ __global__ __launch_bounds__(N) void k_extend(PoolArgs g) {
             auto entry = [&](int i) { return i < had ? table[i] : g.free_pages[n_free - 1 - x.page0 - (i - had)]; };
             if (g.table_out != nullptr) {
                 int32_t* out = g.table_out + (int64_t)(b0 + at) * g.table_out_stride;
-                for (int64_t i = i0; i < g.W; i += step) {
-                    const int page = x.row >= 0 && i < has ? entry((int)i) : -1;
-                    out[i] = page;
-                    if (x.row >= 0 && i >= had && i < has) table[i] = page;
+                for (int64_t i = i0; i < g.W; i += kAhead * step) {
+                    int page[kAhead];
+#pragma unroll
+                    for (int u = 0; u < kAhead; u++) {
+                        const int64_t j = i + u * step;
+                        page[u] = x.row >= 0 && j < has ? entry((int)j) : -1;
+                    }
+#pragma unroll
+                    for (int u = 0; u < kAhead; u++) {
+                        const int64_t j = i + u * step;
+                        if (j < g.W) out[j] = page[u];
+                        if (x.row >= 0 && j >= had && j < has) table[j] = page[u];
+                    }
                 }
             } else {
                 for (int64_t i = (int64_t)had + i0; i < has; i += step) table[i] = entry((int)i);
@@ -231,13 +243,14 @@ __device__ __forceinline__ Release release_of(const PoolArgs& g, int b, int row)
     return r;
 }
 
+template <int N>
 __global__ __launch_bounds__(N) void k_release(PoolArgs g) {
     extern __shared__ int claim[];
-    __shared__ Scan s;
+    __shared__ Scan<N> s;
     __shared__ Release what[N];
     __shared__ int2 where[N];  // row, pages given before it
     const int tid = (int)threadIdx.x, n_free = clamp(g.n_free[0], 0, g.n_pages);
-    claim_rows(g, claim);
+    claim_rows<N>(g, claim);
     int turn = 0;
     int64_t total = 0, pages = 0;  // given by all, and by those before
     if (g.B > N)                   // one round says both
@@ -291,25 +304,37 @@ __global__ __launch_bounds__(N) void k_release(PoolArgs g) {
     }
 }
 
-// Parts of a sequence's work, 2048 places (8 of a workgroup's steps) each on average, and the workgroups: all
-// items at once while the chip holds them.
-unsigned groups_of(PoolArgs& g, int64_t work) {
-    const int64_t p = work / (2048 * (int64_t)g.B), n = (int64_t)g.B * (g.parts = (int)(p < 1 ? 1 : p > 64 ? 64 : p));
-    return (unsigned)(n < 1024 ? n : 1024);
+// Threads: a round decides for as many sequences, and each more costs its sums again (300 and 512 sequences, the two calls:
+// 18 and 23 us, in rounds of 256 23 and 29).
+int threads_of(const PoolArgs& g) { return g.B <= 256 ? 256 : g.B <= 512 ? 512 : 1024; }
+
+// Parts of a sequence's work, 8 of a workgroup's steps each on average, and the workgroups.  Each of them decides, and their
+// counts at the end come one after the other: 128, or 256 where there is much to copy (256 / 512 sequences' tables of 513
+// pages: 128 13.6 / 17.1 us, 256 15.6 / 18.0, 64 14.4 / 20.0; tables of 8,192: 30.4 / 33.0, 21.8 / 24.7, 50 / 53).
+unsigned groups_of(PoolArgs& g, int threads, int64_t work) {
+    const int64_t p = work / (8 * (int64_t)threads * g.B);
+    const int64_t n = (int64_t)g.B * (g.parts = (int)(p < 1 ? 1 : p > 64 ? 64 : p)), most = work < 5 << 17 ? 128 : 256;
+    return (unsigned)(n < most ? n : most);
 }
 
 }  // namespace
 
 void launch_pages_extend(const PoolArgs& a, hipStream_t s) {
     PoolArgs g = a;
-    const unsigned groups = groups_of(g, (int64_t)g.T + (g.table_out != nullptr ? (int64_t)g.B * g.W : 0));
-    hipLaunchKernelGGL(k_extend, dim3(groups), dim3(N), g.rows != nullptr ? 4 * (size_t)g.n_rows : 0, s, g);
+    const int threads = threads_of(g);
+    const unsigned groups = groups_of(g, threads, (int64_t)g.T + (g.table_out != nullptr ? (int64_t)g.B * g.W : 0));
+    const size_t lds = g.rows != nullptr ? 4 * (size_t)g.n_rows : 0;
+    const auto k = threads == 256 ? k_extend<256> : threads == 512 ? k_extend<512> : k_extend<1024>;
+    hipLaunchKernelGGL(k, dim3(groups), dim3(threads), lds, s, g);
 }
 
 void launch_pages_release(const PoolArgs& a, hipStream_t s) {
     PoolArgs g = a;
-    const unsigned groups = groups_of(g, (int64_t)g.B * g.W);
-    hipLaunchKernelGGL(k_release, dim3(groups), dim3(N), g.rows != nullptr ? 4 * (size_t)g.n_rows : 0, s, g);
+    const int threads = threads_of(g);
+    const unsigned groups = groups_of(g, threads, (int64_t)g.B * g.W);
+    const size_t lds = g.rows != nullptr ? 4 * (size_t)g.n_rows : 0;
+    const auto k = threads == 256 ? k_release<256> : threads == 512 ? k_release<512> : k_release<1024>;
+    hipLaunchKernelGGL(k, dim3(groups), dim3(threads), lds, s, g);
 }
 
 }  // namespace bpdq
