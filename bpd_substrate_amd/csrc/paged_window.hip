@@ -30,6 +30,19 @@ constexpr int64_t kMostItems = 1 << 22;  // workgroups of 512 threads in a launc
 
 bool whole_pages(const Paged& a) { return a.page.d % 16 == 0 && a.row_stride < 1 << 26; }
 
+// Waves of a workgroup so that `items` workgroups are on the chip at once.  With few rows a wave's time is latency that more
+// waves do not shorten, and a second round of workgroups doubles it.  Measured (us, 4 / 2 / 1 waves; 4 query heads to each
+// kv head, 128 wide, bf16; lengths from a quarter of the rows to all): 512 items, 132 rows 10.7, 11.0, 12.5; 600 15.4, 11.7,
+// 13.3; 1,024 17.8, 14.3, 15.0; 1,408 24.1, 21.0, 17.8; 2,048 items, 68 / 260 / 516 rows 29.2, 20.2, 14.7 / 50.6, 41.6,
+// 37.4 / 66.6, 61.0, 60.8, but 2,052 rows 227, 235, 234, where memory bounds it; heads of 256, 1,024 items, 132 rows 37.2,
+// 28.3, 22.2; fp32 queries, 480 items, pages of 21, 132 / 520 rows 8.7, 10.8, 14.0 / 19.5, 28.5, 42.7.
+int chip_waves(int DT) { return DT == 256 ? 1024 : 2048; }  // that the registers hold
+bool few_rows(int DT, bool single, int64_t rows) { return rows <= (single || DT == 256 ? 320 : 640); }
+int waves_at_once(int most, int64_t items, int64_t waves) {
+    while (most > 1 && items * most > waves) most >>= 1;
+    return most;
+}
+
 // Waves of a workgroup for each (sequence, head), or 0: the units dealt to all waves of the chip, and a second launch.
 // `rows` is what a token sees at most, `items` sequences times kv heads.  One launch spares the dealing and the join, 6 to
 // 9 us, and costs where few items with many rows leave CUs idle.  Measured (us, one launch with 8 and with 4 waves,
@@ -42,9 +55,10 @@ bool whole_pages(const Paged& a) { return a.page.d % 16 == 0 && a.row_stride < 1
 // 30.8, 23.8, 27.8 / 49.0, 41.6, 40.5).  Heads of 256 fill the registers with 4 waves (2 heads, 2 items, 516 / 1,028 rows:
 // -, 17.0, 17.8 / -, 24.0, 21.0; 128 items: -, 21.3, 43.6 / -, 37.0, 56.0).
 int head_waves(int DT, bool single, int64_t items, int64_t rows) {
-    if (DT == 256) return items >= 128 || rows <= 640 ? 4 : 0;
-    if (single ? rows > 640 : items < 128 && rows > 2304) return 0;
-    return items <= 256 ? 8 : 4;
+    if (DT == 256 ? items < 128 && rows > 640 : single ? rows > 640 : items < 128 && rows > 2304) return 0;
+    const int most = DT == 256 ? 4 : 8;
+    if (few_rows(DT, single, rows)) return waves_at_once(most, items, chip_waves(DT));
+    return items <= 256 ? most : 4;
 }
 
 // Rows that a token sees at most.
@@ -68,24 +82,30 @@ int64_t even_tiles(const Paged& a, int G, int R) {
 //   1, 2,052 rows, 128                                    20, 42
 // heads of 64 (5 to a kv head), 64 sequences, 2,052 rows, 8 / 32: 103, 135 / 240, 149; of 256 (2 kv heads, 8 each), 4 / 8:
 // 76, 98 / 147, 104.
-int rows_waves(const Paged& a, int G, int R, int64_t rows) {
+// Of the workgroups up to one per sequence has no tokens and ends at once: the chip is taken for a quarter larger (us, 4 / 2 / 1
+// waves; 64 sequences, 516 rows, up to 4 and 8 tokens 31.1, 28.0, 40.7 and 40.2, 37.2, 43.9; 107, heads of 64, 122 rows, 6
+// tokens 29.3, 19.5, 15.3; 128, 132 rows, 4 tokens 30.2, 24.9, 21.7).
+int rows_waves(const Paged& a, int G, int R, bool single, int64_t rows) {
     const int DT = padded(a.D);
     const double head = DT == 64 ? 0.95 : DT == 128 ? 1.6 : 4.2, tile = DT == 64 ? 6 : DT == 128 ? 9 : 14;
     const int64_t items = even_tiles(a, G, 16) * a.hkv;
     const double one = head * (double)items * (double)((rows + 63) / 32);
     const double plan = 40e3 + tile * (double)(even_tiles(a, G, R) * a.hkv) * (double)((rows + 127) / 64);
     if (one >= plan || tiles_of(a, G, 16) * a.hkv > kMostItems) return 0;
-    return DT == 256 || items > 256 ? 4 : 8;
+    const int most = DT == 256 ? 4 : 8;
+    if (few_rows(DT, single, rows)) return waves_at_once(most, tiles_of(a, G, 16) * a.hkv, chip_waves(DT) * 5 / 4);
+    return items <= 256 ? most : 4;
 }
 
 // head_waves or rows_waves of a call.
 int waves_of(const Paged& a, int q_type, int G, int window, int sinks) {
     const int DT = padded(a.D);
     const int64_t rows = rows_seen(a, window, sinks);
-    if (planned_way(a.q_start, G)) return rows_waves(a, G, rows_of(a.D, q_type == BPD_T_F32 ? 2 : 1), rows);
+    const bool single = !whole_pages(a) || (q_type == BPD_T_F32 && DT > 64);
+    if (planned_way(a.q_start, G)) return rows_waves(a, G, rows_of(a.D, q_type == BPD_T_F32 ? 2 : 1), single, rows);
     const int64_t items = (int64_t)a.B * a.hkv;
     if (items > kMostItems) return 0;
-    return head_waves(DT, !whole_pages(a) || (q_type == BPD_T_F32 && DT > 64), items, rows);
+    return head_waves(DT, single, items, rows);
 }
 
 template <int QT, int CT, int NS, int DT, bool UNI, int NW>
@@ -104,6 +124,10 @@ void launch_dim(const AttnArgs& g, hipStream_t s) {
         launch_head<QT, CT, NS, DT, UNI, DT < 256 ? 8 : 4>(g, s);
     else if (g.waves == 4)
         launch_head<QT, CT, NS, DT, UNI, 4>(g, s);
+    else if (g.waves == 2)
+        launch_head<QT, CT, NS, DT, UNI, 2>(g, s);
+    else if (g.waves == 1)
+        launch_head<QT, CT, NS, DT, UNI, 1>(g, s);
     else if (g.planned)
         hipLaunchKernelGGL((k_attn_tile<QT, CT, NS, DT, MT, NW, UNI, true>), dim3((unsigned)g.groups), dim3(64 * NW), 0, s,
                            g);

@@ -74,6 +74,33 @@ DEALT = [
 ]
 
 
+def many(B, n, longest, H, HKV, D, q, kv, page, P=0):
+    """Lengths of 0 to `longest`, with up to n new tokens each."""
+    r = np.random.default_rng(B + D)
+    lens = [int(x) for x in r.integers(0, longest + 1, B - 1)] + [longest]
+    new = [1 if n == 1 else min(int(x), k) for x, k in zip(r.integers(0, n + 1, B), lens)]
+    return new, lens, P, H, HKV, D, q, kv, page, True, 0 if n == 1 else 2
+
+
+# many sequences of few rows: two waves to a workgroup, or one
+CROWDS = [
+    (many(120, 1, 60, 8, 8, 64, "f16", "f16", 16), (40, 3), 2),
+    (many(260, 1, 70, 16, 8, 128, "bf16", "bf16", 16), (64, 4), 1),
+    (many(120, 1, 90, 20, 5, 96, "f32", "f16", 21, 30), (50, 33), 2),
+    (many(300, 1, 50, 20, 5, 80, "f32", "bf16", 8), (45, 0), 1),
+    (many(100, 1, 40, 8, 4, 256, "bf16", "bf16", 32), (33, 1), 2),
+    (many(200, 1, 40, 8, 4, 256, "f16", "f16", 8), (100, 5), 1),
+    (many(130, 5, 70, 16, 4, 128, "f16", "f16", 16), (60, 4), 2),
+    (many(300, 4, 50, 8, 4, 64, "f32", "bf16", 21, 20), (30, 25), 1),
+]
+
+
+@pytest.mark.parametrize("case", range(len(CROWDS)))
+def test_many_sequences(dev, case):
+    args, win, _ = CROWDS[case]
+    check(Batch(860 + case, *args, decode=max(args[0]) == 1), dev, *win)
+
+
 @pytest.mark.parametrize("slide", [False, True])
 @pytest.mark.parametrize("case", range(len(TILES)))
 def test_tiles(dev, case, slide):

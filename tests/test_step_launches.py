@@ -6,7 +6,7 @@ import pytest
 
 from launches import Recorder
 from test_gpu_norm_append import MANY
-from test_gpu_window import CASES, DEALT, TILES
+from test_gpu_window import CASES, CROWDS, DEALT, TILES
 from test_serve_host import batch, cache
 from test_step_host import pool, rules
 
@@ -59,6 +59,13 @@ def test_a_workgroup_for_each_sequence_and_head(launched):
         _, (one,) = window(launched, ([1] * B, [600] * B, 0, 4 * HKV, HKV, D, "bf16", "bf16", 64, True, 0), (512, 4), decode=True)
         assert one.kernel == "k_attn_head" and one.grid[0] == B * HKV
         assert one.block[0] == (256 if D == 256 or B * HKV > 256 else 512)
+
+
+@pytest.mark.parametrize("case", range(len(CROWDS)))
+def test_waves_of_many_sequences(launched, case):
+    args, win, waves = CROWDS[case]
+    need, (one,) = window(launched, args, win, decode=max(args[0]) == 1)
+    assert one.kernel == "k_attn_head" and need == 0 and one.block[0] == 64 * waves
 
 
 def test_slices_of_logits(launched):
