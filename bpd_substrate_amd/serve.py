@@ -73,6 +73,16 @@ def _bad(what):
     raise BpdqError(BPDQ_ERR_SHAPE, what)
 
 
+_TOP = 0x7FFFFFFF   # of a C int
+
+
+def _int(n, what):
+    """n, which ctypes would pass on modulo 2^32."""
+    if not -_TOP - 1 <= n <= _TOP:
+        _bad(f"{what} {n} does not fit 32 bits")
+    return n
+
+
 def _tensor(t, what, dtypes, ndim, device=None, contiguous=False):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what} is no tensor")
@@ -127,7 +137,8 @@ class PagedCache:
         self.k, self.v, self.dtype, self.device = k, v, k.dtype, k.device
         self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = k.shape
         s = [0 if n == 1 else st for n, st in zip(k.shape, k.stride())]   # of one page, row or head: never used
-        self.c = _Cache(k.data_ptr(), v.data_ptr(), TYPES[k.dtype], *k.shape, s[0], s[1], s[2])
+        self.c = _Cache(k.data_ptr(), v.data_ptr(), TYPES[k.dtype], *(_int(n, "a dimension of the pages") for n in k.shape),
+                        *s[:3])
         self._geometry = (k.shape[1:], s[1])   # what a workspace goes by
         self._p = ctypes.addressof(self.c)
 
@@ -173,8 +184,8 @@ class PagedBatch:
         self.table, self.lens, self.q_start, self.prefix = table, lens, q_start, prefix
         self.n_seqs, self.n_tokens, self.prefix_len = n, n if n_tokens is None else n_tokens, prefix_len
         p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        self.c = _Batch(p(table), table.stride(0) if n > 1 else w, w, p(lens), p(q_start), n, self.n_tokens, p(prefix),
-                        prefix_len)
+        self.c = _Batch(p(table), table.stride(0) if n > 1 else w, _int(w, "table's width"), p(lens), p(q_start),
+                        _int(n, "n_seqs"), _int(self.n_tokens, "n_tokens"), p(prefix), _int(prefix_len, "prefix_len"))
         self._p = ctypes.addressof(self.c)
         self._bytes = {}
 
@@ -183,7 +194,6 @@ class PagedBatch:
             _bad(f"the batch is on {self.device}, the cache on {cache.device}")
         if self.prefix_len > (0 if self.prefix is None else self.prefix.shape[0]) * cache.page_size:
             _bad(f"prefix_len {self.prefix_len} is more than its pages hold")
-
 
     def _workspace(self, cache, dtype, heads, window, sinks):
         """Bytes that an attention call needs, which go by shapes alone."""
@@ -265,9 +275,9 @@ class PagePool:
                 _bad(f"{what} is {list(t.shape)}, not {list(shape)}")
         self.table, self.lens, self.free, self.n_free, self.gone = table, lens, free, n_free, gone
         self.n_rows, self.width, self.n_pages, self.page_size = R, W, free.shape[0], page_size
-        self.c = _Pool(table.data_ptr(), table.stride(0) if R > 1 else W, W, lens.data_ptr(),
-                       None if gone is None else gone.data_ptr(), free.data_ptr(), n_free.data_ptr(), R, free.shape[0],
-                       page_size)
+        self.c = _Pool(table.data_ptr(), table.stride(0) if R > 1 else W, _int(W, "table's width"), lens.data_ptr(),
+                       None if gone is None else gone.data_ptr(), free.data_ptr(), n_free.data_ptr(), _int(R, "n_rows"),
+                       _int(self.n_pages, "n_pages"), _int(page_size, "page_size"))
         self._p = ctypes.addressof(self.c)
 
     @classmethod
@@ -290,7 +300,7 @@ class PagePool:
             if rows is not None and rows.shape != t.shape:
                 _bad(f"{what} has {t.shape[0]} values and rows {rows.shape[0]}")
         n = t.shape[0] if t is not None else rows.shape[0] if rows is not None else self.n_rows
-        return n, None if rows is None else rows.data_ptr(), None if t is None else t.data_ptr()
+        return _int(n, "n_seqs"), None if rows is None else rows.data_ptr(), None if t is None else t.data_ptr()
 
     def extend(self, new, n_tokens, rows=None, prefix_len=0):
         """Sequence b, row rows[b] of the pool (None: row b), grows by new[b] rows (int32, on the device): a PageStep.
@@ -301,6 +311,8 @@ class PagePool:
         dev, T, W = self.device, n_tokens, self.width
         if T < 0:
             _bad("n_tokens is negative")
+        _int(T, "n_tokens")
+        _int(prefix_len, "prefix_len")
         sizes = (B, B + 1, T, T, B, 0 if rows is None else B * W)
         out = torch.empty(sum(sizes), dtype=torch.int32, device=dev)
         lens, q_start, slots, pos, refused, table = out.split_with_sizes(sizes)
@@ -323,8 +335,9 @@ class PagePool:
             _bad(f"window {window} is below 1, or the pool is without gone")
         if sinks < 0 or prefix_len < 0:
             _bad("sinks or prefix_len is negative")
-        _launch(self.device, gpu._fn("bpd_pages_release_on_gpu"), self._p, rp, kp, B, 0 if window is None else window,
-                max(0, sinks - prefix_len))
+        # rows end below _TOP: beyond it a window, or first rows, are all of them
+        _launch(self.device, gpu._fn("bpd_pages_release_on_gpu"), self._p, rp, kp, B, 0 if window is None else min(window, _TOP),
+                min(max(0, sinks - prefix_len), _TOP))
 
 
 def _weights(w, what, x, heads, D):
@@ -405,8 +418,12 @@ def attention(cache, batch, q, scale=None, out=None, return_lse=False, window=No
         _bad(f"q has {q.dim()} dimensions, not 3")
     if window is None and sinks != 0:
         _bad("sinks without a window")
-    if window is not None:   # beyond these limits every position is seen
-        window, sinks = min(window, 0x7FFFFFFF), min(sinks, 0x7FFFFFFF)
+    if window is not None:
+        if window < 1:
+            _bad("window is below 1")
+        if sinks < 0:
+            _bad("sinks is negative")
+        window, sinks = min(window, _TOP), min(sinks, _TOP)   # positions end below _TOP: beyond it every one is seen
     T, H, D, dev = batch.n_tokens, q.shape[1], cache.head_dim, cache.device
     if q.dtype not in (cache.dtype, torch.float32):
         _bad(f"q is {q.dtype}, neither float32 nor the cache's {cache.dtype}")
@@ -489,6 +506,8 @@ def adjust_logits(logits, tokens=None, lens=None, prompt=None, repetition=None, 
     if logits.dim() != 2:
         _bad(f"logits have {logits.dim()} dimensions, not 2")
     B, V = logits.shape
+    _int(B, "rows of logits")
+    _int(V, "vocab")
     dev = logits.device
     xs = _pitch(logits, "logits")
     if out is None:
@@ -520,7 +539,7 @@ def adjust_logits(logits, tokens=None, lens=None, prompt=None, repetition=None, 
         h, w = tokens.shape
         if h != B:
             _bad(f"tokens has {h} rows and logits {B}")
-        r.tokens, r.token_stride, r.token_width = tokens.data_ptr(), _pitch(tokens, "tokens"), w
+        r.tokens, r.token_stride, r.token_width = tokens.data_ptr(), _pitch(tokens, "tokens"), _int(w, "tokens' width")
         r.lens, r.prompt = per_row(lens, "lens", torch.int32), per_row(prompt, "prompt", torch.int32)
         r.repetition = per_row(repetition, "repetition", torch.float32)
         r.frequency = per_row(frequency, "frequency", torch.float32)
@@ -529,7 +548,7 @@ def adjust_logits(logits, tokens=None, lens=None, prompt=None, repetition=None, 
         _tensor(mask, "mask", i32, 2, dev)
         if mask.shape[1] < (V + 31) // 32:
             _bad(f"mask has {mask.shape[1]} words a row for {V} tokens")
-        r.mask, r.mask_stride, r.n_masks = mask.data_ptr(), _pitch(mask, "mask"), mask.shape[0]
+        r.mask, r.mask_stride, r.n_masks = mask.data_ptr(), _pitch(mask, "mask"), _int(mask.shape[0], "the number of masks")
         r.mask_row = per_row(mask_row, "mask_row", torch.int32)
     if bias is not None:
         start, token, value = bias
@@ -539,7 +558,7 @@ def adjust_logits(logits, tokens=None, lens=None, prompt=None, repetition=None, 
         if start.shape[0] != B + 1 or token.shape != value.shape:
             _bad(f"bias has {start.shape[0]} offsets for {B} rows, or {token.shape[0]} tokens and {value.shape[0]} values")
         r.bias_start, r.bias_token, r.bias_value, r.n_bias = (start.data_ptr(), token.data_ptr(), value.data_ptr(),
-                                                              token.shape[0])
+                                                              _int(token.shape[0], "the number of biases"))
     _launch(dev, gpu._fn("bpd_adjust_logits_on_gpu"), logits.data_ptr(), TYPES[logits.dtype], xs, out.data_ptr(),
             TYPES[out.dtype], ys, B, V, ctypes.addressof(r))
     return out
