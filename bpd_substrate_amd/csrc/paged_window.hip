@@ -27,6 +27,7 @@ namespace bpdq {
 namespace {
 
 constexpr int64_t kMostItems = 1 << 22;  // workgroups of 512 threads in a launch
+constexpr int64_t kMostRows = 8192;      // that one workgroup may have to take for 16 rows of queries
 
 bool whole_pages(const Paged& a) { return a.page.d % 16 == 0 && a.row_stride < 1 << 26; }
 
@@ -82,6 +83,13 @@ int64_t even_tiles(const Paged& a, int G, int R) {
 //   1, 2,052 rows, 128                                    20, 42
 // heads of 64 (5 to a kv head), 64 sequences, 2,052 rows, 8 / 32: 103, 135 / 240, 149; of 256 (2 kv heads, 8 each), 4 / 8:
 // 76, 98 / 147, 104.
+// Fewer of them than CUs take as long as one per CU would, and nearly the same for each row however few they are (one
+// sequence of 1 / 4 tokens: 2,052 rows 24.5, 24.5 / 25.3, 27.9; 4,100 38.9, 26.0 / 39.6, 29.5; 16,388 165, 40 / 166, 43;
+// 131,076 1,724, 150 / 1,730, 153; 2,052 and 4,100 rows with fp32 queries 23.5, 22.2 and 36.5, 24.1, in pages of 21
+// 27.2, 24.0 and 45.0, 26.7; heads of 256, 1,028 and 4,100 27.4, 25.4 and 75.0, 34.6).
+// The lengths are on the device: a workgroup may get all the rows and the others few, while tiles deal what is there.
+// Beyond kMostRows that risk is not taken (64 sequences of one token, lengths from a quarter of the rows to all: 8,196 rows
+// 301, 355, 16,388 548, 613; 65 of two tokens, one of 19,264 rows and the others of 512: 473, 94).
 // Of the workgroups up to one per sequence has no tokens and ends at once: the chip is taken for a quarter larger (us, 4 / 2 / 1
 // waves; 64 sequences, 516 rows, up to 4 and 8 tokens 31.1, 28.0, 40.7 and 40.2, 37.2, 43.9; 107, heads of 64, 122 rows, 6
 // tokens 29.3, 19.5, 15.3; 128, 132 rows, 4 tokens 30.2, 24.9, 21.7).
@@ -89,9 +97,9 @@ int rows_waves(const Paged& a, int G, int R, bool single, int64_t rows) {
     const int DT = padded(a.D);
     const double head = DT == 64 ? 0.95 : DT == 128 ? 1.6 : 4.2, tile = DT == 64 ? 6 : DT == 128 ? 9 : 14;
     const int64_t items = even_tiles(a, G, 16) * a.hkv;
-    const double one = head * (double)items * (double)((rows + 63) / 32);
+    const double one = head * (double)(items > kGroups ? items : kGroups) * (double)((rows + 63) / 32);
     const double plan = 40e3 + tile * (double)(even_tiles(a, G, R) * a.hkv) * (double)((rows + 127) / 64);
-    if (one >= plan || tiles_of(a, G, 16) * a.hkv > kMostItems) return 0;
+    if (rows > kMostRows || one >= plan || tiles_of(a, G, 16) * a.hkv > kMostItems) return 0;
     const int most = DT == 256 ? 4 : 8;
     if (few_rows(DT, single, rows)) return waves_at_once(most, tiles_of(a, G, 16) * a.hkv, chip_waves(DT) * 5 / 4);
     return items <= 256 ? most : 4;
@@ -170,7 +178,7 @@ void launch_attn_window(const Paged& a, int cache_type, const void* q, int64_t q
     AttnArgs g = attn_args(a, cache_type, q, qs, out, os, lse, q_type, H, scale, 0, ws);
     g.window = window;
     g.sinks = sinks;
-    const int n = waves_of(g.a, q_type, g.G, window, sinks);
+    const int n = waves_of(a, q_type, g.G, window, sinks);  // as the workspace's size goes by
     if (n > 0) g.waves = n;
     // as k_attn_wave's
     g.past_mall = (int64_t)a.B * a.hkv * rows_seen(g.a, window, sinks) * a.D * 4 > (int64_t)256 << 20;
