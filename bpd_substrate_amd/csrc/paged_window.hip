@@ -51,12 +51,18 @@ int waves_at_once(int most, int64_t items, int64_t waves) {
 //   8 items, 132 / 2,052 / 4,100 rows      7.7, 8.3, 13.1 / 19.2, 25.5, 20.4 / 31.9, 45.4, 29.7
 //   128, 1,028 / 4,100                     18.1, 19.5, 27.1 / 62.7, 66.6, 68.6
 //   512, 1,028 / 4,100                     52.0, 46.6, 64.6 / 172.7, 170.5, 182.8
+// The lengths are on the device, and one sequence may have most of the rows: beyond 4,096, where dealing and join are little
+// beside them, they are dealt for any number of items (one launch, two; all lengths the same, a quarter of the rows to all,
+// one sequence of all and the others of 512):
+//   512, 4,100 / 16,388    179, 182 / 679, 641    135, 129 / 431, 392    65, 38 / 196, 50
+//   128, 4,100 / 16,388    52, 54 / 199, 171      45, 39 / 161, 109      44, 32 / 148, 47
+//   128 of 256, 4,100      110, 116               98, 95                 83, 62
 // Waves with one unit in flight (`single`: fp32 queries, pages that are no multiple of 16 rows) take more than twice as
 // long for a row (5 heads of 96, page 21, 5 items, 516 / 1,028 rows: 14.7, 18.4, 14.2 / 21.7, 30.0, 15.8; 320 items:
 // 30.8, 23.8, 27.8 / 49.0, 41.6, 40.5).  Heads of 256 fill the registers with 4 waves (2 heads, 2 items, 516 / 1,028 rows:
 // -, 17.0, 17.8 / -, 24.0, 21.0; 128 items: -, 21.3, 43.6 / -, 37.0, 56.0).
 int head_waves(int DT, bool single, int64_t items, int64_t rows) {
-    if (DT == 256 ? items < 128 && rows > 640 : single ? rows > 640 : items < 128 && rows > 2304) return 0;
+    if (rows > 4096 || (DT == 256 ? items < 128 && rows > 640 : single ? rows > 640 : items < 128 && rows > 2304)) return 0;
     const int most = DT == 256 ? 4 : 8;
     if (few_rows(DT, single, rows)) return waves_at_once(most, items, chip_waves(DT));
     return items <= 256 ? most : 4;

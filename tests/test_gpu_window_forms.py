@@ -32,3 +32,22 @@ def test_few_tokens_before_many_rows(dev, case, slide):
         b.slide(*win)
     assert needs_workspace(b, dev, *win)
     check(b, dev, *win)
+
+
+# one token each, of sequences of which one is long: its units go to all waves
+LONG = [
+    (([1] * 17, [30] * 9 + [4800] + [1, 2, 64, 0, 700, 33, 32], 0, 16, 8, 128, "bf16", "bf16", 64, True, 0), (4500, 4)),
+    (([1] * 65, [40] * 64 + [4300], 50, 4, 2, 64, "f32", "f16", 16, False, 0), (4200, 60)),
+    (([1] * 65, [4700] + [3] * 64, 0, 4, 2, 256, "f16", "f16", 32, True, 0), (2 ** 31 - 1, 0)),
+]
+
+
+@pytest.mark.parametrize("slide", [False, True])
+@pytest.mark.parametrize("case", range(len(LONG)))
+def test_one_long_sequence_among_many(dev, case, slide):
+    args, win = LONG[case]
+    b = Batch(920 + case, *args, decode=True)
+    if slide:
+        b.slide(*win)
+    assert needs_workspace(b, dev, *win)
+    check(b, dev, *win)

@@ -43,3 +43,13 @@ def test_many_sequences_of_which_one_may_be_long(launched):
     for new in ([1] * 64, [2] * 64):
         assert kernels(launched, new, 8192, 32, 8, 128, "bf16", "bf16", 64) == ONE
         assert kernels(launched, new, 8196, 32, 8, 128, "bf16", "bf16", 64) == TILES
+
+
+@pytest.mark.parametrize("B,shape", [(16, (32, 8, 128, "bf16", "bf16", 64)), (64, (32, 8, 128, "f16", "f16", 16)), (64, (40, 8, 64, "f16", "f16", 16)),
+                                     (64, (16, 2, 256, "bf16", "bf16", 64)), (200, (8, 8, 64, "f32", "bf16", 16))])
+def test_one_token_each_of_many_sequences(launched, B, shape):
+    assert kernels(launched, [1] * B, 2052, *shape, decode=True) == ONE
+    assert kernels(launched, [1] * B, 4096, *shape, decode=True) == ONE
+    for rows in (4100, 131072):
+        assert kernels(launched, [1] * B, rows, *shape, decode=True) == DEALT
+    assert kernels(launched, [1] * B, 131072, *shape, decode=True, win=2048) == ONE
