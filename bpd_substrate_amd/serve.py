@@ -299,6 +299,9 @@ class PagePool:
             _tensor(t, what, (torch.int32,), 1, self.device, contiguous=True)
             if rows is not None and rows.shape != t.shape:
                 _bad(f"{what} has {t.shape[0]} values and rows {rows.shape[0]}")
+            # read for one sequence while another's length is written
+            if rows is not None and -4 * t.shape[0] < t.data_ptr() - self.c.lens < 4 * self.n_rows:
+                _bad(f"{what} lies in the pool's lens: pass a copy, or no rows")
         n = t.shape[0] if t is not None else rows.shape[0] if rows is not None else self.n_rows
         return _int(n, "n_seqs"), None if rows is None else rows.data_ptr(), None if t is None else t.data_ptr()
 

@@ -147,7 +147,8 @@ int64_t bpd_sample_workspace(int n_rows, int vocab);
  * back.  free_pages[0 .. n_free[0]) are the pages that no sequence holds.  gone (may be NULL, without windows):
  * pages [gone[2 r], gone[2 r + 1]) of row r have slid out of its window and were given back.  All of it is
  * device memory that the caller fills once (tables -1, lens, gone and n_free[1] 0) and the two calls below keep.
- * Calls on one pool follow each other, on one stream or by events.
+ * Calls on one pool follow each other, on one stream or by events.  Their rows, n_new and keep lie in none of its
+ * arrays; with rows NULL n_new and keep may be lens.
  * Pages that are no part of the pool (a shared prefix's) are left out of free_pages.  n_pages and table_width times
  * page_size stay below 2^31; n_rows up to 16384 (BPDQ_ERR_LIMIT). */
 typedef struct {
