@@ -4,8 +4,8 @@
 // paged_attn.hip with the units that no token of an item sees left out (span_of): at most four runs, the first
 // rows and the window's in the prefix and in the sequence's own part.  Every sequence reads the prefix's rows that it sees
 // for itself, as a window passes the prefix soon: its tokens are not packed.  Windows bound what a token sees, so the host
-// knows the work of most batches: those take one launch of k_attn_head, a workgroup for each (sequence, kv head) or each 16
-// rows of a few tokens.
+// knows the work of most batches: up to a few thousand rows they take one launch of k_attn_head, a workgroup for each
+// (sequence, kv head) or each 16 rows of a few tokens.
 //
 // Measured (H 32, 8 kv heads, D 128, bf16 unless said; calls back to back):
 //   64 sequences of one token, windows of 1,024, 268 MB    47 us   5.7 TB/s (reads alone: 7.1): 8 waves of a CU and what
@@ -16,6 +16,7 @@
 //                                                                  which it issues 2,600 (283 vector, 228 scalar instructions)
 //   17 sequences, fp32 q, 5 heads of 96, pages of 21, 2,500    33 us   2.5 TB/s: waves with one unit in flight wait for it
 //                                                                  half of their time
+//   the chunks with fp32 queries, f16 / bf16 pages       487 / 595 us   two and three products for each
 //   1 sequence, D 64, f16, 512                              9 us   latency of one workgroup
 // Measured and left: 64 rows a wave with 4 waves and all 512 registers (433 us for the chunks, 822 with accumulation
 // registers); one lookup for units in one page (313, but 47 -> 51 for 64 sequences behind 8,192 shared keys, which share

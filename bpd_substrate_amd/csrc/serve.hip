@@ -201,13 +201,13 @@ void append(const char* fn, void* hip_stream, const bpd_paged_cache* kv, const b
     const double* turns = rot > 0 ? rope->turns : nullptr;
     const bool neox = rot > 0 && rope->neox == 1;
     if (norm != nullptr && (norm->q != nullptr || norm->k != nullptr))
-        bpdq::launch_norm_append(paged(*kv, *b), kv->type, *norm, turns, rot, neox, pos, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, x_type, n_heads, stream);
+        bpdq::launch_norm_append(paged(*kv, *b), kv->type, *norm, turns, rot, neox, pos, q, q_stride, k, k_stride, v, v_stride,
+                                 q_out, q_out_stride, x_type, n_heads, stream);
     else
         bpdq::launch_rope_append(paged(*kv, *b), kv->type, turns, rot, neox, pos, q, q_stride, k, k_stride, v, v_stride,
                                  q_out, q_out_stride, x_type, n_heads, stream);
     bpdq::abi_hip_ok(hipGetLastError(), fn);
 }
-
 
 void check_window(Args& c, int window, int sinks) {
     c.shape(window >= 1, "window is below 1").shape(sinks >= 0, "sinks is negative");
