@@ -7,7 +7,7 @@
 // Memory bounds it, then the history's latency before a slice's logits can change: 256 x 128,256 binary16 to fp32 with
 // 1,000 tokens and a mask each, 202 MB, 47.5 us = 4.25 TB/s (a copy: 5.1); 64 x 128,256 fp32 with up to 16,384 tokens, 300
 // biases, some masks, 68 MB, 18 us (with the logits read behind the counts and 4-byte reads of the history: 36).  In place,
-where the counts say what to read, 18 us for the 64, with penalties alone 15.6 (a new tensor 19.2).  Measured
+// where the counts say what to read, 18 us for the 64, with penalties alone 15.6 (a new tensor 19.2).  Measured
 // and left: stores past the caches, 43 us for the 256, but 5 to 6 more for the sampling that reads them; slices of 4,096 or
 // 16,384 and workgroups of 256 or 1,024 (48 to 56 us).
 #include "bpdq_paged.h"
