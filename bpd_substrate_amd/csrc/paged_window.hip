@@ -82,7 +82,7 @@ int64_t even_tiles(const Paged& a, int G, int R) {
 }
 
 // The same for several tokens of a sequence, whose rows go 16 to a workgroup or by k_attn_plan, k_attn_tile and k_attn_join.
-// Those have 40 us of launches and uneven shares, and read the keys once for R rows; the cost of a unit, all CUs working,
+// Those have 20 us of launches (few workgroups) to 40 (uneven shares), and read the keys once for R rows; the cost of a unit, all CUs working,
 // is in ns.  Measured (us, 16 rows to a workgroup / tiles; 8 kv heads of 128, 4 query heads each, bf16):
 //   64 sequences, 516 rows, 2 / 4 / 8 / 16 / 32 tokens    35, 81 / 36, 83 / 54, 90 / 82, 106 / 142, 109
 //   64, 2,052 rows, 4 / 8 / 16                            92, 172 / 152, 180 / 238, 196

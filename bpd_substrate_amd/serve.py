@@ -278,6 +278,7 @@ class PagePool:
         self.c = _Pool(table.data_ptr(), table.stride(0) if R > 1 else W, _int(W, "table's width"), lens.data_ptr(),
                        None if gone is None else gone.data_ptr(), free.data_ptr(), n_free.data_ptr(), _int(R, "n_rows"),
                        _int(self.n_pages, "n_pages"), _int(page_size, "page_size"))
+        self._lens = lens.data_ptr(), lens.data_ptr() + 4 * R
         self._p = ctypes.addressof(self.c)
 
     @classmethod
@@ -299,11 +300,14 @@ class PagePool:
             _tensor(t, what, (torch.int32,), 1, self.device, contiguous=True)
             if rows is not None and rows.shape != t.shape:
                 _bad(f"{what} has {t.shape[0]} values and rows {rows.shape[0]}")
-            # read for one sequence while another's length is written
-            if rows is not None and -4 * t.shape[0] < t.data_ptr() - self.c.lens < 4 * self.n_rows:
-                _bad(f"{what} lies in the pool's lens: pass a copy, or no rows")
         n = t.shape[0] if t is not None else rows.shape[0] if rows is not None else self.n_rows
-        return _int(n, "n_seqs"), None if rows is None else rows.data_ptr(), None if t is None else t.data_ptr()
+        if n > _TOP:
+            _int(n, "n_seqs")
+        at = None if t is None else t.data_ptr()
+        # read for one sequence while another's length is written
+        if rows is not None and at is not None and self._lens[0] - 4 * n < at < self._lens[1]:
+            _bad(f"{what} lies in the pool's lens: pass a copy, or no rows")
+        return n, None if rows is None else rows.data_ptr(), at
 
     def extend(self, new, n_tokens, rows=None, prefix_len=0):
         """Sequence b, row rows[b] of the pool (None: row b), grows by new[b] rows (int32, on the device): a PageStep.
@@ -314,8 +318,8 @@ class PagePool:
         dev, T, W = self.device, n_tokens, self.width
         if T < 0:
             _bad("n_tokens is negative")
-        _int(T, "n_tokens")
-        _int(prefix_len, "prefix_len")
+        if T > _TOP or not 0 <= prefix_len <= _TOP:
+            _bad(f"n_tokens {T} or prefix_len {prefix_len} does not fit 31 bits")
         sizes = (B, B + 1, T, T, B, 0 if rows is None else B * W)
         out = torch.empty(sum(sizes), dtype=torch.int32, device=dev)
         lens, q_start, slots, pos, refused, table = out.split_with_sizes(sizes)
@@ -339,8 +343,9 @@ class PagePool:
         if sinks < 0 or prefix_len < 0:
             _bad("sinks or prefix_len is negative")
         # rows end below _TOP: beyond it a window, or first rows, are all of them
-        _launch(self.device, gpu._fn("bpd_pages_release_on_gpu"), self._p, rp, kp, B, 0 if window is None else min(window, _TOP),
-                min(max(0, sinks - prefix_len), _TOP))
+        w, own = 0 if window is None else window if window < _TOP else _TOP, sinks - prefix_len
+        _launch(self.device, gpu._fn("bpd_pages_release_on_gpu"), self._p, rp, kp, B, w,
+                0 if own < 0 else own if own < _TOP else _TOP)
 
 
 def _weights(w, what, x, heads, D):
@@ -509,8 +514,8 @@ def adjust_logits(logits, tokens=None, lens=None, prompt=None, repetition=None, 
     if logits.dim() != 2:
         _bad(f"logits have {logits.dim()} dimensions, not 2")
     B, V = logits.shape
-    _int(B, "rows of logits")
-    _int(V, "vocab")
+    if B > _TOP or V > _TOP:
+        _bad(f"logits are {B} x {V}: neither may pass 31 bits")
     dev = logits.device
     xs = _pitch(logits, "logits")
     if out is None:
