@@ -28,7 +28,8 @@ namespace bpdq {
 namespace {
 
 constexpr int64_t kMostItems = 1 << 22;  // workgroups of 512 threads in a launch
-constexpr int64_t kMostRows = 8192;      // that one workgroup may have to take for 16 rows of queries
+// Rows that one workgroup may have to take for 16 rows of queries, where there are no more workgroups than these.
+constexpr int64_t kMostRows = 8192, kManyItems = 512;
 
 bool whole_pages(const Paged& a) { return a.page.d % 16 == 0 && a.row_stride < 1 << 26; }
 
@@ -53,17 +54,20 @@ int waves_at_once(int most, int64_t items, int64_t waves) {
 //   128, 1,028 / 4,100                     18.1, 19.5, 27.1 / 62.7, 66.6, 68.6
 //   512, 1,028 / 4,100                     52.0, 46.6, 64.6 / 172.7, 170.5, 182.8
 // The lengths are on the device, and one sequence may have most of the rows: beyond 4,096, where dealing and join are little
-// beside them, they are dealt for any number of items (one launch, two; all lengths the same, a quarter of the rows to all,
-// one sequence of all and the others of 512):
+// beside them, they are dealt unless more than 4,096 items keep the chip busy beside it (one launch, two; all lengths the
+// same, a quarter of the rows to all, one sequence of all and the others of 512):
 //   512, 4,100 / 16,388    179, 182 / 679, 641    135, 129 / 431, 392    65, 38 / 196, 50
 //   128, 4,100 / 16,388    52, 54 / 199, 171      45, 39 / 161, 109      44, 32 / 148, 47
 //   128 of 256, 4,100      110, 116               98, 95                 83, 62
+//   2,048, 4,100 / 16,388  -                      421, 421 / 1,698, 1,549    99, 107 / 229, 117
+//   8,192, 4,100 / 16,388  -                      1,706, 1,744 / 6,942, 6,854    367, 395 / 382, 402
 // Waves with one unit in flight (`single`: fp32 queries, pages that are no multiple of 16 rows) take more than twice as
 // long for a row (5 heads of 96, page 21, 5 items, 516 / 1,028 rows: 14.7, 18.4, 14.2 / 21.7, 30.0, 15.8; 320 items:
 // 30.8, 23.8, 27.8 / 49.0, 41.6, 40.5).  Heads of 256 fill the registers with 4 waves (2 heads, 2 items, 516 / 1,028 rows:
 // -, 17.0, 17.8 / -, 24.0, 21.0; 128 items: -, 21.3, 43.6 / -, 37.0, 56.0).
 int head_waves(int DT, bool single, int64_t items, int64_t rows) {
-    if (rows > 4096 || (DT == 256 ? items < 128 && rows > 640 : single ? rows > 640 : items < 128 && rows > 2304)) return 0;
+    if (rows > 4096 && items <= 4096) return 0;
+    if (DT == 256 ? items < 128 && rows > 640 : single ? rows > 640 : items < 128 && rows > 2304) return 0;
     const int most = DT == 256 ? 4 : 8;
     if (few_rows(DT, single, rows)) return waves_at_once(most, items, chip_waves(DT));
     return items <= 256 ? most : 4;
@@ -82,8 +86,8 @@ int64_t even_tiles(const Paged& a, int G, int R) {
 }
 
 // The same for several tokens of a sequence, whose rows go 16 to a workgroup or by k_attn_plan, k_attn_tile and k_attn_join.
-// Those have 20 us of launches (few workgroups) to 40 (uneven shares), and read the keys once for R rows; the cost of a unit, all CUs working,
-// is in ns.  Measured (us, 16 rows to a workgroup / tiles; 8 kv heads of 128, 4 query heads each, bf16):
+// Those have 20 us of launches (few workgroups) to 40 (uneven shares), and read the keys once for R rows; the cost of a
+// unit, all CUs working, is in ns.  Measured (us, 16 rows to a workgroup / tiles; 8 kv heads of 128, 4 query heads each, bf16):
 //   64 sequences, 516 rows, 2 / 4 / 8 / 16 / 32 tokens    35, 81 / 36, 83 / 54, 90 / 82, 106 / 142, 109
 //   64, 2,052 rows, 4 / 8 / 16                            92, 172 / 152, 180 / 238, 196
 //   8, 516 and 2,052 rows, 64                             35, 57 and 86, 74
@@ -95,8 +99,13 @@ int64_t even_tiles(const Paged& a, int G, int R) {
 // 131,076 1,724, 150 / 1,730, 153; 2,052 and 4,100 rows with fp32 queries 23.5, 22.2 and 36.5, 24.1, in pages of 21
 // 27.2, 24.0 and 45.0, 26.7; heads of 256, 1,028 and 4,100 27.4, 25.4 and 75.0, 34.6).
 // The lengths are on the device: a workgroup may get all the rows and the others few, while tiles deal what is there.
-// Beyond kMostRows that risk is not taken (64 sequences of one token, lengths from a quarter of the rows to all: 8,196 rows
-// 301, 355, 16,388 548, 613; 65 of two tokens, one of 19,264 rows and the others of 512: 473, 94).
+// Beyond kMostRows that risk is taken only where more than kManyItems workgroups keep the chip busy beside it, which tiles
+// of few rows do worse (sequences of one token, 8 workgroups to each; 8,196 and 16,388 rows; lengths from a quarter of the
+// rows to all / one of all and the others of 512:
+//   64 sequences     301, 355 and 548, 613 / 65 of two tokens, 19,264 rows 473, 94
+//   128              514, 682 and 999, 1,223 / 212, 125 and 411, 134
+//   256              981, 1,324 and 1,869, 2,489 / 234, 215 and 425, 222
+//   1,024            3,587, 5,241 and 7,064, 9,914 / 462, 743 and 500, 747).
 // Of the workgroups up to one per sequence has no tokens and ends at once: the chip is taken for a quarter larger (us, 4 / 2 / 1
 // waves; 64 sequences, 516 rows, up to 4 and 8 tokens 31.1, 28.0, 40.7 and 40.2, 37.2, 43.9; 107, heads of 64, 122 rows, 6
 // tokens 29.3, 19.5, 15.3; 128, 132 rows, 4 tokens 30.2, 24.9, 21.7).
@@ -106,7 +115,7 @@ int rows_waves(const Paged& a, int G, int R, bool single, int64_t rows) {
     const int64_t items = even_tiles(a, G, 16) * a.hkv;
     const double one = head * (double)(items > kGroups ? items : kGroups) * (double)((rows + 63) / 32);
     const double plan = 40e3 + tile * (double)(even_tiles(a, G, R) * a.hkv) * (double)((rows + 127) / 64);
-    if (rows > kMostRows || one >= plan || tiles_of(a, G, 16) * a.hkv > kMostItems) return 0;
+    if ((rows > kMostRows && items <= kManyItems) || one >= plan || tiles_of(a, G, 16) * a.hkv > kMostItems) return 0;
     const int most = DT == 256 ? 4 : 8;
     if (few_rows(DT, single, rows)) return waves_at_once(most, tiles_of(a, G, 16) * a.hkv, chip_waves(DT) * 5 / 4);
     return items <= 256 ? most : 4;

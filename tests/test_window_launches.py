@@ -53,3 +53,12 @@ def test_one_token_each_of_many_sequences(launched, B, shape):
     for rows in (4100, 131072):
         assert kernels(launched, [1] * B, rows, *shape, decode=True) == DEALT
     assert kernels(launched, [1] * B, 131072, *shape, decode=True, win=2048) == ONE
+
+
+def test_so_many_sequences_that_one_may_be_long(launched):
+    """The others keep the chip busy beside it, and tiles or dealt units would need a workspace of gigabytes."""
+    for rows in (8196, 131072):
+        assert kernels(launched, [1] * 65, rows, 32, 8, 128, "bf16", "bf16", 64) == ONE
+        assert kernels(launched, [1] * 64, rows, 32, 8, 128, "bf16", "bf16", 64) == TILES
+        assert kernels(launched, [1] * 513, rows, 32, 8, 128, "bf16", "bf16", 64, decode=True) == ONE
+        assert kernels(launched, [1] * 512, rows, 32, 8, 128, "bf16", "bf16", 64, decode=True) == DEALT
